@@ -518,6 +518,125 @@ int sparkmv_model_embed_row(void * model, uint32_t id, float * out, void * strea
  * keeps the lowest thread's candidate on ties instead. */
 int sparkmv_argmax(const float * logits, int n, int * out, void * stream);
 
+/* ---- several sequences: a paged cache that holds keys and values in 8 bits ----
+ * No counterpart in the reference, which serves one sequence from f32 rows.
+ * A page holds SPARKMV_KV_PAGE positions of every kv head; a page and kv head
+ * have one scale for the keys and one for the values, and a cached value is
+ * its code (-127..127) times the scale. A sequence is a slot: a row of the
+ * page table, entry j naming the page of positions 64 j .. 64 j + 63. The
+ * caller owns every array, hands out pages and keeps the lengths; several
+ * slots may name one page as long as none appends to it. Codes of a page's
+ * kv head lie as
+ *   keys    [head_dim / 64][64 positions][64]
+ *   values  [g 4][head_dim][t 4][i 4], position 16 t + 4 g + i.
+ *
+ * Every call is asynchronous on its stream, allocates nothing, clears nothing
+ * with a memset and reads slots, positions, lengths and page numbers from
+ * device memory, so it may be captured into a HIP graph and replayed as they
+ * change. What device memory says is checked there: a slot or page number out
+ * of range, a negative position, rows outside the call's are left out (neither
+ * read nor written), never followed. */
+#define SPARKMV_KV_PAGE 64
+
+typedef struct {
+    int kv_heads, head_dim;        /* head_dim 64, 128 or 256 */
+    int npages;                    /* pages of the pool */
+    int nslots, max_pages;         /* the page table's rows and entries per row */
+    int8_t * k, * v;               /* codes [npages][kv_heads][64 * head_dim], 16-byte aligned */
+    float * k_scale, * v_scale;    /* [npages][kv_heads] */
+    const int * pages;             /* [nslots][max_pages], device */
+} sparkmv_kv_cache;
+
+/* The sequences of one call: sequence i is slot[i] (NULL: slot i), its new
+ * tokens are rows qstart[i] .. qstart[i + 1] - 1 of the call's ntok rows (NULL:
+ * row i alone) at positions pos[i] .. A negative pos leaves the sequence out.
+ * Rows of no sequence are left as they were. max_q bounds the new tokens of
+ * one sequence (further ones are left out); max_len is the longest length
+ * after the call as far as the host knows: it shapes launches only, and a
+ * longer sequence is still served in full. nseq is at most 4096. */
+typedef struct {
+    int nseq, ntok, max_q, max_len;
+    const int * slot, * pos, * qstart;   /* device */
+} sparkmv_kv_batch;
+
+/* The new tokens' rows: q [ntok][ldq] holds heads x head_dim values a token, k
+ * and v kv_heads x head_dim, in x_dtype; rows start 16-byte aligned. */
+typedef struct {
+    const void * q, * k, * v;      /* q NULL (and heads 0): no queries to rotate */
+    int ldq, ldk, ldv, x_dtype, heads;
+    const float * rope;            /* [rope_rows][rope_dim]: cosines, then sines; NULL with rope_dim 0 */
+    int rope_rows, rope_dim;
+    void * q_out;                  /* [ntok][ldqo], x_dtype; may be q itself */
+    int ldqo;
+} sparkmv_kv_new;
+
+/* cos and sin of position * theta^(-2 i / rope_dim), i < rope_dim / 2, for
+ * positions 0 .. rows - 1, with the model's own f32 expressions
+ * (tools/vq-runtime/src/model.rs:416-428). */
+int sparkmv_rope_table(float * table, int rows, int rope_dim, double theta, void * stream);
+
+/* Append: elements e < rope_dim / 2 of each q and k head turn with e + rope_dim / 2
+ * by their position's row of the table (products and sums in 64 bits, one
+ * rounding to f32 for a key, to x_dtype for a query), and keys and values enter
+ * their pages. A page opened here (its first position is new), or whose scale
+ * no longer covers its new values, takes the scale
+ *   f32(largest |new value| * h / 127),  h = 1 if the page is full after the call, else 1.25
+ * and its older codes are rounded anew to it; a code is the value over the
+ * scale, rounded to nearest even. The headroom h makes a later growth rare and
+ * keeps the sum of all roundings under 2.5 steps however often it happens. A
+ * value that is not finite makes the scale NaN, and the page's head reads as
+ * NaN until its first position is appended again. A sequence may be cut back
+ * to any length (append again at a smaller pos): a page keeps its scale then. A slot may appear
+ * once in an append. The table must cover 64 * max_pages positions. */
+int sparkmv_kv_append(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_new * rows,
+                      void * stream);
+
+/* Cached positions as values: k_out and v_out (either may be NULL) are
+ * [nseq][n][kv_heads][head_dim] in out_dtype; row j of sequence i is position
+ * from[i] + j of slot[i] (NULL: slot i). Positions without a page are zero. */
+int sparkmv_kv_read(const sparkmv_kv_cache * cache, int nseq, const int * slot, const int * from, int n, void * k_out,
+                    void * v_out, int out_dtype, void * stream);
+
+/* The new tokens' queries and what attention returns. */
+typedef struct {
+    const void * q;                /* [ntok][ldq] rotated queries, heads x head_dim a token, rows 16-byte aligned */
+    int ldq, q_dtype, heads;       /* heads: a multiple of kv_heads, at most 16 times */
+    float scale;                   /* of the scores */
+    int window;                    /* positions a token sees, its own included; 0: all */
+    const float * gate;            /* [ntok][ldg]: a head's output times sigmoid of it; NULL: none */
+    int ldg;
+    void * out;                    /* [ntok][ldo], heads x head_dim a token, rows 16-byte aligned */
+    int ldo, out_dtype;
+    void * work;                   /* sparkmv_kv_attend_work bytes, 256-byte aligned; not shared by calls that overlap */
+    size_t work_bytes;
+} sparkmv_kv_query;
+
+/* Bytes of workspace an attention call of these sizes needs on the current
+ * device (pointers are not read). */
+size_t sparkmv_kv_attend_work(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, int heads);
+/* Attention over the cache after the append: token j of a sequence, at
+ * position pos + j, sees positions up to its own (the last `window` of them).
+ * Softmax statistics and sums are f32. A token none of whose positions has a
+ * page gives zeros. Queries and outputs may be f32 or bf16 apart. */
+int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_query * query,
+                      void * stream);
+
+/* ---- log probabilities ----
+ * Beside sparkmv_argmax: for each of `rows` rows of n logits (x_dtype, row
+ * stride ld), with lse = log sum e^x: logprob[r] = x[tokens[r]] - lse,
+ * entropy[r] = -sum p log p with p = e^(x - lse), and the k <= 32 largest
+ * logits in order (equal ones by lower index): top_id[r][k], top_logprob[r][k].
+ * tokens and logprob, entropy, and with k = 0 the tops, may be NULL. -inf is a
+ * masked logit (p = 0, log probability -inf); a row of nothing else has
+ * entropy 0. A NaN or +inf makes the row's values NaN and NaN is never chosen;
+ * where fewer than k can be, the rest are id -1, -inf. A token outside the row
+ * gives NaN. No counterpart in the reference. work: sparkmv_logprobs_work
+ * bytes, 256-byte aligned, not shared by calls that overlap. */
+size_t sparkmv_logprobs_work(int rows, int n, int k);
+int sparkmv_logprobs(const void * logits, int x_dtype, int rows, int n, size_t ld, const int * tokens, int k,
+                     float * logprob, float * entropy, int * top_id, float * top_logprob, void * work,
+                     size_t work_bytes, void * stream);
+
 /* A checkpoint's config.json (tools/vq-runtime/src/config.rs:39-85,
  * Config::load): hidden_size, num_hidden_layers, num_attention_heads,
  * num_key_value_heads, head_dim, intermediate_size, vocab_size,

@@ -80,6 +80,31 @@ class ChainMatrix(ctypes.Structure):
                 ("y_add", ctypes.c_void_p), ("rows", ctypes.c_int)]
 
 
+class KvCache(ctypes.Structure):
+    _fields_ = [("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("npages", ctypes.c_int),
+                ("nslots", ctypes.c_int), ("max_pages", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("pages", ctypes.c_void_p)]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("nseq", ctypes.c_int), ("ntok", ctypes.c_int), ("max_q", ctypes.c_int), ("max_len", ctypes.c_int),
+                ("slot", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("qstart", ctypes.c_void_p)]
+
+
+class KvNew(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ldq", ctypes.c_int),
+                ("ldk", ctypes.c_int), ("ldv", ctypes.c_int), ("x_dtype", ctypes.c_int), ("heads", ctypes.c_int),
+                ("rope", ctypes.c_void_p), ("rope_rows", ctypes.c_int), ("rope_dim", ctypes.c_int),
+                ("q_out", ctypes.c_void_p), ("ldqo", ctypes.c_int)]
+
+
+class KvQuery(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("ldq", ctypes.c_int), ("q_dtype", ctypes.c_int), ("heads", ctypes.c_int),
+                ("scale", ctypes.c_float), ("window", ctypes.c_int), ("gate", ctypes.c_void_p), ("ldg", ctypes.c_int),
+                ("out", ctypes.c_void_p), ("ldo", ctypes.c_int), ("out_dtype", ctypes.c_int),
+                ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_size_t)]
+
+
 # chain op input transforms (sparkmv_chain_add_vq x_mode)
 X_MODE_BF16, X_MODE_F32, X_MODE_NORM = 0, 1, 2
 
@@ -187,6 +212,13 @@ SIGNATURES = {
     "sparkmv_model_captured": (_I, [_P, _I, _PP]),
     "sparkmv_model_embed_row": (_I, [_P, ctypes.c_uint32, _P, _P]),
     "sparkmv_argmax": (_I, [_P, _I, _P, _P]),
+    "sparkmv_rope_table": (_I, [_P, _I, _I, ctypes.c_double, _P]),
+    "sparkmv_kv_append": (_I, [_P, _P, _P, _P]),
+    "sparkmv_kv_read": (_I, [_P, _I, _P, _P, _I, _P, _P, _I, _P]),
+    "sparkmv_kv_attend_work": (_S, [_P, _P, _I]),
+    "sparkmv_kv_attend": (_I, [_P, _P, _P, _P]),
+    "sparkmv_logprobs_work": (_S, [_I] * 3),
+    "sparkmv_logprobs": (_I, [_P, _I, _I, _I, _S, _P, _I, _P, _P, _P, _P, _P, _S, _P]),
     "sparkmv_config_load": (_I, [ctypes.c_char_p, ctypes.POINTER(ModelCfg), ctypes.POINTER(_I), _I]),
     "sparkmv_model_load": (_P, [ctypes.c_char_p, ctypes.c_char_p, _I, _I, _I]),
     "sparkmv_model_apply_profile": (_I, [_P, _P, _U64, ctypes.c_char_p]),
@@ -759,6 +791,276 @@ def argmax(logits, stream=None):
     out = torch.empty(1, dtype=torch.int32, device=logits.device)
     check(lib().sparkmv_argmax(logits.data_ptr(), logits.numel(), out.data_ptr(), _stream_ptr(stream)), "argmax")
     return out
+
+
+class _Call:
+    """One operator's call with its arguments laid out once: call it (on the
+    current stream, or the given one) as often as the tensors it holds change
+    their values. It runs on the device of its tensors."""
+
+    def __init__(self, fn, args, device, what, keep):
+        self.fn, self.args, self.what, self.keep = fn, args, what, keep
+        self.device = device.index if device.index is not None else _torch().cuda.current_device()
+
+    def __call__(self, stream=None):
+        cuda = _torch().cuda
+        if cuda.current_device() != self.device:
+            with cuda.device(self.device):
+                return self(stream)
+        s = (cuda.current_stream() if stream is None else stream).cuda_stream
+        if self.fn(*self.args, s) != 0:
+            raise SparkmvError(f"{self.what}: {last_error()}")
+
+
+def _used_on(stream, *tensors):
+    """Tensors made here on the current stream and used on the caller's: their
+    memory is not handed out again before that stream's work is done"""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
+def _kv_tensor(what, t, dtypes, shape, device):
+    """t checked: a device tensor of one of dtypes; shape entries of None are free"""
+    if t.dtype not in dtypes:
+        raise SparkmvError(f"{what}: type {t.dtype} is none of {', '.join(str(d) for d in dtypes)}")
+    if len(t.shape) != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape)):
+        raise SparkmvError(f"{what}: shape {tuple(t.shape)} is not {tuple('any' if w is None else w for w in shape)}")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise SparkmvError(f"{what}: on {t.device}, not on {device or 'a GPU'}")
+    return t
+
+
+def _kv_flat(what, t, dtypes, shape, device):
+    if not _kv_tensor(what, t, dtypes, shape, device).is_contiguous():
+        raise SparkmvError(f"{what}: not contiguous")
+    return t
+
+
+def _kv_rows(what, t, dtypes, heads, head_dim, device):
+    """[rows, heads, head_dim] or [rows, heads * head_dim] with whole rows: the
+    row count and the row stride"""
+    shape = (None, heads, head_dim) if t.dim() == 3 else (None, heads * head_dim)
+    _kv_tensor(what, t, dtypes, shape, device)
+    if (t.dim() == 3 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim))) or (t.dim() == 2 and t.stride(1) != 1):
+        raise SparkmvError(f"{what}: a row's values are not side by side")
+    return t.shape[0], t.stride(0) if t.shape[0] > 1 else heads * head_dim
+
+
+def rope_table(rows, rope_dim, theta, device="cuda", stream=None):
+    """[rows, rope_dim] f32: cos then sin of position * theta^(-2 i / rope_dim)
+    (sparkmv_rope_table, the model's own expressions)."""
+    torch = _torch()
+    out = torch.empty((rows, rope_dim), dtype=torch.float32, device=device)
+    with torch.cuda.device(out.device):
+        check(lib().sparkmv_rope_table(out.data_ptr(), rows, rope_dim, float(theta), _stream_ptr(stream)), "rope table")
+    return out
+
+
+class KVBatch:
+    """The sequences of one call over a PagedKV (sparkmv_kv_batch). pos: device
+    int32 [nseq], each sequence's first new position (negative: left out).
+    qstart: device int32 [nseq + 1], the rows of its new tokens among ntok (None:
+    row i is sequence i's one token). slot: device int32 [nseq] (None: slot i).
+    max_q bounds a sequence's new tokens, max_len is the longest length the
+    host expects (it shapes launches only). The tensors' values are read when
+    a call runs."""
+
+    def __init__(self, pos, ntok=None, qstart=None, slot=None, max_q=None, max_len=None):
+        i32 = (_torch().int32,)
+        self.device = pos.device
+        nseq = pos.shape[0]
+        self.keep = [_kv_flat("kv batch positions", pos, i32, (None,), None)]
+        if qstart is not None:
+            self.keep.append(_kv_flat("kv batch rows", qstart, i32, (nseq + 1,), self.device))
+        if slot is not None:
+            self.keep.append(_kv_flat("kv batch slots", slot, i32, (nseq,), self.device))
+        self.ntok = nseq if ntok is None else int(ntok)
+        if max_q is None:
+            max_q = max(1, self.ntok) if qstart is not None else 1
+        self.c = KvBatch(nseq=nseq, ntok=self.ntok, max_q=int(max_q), max_len=int(max_len or 0),
+                         slot=_ptr(slot), pos=pos.data_ptr() if nseq else None, qstart=_ptr(qstart))
+
+
+class PagedKV:
+    """Keys and values of several sequences in 8 bits, in pages of 64 positions
+    with one scale per page and kv head (sparkmv_kv_*). pages: the page table,
+    device int32 [nslots, max_pages], -1 where a slot has no page; k, v, the
+    scales and the table are made here unless given (layers share a table).
+    The caller hands out pages and keeps the lengths."""
+
+    PAGE = 64
+
+    def __init__(self, kv_heads, head_dim, npages, nslots, max_pages, pages=None, k=None, v=None, k_scale=None,
+                 v_scale=None, device="cuda"):
+        torch = _torch()
+        self.kv_heads, self.head_dim = int(kv_heads), int(head_dim)
+        self.npages, self.nslots, self.max_pages = int(npages), int(nslots), int(max_pages)
+        given = [t for t in (pages, k, v, k_scale, v_scale) if t is not None]
+        dev = given[0].device if given else torch.empty(0, device=device).device
+        codes, scales = (self.npages, self.kv_heads, self.PAGE * self.head_dim), (self.npages, self.kv_heads)
+        self.pages = torch.full((self.nslots, self.max_pages), -1, dtype=torch.int32, device=dev) if pages is None else pages
+        self.k = torch.zeros(codes, dtype=torch.int8, device=dev) if k is None else k
+        self.v = torch.zeros(codes, dtype=torch.int8, device=dev) if v is None else v
+        self.k_scale = torch.zeros(scales, device=dev) if k_scale is None else k_scale
+        self.v_scale = torch.zeros(scales, device=dev) if v_scale is None else v_scale
+        _kv_flat("kv pages", self.pages, (torch.int32,), (self.nslots, self.max_pages), dev)
+        for what, t in (("kv keys", self.k), ("kv values", self.v)):
+            _kv_flat(what, t, (torch.int8,), codes, dev)
+        for what, t in (("kv key scales", self.k_scale), ("kv value scales", self.v_scale)):
+            _kv_flat(what, t, (torch.float32,), scales, dev)
+        self.device = dev
+        self.c = KvCache(kv_heads=self.kv_heads, head_dim=self.head_dim, npages=self.npages, nslots=self.nslots,
+                         max_pages=self.max_pages, k=self.k.data_ptr(), v=self.v.data_ptr(),
+                         k_scale=self.k_scale.data_ptr(), v_scale=self.v_scale.data_ptr(), pages=self.pages.data_ptr())
+
+    def _same(self, batch):
+        if batch.device != self.device:
+            raise SparkmvError(f"kv batch: on {batch.device}, not on {self.device}")
+
+    def append_op(self, batch, q, k, v, rope=None, q_out=None):
+        """The call that rotates q into q_out and k by the table, and appends k
+        and v ([ntok, heads, head_dim] or flat rows, f32 or bf16). q None: keys
+        and values only."""
+        torch = _torch()
+        self._same(batch)
+        xt = (k.dtype,) if k.dtype in (torch.float32, torch.bfloat16) else (torch.float32, torch.bfloat16)
+        n = KvNew(x_dtype=X_F32 if k.dtype == torch.float32 else X_BF16)
+        for name, t in (("k", k), ("v", v)):
+            rows, ld = _kv_rows("kv append " + name, t, xt, self.kv_heads, self.head_dim, self.device)
+            if rows < batch.ntok:
+                raise SparkmvError(f"kv append {name}: {rows} rows for {batch.ntok} tokens")
+            setattr(n, name, t.data_ptr())
+            setattr(n, "ld" + name, ld)
+        if (q is None) != (q_out is None):
+            raise SparkmvError("kv append: queries and their output do not agree")
+        if q is not None:
+            n.heads = q.shape[1] if q.dim() == 3 else q.shape[1] // self.head_dim
+            for name, ldn, t in (("q", "ldq", q), ("q_out", "ldqo", q_out)):
+                rows, ld = _kv_rows("kv append " + name, t, xt, n.heads, self.head_dim, self.device)
+                if rows < batch.ntok:
+                    raise SparkmvError(f"kv append {name}: {rows} rows for {batch.ntok} tokens")
+                setattr(n, name, t.data_ptr())
+                setattr(n, ldn, ld)
+        if rope is not None:
+            _kv_flat("kv append rope", rope, (torch.float32,), (None, None), self.device)
+            n.rope, n.rope_rows, n.rope_dim = rope.data_ptr(), rope.shape[0], rope.shape[1]
+        return _Call(lib().sparkmv_kv_append, (ctypes.addressof(self.c), ctypes.addressof(batch.c), ctypes.addressof(n)),
+                     self.device, "kv append", (self, batch, q, k, v, rope, q_out, n))
+
+    def append(self, batch, q, k, v, rope=None, q_out=None, stream=None):
+        self.append_op(batch, q, k, v, rope, q_out)(stream)
+
+    def read_op(self, start, k_out=None, v_out=None, slot=None):
+        """The call that reads positions start[i] .. of slot[i] (None: slot i) into
+        k_out and v_out ([nseq, n, kv_heads, head_dim], f32 or bf16)."""
+        torch = _torch()
+        i32, ft = (torch.int32,), (torch.float32, torch.bfloat16)
+        outs = [t for t in (k_out, v_out) if t is not None]
+        if not outs:
+            raise SparkmvError("kv read: nothing to read into")
+        _kv_flat("kv read start", start, i32, (None,), self.device)
+        for t in outs:
+            _kv_flat("kv read", t, ft, (start.shape[0], outs[0].shape[1], self.kv_heads, self.head_dim), self.device)
+            if t.dtype != outs[0].dtype:
+                raise SparkmvError("kv read: keys and values of two types")
+        if slot is not None:
+            _kv_flat("kv read slots", slot, i32, (start.shape[0],), self.device)
+        return _Call(lib().sparkmv_kv_read,
+                     (ctypes.addressof(self.c), start.shape[0], _ptr(slot), start.data_ptr(), outs[0].shape[1],
+                      _ptr(k_out), _ptr(v_out), X_F32 if outs[0].dtype == torch.float32 else X_BF16),
+                     self.device, "kv read", (self, start, k_out, v_out, slot))
+
+    def read(self, start, k_out=None, v_out=None, slot=None, stream=None):
+        self.read_op(start, k_out, v_out, slot)(stream)
+
+    def attend_op(self, batch, q, out, scale=None, window=0, gate=None, work=None):
+        """The call that attends q (rotated, [ntok, heads, head_dim] or flat rows,
+        f32 or bf16) over the cache into out (the same shape, f32 or bf16).
+        scale: of the scores (None: head_dim ** -0.5). window: positions a token
+        sees, its own included (0: all). gate: f32 [ntok, heads]; a head's output
+        times its sigmoid. work: uint8 tensor (None: made here); calls that may
+        overlap need one each."""
+        torch = _torch()
+        self._same(batch)
+        ft = (torch.float32, torch.bfloat16)
+        heads = q.shape[1] if q.dim() == 3 else q.shape[1] // self.head_dim
+        n = KvQuery(heads=heads, scale=self.head_dim ** -0.5 if scale is None else float(scale), window=int(window),
+                    q_dtype=X_F32 if q.dtype == torch.float32 else X_BF16,
+                    out_dtype=X_F32 if out.dtype == torch.float32 else X_BF16)
+        for name, ldn, t in (("q", "ldq", q), ("out", "ldo", out)):
+            rows, ld = _kv_rows("kv attend " + name, t, ft, heads, self.head_dim, self.device)
+            if rows < batch.ntok:
+                raise SparkmvError(f"kv attend {name}: {rows} rows for {batch.ntok} tokens")
+            setattr(n, name, t.data_ptr())
+            setattr(n, ldn, ld)
+        if gate is not None:
+            _kv_tensor("kv attend gate", gate, (torch.float32,), (None, heads), self.device)
+            if gate.shape[0] < batch.ntok or (heads > 1 and gate.stride(1) != 1):
+                raise SparkmvError("kv attend gate: rows of heads side by side, one a token, are needed")
+            n.gate, n.ldg = gate.data_ptr(), gate.stride(0) if gate.shape[0] > 1 else heads
+        with torch.cuda.device(self.device):
+            need = lib().sparkmv_kv_attend_work(ctypes.addressof(self.c), ctypes.addressof(batch.c), heads)
+        if work is None and need:
+            work = torch.empty(need, dtype=torch.uint8, device=self.device)
+        if work is not None:
+            _kv_flat("kv attend work", work, (torch.uint8,), (None,), self.device)
+            n.work, n.work_bytes = work.data_ptr(), work.numel()
+        return _Call(lib().sparkmv_kv_attend, (ctypes.addressof(self.c), ctypes.addressof(batch.c), ctypes.addressof(n)),
+                     self.device, "kv attend", (self, batch, q, out, gate, work, n))
+
+    def attend(self, batch, q, out, scale=None, window=0, gate=None, work=None, stream=None):
+        op = self.attend_op(batch, q, out, scale, window, gate, work)
+        op(stream)
+        _used_on(stream, op.keep[5])
+
+
+def logprobs_op(logits, tokens=None, logprob=None, entropy=None, top_id=None, top_logprob=None, work=None):
+    """The call that fills, for every row of logits ([rows, n] f32 or bf16), the
+    log probability of tokens[row] (int32), the entropy, and the top_id.shape[1]
+    <= 32 largest logits' ids (int32) and log probabilities (sparkmv_logprobs);
+    outputs that are None are left out."""
+    torch = _torch()
+    _kv_tensor("logits", logits, (torch.float32, torch.bfloat16), (None, None), None)
+    dev, (rows, n) = logits.device, logits.shape
+    if n > 1 and logits.stride(1) != 1:
+        raise SparkmvError("logits: a row's values are not side by side")
+    i32, f32 = (torch.int32,), (torch.float32,)
+    if (tokens is None) != (logprob is None) or (top_id is None) != (top_logprob is None):
+        raise SparkmvError("logprobs: an input or output without its other half")
+    k = 0 if top_id is None else top_id.shape[1]
+    for what, t, dt, shape in (("tokens", tokens, i32, (rows,)), ("logprob", logprob, f32, (rows,)),
+                               ("entropy", entropy, f32, (rows,)), ("top ids", top_id, i32, (rows, k)),
+                               ("top log probabilities", top_logprob, f32, (rows, k))):
+        if t is not None:
+            _kv_flat("logprobs " + what, t, dt, shape, dev)
+    with torch.cuda.device(dev):
+        need = lib().sparkmv_logprobs_work(rows, n, k)
+    if work is None and need:
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+    if work is not None:
+        _kv_flat("logprobs work", work, (torch.uint8,), (None,), dev)
+    return _Call(lib().sparkmv_logprobs,
+                 (logits.data_ptr(), X_F32 if logits.dtype == torch.float32 else X_BF16, rows, n,
+                  logits.stride(0) if rows > 1 else n, _ptr(tokens), k, _ptr(logprob), _ptr(entropy),
+                  _ptr(top_id) if k else None, _ptr(top_logprob) if k else None, _ptr(work),
+                  0 if work is None else work.numel()),
+                 dev, "logprobs", (logits, tokens, logprob, entropy, top_id, top_logprob, work))
+
+
+def logprobs(logits, tokens=None, k=0, stream=None):
+    """(logprob [rows] or None, entropy [rows], top_id [rows, k], top_logprob
+    [rows, k]) of logits [rows, n], as new tensors."""
+    torch = _torch()
+    rows, dev = logits.shape[0], logits.device
+    f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
+    lp = f(rows) if tokens is not None else None
+    ent, ids, tops = f(rows), torch.empty((rows, k), dtype=torch.int32, device=dev), f(rows, k)
+    op = logprobs_op(logits, tokens, lp, ent, ids, tops)
+    op(stream)
+    _used_on(stream, lp, ent, ids, tops, op.keep[6])
+    return lp, ent, ids, tops
 
 
 def _hip_copy(dst, src, nbytes):
