@@ -19,7 +19,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "lib", "libsparkmv.so")
 
 HIP_SOURCES = ["vq_kernels.hip", "kq_kernels.hip", "prefill.hip", "forward.hip", "chain.hip", "probe.hip", "kv.hip",
-               "logprobs.hip"]
+               "kv_attend.hip", "logprobs.hip"]
 CXX_SOURCES = ["abi.cpp", "lds_allow.cpp", "plan.cpp", "host/vq_format.cpp", "host/synth.cpp", "host/artifacts.cpp", "host/profile.cpp",
                "host/model_load.cpp"]
 

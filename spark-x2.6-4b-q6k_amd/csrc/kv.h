@@ -44,8 +44,23 @@ __device__ __forceinline__ KvSeq kv_seq(const sparkmv_kv_batch & b, int i, int n
     return s;
 }
 
-/* the host's checks of a cache and a batch: 0, or -1 with the message set */
+__device__ __forceinline__ float kv_load(const float * p) { return *p; }
+__device__ __forceinline__ float kv_load(const uint16_t * p) { return __uint_as_float((uint32_t) *p << 16); }
+__device__ __forceinline__ uint16_t kv_bf16(float f) {
+    uint32_t u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t) ((u >> 16) | 0x40u);
+    return (uint16_t) ((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ void kv_store(float * p, float v) { *p = v; }
+__device__ __forceinline__ void kv_store(uint16_t * p, float v) { *p = kv_bf16(v); }
+
+/* the host's checks: 0, or -1 with the message set. kv_check_rows: nrows rows of
+ * n values at stride ld, each starting 16-byte aligned */
+bool kv_aligned(const void * p, size_t n);
+int kv_check_dtype(const char * what, int dtype);
+int kv_check_rows(const char * what, const void * p, int ld, long n, int dtype, int nrows);
 int kv_check_cache(const sparkmv_kv_cache * c);
 int kv_check_batch(const sparkmv_kv_batch * b);
+int kv_check_launch(const char * what);
 
 }  // namespace sparkmv

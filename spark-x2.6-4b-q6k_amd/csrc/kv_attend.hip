@@ -1,0 +1,881 @@
+/* kv_attend.hip — attention over the paged 8-bit cache (include/sparkmv.h):
+ *   out = sum_p softmax_p(scale * q . k_p) v_p (* sigmoid(gate))
+ * over the positions p that a token sees.
+ *
+ * Both products run on the 8-bit integer matrix instructions, 16 x 16 x 64,
+ * with the codes as they lie in memory: nothing is converted. What meets them
+ * is an f32 query element or weight as an integer, written in D signed digits
+ * of base 256 (d0 2^8(D-1) + .. + d(D-1)); a digit's sums are exact in i32
+ * (256 * 127 * 128 < 2^23), and D digits' sums make the product.
+ *
+ *   A query element is an integer at a power of two that the head's largest
+ *   element sets: 31 bits with four digits, more than f32 holds; 15 with two.
+ *
+ *   A weight e^(s - m) takes as m the largest score of its own page, so its
+ *   integer (31 or 15 bits) is fine against the page's largest weight whatever
+ *   the rest of the sequence holds. The page's sum enters the f32 output times
+ *   value scale * e^(m - M), where M, a running reference, moves only when a
+ *   page passes it by 2^kKvLag.
+ *
+ * Four digits serve f32 outputs; two (2^-15, under bf16's half step of 2^-9
+ * even where 64 weights add up) serve bf16 ones, except where four cost
+ * nothing. Scores, weights' sums and outputs are f32. */
+#include "kv.h"
+
+#include <math.h>
+
+namespace sparkmv {
+
+namespace {
+
+constexpr float kKvLag = 16.0f;
+constexpr float kKvLog2e = 1.44269504088896340736f;
+
+typedef int kv_i4 __attribute__((ext_vector_type(4)));
+typedef float kv_f4 __attribute__((ext_vector_type(4)));
+
+/* the pages that tokens t0 .. t1 - 1 of a sequence see: the first and how many */
+__device__ __forceinline__ int kv_span(const KvSeq & s, int t0, int t1, int window, int & first) {
+    const int p = s.pos + t0;
+    first = (window > 0 && p + 1 > window ? p + 1 - window : 0) / kKvPage;
+    return (s.pos + t1 - 1) / kKvPage - first + 1;
+}
+
+template <int CTRL>
+__device__ __forceinline__ float kv_quad(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+/* the sum over the four lanes of a quad, the same bits in each */
+__device__ __forceinline__ float kv_quad_sum(float v) {
+    v += kv_quad<0xb1>(v);          /* lanes 1 0 3 2 */
+    return v + kv_quad<0x4e>(v);    /* lanes 2 3 0 1 */
+}
+
+/* 16 query elements as f32 */
+__device__ __forceinline__ void kv_load16(const sparkmv_kv_query & q, size_t at, float * x) {
+    if (q.q_dtype == SPARKMV_X_F32) {
+        const float * p = (const float *) q.q + at;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const kv_f4 v = *(const kv_f4 *) (p + 4 * k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[4 * k + i] = v[i];
+        }
+    } else {
+        const uint16_t * p = (const uint16_t *) q.q + at;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const kv_i4 v = *(const kv_i4 *) (p + 8 * k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[8 * k + 2 * i] = __uint_as_float((uint32_t) v[i] << 16);
+                x[8 * k + 2 * i + 1] = __uint_as_float((uint32_t) v[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+
+/* the exponent that the largest element sets, over the lanes of a column (which
+ * hold its elements between them); bad: one is not finite */
+template <int NC>
+__device__ __forceinline__ int kv_q_exponent(const float (&x)[NC][16], bool & bad) {
+    uint32_t big = 0;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) big = max(big, __float_as_uint(x[c][e]) & 0x7fffffffu);
+    big = max(big, (uint32_t) __shfl_xor((int) big, 16, 64));
+    big = max(big, (uint32_t) __shfl_xor((int) big, 32, 64));
+    bad = big >= 0x7f800000u;
+    int ex = 0;
+    (void) frexpf(__uint_as_float(bad ? 0u : big), &ex);
+    return ex;
+}
+
+/* out[row][head][d] = o / l, gated; no weight at all gives 0 */
+__device__ __forceinline__ void kv_write(const sparkmv_kv_query & q, int row, int head, int hd, int d, float o, float l) {
+    float f = l == 0.0f ? 0.0f : 1.0f / l;
+    if (q.gate) f *= 1.0f / (1.0f + expf(-q.gate[(size_t) row * q.ldg + head]));
+    const float v = l == 0.0f ? 0.0f : o * f;
+    const size_t at = (size_t) row * q.ldo + (size_t) head * hd + d;
+    if (q.out_dtype == SPARKMV_X_F32) ((float *) q.out)[at] = v;
+    else ((uint16_t *) q.out)[at] = kv_bf16(v);
+}
+
+/* ------------------------------------------------------------- few columns
+ *
+ * Up to four columns (token, query head) of a kv head: a decode step of up to
+ * four query heads per kv head. Bound by reading the codes once. The sixteen
+ * columns of a tile are the four columns times four digits, so f32's whole
+ * precision costs no further instruction; a column's value is the sum of its
+ * digits' sums, two cross-lane additions in a quad.
+ *
+ * Workgroups take equal shares of all (sequence, kv head, page) in that order,
+ * so lengths may differ by any amount; a kv head of a sequence counts kKvItem
+ * pages more than it has, for what beginning it costs. A share's pages of one
+ * kv head go to the four waves in turn, whose results meet in LDS; a kv head's
+ * pages that lie in one share are written out at once, others as a partial
+ * result that a second launch joins. */
+constexpr int kKvItem = 8;
+constexpr int kKvFlatMost = 1024;   /* workgroups, at most */
+
+struct KvFlat {
+    sparkmv_kv_cache c;
+    sparkmv_kv_batch b;
+    sparkmv_kv_query q;
+    int least;       /* pages of a share, at least */
+    int * pre;       /* [nseq + 2]: what one kv head of the sequences before counts; the share */
+    float * po;      /* [workgroups][2][4][HD] */
+    float * pml;     /* [workgroups][2][4][2] */
+};
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void kv_flat_kernel(const KvFlat A) {
+    constexpr int NC = HD / 64, ND = HD / 16;
+    extern __shared__ int lpre[];                     /* [nseq + 1] */
+    __shared__ int lsum[4];
+    __shared__ __attribute__((aligned(16))) float lo[4][4][HD];
+    __shared__ float lm[4][4], ll[4][4];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c16 = lane & 15, col = c16 >> 2, dg = c16 & 3;
+    const int kvh = A.c.kv_heads, G = A.q.heads / kvh, nseq = A.b.nseq;
+    {
+        const int per = (nseq + 255) / 256, i0 = min(nseq, tid * per), i1 = min(nseq, i0 + per);
+        int sum = 0;
+        for (int i = i0; i < i1; i++) {
+            int first;
+            const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
+            lpre[i] = sum;
+            if (s.count > 0) sum += kv_span(s, 0, s.count, A.q.window, first) + kKvItem;
+        }
+        int scan = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(scan, o, 64);
+            if (lane >= o) scan += v;
+        }
+        if (lane == 63) lsum[wave] = scan;
+        __syncthreads();
+        int before = scan - sum;
+        for (int w = 0; w < wave; w++) before += lsum[w];
+        for (int i = i0; i < i1; i++) lpre[i] += before;
+        if (tid == 255) lpre[nseq] = before + sum;
+        __syncthreads();
+    }
+    const int total = lpre[nseq] * kvh, share = max((total + (int) gridDim.x - 1) / (int) gridDim.x, A.least);
+    if (blockIdx.x == 0) {
+        for (int i = tid; i <= nseq; i += 256) A.pre[i] = lpre[i];
+        if (tid == 0) A.pre[nseq + 1] = share;
+    }
+    const int ubeg = (int) blockIdx.x * share, uend = min(total, ubeg + share);
+    const float wdig = (float) (1 << (8 * (3 - dg)));
+    const uint32_t sel = (uint32_t) (3 - dg) | (uint32_t) (7 - dg) << 8 | 0x0c0c0000u, flip = dg ? 0x80808080u : 0u;
+    /* byte 3 - dg of four integers with 0x808080 added: the digit, its sign bit
+     * turned in the lower three */
+    auto digits = [&](uint32_t a, uint32_t b, uint32_t c, uint32_t d) -> int {
+        const uint32_t lo2 = __builtin_amdgcn_perm(b, a, sel), hi2 = __builtin_amdgcn_perm(d, c, sel);
+        return (int) ((lo2 | hi2 << 16) ^ flip);
+    };
+    for (int u = ubeg; u < uend;) {
+        /* the sequence: the last one that begins at or before u */
+        int i = 0;
+        for (int b = nseq; b - i > 1;) {
+            const int mid = (i + b) >> 1;
+            if (lpre[mid] * kvh <= u) i = mid;
+            else b = mid;
+        }
+        const int n = lpre[i + 1] - lpre[i] - kKvItem, in = u - lpre[i] * kvh, h = in / (n + kKvItem), off = in - h * (n + kKvItem);
+        if (off >= n) {
+            u += n + kKvItem - off;
+            continue;
+        }
+        const int seg = min(n - off, uend - u);
+        const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
+        int first;
+        kv_span(s, 0, s.count, A.q.window, first);
+        const int ncol = s.count * G, tok = min(col / G, s.count - 1), head = h * G + col % G;
+        const int pos_c = s.pos + tok, beg_c = A.q.window > 0 && pos_c + 1 > A.q.window ? pos_c + 1 - A.q.window : 0;
+        /* positions that every column sees */
+        const int all_lo = A.q.window > 0 && s.pos + s.count > A.q.window ? s.pos + s.count - A.q.window : 0, all_hi = s.pos;
+        /* the columns' digits */
+        kv_i4 qd[NC];
+        float cs;
+        bool qbad;
+        {
+            float x[NC][16];
+            const size_t at = (size_t) (s.row + tok) * A.q.ldq + (size_t) head * HD + 16 * g;
+#pragma unroll
+            for (int c = 0; c < NC; c++) kv_load16(A.q, at + 64 * c, x[c]);
+            const int ex = kv_q_exponent<NC>(x, qbad);
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        y[e] = (uint32_t) (int) rintf(ldexpf(qbad ? 0.0f : x[c][4 * w + e], 30 - ex)) + 0x808080u;
+                    const int d = digits(y[0], y[1], y[2], y[3]);
+                    qd[c][w] = col < ncol ? d : 0;
+                }
+            cs = ldexpf(A.q.scale * kKvLog2e, ex - 30);
+        }
+        float m = -INFINITY, l = 0.0f;
+        kv_f4 o[ND];
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] = kv_f4{0.f, 0.f, 0.f, 0.f};
+        const int * table = A.c.pages + (size_t) s.slot * A.c.max_pages + first + off;
+        /* 64 pages of this wave at a time: their numbers and scales are held one a lane */
+        for (int base = wave; base < seg; base += 256) {
+            const int mine = min((seg - base + 3) / 4, 64);
+            int id = 0;
+            float ks = 0.0f, vs = 0.0f;
+            bool have = false;
+            if (lane < mine) {
+                id = table[base + 4 * lane];
+                have = id >= 0 && id < A.c.npages;
+                id = have ? id : 0;
+                ks = A.c.k_scale[(size_t) id * kvh + h];
+                vs = A.c.v_scale[(size_t) id * kvh + h];
+            }
+            const uint64_t there = __ballot(have);
+            kv_i4 kr[NC][4], vr[ND];
+            auto fetch_k = [&](int j) {
+                const int8_t * p = A.c.k + ((size_t) __builtin_amdgcn_readlane(id, j) * kvh + h) * (size_t) (kKvPage * HD) + c16 * 64 + 16 * g;
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) kr[c][t] = *(const kv_i4 *) (p + c * 4096 + t * 1024);
+            };
+            auto fetch_v = [&](int j) {
+                const int8_t * p = A.c.v + ((size_t) __builtin_amdgcn_readlane(id, j) * kvh + h) * (size_t) (kKvPage * HD) + (g * HD + c16) * 16;
+#pragma unroll
+                for (int d = 0; d < ND; d++) vr[d] = *(const kv_i4 *) (p + d * 256);
+            };
+            fetch_k(0);
+            fetch_v(0);
+            __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < mine; j++) {
+                const int nx = min(j + 1, mine - 1);
+                float x[4][4];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    kv_i4 acc = kv_i4{0, 0, 0, 0};
+#pragma unroll
+                    for (int c = 0; c < NC; c++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[c][t], qd[c], acc, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[t][e] = (float) acc[e] * wdig;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                fetch_k(nx);
+                __builtin_amdgcn_sched_barrier(0);
+                const float kscale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), j));
+                const float vscale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), j));
+                const float f = cs * kscale;
+                const int p0 = (first + off + base + 4 * j) * kKvPage;
+                const bool ok = there >> j & 1;
+                float mp = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[t][e] = kv_quad_sum(x[t][e]) * f;
+                if (!ok || p0 < all_lo || p0 + kKvPage - 1 > all_hi || kscale != kscale) {
+                    bool any = false;
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int p = p0 + 16 * t + 4 * g + e;
+                            const bool seen = ok && p >= beg_c && p <= pos_c;
+                            any = any || seen;
+                            x[t][e] = seen && kscale == kscale ? x[t][e] : -INFINITY;
+                        }
+                    if (any && kscale != kscale) l = kscale;   /* NaN to the end for a column that sees some of it */
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mp = fmaxf(mp, x[t][e]);
+                mp = fmaxf(mp, __shfl_xor(mp, 16, 64));
+                mp = fmaxf(mp, __shfl_xor(mp, 32, 64));
+                if (__any(mp > m + kKvLag)) {
+                    const float mn = fmaxf(m, mp);
+                    const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                    l *= a;
+#pragma unroll
+                    for (int d = 0; d < ND; d++) o[d] *= a;
+                    m = mn;
+                }
+                const float mref = mp == -INFINITY ? 0.0f : mp;
+                kv_i4 P;
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float p = __builtin_amdgcn_exp2f(x[t][e] - mref);
+                        sum += p;
+                        y[e] = (uint32_t) (int) (p * 1073741824.0f) + 0x808080u;
+                    }
+                    P[t] = digits(y[0], y[1], y[2], y[3]);
+                }
+                const float step = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - m);
+                l += sum * step;
+                const float w = mp == -INFINITY ? 0.0f : step * vscale;
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const kv_i4 acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[d], P, kv_i4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[d][e] += w * (float) acc[e];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                fetch_v(nx);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (qbad) l = __uint_as_float(0x7fc00000u);
+        /* the digits of a column, then the waves */
+        const float down = wdig * 9.313225746154785e-10f;   /* 2^-30 */
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            kv_f4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = kv_quad_sum(o[d][e] * down);
+            if ((d & 3) == dg) *(kv_f4 *) &lo[wave][col][16 * d + 4 * g] = v;
+        }
+        if (g == 0 && dg == 0) {
+            lm[wave][col] = m;
+            ll[wave][col] = l;
+        }
+        __syncthreads();
+        const bool whole = seg == n;
+        const size_t at = 2 * (size_t) blockIdx.x + (off == 0 ? 1 : 0);
+        for (int k = tid; k < ncol * HD; k += 256) {
+            const int cc = k / HD, d = k - cc * HD;
+            float M = lm[0][cc];
+#pragma unroll
+            for (int w = 1; w < 4; w++) M = fmaxf(M, lm[w][cc]);
+            float L = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float a = lm[w][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[w][cc] - M);
+                L += lm[w][cc] == -INFINITY ? ll[w][cc] : a * ll[w][cc];
+                v += a * lo[w][cc][d];
+            }
+            if (whole) {
+                kv_write(A.q, s.row + cc / G, h * G + cc % G, HD, d, v, L);
+            } else {
+                A.po[(at * 4 + cc) * HD + d] = v;
+                if (d == 0) {
+                    A.pml[(at * 4 + cc) * 2] = M;
+                    A.pml[(at * 4 + cc) * 2 + 1] = L;
+                }
+            }
+        }
+        __syncthreads();
+        u += seg;
+    }
+}
+
+/* The join of one column's partials at[0 .. n - 1] by four waves (sub 0..3 of the
+ * column): weights e^(m - M) in LDS, then each wave adds every fourth row with
+ * eight of them in flight, and the four sums add up in order. rows[k] is the
+ * k-th partial's index. Returns the sum of weights; o has this lane's HD / 64
+ * elements, complete in sub 0. */
+template <int HD, class At>
+__device__ __forceinline__ float kv_join(const float * po, const float * pml, int n, At at, float * wts, float * acc, int sub,
+                                         int lane, float (&o)[HD / 64]) {
+    constexpr int E = HD / 64;
+    typedef float fe __attribute__((ext_vector_type(E)));
+    float M = -INFINITY;
+    for (int k = lane; k < n; k += 64) M = fmaxf(M, pml[2 * at(k)]);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor(M, s, 64));
+    float L = 0.0f;
+    for (int k = lane; k < n; k += 64) {
+        const float m = pml[2 * at(k)], l = pml[2 * at(k) + 1], f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+        L += m == -INFINITY ? l : f * l;
+        if (sub == 0) wts[k] = f;
+    }
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) L += __shfl_xor(L, s, 64);
+    __syncthreads();
+    fe sum = (fe) 0.0f;
+    for (int k0 = sub; k0 < n; k0 += 32) {
+        fe v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = *(const fe *) (po + at(min(k0 + 4 * j, n - 1)) * HD + E * lane);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (k0 + 4 * j < n) sum += wts[k0 + 4 * j] * v[j];
+    }
+    if (sub) *(fe *) (acc + (sub - 1) * HD + E * lane) = sum;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 3; j++) sum += *(const fe *) (acc + j * HD + E * lane);
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = sum[e];
+    return L;
+}
+
+/* Joins the partial results of one (sequence, kv head), in the order of its
+ * pages: its first share wrote slot 1, the later ones slot 0. Four waves a
+ * column. */
+template <int HD>
+__global__ __launch_bounds__(1024) void kv_flat_join_kernel(const KvFlat A) {
+    __shared__ float wts[4][kKvFlatMost];
+    __shared__ __attribute__((aligned(16))) float acc[4][3 * HD];
+    const int i = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = wave >> 2, sub = wave & 3;
+    const int kvh = A.c.kv_heads, G = A.q.heads / kvh;
+    const int before = A.pre[i], all = A.pre[i + 1] - before, n = all - kKvItem, share = A.pre[A.b.nseq + 1];
+    if (all == 0) return;
+    const int a = before * kvh + h * all, w0 = a / share, w1 = (a + n - 1) / share;
+    if (w0 == w1) return;
+    const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
+    const int cc = min(col, s.count * G - 1);
+    float o[HD / 64];
+    const float L = kv_join<HD>(A.po, A.pml, w1 - w0 + 1, [&](int k) { return (2 * (size_t) (w0 + k) + (k == 0)) * 4 + cc; },
+                                wts[col], acc[col], sub, lane, o);
+    if (sub || col != cc) return;
+#pragma unroll
+    for (int e = 0; e < HD / 64; e++) kv_write(A.q, s.row + cc / G, h * G + cc % G, HD, HD / 64 * lane + e, o[e], L);
+}
+
+/* -------------------------------------------------------------- many columns
+ *
+ * A workgroup takes 16 * WQ columns (token, query head) of a kv head and a share
+ * of the pages they see. A page's codes go to LDS as they lie (direct loads, the
+ * next page's while this one is worked). WQ waves take 16 columns each; with
+ * WQ < 4 the other waves work on the same columns and take a part of the
+ * elements in the product with the values (and repeat the scores). Each digit is
+ * an instruction of its own here, on the same codes. Work that is split over the
+ * pages is joined by a second launch. */
+struct KvTile {
+    sparkmv_kv_cache c;
+    sparkmv_kv_batch b;
+    sparkmv_kv_query q;
+    int nsplit;
+    float * po;      /* [tiles][kv_heads][columns][nsplit][HD] */
+    float * pml;     /* [tiles][kv_heads][columns][nsplit][2] */
+};
+
+constexpr int kKvIds = 256;   /* page numbers held at a time */
+
+/* tile number `tile` of the batch, tiles of `cols` columns: its sequence and its
+ * place there; false past the last one. Every thread of the workgroup calls it. */
+__device__ __forceinline__ bool kv_find_tile(const sparkmv_kv_batch & b, const sparkmv_kv_cache & c, int G, int cols, int tile,
+                                             int * lds, KvSeq & s, int & place) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
+    if (tid == 0) lds[0] = -1;
+    int before = 0;
+    for (int i0 = 0; i0 < b.nseq; i0 += blockDim.x) {
+        KvSeq mine = {0, 0, 0, 0};
+        if (i0 + tid < b.nseq) mine = kv_seq(b, i0 + tid, c.nslots, c.max_pages);
+        const int n = (int) (((long) mine.count * G + cols - 1) / cols);
+        int scan = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(scan, o, 64);
+            if (lane >= o) scan += v;
+        }
+        __syncthreads();
+        if (lane == 63) lds[2 + wave] = scan;
+        __syncthreads();
+        int at = before + scan - n;
+        for (int w = 0; w < nw; w++) {
+            if (w < wave) at += lds[2 + w];
+            before += lds[2 + w];
+        }
+        if (tile >= at && tile < at + n) {
+            lds[0] = i0 + tid;
+            lds[1] = tile - at;
+        }
+        if (tile < before) break;
+    }
+    __syncthreads();
+    if (lds[0] < 0) return false;
+    s = kv_seq(b, lds[0], c.nslots, c.max_pages);
+    place = lds[1];
+    return true;
+}
+
+template <int HD, int D, int WQ>
+__global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
+    constexpr int NC = HD / 64, WD = 4 / WQ, ND = HD / 16 / WD, HALF = kKvPage * HD;
+    constexpr float PMAX = D == 2 ? 32512.0f : 1073741824.0f;   /* a weight of 1: 127 * 256, or 2^30 */
+    constexpr uint32_t BIAS = D == 2 ? 0x80u : 0x808080u;
+    typedef __attribute__((address_space(3))) void lds_void;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lbuf[];   /* [2][keys, values] */
+    __shared__ int lfind[8];
+    __shared__ int lid[kKvIds];
+    __shared__ float lks[kKvIds], lvs[kKvIds];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c16 = lane & 15;
+    const int wq = wave % WQ, wd = wave / WQ, kvh = A.c.kv_heads, G = A.q.heads / kvh, h = blockIdx.y;
+    KvSeq s;
+    int place;
+    if (!kv_find_tile(A.b, A.c, G, 16 * WQ, blockIdx.x, lfind, s, place)) return;
+    const int ncol = s.count * G, col0 = place * 16 * WQ, t0 = col0 / G, t1 = min(col0 + 16 * WQ - 1, ncol - 1) / G + 1;
+    int first;
+    const int npages = kv_span(s, t0, t1, A.q.window, first), per = (npages + A.nsplit - 1) / A.nsplit;
+    const int jbeg = (int) blockIdx.z * per, jend = min(npages, jbeg + per);
+    if (jbeg >= jend) return;
+    first += jbeg;
+    const int n = jend - jbeg;
+    const int * table = A.c.pages + (size_t) s.slot * A.c.max_pages + first;
+    auto ids = [&](int j0) {   /* pages j0 .. of the share; a barrier on both sides */
+        __syncthreads();
+        if (j0 + tid < n) {
+            int id = table[j0 + tid];
+            const bool have = id >= 0 && id < A.c.npages;
+            lid[tid] = have ? id : -1;
+            lks[tid] = have ? A.c.k_scale[(size_t) id * kvh + h] : 0.0f;
+            lvs[tid] = have ? A.c.v_scale[(size_t) id * kvh + h] : 0.0f;
+        }
+        __syncthreads();
+    };
+    auto fetch = [&](int j, int b) {
+        const size_t at = ((size_t) max(__builtin_amdgcn_readfirstlane(lid[j & (kKvIds - 1)]), 0) * kvh + h) * (size_t) HALF;
+        const int8_t * kc = A.c.k + at, * vc = A.c.v + at;
+        uint8_t * to = lbuf + (size_t) b * 2 * HALF;
+#pragma unroll
+        for (int k = 0; k < HALF / 4096; k++) {
+            const int o = (4 * k + wave) * 1024;
+            __builtin_amdgcn_global_load_lds((const void *) (kc + o + 16 * lane), (lds_void *) (to + o), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const void *) (vc + o + 16 * lane), (lds_void *) (to + HALF + o), 16, 0, 0);
+        }
+    };
+    ids(0);
+    fetch(0, 0);
+    /* this wave's columns */
+    const int wfirst = col0 + 16 * wq, cc = min(wfirst + c16, ncol - 1), tok = cc / G, head = h * G + cc - tok * G;
+    const bool live = wfirst < ncol;   /* uniform in the wave */
+    const int pos_c = s.pos + tok, beg_c = A.q.window > 0 && pos_c + 1 > A.q.window ? pos_c + 1 - A.q.window : 0;
+    const int tlo = min(wfirst, ncol - 1) / G, thi = min(wfirst + 15, ncol - 1) / G;
+    const int wpos_lo = s.pos + tlo, wpos_hi = s.pos + thi;   /* the wave's first and last token */
+    const int wbeg_lo = A.q.window > 0 && wpos_lo + 1 > A.q.window ? wpos_lo + 1 - A.q.window : 0;
+    const int wbeg_hi = A.q.window > 0 && wpos_hi + 1 > A.q.window ? wpos_hi + 1 - A.q.window : 0;
+    kv_i4 qd[D][NC];
+    float cs;
+    bool qbad;
+    {
+        float x[NC][16];
+        const size_t at = (size_t) (s.row + tok) * A.q.ldq + (size_t) head * HD + 16 * g;
+#pragma unroll
+        for (int c = 0; c < NC; c++) kv_load16(A.q, at + 64 * c, x[c]);
+        const int ex = kv_q_exponent<NC>(x, qbad);
+        constexpr int B = D == 2 ? 14 : 30;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = (uint32_t) (int) rintf(ldexpf(qbad ? 0.0f : x[c][4 * w + e], B - ex)) + BIAS;
+#pragma unroll
+                for (int d = 0; d < D; d++) {
+                    const uint32_t b = D - 1 - d, sel = b | (b + 4) << 8 | 0x0c0c0000u;
+                    const uint32_t lo2 = __builtin_amdgcn_perm(y[1], y[0], sel), hi2 = __builtin_amdgcn_perm(y[3], y[2], sel);
+                    qd[d][c][w] = (int) ((lo2 | hi2 << 16) ^ (d ? 0x80808080u : 0u));
+                }
+            }
+        cs = ldexpf(A.q.scale * kKvLog2e, ex - B);
+    }
+    /* the value of a product's digit sums */
+    auto value = [&](const kv_i4 * a, int e) -> float {
+        if constexpr (D == 2) return (float) (a[0][e] * 256 + a[1][e]);
+        else return fmaf((float) (a[0][e] * 256 + a[1][e]), 65536.0f, (float) (a[2][e] * 256 + a[3][e]));
+    };
+    float m = -INFINITY, l = 0.0f;
+    kv_f4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = kv_f4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < n; j++) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   /* this wave's part of page j */
+        __syncthreads();                                    /* everyone's, and everyone is done with the other buffer */
+        const int k = j & (kKvIds - 1);
+        const int id = lid[k];
+        const float kscale = lks[k], vscale = lvs[k];
+        if (j + 1 < n) {
+            if (k == kKvIds - 1) ids(j + 1);
+            fetch(j + 1, (j + 1) & 1);
+        }
+        const int p0 = (first + j) * kKvPage;
+        if (!live || id < 0 || p0 > wpos_hi || p0 + kKvPage - 1 < wbeg_lo) continue;   /* uniform in the wave */
+        const uint8_t * kp = lbuf + (size_t) (j & 1) * 2 * HALF + 16 * g + 64 * c16;
+        const uint8_t * vp = lbuf + (size_t) (j & 1) * 2 * HALF + HALF + (g * HD + 16 * ND * wd + c16) * 16;
+        float x[4][4];
+        const float f = cs * kscale;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            kv_i4 acc[D];
+#pragma unroll
+            for (int d = 0; d < D; d++) acc[d] = kv_i4{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const kv_i4 kf = *(const kv_i4 *) (kp + c * 4096 + t * 1024);
+#pragma unroll
+                for (int d = 0; d < D; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qd[d][c], acc[d], 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[t][e] = value(acc, e) * f;
+        }
+        if (p0 < wbeg_hi || p0 + kKvPage - 1 > wpos_lo || kscale != kscale) {
+            bool any = false;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int p = p0 + 16 * t + 4 * g + e;
+                    const bool seen = p >= beg_c && p <= pos_c;
+                    any = any || seen;
+                    x[t][e] = seen && kscale == kscale ? x[t][e] : -INFINITY;
+                }
+            if (any && kscale != kscale) l = kscale;   /* NaN to the end for a column that sees some of it */
+        }
+        float mp = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) mp = fmaxf(mp, x[t][e]);
+        mp = fmaxf(mp, __shfl_xor(mp, 16, 64));
+        mp = fmaxf(mp, __shfl_xor(mp, 32, 64));
+        if (__any(mp > m + kKvLag)) {
+            const float mn = fmaxf(m, mp);
+            const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= a;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= a;
+            m = mn;
+        }
+        const float mref = mp == -INFINITY ? 0.0f : mp;
+        kv_i4 P[D];
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float p = __builtin_amdgcn_exp2f(x[t][e] - mref);
+                sum += p;
+                y[e] = (uint32_t) (int) (D == 2 ? p * PMAX + 0.5f : p * PMAX) + BIAS;
+            }
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                const uint32_t b = D - 1 - d, sel = b | (b + 4) << 8 | 0x0c0c0000u;
+                const uint32_t lo2 = __builtin_amdgcn_perm(y[1], y[0], sel), hi2 = __builtin_amdgcn_perm(y[3], y[2], sel);
+                P[d][t] = (int) ((lo2 | hi2 << 16) ^ (d ? 0x80808080u : 0u));
+            }
+        }
+        const float step = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - m);
+        l += sum * step;
+        const float w = mp == -INFINITY ? 0.0f : step * vscale * (1.0f / PMAX);
+        if (vscale == vscale) {
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const kv_i4 vf = *(const kv_i4 *) (vp + d * 256);
+                kv_i4 acc[D];
+#pragma unroll
+                for (int k2 = 0; k2 < D; k2++) acc[k2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf, P[k2], kv_i4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[d][e] += w * value(acc, e);
+            }
+        } else if (mp != -INFINITY) {
+            l = vscale;
+        }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (qbad) l = __uint_as_float(0x7fc00000u);
+    if (wfirst + c16 >= ncol) return;
+    if (A.nsplit == 1) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) kv_write(A.q, s.row + tok, head, HD, 16 * (ND * wd + d) + 4 * g + e, o[d][e], l);
+        return;
+    }
+    const size_t at = (((size_t) blockIdx.x * kvh + h) * (16 * WQ) + 16 * wq + c16) * A.nsplit + blockIdx.z;
+#pragma unroll
+    for (int d = 0; d < ND; d++) *(kv_f4 *) (A.po + at * HD + 16 * (ND * wd + d) + 4 * g) = o[d];
+    if (wd == 0 && g == 0) {
+        A.pml[2 * at] = m;
+        A.pml[2 * at + 1] = l;
+    }
+}
+
+/* Joins the splits of a tile: four waves a column, four columns at a time. */
+constexpr int kKvSplits = 64;
+template <int HD>
+__global__ __launch_bounds__(1024) void kv_tile_join_kernel(const KvTile A, int cols) {
+    __shared__ float wts[4][kKvSplits];
+    __shared__ __attribute__((aligned(16))) float acc[4][3 * HD];
+    __shared__ int lfind[20];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = wave >> 2, sub = wave & 3;
+    const int kvh = A.c.kv_heads, G = A.q.heads / kvh, h = blockIdx.y;
+    KvSeq s;
+    int place;
+    if (!kv_find_tile(A.b, A.c, G, cols, blockIdx.x, lfind, s, place)) return;
+    const int ncol = s.count * G, col0 = place * cols, t0 = col0 / G, t1 = min(col0 + cols - 1, ncol - 1) / G + 1;
+    int first;
+    const int npages = kv_span(s, t0, t1, A.q.window, first), per = (npages + A.nsplit - 1) / A.nsplit, n = (npages + per - 1) / per;
+    const int c = 4 * (int) blockIdx.z + col;
+    if (col0 + 4 * (int) blockIdx.z >= ncol) return;
+    const int cc = min(col0 + c, ncol - 1);
+    const size_t row = (((size_t) blockIdx.x * kvh + h) * cols + (cc - col0)) * A.nsplit;
+    float o[HD / 64];
+    const float L = kv_join<HD>(A.po, A.pml, n, [&](int k) { return row + k; }, wts[col], acc[col], sub, lane, o);
+    if (sub || cc != col0 + c) return;
+    const int tok = cc / G;
+#pragma unroll
+    for (int e = 0; e < HD / 64; e++) kv_write(A.q, s.row + tok, h * G + cc - tok * G, HD, HD / 64 * lane + e, o[e], L);
+}
+
+/* -------------------------------------------------------------------- host */
+
+struct KvPlan {
+    int flat;                 /* the few-column kernel */
+    int groups, least;        /* its workgroups and least share */
+    int wq, tiles, nsplit;    /* the many-column kernel's */
+    size_t pre, po, pml, bytes;
+};
+
+KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads) {
+    KvPlan p = {};
+    const int G = heads / c->kv_heads, max_q = b->qstart ? (b->max_q < b->ntok ? b->max_q : b->ntok) : 1;
+    const long cols = (long) (max_q > 0 ? max_q : 1) * G, hd = c->head_dim;
+    long len = b->max_len > 0 ? b->max_len : (long) c->max_pages * kKvPage;
+    const long pages = (len + kKvPage - 1) / kKvPage;
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t o = off; off += (bytes + 255) & ~(size_t) 255; return o; };
+    if (cols <= 4) {
+        p.flat = 1;
+        const long most = 2 * cu_count() < kKvFlatMost ? 2 * cu_count() : kKvFlatMost, all = pages * b->nseq * c->kv_heads;
+        p.groups = (int) (all < 1 ? 1 : (all < most ? all : most));
+        p.least = 1;
+        p.pre = take(((size_t) b->nseq + 2) * 4);
+        p.po = take((size_t) p.groups * 2 * 4 * hd * 4);
+        p.pml = take((size_t) p.groups * 2 * 4 * 2 * 4);
+    } else {
+        p.wq = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
+        p.tiles = (int) ((long) b->ntok * G / (16 * p.wq) + b->nseq);
+        const long busy = ((long) b->ntok * G + 16 * p.wq - 1) / (16 * p.wq) * c->kv_heads;
+        /* two workgroups a CU, eight pages a split */
+        long n = (2 * cu_count() + busy - 1) / busy;
+        if (n > pages / 8) n = pages / 8;
+        p.nsplit = (int) (n < 1 ? 1 : (n > kKvSplits ? kKvSplits : n));
+        if (p.nsplit > 1) {
+            const size_t rows = (size_t) p.tiles * c->kv_heads * 16 * p.wq * p.nsplit;
+            p.po = take(rows * hd * 4);
+            p.pml = take(rows * 2 * 4);
+        }
+    }
+    p.bytes = off;
+    return p;
+}
+
+}  // namespace
+
+}  // namespace sparkmv
+
+using namespace sparkmv;
+
+extern "C" {
+
+size_t sparkmv_kv_attend_work(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, int heads) {
+    if (kv_check_cache(cache) || kv_check_batch(batch) || heads < 1 || heads % cache->kv_heads) return 0;
+    if (batch->nseq == 0 || batch->ntok == 0) return 0;
+    return kv_plan(cache, batch, heads).bytes;
+}
+
+int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_query * query,
+                      void * stream) {
+    if (kv_check_cache(cache) || kv_check_batch(batch)) return -1;
+    if (!query) { set_error("kv query is null"); return -1; }
+    const sparkmv_kv_query & q = *query;
+    if (kv_check_dtype("queries", q.q_dtype) || kv_check_dtype("attention output", q.out_dtype)) return -1;
+    if (q.heads < 1 || q.heads % cache->kv_heads || q.heads / cache->kv_heads > kKvMaxGroup) {
+        set_error("%d query heads are not 1..%d times %d kv heads", q.heads, kKvMaxGroup, cache->kv_heads);
+        return -1;
+    }
+    if (q.window < 0) { set_error("window %d is negative", q.window); return -1; }
+    if (!(fabsf(q.scale) < INFINITY)) { set_error("the scale of the scores is not finite"); return -1; }
+    if (batch->nseq == 0 || batch->ntok == 0) return 0;
+    const long qd = (long) q.heads * cache->head_dim;
+    if (kv_check_rows("queries", q.q, q.ldq, qd, q.q_dtype, batch->ntok) ||
+        kv_check_rows("attention output", q.out, q.ldo, qd, q.out_dtype, batch->ntok))
+        return -1;
+    if (q.gate && batch->ntok > 1 && q.ldg < q.heads) {
+        set_error("gate: a row stride of %d holds no %d heads", q.ldg, q.heads);
+        return -1;
+    }
+    if ((long) batch->nseq * (cache->max_pages + kKvItem) * cache->kv_heads > 0x7fffffffl) {
+        set_error("%d sequences of up to %d pages and %d kv heads are too many for one call", batch->nseq, cache->max_pages,
+                  cache->kv_heads);
+        return -1;
+    }
+    const KvPlan p = kv_plan(cache, batch, q.heads);
+    if (p.bytes && (!q.work || !kv_aligned(q.work, 256) || q.work_bytes < p.bytes)) {
+        set_error("attention needs %zu bytes of 256-byte aligned workspace, not %zu", p.bytes, q.work ? q.work_bytes : 0);
+        return -1;
+    }
+    hipStream_t s = (hipStream_t) stream;
+    uint8_t * mem = (uint8_t *) q.work;
+    const int max_q = batch->qstart ? batch->max_q : 1, hd = cache->head_dim;
+    if (p.flat) {
+        KvFlat f;
+        f.c = *cache; f.b = *batch; f.q = q;
+        f.b.max_q = max_q;
+        f.least = p.least;
+        f.pre = (int *) (mem + p.pre); f.po = (float *) (mem + p.po); f.pml = (float *) (mem + p.pml);
+        const dim3 grid((unsigned) p.groups), join((unsigned) batch->nseq, (unsigned) cache->kv_heads);
+        const uint32_t lds = ((uint32_t) batch->nseq + 1) * 4;
+#define KV_FLAT(H)                                                                                                   \
+    do {                                                                                                             \
+        hipLaunchKernelGGL(kv_flat_kernel<H>, grid, dim3(256), lds, s, f);                                           \
+        hipLaunchKernelGGL(kv_flat_join_kernel<H>, join, dim3(1024), 0, s, f);                                       \
+    } while (0)
+        if (hd == 64) KV_FLAT(64);
+        else if (hd == 128) KV_FLAT(128);
+        else KV_FLAT(256);
+#undef KV_FLAT
+        return kv_check_launch("kv attention launch");
+    }
+    KvTile t;
+    t.c = *cache; t.b = *batch; t.q = q;
+    t.b.max_q = max_q;
+    t.nsplit = p.nsplit;
+    t.po = (float *) (mem + p.po); t.pml = (float *) (mem + p.pml);
+    const dim3 grid((unsigned) p.tiles, (unsigned) cache->kv_heads, (unsigned) p.nsplit);
+    const uint32_t lds = 4 * kKvPage * (uint32_t) hd;
+#define KV_TILE(H, D, W)                                                                                             \
+    do {                                                                                                             \
+        static LdsAllowed allowed;                                                                                   \
+        if (lds_allow(allowed, (const void *) kv_tile_kernel<H, D, W>, lds + 4096, "LDS opt-in for the kv attention")) \
+            return -1;                                                                                               \
+        hipLaunchKernelGGL((kv_tile_kernel<H, D, W>), grid, dim3(256), lds, s, t);                                   \
+    } while (0)
+#define KV_TILE_D(H, W)                                                                                              \
+    do {                                                                                                             \
+        if (q.out_dtype == SPARKMV_X_F32) KV_TILE(H, 4, W);                                                          \
+        else KV_TILE(H, 2, W);                                                                                       \
+    } while (0)
+#define KV_TILE_W(H)                                                                                                 \
+    do {                                                                                                             \
+        if (p.wq == 1) KV_TILE_D(H, 1);                                                                              \
+        else if (p.wq == 2) KV_TILE_D(H, 2);                                                                         \
+        else KV_TILE_D(H, 4);                                                                                        \
+        if (p.nsplit > 1)                                                                                            \
+            hipLaunchKernelGGL(kv_tile_join_kernel<H>, dim3(grid.x, grid.y, 4 * p.wq), dim3(1024), 0, s, t, 16 * p.wq); \
+    } while (0)
+    if (hd == 64) KV_TILE_W(64);
+    else if (hd == 128) KV_TILE_W(128);
+    else KV_TILE_W(256);
+#undef KV_TILE_W
+#undef KV_TILE_D
+#undef KV_TILE
+    return kv_check_launch("kv attention launch");
+}
+
+}  // extern "C"

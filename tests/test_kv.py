@@ -90,6 +90,22 @@ def test_bad_queries(sm, bad, text):
     refused(sm, sm.lib().sparkmv_kv_attend(ref(cache(sm)), ref(batch(sm)), ref(query(sm, **bad)), None), text)
 
 
+def test_workspace(sm):
+    L = sm.lib()
+    c = cache(sm)
+    for b, heads in ((batch(sm), 4), (batch(sm, nseq=1, ntok=300, qstart=P, max_q=300, max_len=128), 4), (batch(sm), 32)):
+        need = L.sparkmv_kv_attend_work(ref(c), ref(b), heads)
+        rows = dict(heads=heads, ldq=64 * heads, ldo=64 * heads)
+        if need:
+            for w in (dict(work=None, work_bytes=need), dict(work=P, work_bytes=need - 1), dict(work=P + 128, work_bytes=need)):
+                refused(sm, L.sparkmv_kv_attend(ref(c), ref(b), ref(query(sm, **rows, **w)), None), "workspace")
+    assert L.sparkmv_kv_attend_work(ref(c), ref(batch(sm)), 4) > 0
+    # the count of pages has to fit a 32-bit number
+    big = cache(sm, kv_heads=64, max_pages=1 << 20)
+    refused(sm, L.sparkmv_kv_attend(ref(big), ref(batch(sm, nseq=64, ntok=64)), ref(query(sm, heads=64, ldq=4096, ldo=4096)), None),
+            "too many for one call")
+
+
 def test_null_structures_and_empty_calls(sm):
     L = sm.lib()
     c, b, n, q = cache(sm), batch(sm), new(sm), query(sm)
