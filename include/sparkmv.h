@@ -630,7 +630,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
  * masked logit (p = 0, log probability -inf); a row of nothing else has
  * entropy 0. A NaN or +inf makes the row's values NaN and NaN is never chosen;
  * where fewer than k can be, the rest are id -1, -inf. A token outside the row
- * gives NaN. No counterpart in the reference. work: sparkmv_logprobs_work
+ * gives NaN. n is at most 524288, rows 65535. No counterpart in the reference. work: sparkmv_logprobs_work
  * bytes, 256-byte aligned, not shared by calls that overlap. */
 size_t sparkmv_logprobs_work(int rows, int n, int k);
 int sparkmv_logprobs(const void * logits, int x_dtype, int rows, int n, size_t ld, const int * tokens, int k,

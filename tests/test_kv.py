@@ -133,7 +133,9 @@ def test_bad_rope_tables(sm, args, text):
 
 
 @pytest.mark.parametrize("bad,text", [
-    ({"x_dtype": 9}, "unknown type 9"), ({"rows": -1}, "-1 rows"), ({"n": 0}, "0 logits"), ({"k": 33}, "33 alternatives"),
+    ({"x_dtype": 9}, "unknown type 9"), ({"rows": -1}, "-1 rows"), ({"n": 0}, "0 logits"), ({"n": 524289, "ld": 524289}, "above 524288"),
+    ({"rows": 65536}, "above 65535"), ({"work": None}, "workspace"), ({"work_bytes": 63}, "workspace"), ({"work": P + 16}, "workspace"),
+     ({"k": 33}, "33 alternatives"),
     ({"k": -1}, "-1 alternatives"), ({"logits": None}, "logits are null"), ({"ld": 9}, "holds no 10"),
     ({"tokens": None}, "do not agree"), ({"logprob": None}, "do not agree"), ({"top_id": None}, "without room"),
     ({"top_logprob": None}, "without room")])
