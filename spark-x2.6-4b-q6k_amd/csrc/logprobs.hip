@@ -176,23 +176,32 @@ __device__ __forceinline__ float lp_value(uint64_t key) {
 }
 __device__ __forceinline__ int lp_place(uint64_t key) { return (int) ~(uint32_t) key; }
 
-/* how many of the n keys are larger; the list is padded with a zero to an even count */
+/* how many of the n keys are larger; zeros follow the list up to a multiple of
+ * kLpPad, whose reads are in flight together (one at a time they cost 5 us for
+ * 256 keys, so 1.4) */
+constexpr int kLpPad = 16;
 __device__ __forceinline__ int lp_rank(const uint64_t * keys, int n, uint64_t mine) {
     typedef uint64_t u2 __attribute__((ext_vector_type(2)));
     int c = 0;
-    for (int i = 0; i < n; i += 2) {
-        const u2 v = *(const u2 *) (keys + i);
-        c += (v[0] > mine) + (v[1] > mine);
+    for (int i = 0; i < n; i += kLpPad) {
+        u2 v[kLpPad / 2];
+#pragma unroll
+        for (int j = 0; j < kLpPad / 2; j++) v[j] = *(const u2 *) (keys + i + 2 * j);
+#pragma unroll
+        for (int j = 0; j < kLpPad / 2; j++) c += (v[j][0] > mine) + (v[j][1] > mine);
     }
     return c;
 }
 
 constexpr int kLpList = kLpMaxK * (kLpMaxN / kLpSeg / 256);   /* segments of k threads */
 
+/* segments a thread keeps in registers: rows of up to 163840 logits are not read again */
+constexpr int kLpHeld = 20;
+
 template <typename X>
 __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     __shared__ __attribute__((aligned(16))) uint64_t lkey[256];
-    __shared__ __attribute__((aligned(16))) uint64_t lseg[kLpList + 2];
+    __shared__ __attribute__((aligned(16))) uint64_t lseg[kLpList + kLpPad];
     __shared__ uint64_t lpick[kLpMaxK], lleast;
     __shared__ float red[3][4];
     __shared__ int count[2];
@@ -212,15 +221,17 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     const float * seg = A.seg + (size_t) r * A.nseg;
     const int nseg = k ? A.nseg : 0;
     uint64_t best = 0;
-    for (int i0 = tid; i0 < nseg; i0 += 8 * 256) {
-        float v[8];
+    float held[kLpHeld];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = i0 + 256 * j < nseg ? seg[i0 + 256 * j] : NAN;
+    for (int j = 0; j < kLpHeld; j++) held[j] = tid + 256 * j < nseg ? seg[tid + 256 * j] : NAN;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint64_t key = lp_key(v[j], i0 + 256 * j);
-            best = key > best ? key : best;
-        }
+    for (int j = 0; j < kLpHeld; j++) {
+        const uint64_t key = lp_key(held[j], tid + 256 * j);
+        best = key > best ? key : best;
+    }
+    for (int i = tid + 256 * kLpHeld; i < nseg; i += 256) {
+        const uint64_t key = lp_key(seg[i], i);
+        best = key > best ? key : best;
     }
     if (tid == 0) lleast = 1;
     lkey[tid] = best;
@@ -248,7 +259,12 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     __syncthreads();
     if (place < k) {
         const uint64_t least = lleast;
-        for (int i = tid; i < nseg; i += 256) {
+#pragma unroll
+        for (int j = 0; j < kLpHeld; j++) {
+            const uint64_t key = lp_key(held[j], tid + 256 * j);
+            if (key >= least) lseg[atomicAdd(&count[0], 1)] = key;
+        }
+        for (int i = tid + 256 * kLpHeld; i < nseg; i += 256) {
             const uint64_t key = lp_key(seg[i], i);
             if (key >= least) lseg[atomicAdd(&count[0], 1)] = key;
         }
@@ -265,7 +281,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     }
     if (!k) return;
     const int nc = count[0];
-    if (tid < 2) lseg[nc + tid] = 0;
+    if (tid < kLpPad) lseg[nc + tid] = 0;
     if (tid < kLpMaxK) lpick[tid] = 0;
     __syncthreads();
     for (int i = tid; i < nc; i += 256) {
@@ -286,7 +302,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     }
     __syncthreads();
     const int nl = count[1];
-    if (tid < 2) list[nl + tid] = 0;
+    if (tid < kLpPad) list[nl + tid] = 0;
     __syncthreads();
     for (int i = tid; i < nl; i += 256) {
         const uint64_t key = list[i];
