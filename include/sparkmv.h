@@ -593,7 +593,8 @@ int sparkmv_kv_append(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
 
 /* Cached positions as values: k_out and v_out (either may be NULL) are
  * [nseq][n][kv_heads][head_dim] in out_dtype; row j of sequence i is position
- * from[i] + j of slot[i] (NULL: slot i). Positions without a page are zero. */
+ * from[i] + j of slot[i] (NULL: slot i). Positions without a page are zero.
+ * The outputs are 16-byte aligned. */
 int sparkmv_kv_read(const sparkmv_kv_cache * cache, int nseq, const int * slot, const int * from, int n, void * k_out,
                     void * v_out, int out_dtype, void * stream);
 

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void kv_rope_table_kernel(float * tab, int row
 /* -------------------------------------------------------------------- append
  *
  * Workgroups 0 .. nkv - 1 take one (sequence, touched page, kv head, keys or
- * values) each, the others four query heads of one token.
+ * values) each, the others a few query heads of one token.
  *
  * A page's workgroup turns the new rows into f32 in LDS (at most 64 x hd),
  * takes their largest magnitude, settles the scale, and writes the codes in 16
@@ -73,15 +73,39 @@ __device__ __forceinline__ int kv_pair(int j, int half, int & second) {
     return 2 * j;
 }
 
-template <typename X>
-__device__ __forceinline__ void kv_turn(const X * row, int e0, int e1, const float * rope, int j, int half, double & a,
-                                        double & b) {
-    a = (double) kv_load(row + e0);
-    b = (double) kv_load(row + e1);
-    if (j < half && rope) {
-        const double c = (double) rope[j], s = (double) rope[half + j], x = a;
-        a = x * c - b * s;
-        b = b * c + x * s;
+/* n pairs over NT threads, four of a thread's in flight: at(i, row, table) gives
+ * pair i's place in its head, its row and its table row (NULL: not turned), and
+ * put(i, e0, e1, a, b) takes the two results */
+template <typename X, int NT, typename At, typename Put>
+__device__ __forceinline__ void kv_turn_all(int n, At at, int half, Put put) {
+    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * NT) {
+        int e0[4], e1[4];
+        float x[4], y[4], c[4], s[4];
+        bool turn[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int i = min(i0 + u * NT, n - 1);
+            const X * row;
+            const float * tab;
+            const int j = at(i, row, tab);
+            e0[u] = kv_pair(j, half, e1[u]);
+            x[u] = kv_load(row + e0[u]);
+            y[u] = kv_load(row + e1[u]);
+            turn[u] = j < half && tab;
+            c[u] = turn[u] ? tab[j] : 1.0f;
+            s[u] = turn[u] ? tab[half + j] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (i0 + u * NT >= n) continue;
+            double a = (double) x[u], b = (double) y[u];
+            if (turn[u]) {
+                const double p = a, cc = (double) c[u], ss = (double) s[u];
+                a = p * cc - b * ss;
+                b = b * cc + p * ss;
+            }
+            put(i0 + u * NT, e0[u], e1[u], a, b);
+        }
     }
 }
 
@@ -94,18 +118,20 @@ __device__ __forceinline__ float kv_code(float x, float s, float r, bool tiny) {
     return n;
 }
 
-template <typename X>
-__global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend A) {
+template <typename X, int NT>
+__global__ __launch_bounds__(NT) void kv_append_kernel(const KvAppend A) {
+    constexpr int QH = NT / 64;      /* query heads of a workgroup */
     extern __shared__ __attribute__((aligned(16))) float lrow[];   /* [rows][hd] */
-    __shared__ uint32_t lmax[4];
+    __shared__ uint32_t lmax[NT / 64];
     const int tid = threadIdx.x, hd = A.c.head_dim, kvh = A.c.kv_heads, half = A.half;
+    const int sh = 31 - __clz(hd / 2), pairs = 1 << sh;   /* head_dim is a power of two */
     if ((int) blockIdx.x >= A.nkv) {
         /* queries */
-        const int w = (int) blockIdx.x - A.nkv, t = w / A.qparts, h0 = 4 * (w - t * A.qparts);
+        const int w = (int) blockIdx.x - A.nkv, t = w / A.qparts, h0 = QH * (w - t * A.qparts);
         __shared__ int lpos;
         if (tid == 0) lpos = -1;
         __syncthreads();
-        for (int i = tid; i < A.b.nseq; i += 256) {
+        for (int i = tid; i < A.b.nseq; i += NT) {
             const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
             if (t >= s.row && t - s.row < s.count) lpos = s.pos + t - s.row;
         }
@@ -113,18 +139,18 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend A) {
         const int pos = lpos;
         if (pos < 0) return;
         const float * rope = half ? A.n.rope + (size_t) pos * 2 * half : nullptr;
-        const X * src = (const X *) A.n.q + (size_t) t * A.n.ldq;
-        X * dst = (X *) A.n.q_out + (size_t) t * A.n.ldqo;
-        const int pairs = hd / 2, n = min(4, A.n.heads - h0) * pairs;
-        for (int i = tid; i < n; i += 256) {
-            const int h = h0 + i / pairs, j = i % pairs;
-            int e1;
-            const int e0 = kv_pair(j, half, e1);
-            double a, b;
-            kv_turn(src + (size_t) h * hd, e0, e1, rope, j, half, a, b);
-            kv_store_wide(dst + (size_t) h * hd + e0, a);
-            kv_store_wide(dst + (size_t) h * hd + e1, b);
-        }
+        const X * src = (const X *) A.n.q + (size_t) t * A.n.ldq + (size_t) h0 * hd;
+        X * dst = (X *) A.n.q_out + (size_t) t * A.n.ldqo + (size_t) h0 * hd;
+        const int n = min(QH, A.n.heads - h0) << sh;
+        kv_turn_all<X, NT>(n, [&](int i, const X *& row, const float *& tab) {
+            row = src + (size_t) (i >> sh) * hd;
+            tab = rope;
+            return i & (pairs - 1);
+        }, half, [&](int i, int e0, int e1, double a, double b) {
+            X * to = dst + (size_t) (i >> sh) * hd;
+            kv_store_wide(to + e0, a);
+            kv_store_wide(to + e1, b);
+        });
         return;
     }
     int w = blockIdx.x;
@@ -146,24 +172,25 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend A) {
     int8_t * codes = (which ? A.c.v : A.c.k) + ((size_t) page * kvh + h) * (size_t) (kKvPage * hd);
     const float was = held ? *scale : 0.0f;
     uint32_t big = 0;
-    const int pairs = hd / 2;
-    for (int k = tid; k < rows * pairs; k += 256) {
-        const int r = k / pairs, j = k - r * pairs, p = lo + r;
-        int e1;
-        const int e0 = kv_pair(j, half, e1);
-        double a, b;
-        kv_turn(src + (size_t) (s.row + p - s.pos) * ld + (size_t) h * hd, e0, e1,
-                which || !half ? nullptr : A.n.rope + (size_t) p * 2 * half, j, half, a, b);
+    const X * base = src + (size_t) (s.row + lo - s.pos) * ld + (size_t) h * hd;
+    kv_turn_all<X, NT>(rows << sh, [&](int i, const X *& row, const float *& tab) {
+        const int r = i >> sh;
+        row = base + (size_t) r * ld;
+        tab = which || !half ? nullptr : A.n.rope + (size_t) (lo + r) * 2 * half;
+        return i & (pairs - 1);
+    }, half, [&](int i, int e0, int e1, double a, double b) {
         const float x = (float) a, y = (float) b;
-        lrow[r * hd + e0] = x;
-        lrow[r * hd + e1] = y;
+        float * to = lrow + (i >> sh) * hd;
+        to[e0] = x;
+        to[e1] = y;
         big = max(big, max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu));
-    }
+    });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) big = max(big, (uint32_t) __shfl_xor((int) big, o, 64));
     if ((tid & 63) == 0) lmax[tid >> 6] = big;
     __syncthreads();
-    big = max(max(lmax[0], lmax[1]), max(lmax[2], lmax[3]));
+#pragma unroll
+    for (int w2 = 0; w2 < NT / 64; w2++) big = max(big, lmax[w2]);
     const double need = (double) __uint_as_float(big);
     const bool bad = big >= 0x7f800000u || was != was;
     const bool keep = held && need <= 127.0 * (double) was;
@@ -183,8 +210,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend A) {
     if (which == 0) {
         const int per = hd / 16;   /* pieces of a position */
         const int first = again ? 0 : held;
-        for (int k = tid; k < (held + rows - first) * per; k += 256) {
-            const int r = first + k / per, d = 16 * (k % per);
+        for (int k = tid; k < (held + rows - first) * per; k += NT) {
+            const int r = first + (k >> (sh - 3)), d = 16 * (k & (per - 1));
             int8_t * at = codes + kv_key_at(r, d);
             union { int4 v; int8_t c[16]; } u;
             if (r < held) {
@@ -200,8 +227,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend A) {
         }
     } else {
         const int upto = held + rows;
-        for (int k = tid; k < 4 * hd; k += 256) {
-            const int g = k / hd, d = k - g * hd;
+        for (int k = tid; k < 4 * hd; k += NT) {
+            const int g = k >> (sh + 1), d = k & (hd - 1);
             /* positions 16 t + 4 g + i of this piece */
             bool any = false, all = true;
 #pragma unroll
@@ -224,6 +251,20 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend A) {
             *(int4 *) at = u.v;
         }
     }
+}
+
+/* N neighbouring values, N a multiple of 4, aligned to four of them */
+template <int N>
+__device__ __forceinline__ void kv_store4(float * p, const float * x) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) *(float4 *) (p + k) = float4{x[k], x[k + 1], x[k + 2], x[k + 3]};
+}
+template <int N>
+__device__ __forceinline__ void kv_store4(uint16_t * p, const float * x) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4)
+        *(uint2 *) (p + k) = uint2{(uint32_t) kv_bf16(x[k]) | (uint32_t) kv_bf16(x[k + 1]) << 16,
+                                   (uint32_t) kv_bf16(x[k + 2]) | (uint32_t) kv_bf16(x[k + 3]) << 16};
 }
 
 /* ---------------------------------------------------------------------- read
@@ -249,20 +290,31 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const sparkmv_kv_cache c, 
     const int8_t * codes = (which ? c.v : c.k) + head * (size_t) (kKvPage * hd);
     out += ((size_t) i * n * kvh + h) * hd;
     const size_t row = (size_t) kvh * hd;
-    if (!which || !have) {
-        for (int k = tid; k < (int) (hi - lo) * hd; k += 256) {
-            const int r = (int) (lo - p0) + k / hd, d = k % hd;
-            kv_store(out + (size_t) (p0 + r - f) * row + d, have ? (float) codes[kv_key_at(r, d)] * s : 0.0f);
+    if (!which) {
+        const int per = hd / 16, cnt = (int) (hi - lo) * per;
+        for (int k = tid; k < cnt; k += 256) {
+            const int r = (int) (lo - p0) + k / per, d = 16 * (k % per);
+            union { int4 v; int8_t c[16]; } u;
+            u.v = have ? *(const int4 *) (codes + kv_key_at(r, d)) : int4{0, 0, 0, 0};
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = (float) u.c[e] * s;
+            kv_store4<16>(out + (size_t) (p0 + r - f) * row + d, x);
         }
     } else {
-        for (int k = tid; k < 4 * hd; k += 256) {
-            const int g = k / hd, d = k - g * hd;
-            union { int4 v; int8_t c[16]; } u;
-            u.v = *(const int4 *) (codes + (size_t) k * 16);
+        /* four elements of 16 positions a thread */
+        for (int k = tid; k < hd; k += 256) {
+            const int g = k / (hd / 4), d = 4 * (k % (hd / 4));
+            union { int4 v; int8_t c[16]; } u[4];
+#pragma unroll
+            for (int w = 0; w < 4; w++) u[w].v = have ? *(const int4 *) (codes + (size_t) (g * hd + d + w) * 16) : int4{0, 0, 0, 0};
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const long p = p0 + 16 * (e >> 2) + 4 * g + (e & 3);
-                if (p >= lo && p < hi) kv_store(out + (size_t) (p - f) * row + d, (float) u.c[e] * s);
+                float x[4];
+#pragma unroll
+                for (int w = 0; w < 4; w++) x[w] = (float) u[w].c[e] * s;
+                if (p >= lo && p < hi) kv_store4<4>(out + (size_t) (p - f) * row + d, x);
             }
         }
     }
@@ -382,22 +434,35 @@ int sparkmv_kv_append(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     a.half = n.rope_dim / 2;
     a.nb = (a.b.max_q + kKvPage - 2) / kKvPage + 1;
     if (a.nb > cache->max_pages) a.nb = cache->max_pages;
-    a.qparts = (n.heads + 3) / 4;
+    /* 1024 threads from 9 rows a page on: 64 rows x 256 elements are 8192 pairs,
+     * of which 256 threads took 32 each (a chunk of 512 tokens 33 us); one row
+     * gives 256 threads no work for more */
+    const bool wide = a.b.max_q > 8;
+    const int nt = wide ? 1024 : 256;
+    a.qparts = (n.heads + nt / 64 - 1) / (nt / 64);
     const long nkv = (long) batch->nseq * a.nb * cache->kv_heads * 2, wgs = nkv + (long) batch->ntok * a.qparts;
     if (wgs > 0x7fffffffl) { set_error("an append of %ld workgroups", wgs); return -1; }
     a.nkv = (int) nkv;
     const int lrows = a.b.max_q < kKvPage ? a.b.max_q : kKvPage;
     const uint32_t lds = (uint32_t) (lrows * hd * 4);
-    const bool f32 = n.x_dtype == SPARKMV_X_F32;
-    static LdsAllowed allowed[2];
-    /* a full page of 256 elements takes 64 KB beside the kernel's own words */
-    if (lds_allow(allowed[f32], f32 ? (const void *) kv_append_kernel<float> : (const void *) kv_append_kernel<uint16_t>,
-                  lds + 1024, "LDS opt-in for the kv append"))
-        return -1;
-    const dim3 grid((unsigned) wgs), block(256);
+    const dim3 grid((unsigned) wgs), block((unsigned) nt);
     hipStream_t s = (hipStream_t) stream;
-    if (f32) hipLaunchKernelGGL(kv_append_kernel<float>, grid, block, lds, s, a);
-    else hipLaunchKernelGGL(kv_append_kernel<uint16_t>, grid, block, lds, s, a);
+    /* a full page of 256 elements takes 64 KB beside the kernel's own words */
+#define KV_APPEND(X, NT)                                                                                             \
+    do {                                                                                                             \
+        static LdsAllowed allowed;                                                                                   \
+        if (lds_allow(allowed, (const void *) kv_append_kernel<X, NT>, lds + 1024, "LDS opt-in for the kv append"))  \
+            return -1;                                                                                               \
+        hipLaunchKernelGGL((kv_append_kernel<X, NT>), grid, block, lds, s, a);                                       \
+    } while (0)
+    if (n.x_dtype == SPARKMV_X_F32) {
+        if (wide) KV_APPEND(float, 1024);
+        else KV_APPEND(float, 256);
+    } else {
+        if (wide) KV_APPEND(uint16_t, 1024);
+        else KV_APPEND(uint16_t, 256);
+    }
+#undef KV_APPEND
     return kv_check_launch("kv append launch");
 }
 
@@ -408,6 +473,7 @@ int sparkmv_kv_read(const sparkmv_kv_cache * cache, int nseq, const int * slot, 
     if (n < 0) { set_error("%d positions", n); return -1; }
     if (nseq == 0 || n == 0 || (!k_out && !v_out)) return 0;
     if (!from) { set_error("kv read has no positions"); return -1; }
+    if (!kv_aligned(k_out, 16) || !kv_aligned(v_out, 16)) { set_error("kv read: rows do not start 16-byte aligned"); return -1; }
     const long nb = (n + kKvPage - 2) / kKvPage + 1, wgs = (long) nseq * nb;
     if (wgs > 0x7fffffffl) { set_error("a read of %ld pages", wgs); return -1; }
     const dim3 grid((unsigned) wgs, (unsigned) cache->kv_heads, 2), block(256);

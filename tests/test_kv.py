@@ -122,6 +122,7 @@ def test_null_structures_and_empty_calls(sm):
     refused(sm, L.sparkmv_kv_read(ref(c), 3, None, None, 1, P, P, 1, None), "no positions")
     refused(sm, L.sparkmv_kv_read(ref(c), 5000, None, P, 1, P, P, 1, None), "5000 sequences")
     refused(sm, L.sparkmv_kv_read(ref(c), 3, None, P, -1, P, P, 1, None), "-1 positions")
+    refused(sm, L.sparkmv_kv_read(ref(c), 3, None, P, 1, P + 4, P, 1, None), "16-byte aligned")
     refused(sm, L.sparkmv_kv_read(ref(c), 3, None, P, 1, P, P, 7, None), "unknown type 7")
 
 
