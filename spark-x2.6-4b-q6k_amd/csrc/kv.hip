@@ -40,12 +40,14 @@ __global__ __launch_bounds__(256) void kv_rope_table_kernel(float * tab, int row
 /* -------------------------------------------------------------------- append
  *
  * Workgroups 0 .. nkv - 1 take one (sequence, touched page, kv head, keys or
- * values) each, the others a few query heads of one token.
+ * values) each, the others some of the tokens' queries.
  *
- * A page's workgroup turns the new rows into f32 in LDS (at most 64 x hd),
- * takes their largest magnitude, settles the scale, and writes the codes in 16
- * byte pieces of the layout; pieces that also hold older positions are read
- * first. Nothing else writes the page's head during the launch.
+ * A page's workgroup holds its new rows in registers (a thread up to kKvPairs
+ * pairs of elements), takes their largest magnitude, settles the scale, puts the
+ * codes in LDS and writes them in 16 byte pieces of the layout; pieces that also
+ * hold older positions are read first, as soon as the page is known. Nothing
+ * else writes the page's head during the launch. One token is bound by its chain
+ * of reads (position, page, scale and piece), a chunk by its rows.
  *
  * The arithmetic is fixed to the bit, so that a code does not depend on how a
  * compiler orders a sum: the rotation in 64 bits (products of f32 are exact
@@ -57,9 +59,9 @@ struct KvAppend {
     sparkmv_kv_cache c;
     sparkmv_kv_batch b;
     sparkmv_kv_new n;
-    int nb;          /* pages a sequence's new tokens may touch */
-    int nkv;         /* workgroups of pages */
-    int qparts;      /* workgroups of one token's queries */
+    int nb;              /* pages a sequence's new tokens may touch */
+    int nkv;             /* workgroups of pages */
+    int qtok, qparts;    /* tokens of a workgroup of queries, or workgroups of a token */
     int half;
 };
 
@@ -73,84 +75,99 @@ __device__ __forceinline__ int kv_pair(int j, int half, int & second) {
     return 2 * j;
 }
 
-/* n pairs over NT threads, four of a thread's in flight: at(i, row, table) gives
- * pair i's place in its head, its row and its table row (NULL: not turned), and
- * put(i, e0, e1, a, b) takes the two results */
-template <typename X, int NT, typename At, typename Put>
-__device__ __forceinline__ void kv_turn_all(int n, At at, int half, Put put) {
-    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * NT) {
-        int e0[4], e1[4];
-        float x[4], y[4], c[4], s[4];
-        bool turn[4];
+/* up to four pairs and their turns, requested together and then turned: at(u, row,
+ * tab) gives the u-th pair's place in its head, its row and its table row (NULL:
+ * not turned). Only `live` of them, a uniform count, are there: a call of one
+ * token steps over the others' instructions, which it would otherwise fetch */
+constexpr int kKvPairs = 4;
+template <typename X, typename At>
+__device__ __forceinline__ void kv_turn(At at, int live, int half, double * a, double * b) {
+    float x[kKvPairs], y[kKvPairs], c[kKvPairs], s[kKvPairs];
+    bool turn[kKvPairs];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int i = min(i0 + u * NT, n - 1);
-            const X * row;
-            const float * tab;
-            const int j = at(i, row, tab);
-            e0[u] = kv_pair(j, half, e1[u]);
-            x[u] = kv_load(row + e0[u]);
-            y[u] = kv_load(row + e1[u]);
-            turn[u] = j < half && tab;
-            c[u] = turn[u] ? tab[j] : 1.0f;
-            s[u] = turn[u] ? tab[half + j] : 0.0f;
-        }
+    for (int u = 0; u < kKvPairs; u++) {
+        if (u >= live) break;
+        const X * row;
+        const float * tab;
+        const int j = at(u, row, tab);
+        int e1;
+        const int e0 = kv_pair(j, half, e1);
+        x[u] = kv_load(row + e0);
+        y[u] = kv_load(row + e1);
+        turn[u] = j < half && tab;
+        c[u] = turn[u] ? tab[j] : 1.0f;
+        s[u] = turn[u] ? tab[half + j] : 0.0f;
+    }
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            if (i0 + u * NT >= n) continue;
-            double a = (double) x[u], b = (double) y[u];
-            if (turn[u]) {
-                const double p = a, cc = (double) c[u], ss = (double) s[u];
-                a = p * cc - b * ss;
-                b = b * cc + p * ss;
-            }
-            put(i0 + u * NT, e0[u], e1[u], a, b);
-        }
+    for (int u = 0; u < kKvPairs; u++) {
+        if (u >= live) break;
+        const double p = (double) x[u], q = (double) y[u], cc = (double) c[u], ss = (double) s[u];
+        a[u] = turn[u] ? p * cc - q * ss : p;
+        b[u] = turn[u] ? q * cc + p * ss : q;
     }
 }
 
-/* nearest integer of x / s (ties to even), |x / s| <= 127.5 */
-__device__ __forceinline__ float kv_code(float x, float s, float r, bool tiny) {
-    if (tiny) return (float) rint((double) x / (double) s);
+/* nearest integer of x / s (ties to even), |x / s| <= 127.5; r is f32(1 / s) */
+__device__ __forceinline__ int kv_code(float x, float s, float r) {
     float n = rintf(x * r);
     const float e = fmaf(-s, n, x), e2 = 2.0f * fabsf(e);
     if (e2 > s || (e2 == s && ((int) n & 1))) n += e > 0.0f ? 1.0f : -1.0f;
-    return n;
+    return (int) n;
+}
+/* the same of a product of a code and its old scale, exact in 64 bits */
+__device__ __forceinline__ int kv_code(double x, double s, float r) {
+    double n = rint(x * (double) r);
+    const double e = fma(-s, n, x), e2 = 2.0 * fabs(e);
+    if (e2 > s || (e2 == s && ((int) n & 1))) n += e > 0.0 ? 1.0 : -1.0;
+    return (int) n;
 }
 
+constexpr int kv_append_rows(int nt) { return nt == 256 ? 8 : kKvPage; }   /* new rows of a page, at most */
+
+/* 256 threads: 8 rows of up to 256 elements; 512: 64 rows of up to 128; 1024: 64 of 256 */
 template <typename X, int NT>
-__global__ __launch_bounds__(NT) void kv_append_kernel(const KvAppend A) {
-    constexpr int QH = NT / 64;      /* query heads of a workgroup */
-    extern __shared__ __attribute__((aligned(16))) float lrow[];   /* [rows][hd] */
+__global__ __launch_bounds__(NT, NT == 256 ? 1 : 8) void kv_append_kernel(const KvAppend A) {
+    constexpr int U = NT == 256 ? 4 : 8, NP = NT == 256 ? 4 : 1;   /* pairs and pieces a thread, at most */
+    __shared__ __attribute__((aligned(16))) int8_t lcode[kKvPage * 256];
     __shared__ uint32_t lmax[NT / 64];
     const int tid = threadIdx.x, hd = A.c.head_dim, kvh = A.c.kv_heads, half = A.half;
     const int sh = 31 - __clz(hd / 2), pairs = 1 << sh;   /* head_dim is a power of two */
     if ((int) blockIdx.x >= A.nkv) {
         /* queries */
-        const int w = (int) blockIdx.x - A.nkv, t = w / A.qparts, h0 = QH * (w - t * A.qparts);
-        __shared__ int lpos;
-        if (tid == 0) lpos = -1;
+        int * lpos = (int *) lcode;                        /* [qtok], at most NT * kKvPairs / 32 */
+        const int w = (int) blockIdx.x - A.nkv, t0 = w / A.qparts * A.qtok, per = A.n.heads << sh;
+        const int first = w % A.qparts * (NT * kKvPairs);   /* 0 where a workgroup takes whole tokens */
+        const int n = A.qparts > 1 ? min(per, first + NT * kKvPairs) : min(A.qtok, A.b.ntok - t0) * per;
+        for (int i = tid; i < A.qtok; i += NT) lpos[i] = -1;
         __syncthreads();
         for (int i = tid; i < A.b.nseq; i += NT) {
             const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
-            if (t >= s.row && t - s.row < s.count) lpos = s.pos + t - s.row;
+            for (int t = max(s.row, t0); t < min(s.row + s.count, t0 + A.qtok); t++) lpos[t - t0] = s.pos + t - s.row;
         }
         __syncthreads();
-        const int pos = lpos;
-        if (pos < 0) return;
-        const float * rope = half ? A.n.rope + (size_t) pos * 2 * half : nullptr;
-        const X * src = (const X *) A.n.q + (size_t) t * A.n.ldq + (size_t) h0 * hd;
-        X * dst = (X *) A.n.q_out + (size_t) t * A.n.ldqo + (size_t) h0 * hd;
-        const int n = min(QH, A.n.heads - h0) << sh;
-        kv_turn_all<X, NT>(n, [&](int i, const X *& row, const float *& tab) {
-            row = src + (size_t) (i >> sh) * hd;
-            tab = rope;
-            return i & (pairs - 1);
-        }, half, [&](int i, int e0, int e1, double a, double b) {
-            X * to = dst + (size_t) (i >> sh) * hd;
-            kv_store_wide(to + e0, a);
-            kv_store_wide(to + e1, b);
-        });
+        for (int j0 = first; j0 < n; j0 += NT * kKvPairs) {
+            const int i0 = j0 + tid, live = (n - j0 + NT - 1) / NT;
+            double a[kKvPairs], b[kKvPairs];
+            kv_turn<X>([&](int u, const X *& row, const float *& tab) {
+                const int k = min(i0 + u * NT, n - 1), t = A.qparts > 1 ? 0 : k / per, e = k - t * per, pos = lpos[t];
+                row = (const X *) A.n.q + (size_t) (t0 + t) * A.n.ldq + (size_t) (e >> sh) * hd;
+                tab = half && pos >= 0 ? A.n.rope + (size_t) pos * 2 * half : nullptr;
+                return e & (pairs - 1);
+            }, live, half, a, b);
+#pragma unroll
+            for (int u = 0; u < kKvPairs; u++) {
+                if (u >= live) break;
+                const int k = i0 + u * NT;
+                if (k >= n) continue;
+                const int t = A.qparts > 1 ? 0 : k / per, e = k - t * per;
+                if (lpos[t] < 0) continue;
+                X * to = (X *) A.n.q_out + (size_t) (t0 + t) * A.n.ldqo + (size_t) (e >> sh) * hd;
+                int e1;
+                const int e0 = kv_pair(e & (pairs - 1), half, e1);
+                kv_store_wide(to + e0, a[u]);
+                kv_store_wide(to + e1, b[u]);
+            }
+        }
         return;
     }
     int w = blockIdx.x;
@@ -164,92 +181,125 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(const KvAppend A) {
     const int blk = s.pos / kKvPage + (w - i * A.nb), p0 = blk * kKvPage, end = s.pos + s.count;
     if (p0 >= end) return;
     const int page = A.c.pages[(size_t) s.slot * A.c.max_pages + blk];
+    const int lo = max(s.pos, p0), hi = min(end, p0 + kKvPage), held = lo - p0, rows = hi - lo, upto = held + rows;
+    /* the rows' pairs, requested before the page is looked at */
+    const X * src = (const X *) (which ? A.n.v : A.n.k) + (size_t) h * hd;
+    const int ld = which ? A.n.ldv : A.n.ldk, np = rows << sh;
+    float x[U], y[U];
+    uint32_t big = 0;
+    const int live = (np + NT - 1) / NT;
+#pragma unroll
+    for (int v = 0; v < U; v += kKvPairs) {
+        if (v >= live) break;
+        double a[kKvPairs], b[kKvPairs];
+        kv_turn<X>([&](int u, const X *& row, const float *& tab) {
+            const int k = min(tid + (v + u) * NT, np - 1), r = k >> sh;
+            row = src + (size_t) (s.row + lo + r - s.pos) * ld;
+            tab = which || !half ? nullptr : A.n.rope + (size_t) (lo + r) * 2 * half;
+            return k & (pairs - 1);
+        }, live - v, half, a, b);
+#pragma unroll
+        for (int u = 0; u < kKvPairs; u++) {
+            if (v + u >= live) break;
+            x[v + u] = (float) a[u];
+            y[v + u] = (float) b[u];
+            big = max(big, max(__float_as_uint(x[v + u]) & 0x7fffffffu, __float_as_uint(y[v + u]) & 0x7fffffffu));
+        }
+    }
     if (page < 0 || page >= A.c.npages) return;
-    const int lo = max(s.pos, p0), hi = min(end, p0 + kKvPage), held = lo - p0, rows = hi - lo;
-    const X * src = (const X *) (which ? A.n.v : A.n.k);
-    const int ld = which ? A.n.ldv : A.n.ldk;
     float * scale = (which ? A.c.v_scale : A.c.k_scale) + (size_t) page * kvh + h;
     int8_t * codes = (which ? A.c.v : A.c.k) + ((size_t) page * kvh + h) * (size_t) (kKvPage * hd);
     const float was = held ? *scale : 0.0f;
-    uint32_t big = 0;
-    const X * base = src + (size_t) (s.row + lo - s.pos) * ld + (size_t) h * hd;
-    kv_turn_all<X, NT>(rows << sh, [&](int i, const X *& row, const float *& tab) {
-        const int r = i >> sh;
-        row = base + (size_t) r * ld;
-        tab = which || !half ? nullptr : A.n.rope + (size_t) (lo + r) * 2 * half;
-        return i & (pairs - 1);
-    }, half, [&](int i, int e0, int e1, double a, double b) {
-        const float x = (float) a, y = (float) b;
-        float * to = lrow + (i >> sh) * hd;
-        to[e0] = x;
-        to[e1] = y;
-        big = max(big, max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu));
-    });
+    /* the values' pieces that hold older positions beside new ones: piece u of a
+     * thread is of group gu; only groups with a new position are touched */
+    union Piece { int4 v; uint32_t w[4]; int8_t c[16]; };
+    Piece piece[NP];
+    auto group = [&](int u) { return (tid + u * NT) >> (sh + 1); };
+    auto touched = [&](int g, int from) {   /* whether one of from .. upto - 1 is in group g */
+        return ((g - (from >> 2)) & 3) <= ((upto - 1) >> 2) - (from >> 2);
+    };
+    if (which && (held > 0 || upto < kKvPage)) {
+#pragma unroll
+        for (int u = 0; u < NP; u++)
+            if (group(u) < 4 && touched(group(u), held)) piece[u].v = *(const int4 *) (codes + (size_t) (tid + u * NT) * 16);
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) big = max(big, (uint32_t) __shfl_xor((int) big, o, 64));
     if ((tid & 63) == 0) lmax[tid >> 6] = big;
     __syncthreads();
 #pragma unroll
-    for (int w2 = 0; w2 < NT / 64; w2++) big = max(big, lmax[w2]);
+    for (int k = 0; k < NT / 64; k++) big = max(big, lmax[k]);
     const double need = (double) __uint_as_float(big);
     const bool bad = big >= 0x7f800000u || was != was;
     const bool keep = held && need <= 127.0 * (double) was;
     const float now = bad ? __uint_as_float(0x7fc00000u)
                           : (keep ? was : (float) (need * (hi == p0 + kKvPage ? 1.0 : 1.25) / 127.0));
-    if (!keep || bad) {
-        if (tid == 0) *scale = now;
-    }
-    /* below 2^-100 the reciprocal or the remainder could leave f32's range */
-    const bool none = bad || !(now > 0.0f), tiny = now < 7.9e-31f;
-    const float inv = none ? 0.0f : 1.0f / now;
+    if ((!keep || bad) && tid == 0) *scale = now;
+    /* a scale below 2^-100 and what it divides go up by 2^100, exactly, so that
+     * the reciprocal and the remainders stay in f32's range */
+    const bool none = bad || !(now > 0.0f);
+    const float up = now < 7.888609e-31f ? 1.2676506e30f : 1.0f, div = now * up, inv = none ? 0.0f : 1.0f / div;
     const bool again = held && !keep && !bad;   /* older codes rounded anew */
-    auto code = [&](int old, int r) -> int {    /* position p0 + r's code; old is what is there */
-        if (r < held) return again ? (none ? 0 : (int) rint((double) old * (double) was / (double) now)) : old;
-        return 0;
-    };
-    if (which == 0) {
+    const double was_up = (double) was * (double) up;
+    auto old_code = [&](int c) -> int8_t { return none ? 0 : (int8_t) kv_code((double) c * was_up, (double) div, inv); };
+    /* codes to LDS: keys by row, values as they lie in a page */
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (u >= live) break;
+        const int k = tid + u * NT, r = k >> sh;
+        if (k >= np) continue;
+        int e1;
+        const int e0 = kv_pair(k & (pairs - 1), half, e1);
+        const int a = none ? 0 : kv_code(x[u] * up, div, inv), b = none ? 0 : kv_code(y[u] * up, div, inv);
+        lcode[which ? kv_value_at(held + r, e0, hd) : r * hd + e0] = (int8_t) a;
+        lcode[which ? kv_value_at(held + r, e1, hd) : r * hd + e1] = (int8_t) b;
+    }
+    __syncthreads();
+    if (!which) {
         const int per = hd / 16;   /* pieces of a position */
-        const int first = again ? 0 : held;
-        for (int k = tid; k < (held + rows - first) * per; k += NT) {
-            const int r = first + (k >> (sh - 3)), d = 16 * (k & (per - 1));
-            int8_t * at = codes + kv_key_at(r, d);
-            union { int4 v; int8_t c[16]; } u;
-            if (r < held) {
-                u.v = *(const int4 *) at;
-#pragma unroll
-                for (int e = 0; e < 16; e++) u.c[e] = (int8_t) code(u.c[e], r);
-            } else {
-                const float * x = lrow + (r - held) * hd + d;
-#pragma unroll
-                for (int e = 0; e < 16; e++) u.c[e] = none ? 0 : (int8_t) (int) kv_code(x[e], now, inv, tiny);
-            }
-            *(int4 *) at = u.v;
+        for (int k = tid; k < rows * per; k += NT) {
+            const int r = k >> (sh - 3), d = 16 * (k & (per - 1));
+            *(int4 *) (codes + kv_key_at(held + r, d)) = *(const int4 *) (lcode + r * hd + d);
         }
-    } else {
-        const int upto = held + rows;
+        if (again)
+            for (int k = tid; k < held * per; k += NT) {
+                Piece q;
+                int4 * at = (int4 *) (codes + kv_key_at(k >> (sh - 3), 16 * (k & (per - 1))));
+                q.v = *at;
+#pragma unroll
+                for (int e = 0; e < 16; e++) q.c[e] = old_code(q.c[e]);
+                *at = q.v;
+            }
+        return;
+    }
+    /* positions from .. upto - 1 of a page come from LDS, the others stay */
+    const int from = again ? 0 : held;
+    if (again) {
         for (int k = tid; k < 4 * hd; k += NT) {
-            const int g = k >> (sh + 1), d = k & (hd - 1);
-            /* positions 16 t + 4 g + i of this piece */
-            bool any = false, all = true;
+            Piece q;
+            q.v = *(const int4 *) (codes + (size_t) k * 16);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int r = 16 * (e >> 2) + 4 * g + (e & 3);
-                const bool in = r >= (again ? 0 : held) && r < upto;
-                any = any || in;
-                all = all && r >= held && r < upto;
-            }
-            if (!any) continue;
-            int8_t * at = codes + (size_t) k * 16;
-            union { int4 v; int8_t c[16]; } u;
-            if (!all) u.v = *(const int4 *) at;
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int r = 16 * (e >> 2) + 4 * g + (e & 3);
-                if (r < held) u.c[e] = (int8_t) code(u.c[e], r);
-                else if (r < upto) u.c[e] = none ? 0 : (int8_t) (int) kv_code(lrow[(r - held) * hd + d], now, inv, tiny);
-            }
-            *(int4 *) at = u.v;
+            for (int e = 0; e < 16; e++)
+                if (16 * (e >> 2) + 4 * (k >> (sh + 1)) + (e & 3) < held) lcode[16 * k + e] = old_code(q.c[e]);
         }
+    }
+#pragma unroll
+    for (int u = 0; u < NP; u++) {
+        const int k = tid + u * NT, g = group(u);
+        if (g >= 4 || !touched(g, from)) continue;
+        Piece q;
+        q.v = *(const int4 *) (lcode + 16 * k);
+        if (from > 0 || upto < kKvPage) {
+            if (again) piece[u].v = *(const int4 *) (codes + (size_t) k * 16);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                /* bytes lo4 .. hi4 - 1 of the word */
+                const int b = 16 * t + 4 * g, lo4 = min(max(from - b, 0), 4), hi4 = min(max(upto - b, 0), 4);
+                const uint32_t m = (uint32_t) ((1ull << (8 * hi4)) - (1ull << (8 * lo4)));
+                q.w[t] = hi4 > lo4 ? (q.w[t] & m) | (piece[u].w[t] & ~m) : piece[u].w[t];
+            }
+        }
+        *(int4 *) (codes + (size_t) k * 16) = q.v;
     }
 }
 
@@ -434,34 +484,29 @@ int sparkmv_kv_append(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     a.half = n.rope_dim / 2;
     a.nb = (a.b.max_q + kKvPage - 2) / kKvPage + 1;
     if (a.nb > cache->max_pages) a.nb = cache->max_pages;
-    /* 1024 threads from 9 rows a page on: 64 rows x 256 elements are 8192 pairs,
-     * of which 256 threads took 32 each (a chunk of 512 tokens 33 us); one row
-     * gives 256 threads no work for more */
-    const bool wide = a.b.max_q > 8;
-    const int nt = wide ? 1024 : 256;
-    a.qparts = (n.heads + nt / 64 - 1) / (nt / 64);
-    const long nkv = (long) batch->nseq * a.nb * cache->kv_heads * 2, wgs = nkv + (long) batch->ntok * a.qparts;
+    /* 256 threads hold eight rows of a page, 512 all 64 of up to 128 elements, 1024
+     * of 256: with 256 for a chunk of 512 tokens the rows came in 32 turns and took
+     * 33 us instead of 12; one row gives no more than 128 threads a pair */
+    const int nt = a.b.max_q <= kv_append_rows(256) ? 256 : (hd <= 128 ? 512 : 1024);
+    const int qpairs = nt * kKvPairs, per = n.heads * (hd / 2);
+    a.qtok = per && per <= qpairs ? qpairs / per : 1;
+    a.qparts = per > qpairs ? (per + qpairs - 1) / qpairs : 1;
+    const long nkv = (long) batch->nseq * a.nb * cache->kv_heads * 2;
+    const long wgs = nkv + (n.heads ? (long) ((batch->ntok + a.qtok - 1) / a.qtok) * a.qparts : 0);
     if (wgs > 0x7fffffffl) { set_error("an append of %ld workgroups", wgs); return -1; }
     a.nkv = (int) nkv;
-    const int lrows = a.b.max_q < kKvPage ? a.b.max_q : kKvPage;
-    const uint32_t lds = (uint32_t) (lrows * hd * 4);
     const dim3 grid((unsigned) wgs), block((unsigned) nt);
     hipStream_t s = (hipStream_t) stream;
-    /* a full page of 256 elements takes 64 KB beside the kernel's own words */
-#define KV_APPEND(X, NT)                                                                                             \
+#define KV_APPEND(X, NT) hipLaunchKernelGGL((kv_append_kernel<X, NT>), grid, block, 0, s, a)
+#define KV_APPEND_NT(X)                                                                                              \
     do {                                                                                                             \
-        static LdsAllowed allowed;                                                                                   \
-        if (lds_allow(allowed, (const void *) kv_append_kernel<X, NT>, lds + 1024, "LDS opt-in for the kv append"))  \
-            return -1;                                                                                               \
-        hipLaunchKernelGGL((kv_append_kernel<X, NT>), grid, block, lds, s, a);                                       \
+        if (nt == 256) KV_APPEND(X, 256);                                                                            \
+        else if (nt == 512) KV_APPEND(X, 512);                                                                       \
+        else KV_APPEND(X, 1024);                                                                                     \
     } while (0)
-    if (n.x_dtype == SPARKMV_X_F32) {
-        if (wide) KV_APPEND(float, 1024);
-        else KV_APPEND(float, 256);
-    } else {
-        if (wide) KV_APPEND(uint16_t, 1024);
-        else KV_APPEND(uint16_t, 256);
-    }
+    if (n.x_dtype == SPARKMV_X_F32) KV_APPEND_NT(float);
+    else KV_APPEND_NT(uint16_t);
+#undef KV_APPEND_NT
 #undef KV_APPEND
     return kv_check_launch("kv append launch");
 }
