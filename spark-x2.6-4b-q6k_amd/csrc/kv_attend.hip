@@ -42,13 +42,23 @@ __device__ __forceinline__ int kv_span(const KvSeq & s, int t0, int t1, int wind
 }
 
 template <int CTRL>
-__device__ __forceinline__ float kv_quad(float v) {
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+__device__ __forceinline__ int kv_quad(int v) { return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true); }
+template <int CTRL>
+__device__ __forceinline__ float kv_quad(float v) { return __int_as_float(kv_quad<CTRL>(__float_as_int(v))); }
+constexpr int kKvXor1 = 0xb1, kKvXor2 = 0x4e;   /* quad permutations: lanes 1 0 3 2, 2 3 0 1 */
+
+/* the largest, or the sum, of the four lanes 16 apart, in each of them */
+__device__ __forceinline__ float kv_rows_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
-/* the sum over the four lanes of a quad, the same bits in each */
-__device__ __forceinline__ float kv_quad_sum(float v) {
-    v += kv_quad<0xb1>(v);          /* lanes 1 0 3 2 */
-    return v + kv_quad<0x4e>(v);    /* lanes 2 3 0 1 */
+__device__ __forceinline__ float kv_rows_sum(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
 /* 16 query elements as f32 */
@@ -107,17 +117,24 @@ __device__ __forceinline__ void kv_write(const sparkmv_kv_query & q, int row, in
  * Up to four columns (token, query head) of a kv head: a decode step of up to
  * four query heads per kv head. Bound by reading the codes once. The sixteen
  * columns of a tile are the four columns times four digits, so f32's whole
- * precision costs no further instruction; a column's value is the sum of its
- * digits' sums, two cross-lane additions in a quad.
+ * precision costs no further instruction. The four lanes of a quad add their
+ * digits' sums up so that each ends with a quarter of the column's scores, takes
+ * their weights, and hands them back as integers for the others' digits.
  *
  * Workgroups take equal shares of all (sequence, kv head, page) in that order,
  * so lengths may differ by any amount; a kv head of a sequence counts kKvItem
  * pages more than it has, for what beginning it costs. A share's pages of one
  * kv head go to the four waves in turn, whose results meet in LDS; a kv head's
  * pages that lie in one share are written out at once, others as a partial
- * result that a second launch joins. */
+ * result that a second launch joins.
+ *
+ * A short call is bound by its chain of reads (positions, page numbers, codes)
+ * and by fetching instructions that run once, about 0.5 us a kilobyte: so the
+ * codes are requested before the queries are looked at, and what runs once is
+ * kept in loops. */
 constexpr int kKvItem = 8;
 constexpr int kKvFlatMost = 1024;   /* workgroups, at most */
+constexpr int kKvWhole = 24;        /* pages of a sequence that one workgroup takes alone */
 
 struct KvFlat {
     sparkmv_kv_cache c;
@@ -129,44 +146,82 @@ struct KvFlat {
     float * pml;     /* [workgroups][2][4][2] */
 };
 
-template <int HD>
-__global__ __launch_bounds__(256, 2) void kv_flat_kernel(const KvFlat A) {
-    constexpr int NC = HD / 64, ND = HD / 16;
-    extern __shared__ int lpre[];                     /* [nseq + 1] */
+constexpr int kv_flat_lds(int hd, int waves) { return waves * 16 * (hd + 4) * 4 + 16 * hd; }
+
+/* WAVES 4: shares; 8: workgroup i * kv_heads + h takes the whole of a sequence's
+ * kv head, and no join follows */
+template <int HD, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void kv_flat_kernel(const KvFlat A) {
+    constexpr int NC = HD / 64, ND = HD / 16, NT = 64 * WAVES, E = HD / 64, LO = HD + 4;
+    constexpr bool WHOLE = WAVES == 8;
+    extern __shared__ __attribute__((aligned(16))) uint8_t ldyn[];
+    float * lo = (float *) ldyn;                      /* [WAVES][16][LO]: a wave's output, digit by digit */
+    uint8_t * lq = ldyn + WAVES * 16 * LO * 4;        /* [16 * HD]: query digits as the matrix instruction's lanes take them */
+    int * lpre = (int *) (lq + 16 * HD);              /* [nseq + 1], shares of more than 64 sequences only */
     __shared__ int lsum[4];
-    __shared__ __attribute__((aligned(16))) float lo[4][4][HD];
-    __shared__ float lm[4][4], ll[4][4];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c16 = lane & 15, col = c16 >> 2, dg = c16 & 3;
+    __shared__ float lcs[4], lbad[4], lm[WAVES][4], ll[WAVES][4];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c16 = lane & 15;
+    const int col = c16 >> 2, dg = c16 & 3;
     const int kvh = A.c.kv_heads, G = A.q.heads / kvh, nseq = A.b.nseq;
-    {
-        const int per = (nseq + 255) / 256, i0 = min(nseq, tid * per), i1 = min(nseq, i0 + per);
-        int sum = 0;
-        for (int i = i0; i < i1; i++) {
+    /* shares: what a kv head of each sequence counts. Up to 64 sequences a lane
+     * each, in every wave; more through LDS */
+    const bool few = nseq <= 64;
+    KvSeq mine = {0, 0, 0, 0};
+    int cost = 0, before = 0;
+    int ubeg = blockIdx.x, uend = ubeg + 1;
+    if constexpr (!WHOLE) {
+        int total;
+        if (few) {
+            if (lane < nseq) mine = kv_seq(A.b, lane, A.c.nslots, A.c.max_pages);
             int first;
-            const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
-            lpre[i] = sum;
-            if (s.count > 0) sum += kv_span(s, 0, s.count, A.q.window, first) + kKvItem;
-        }
-        int scan = sum;
+            if (mine.count > 0) cost = kv_span(mine, 0, mine.count, A.q.window, first) + kKvItem;
+            int scan = cost;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(scan, o, 64);
-            if (lane >= o) scan += v;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(scan, o, 64);
+                if (lane >= o) scan += v;
+            }
+            before = scan - cost;
+            total = __builtin_amdgcn_readlane(scan, 63);
+        } else {
+            const int per = (nseq + 255) / 256, i0 = min(nseq, tid * per), i1 = min(nseq, i0 + per);
+            int sum = 0;
+            for (int i = i0; i < i1; i++) {
+                int first;
+                const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
+                lpre[i] = sum;
+                if (s.count > 0) sum += kv_span(s, 0, s.count, A.q.window, first) + kKvItem;
+            }
+            int scan = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(scan, o, 64);
+                if (lane >= o) scan += v;
+            }
+            if (lane == 63) lsum[wave] = scan;
+            __syncthreads();
+            int base = scan - sum;
+            for (int w = 0; w < wave; w++) base += lsum[w];
+            for (int i = i0; i < i1; i++) lpre[i] += base;
+            if (tid == 255) lpre[nseq] = base + sum;
+            __syncthreads();
+            total = __builtin_amdgcn_readfirstlane(lpre[nseq]);
         }
-        if (lane == 63) lsum[wave] = scan;
-        __syncthreads();
-        int before = scan - sum;
-        for (int w = 0; w < wave; w++) before += lsum[w];
-        for (int i = i0; i < i1; i++) lpre[i] += before;
-        if (tid == 255) lpre[nseq] = before + sum;
-        __syncthreads();
+        const int share = max((total * kvh + (int) gridDim.x - 1) / (int) gridDim.x, A.least);
+        if (blockIdx.x == 0) {
+            if (few) {
+                if (tid < nseq) A.pre[tid] = before;
+            } else {
+                for (int i = tid; i < nseq; i += 256) A.pre[i] = lpre[i];
+            }
+            if (tid == 0) {
+                A.pre[nseq] = total;
+                A.pre[nseq + 1] = share;
+            }
+        }
+        ubeg = (int) blockIdx.x * share;
+        uend = min(total * kvh, ubeg + share);
     }
-    const int total = lpre[nseq] * kvh, share = max((total + (int) gridDim.x - 1) / (int) gridDim.x, A.least);
-    if (blockIdx.x == 0) {
-        for (int i = tid; i <= nseq; i += 256) A.pre[i] = lpre[i];
-        if (tid == 0) A.pre[nseq + 1] = share;
-    }
-    const int ubeg = (int) blockIdx.x * share, uend = min(total, ubeg + share);
     const float wdig = (float) (1 << (8 * (3 - dg)));
     const uint32_t sel = (uint32_t) (3 - dg) | (uint32_t) (7 - dg) << 8 | 0x0c0c0000u, flip = dg ? 0x80808080u : 0u;
     /* byte 3 - dg of four integers with 0x808080 added: the digit, its sign bit
@@ -176,94 +231,156 @@ __global__ __launch_bounds__(256, 2) void kv_flat_kernel(const KvFlat A) {
         return (int) ((lo2 | hi2 << 16) ^ flip);
     };
     for (int u = ubeg; u < uend;) {
-        /* the sequence: the last one that begins at or before u */
-        int i = 0;
-        for (int b = nseq; b - i > 1;) {
-            const int mid = (i + b) >> 1;
-            if (lpre[mid] * kvh <= u) i = mid;
-            else b = mid;
+        int h, off = 0, n, seg, first;
+        KvSeq s;
+        if constexpr (WHOLE) {
+            const int i = u / kvh;
+            h = u - i * kvh;
+            s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
+            if (s.count <= 0) return;
+            seg = n = kv_span(s, 0, s.count, A.q.window, first);
+        } else {
+            /* the sequence: the last one that begins at or before u */
+            int in;
+            if (few) {
+                const int i = 63 - __builtin_clzll(__ballot(lane < nseq && before * kvh <= u));
+                s.slot = __builtin_amdgcn_readlane(mine.slot, i);
+                s.pos = __builtin_amdgcn_readlane(mine.pos, i);
+                s.row = __builtin_amdgcn_readlane(mine.row, i);
+                s.count = __builtin_amdgcn_readlane(mine.count, i);
+                in = u - __builtin_amdgcn_readlane(before, i) * kvh;
+            } else {
+                int i = 0;
+                for (int b = nseq; b - i > 1;) {
+                    const int mid = (i + b) >> 1;
+                    if (__builtin_amdgcn_readfirstlane(lpre[mid]) * kvh <= u) i = mid;
+                    else b = mid;
+                }
+                s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
+                s.slot = __builtin_amdgcn_readfirstlane(s.slot);
+                s.pos = __builtin_amdgcn_readfirstlane(s.pos);
+                s.row = __builtin_amdgcn_readfirstlane(s.row);
+                s.count = __builtin_amdgcn_readfirstlane(s.count);
+                in = u - __builtin_amdgcn_readfirstlane(lpre[i]) * kvh;
+            }
+            n = kv_span(s, 0, s.count, A.q.window, first);
+            h = in / (n + kKvItem);
+            off = in - h * (n + kKvItem);
+            if (off >= n) {
+                u += n + kKvItem - off;
+                continue;
+            }
+            seg = min(n - off, uend - u);
         }
-        const int n = lpre[i + 1] - lpre[i] - kKvItem, in = u - lpre[i] * kvh, h = in / (n + kKvItem), off = in - h * (n + kKvItem);
-        if (off >= n) {
-            u += n + kKvItem - off;
-            continue;
-        }
-        const int seg = min(n - off, uend - u);
-        const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
-        int first;
-        kv_span(s, 0, s.count, A.q.window, first);
-        const int ncol = s.count * G, tok = min(col / G, s.count - 1), head = h * G + col % G;
+        const int ncol = s.count * G, tok = min(col / G, s.count - 1);
         const int pos_c = s.pos + tok, beg_c = A.q.window > 0 && pos_c + 1 > A.q.window ? pos_c + 1 - A.q.window : 0;
         /* positions that every column sees */
         const int all_lo = A.q.window > 0 && s.pos + s.count > A.q.window ? s.pos + s.count - A.q.window : 0, all_hi = s.pos;
-        /* the columns' digits */
-        kv_i4 qd[NC];
-        float cs;
-        bool qbad;
-        {
-            float x[NC][16];
-            const size_t at = (size_t) (s.row + tok) * A.q.ldq + (size_t) head * HD + 16 * g;
-#pragma unroll
-            for (int c = 0; c < NC; c++) kv_load16(A.q, at + 64 * c, x[c]);
-            const int ex = kv_q_exponent<NC>(x, qbad);
+        const int * table = A.c.pages + (size_t) s.slot * A.c.max_pages + first + off;
+        /* 64 pages of this wave at a time: their numbers and scales are held one a lane */
+        int id, count;
+        float ks, vs;
+        uint64_t there;
+        kv_i4 kr[NC][4], vr[ND];
+        /* buffer loads: a page's base is uniform, so all of its 32 addresses take
+         * one register a lane (64-bit ones took 60, which then spilled) */
+        const uint32_t klane = c16 * 64 + 16 * g, vlane = (g * HD + c16) * 16;
+        auto page_at = [&](const int8_t * p, int j) {
+            const uint64_t at = (uint64_t) p + ((uint64_t) (uint32_t) __builtin_amdgcn_readlane(id, j) * (uint32_t) kvh + (uint32_t) h) * (kKvPage * HD);
+            const uint64_t lo = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) at);
+            const uint64_t hi = (uint32_t) __builtin_amdgcn_readfirstlane((int) (at >> 32));
+            return __builtin_amdgcn_make_buffer_rsrc((void *) (hi << 32 | lo), 0, kKvPage * HD, 0x00027000);
+        };
+        auto fetch_k = [&](int j) {
+            const auto p = page_at(A.c.k, j);
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    uint32_t y[4];
+                for (int t = 0; t < 4; t++) kr[c][t] = (kv_i4) __builtin_amdgcn_raw_buffer_load_b128(p, klane, c * 4096 + t * 1024, 0);
+        };
+        auto begin = [&](int base) {
+            count = min((seg - base + WAVES - 1) / WAVES, 64);
+            id = 0;
+            ks = vs = 0.0f;
+            bool have = false;
+            if (lane < count) {
+                id = table[base + WAVES * lane];
+                have = id >= 0 && id < A.c.npages;
+                id = have ? id : 0;
+                const uint64_t at = (uint64_t) (uint32_t) id * (uint32_t) kvh + (uint32_t) h;
+                ks = A.c.k_scale[at];
+                vs = A.c.v_scale[at];
+            }
+            there = __ballot(have);
+            fetch_k(0);
+            const auto p = page_at(A.c.v, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        y[e] = (uint32_t) (int) rintf(ldexpf(qbad ? 0.0f : x[c][4 * w + e], 30 - ex)) + 0x808080u;
-                    const int d = digits(y[0], y[1], y[2], y[3]);
-                    qd[c][w] = col < ncol ? d : 0;
-                }
-            cs = ldexpf(A.q.scale * kKvLog2e, ex - 30);
+            for (int d = 0; d < ND; d++) vr[d] = (kv_i4) __builtin_amdgcn_raw_buffer_load_b128(p, vlane, d * 256, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        /* the columns' digits, a wave a column and E elements a lane. The elements
+         * are requested before the codes: loads return in order */
+        const bool live = wave < ncol;
+        float x[E];
+        if (wave < 4) {
+            const int t = live ? wave / G : 0, head = h * G + (live ? wave % G : 0);
+            const size_t at = (size_t) (s.row + t) * A.q.ldq + (size_t) head * HD + E * lane;
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                x[e] = A.q.q_dtype == SPARKMV_X_F32 ? kv_load((const float *) A.q.q + at + e) : kv_load((const uint16_t *) A.q.q + at + e);
         }
+        if (wave < seg) begin(wave);
+        if (wave < 4) {
+            uint32_t big = 0, y[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < E; e++) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
+            /* non-negative floats, a NaN above the infinities, order as integers do */
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) big = max(big, (uint32_t) __shfl_xor((int) big, o, 64));
+            const bool bad = big >= 0x7f800000u;
+            int ex = 0;
+            (void) frexpf(__uint_as_float(bad ? 0u : big), &ex);
+#pragma unroll
+            for (int e = 0; e < E; e++) y[e] = (live && !bad ? (uint32_t) (int) rintf(ldexpf(x[e], 30 - ex)) : 0u) + 0x808080u;
+            /* element d of digit column n at ((d / 64 * 64 + d / 16 % 4 * 16 + n) * 16 + d % 16 */
+            const int d0 = E * lane;
+            uint8_t * to = lq + (((d0 >> 6) * 64 + (d0 >> 4 & 3) * 16 + 4 * wave) * 16 + (d0 & 15));
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const uint32_t b = 3 - d, pick = b | (b + 4) << 8 | 0x0c0c0000u, turn = d ? 0x80808080u : 0u;
+                const uint32_t w = (__builtin_amdgcn_perm(y[1], y[0], pick) | __builtin_amdgcn_perm(y[3], y[2], pick) << 16) ^ turn;
+                if constexpr (E == 4) *(uint32_t *) (to + 16 * d) = w;
+                else if constexpr (E == 2) *(uint16_t *) (to + 16 * d) = (uint16_t) w;
+                else to[16 * d] = (uint8_t) w;
+            }
+            if (lane == 0) {
+                lcs[wave] = ldexpf(A.q.scale * kKvLog2e, ex - 30);
+                lbad[wave] = bad ? __uint_as_float(0x7fc00000u) : 0.0f;
+            }
+        }
+        __syncthreads();
+        const float cs = lcs[col];
         float m = -INFINITY, l = 0.0f;
         kv_f4 o[ND];
 #pragma unroll
         for (int d = 0; d < ND; d++) o[d] = kv_f4{0.f, 0.f, 0.f, 0.f};
-        const int * table = A.c.pages + (size_t) s.slot * A.c.max_pages + first + off;
-        /* 64 pages of this wave at a time: their numbers and scales are held one a lane */
-        for (int base = wave; base < seg; base += 256) {
-            const int mine = min((seg - base + 3) / 4, 64);
-            int id = 0;
-            float ks = 0.0f, vs = 0.0f;
-            bool have = false;
-            if (lane < mine) {
-                id = table[base + 4 * lane];
-                have = id >= 0 && id < A.c.npages;
-                id = have ? id : 0;
-                ks = A.c.k_scale[(size_t) id * kvh + h];
-                vs = A.c.v_scale[(size_t) id * kvh + h];
-            }
-            const uint64_t there = __ballot(have);
-            kv_i4 kr[NC][4], vr[ND];
-            auto fetch_k = [&](int j) {
-                const int8_t * p = A.c.k + ((size_t) __builtin_amdgcn_readlane(id, j) * kvh + h) * (size_t) (kKvPage * HD) + c16 * 64 + 16 * g;
+        for (int base = wave; base < seg; base += 64 * WAVES) {
+            if (base > wave) begin(base);
+            for (int j = 0; j < count; j++) {
+                const int nx = min(j + 1, count - 1);
+                float a[4][4];
+                /* read again for each page: held, they would leave too few registers */
+                asm volatile("" ::: "memory");
+                kv_i4 qd[NC];
 #pragma unroll
-                for (int c = 0; c < NC; c++)
-#pragma unroll
-                    for (int t = 0; t < 4; t++) kr[c][t] = *(const kv_i4 *) (p + c * 4096 + t * 1024);
-            };
-            auto fetch_v = [&](int j) {
-                const int8_t * p = A.c.v + ((size_t) __builtin_amdgcn_readlane(id, j) * kvh + h) * (size_t) (kKvPage * HD) + (g * HD + c16) * 16;
-#pragma unroll
-                for (int d = 0; d < ND; d++) vr[d] = *(const kv_i4 *) (p + d * 256);
-            };
-            fetch_k(0);
-            fetch_v(0);
-            __builtin_amdgcn_sched_barrier(0);
-            for (int j = 0; j < mine; j++) {
-                const int nx = min(j + 1, mine - 1);
-                float x[4][4];
+                for (int c = 0; c < NC; c++) qd[c] = *(const kv_i4 *) (lq + (c * 64 + lane) * 16);
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
                     kv_i4 acc = kv_i4{0, 0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < NC; c++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[c][t], qd[c], acc, 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[t][e] = (float) acc[e] * wdig;
+                    for (int e = 0; e < 4; e++) a[t][e] = (float) acc[e] * wdig;
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 fetch_k(nx);
@@ -271,98 +388,100 @@ __global__ __launch_bounds__(256, 2) void kv_flat_kernel(const KvFlat A) {
                 const float kscale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), j));
                 const float vscale = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), j));
                 const float f = cs * kscale;
-                const int p0 = (first + off + base + 4 * j) * kKvPage;
+                /* x[e]: the score of position 16 dg + 4 g + e, the digits' sums of the quad added up */
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float k0 = (dg & 2 ? a[2][e] : a[0][e]) + kv_quad<kKvXor2>(dg & 2 ? a[0][e] : a[2][e]);
+                    const float k1 = (dg & 2 ? a[3][e] : a[1][e]) + kv_quad<kKvXor2>(dg & 2 ? a[1][e] : a[3][e]);
+                    x[e] = ((dg & 1 ? k1 : k0) + kv_quad<kKvXor1>(dg & 1 ? k0 : k1)) * f;
+                }
+                const int p0 = (first + off + base + WAVES * j) * kKvPage;
                 const bool ok = there >> j & 1;
-                float mp = -INFINITY;
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[t][e] = kv_quad_sum(x[t][e]) * f;
                 if (!ok || p0 < all_lo || p0 + kKvPage - 1 > all_hi || kscale != kscale) {
                     bool any = false;
 #pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int p = p0 + 16 * t + 4 * g + e;
-                            const bool seen = ok && p >= beg_c && p <= pos_c;
-                            any = any || seen;
-                            x[t][e] = seen && kscale == kscale ? x[t][e] : -INFINITY;
-                        }
+                    for (int e = 0; e < 4; e++) {
+                        const int p = p0 + 16 * dg + 4 * g + e;
+                        const bool seen = ok && p >= beg_c && p <= pos_c;
+                        any = any || seen;
+                        x[e] = seen && kscale == kscale ? x[e] : -INFINITY;
+                    }
                     if (any && kscale != kscale) l = kscale;   /* NaN to the end for a column that sees some of it */
                 }
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mp = fmaxf(mp, x[t][e]);
-                mp = fmaxf(mp, __shfl_xor(mp, 16, 64));
-                mp = fmaxf(mp, __shfl_xor(mp, 32, 64));
+                float mp = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                mp = fmaxf(mp, kv_quad<kKvXor1>(mp));
+                mp = fmaxf(mp, kv_quad<kKvXor2>(mp));
+                mp = kv_rows_max(mp);
                 if (__any(mp > m + kKvLag)) {
                     const float mn = fmaxf(m, mp);
-                    const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-                    l *= a;
+                    const float r = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                    l *= r;
 #pragma unroll
-                    for (int d = 0; d < ND; d++) o[d] *= a;
+                    for (int d = 0; d < ND; d++) o[d] *= r;
                     m = mn;
                 }
                 const float mref = mp == -INFINITY ? 0.0f : mp;
-                kv_i4 P;
                 float sum = 0.0f;
+                int y[4];
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    uint32_t y[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float p = __builtin_amdgcn_exp2f(x[t][e] - mref);
-                        sum += p;
-                        y[e] = (uint32_t) (int) (p * 1073741824.0f) + 0x808080u;
-                    }
-                    P[t] = digits(y[0], y[1], y[2], y[3]);
+                for (int e = 0; e < 4; e++) {
+                    const float p = __builtin_amdgcn_exp2f(x[e] - mref);
+                    sum += p;
+                    y[e] = (int) (p * 1073741824.0f) + 0x808080;
                 }
+                /* tile t's weights are lane t's of the quad */
+                kv_i4 P;
+                P[0] = digits(kv_quad<0x00>(y[0]), kv_quad<0x00>(y[1]), kv_quad<0x00>(y[2]), kv_quad<0x00>(y[3]));
+                P[1] = digits(kv_quad<0x55>(y[0]), kv_quad<0x55>(y[1]), kv_quad<0x55>(y[2]), kv_quad<0x55>(y[3]));
+                P[2] = digits(kv_quad<0xaa>(y[0]), kv_quad<0xaa>(y[1]), kv_quad<0xaa>(y[2]), kv_quad<0xaa>(y[3]));
+                P[3] = digits(kv_quad<0xff>(y[0]), kv_quad<0xff>(y[1]), kv_quad<0xff>(y[2]), kv_quad<0xff>(y[3]));
                 const float step = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - m);
                 l += sum * step;
                 const float w = mp == -INFINITY ? 0.0f : step * vscale;
+                /* four at a time: with all of them ahead their sums would not fit the registers */
+                const auto vnext = page_at(A.c.v, nx);
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const kv_i4 acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[d], P, kv_i4{0, 0, 0, 0}, 0, 0, 0);
+                for (int d0 = 0; d0 < ND; d0 += 4) {
+                    kv_i4 acc[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[d][e] += w * (float) acc[e];
+                    for (int d = 0; d < 4; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[d0 + d], P, kv_i4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                    for (int d = 0; d < 4; d++) vr[d0 + d] = (kv_i4) __builtin_amdgcn_raw_buffer_load_b128(vnext, vlane, (d0 + d) * 256, 0);
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[d0 + d][e] += w * (float) acc[d][e];
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                fetch_v(nx);
-                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
-        if (qbad) l = __uint_as_float(0x7fc00000u);
-        /* the digits of a column, then the waves */
-        const float down = wdig * 9.313225746154785e-10f;   /* 2^-30 */
+        l += kv_quad<kKvXor1>(l);
+        l += kv_quad<kKvXor2>(l);
+        l = kv_rows_sum(l);
+        /* the waves' outputs meet in LDS */
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            kv_f4 v;
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = kv_quad_sum(o[d][e] * down);
-            if ((d & 3) == dg) *(kv_f4 *) &lo[wave][col][16 * d + 4 * g] = v;
-        }
+        for (int d = 0; d < ND; d++) *(kv_f4 *) (lo + (wave * 16 + c16) * LO + 16 * d + 4 * g) = o[d];
         if (g == 0 && dg == 0) {
             lm[wave][col] = m;
-            ll[wave][col] = l;
+            ll[wave][col] = l + lbad[col];
         }
         __syncthreads();
-        const bool whole = seg == n;
+        const bool whole = WHOLE || seg == n;
         const size_t at = 2 * (size_t) blockIdx.x + (off == 0 ? 1 : 0);
-        for (int k = tid; k < ncol * HD; k += 256) {
+        for (int k = tid; k < ncol * HD; k += NT) {
             const int cc = k / HD, d = k - cc * HD;
             float M = lm[0][cc];
 #pragma unroll
-            for (int w = 1; w < 4; w++) M = fmaxf(M, lm[w][cc]);
+            for (int w = 1; w < WAVES; w++) M = fmaxf(M, lm[w][cc]);
             float L = 0.0f, v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float a = lm[w][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[w][cc] - M);
-                L += lm[w][cc] == -INFINITY ? ll[w][cc] : a * ll[w][cc];
-                v += a * lo[w][cc][d];
+#pragma unroll 1
+            for (int w = 0; w < WAVES; w++) {
+                const float * p = lo + (w * 16 + 4 * cc) * LO + d;
+                const float r = lm[w][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[w][cc] - M);
+                L += lm[w][cc] == -INFINITY ? ll[w][cc] : r * ll[w][cc];
+                /* digits 2^24 .. 2^0, over the weight's 2^30 */
+                v += r * (((p[3 * LO] * 0x1p-30f + p[2 * LO] * 0x1p-22f) + p[LO] * 0x1p-14f) + p[0] * 0x1p-6f);
             }
             if (whole) {
                 kv_write(A.q, s.row + cc / G, h * G + cc % G, HD, d, v, L);
@@ -379,13 +498,12 @@ __global__ __launch_bounds__(256, 2) void kv_flat_kernel(const KvFlat A) {
     }
 }
 
-/* The join of one column's partials at[0 .. n - 1] by four waves (sub 0..3 of the
- * column): weights e^(m - M) in LDS, then each wave adds every fourth row with
- * eight of them in flight, and the four sums add up in order. rows[k] is the
- * k-th partial's index. Returns the sum of weights; o has this lane's HD / 64
- * elements, complete in sub 0. */
-template <int HD, class At>
-__device__ __forceinline__ float kv_join(const float * po, const float * pml, int n, At at, float * wts, float * acc, int sub,
+/* The join of one column's n partials by W waves: weights e^(m - M) in LDS, then
+ * each wave adds every W-th row with eight of them in flight, and the waves' sums
+ * add up in order. at(k) is the k-th partial's index. Returns the sum of weights;
+ * o has this lane's HD / 64 elements, complete in wave 0. */
+template <int HD, int W, class At>
+__device__ __forceinline__ float kv_join(const float * po, const float * pml, int n, At at, float * wts, float * acc, int wave,
                                          int lane, float (&o)[HD / 64]) {
     constexpr int E = HD / 64;
     typedef float fe __attribute__((ext_vector_type(E)));
@@ -397,50 +515,49 @@ __device__ __forceinline__ float kv_join(const float * po, const float * pml, in
     for (int k = lane; k < n; k += 64) {
         const float m = pml[2 * at(k)], l = pml[2 * at(k) + 1], f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
         L += m == -INFINITY ? l : f * l;
-        if (sub == 0) wts[k] = f;
+        if (wave == 0) wts[k] = f;
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) L += __shfl_xor(L, s, 64);
     __syncthreads();
     fe sum = (fe) 0.0f;
-    for (int k0 = sub; k0 < n; k0 += 32) {
+    for (int k0 = wave; k0 < n; k0 += 8 * W) {
         fe v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = *(const fe *) (po + at(min(k0 + 4 * j, n - 1)) * HD + E * lane);
+        for (int j = 0; j < 8; j++) v[j] = *(const fe *) (po + at(min(k0 + W * j, n - 1)) * HD + E * lane);
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (k0 + 4 * j < n) sum += wts[k0 + 4 * j] * v[j];
+            if (k0 + W * j < n) sum += wts[k0 + W * j] * v[j];
     }
-    if (sub) *(fe *) (acc + (sub - 1) * HD + E * lane) = sum;
+    if (wave) *(fe *) (acc + (wave - 1) * HD + E * lane) = sum;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 3; j++) sum += *(const fe *) (acc + j * HD + E * lane);
+    for (int j = 0; j < W - 1; j++) sum += *(const fe *) (acc + j * HD + E * lane);
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = sum[e];
     return L;
 }
 
-/* Joins the partial results of one (sequence, kv head), in the order of its
- * pages: its first share wrote slot 1, the later ones slot 0. Four waves a
- * column. */
+/* Joins the partial results of one column of a (sequence, kv head), in the order
+ * of its pages: its first share wrote slot 1, the later ones slot 0. */
 template <int HD>
-__global__ __launch_bounds__(1024) void kv_flat_join_kernel(const KvFlat A) {
-    __shared__ float wts[4][kKvFlatMost];
-    __shared__ __attribute__((aligned(16))) float acc[4][3 * HD];
-    const int i = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = wave >> 2, sub = wave & 3;
+__global__ __launch_bounds__(512) void kv_flat_join_kernel(const KvFlat A) {
+    __shared__ float wts[kKvFlatMost];
+    __shared__ __attribute__((aligned(16))) float acc[7 * HD];
+    const int i = blockIdx.x, h = blockIdx.y, c = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int kvh = A.c.kv_heads, G = A.q.heads / kvh;
     const int before = A.pre[i], all = A.pre[i + 1] - before, n = all - kKvItem, share = A.pre[A.b.nseq + 1];
     if (all == 0) return;
     const int a = before * kvh + h * all, w0 = a / share, w1 = (a + n - 1) / share;
     if (w0 == w1) return;
     const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
-    const int cc = min(col, s.count * G - 1);
+    if (c >= s.count * G) return;
     float o[HD / 64];
-    const float L = kv_join<HD>(A.po, A.pml, w1 - w0 + 1, [&](int k) { return (2 * (size_t) (w0 + k) + (k == 0)) * 4 + cc; },
-                                wts[col], acc[col], sub, lane, o);
-    if (sub || col != cc) return;
+    const float L = kv_join<HD, 8>(A.po, A.pml, w1 - w0 + 1, [&](int k) { return (2 * (size_t) (w0 + k) + (k == 0)) * 4 + c; },
+                                   wts, acc, wave, lane, o);
+    if (wave) return;
 #pragma unroll
-    for (int e = 0; e < HD / 64; e++) kv_write(A.q, s.row + cc / G, h * G + cc % G, HD, HD / 64 * lane + e, o[e], L);
+    for (int e = 0; e < HD / 64; e++) kv_write(A.q, s.row + c / G, h * G + c % G, HD, HD / 64 * lane + e, o[e], L);
 }
 
 /* -------------------------------------------------------------- many columns
@@ -639,8 +756,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) mp = fmaxf(mp, x[t][e]);
-        mp = fmaxf(mp, __shfl_xor(mp, 16, 64));
-        mp = fmaxf(mp, __shfl_xor(mp, 32, 64));
+        mp = kv_rows_max(mp);
         if (__any(mp > m + kKvLag)) {
             const float mn = fmaxf(m, mp);
             const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -685,8 +801,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
             l = vscale;
         }
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = kv_rows_sum(l);
     if (qbad) l = __uint_as_float(0x7fc00000u);
     if (wfirst + c16 >= ncol) return;
     if (A.nsplit == 1) {
@@ -725,7 +840,7 @@ __global__ __launch_bounds__(1024) void kv_tile_join_kernel(const KvTile A, int 
     const int cc = min(col0 + c, ncol - 1);
     const size_t row = (((size_t) blockIdx.x * kvh + h) * cols + (cc - col0)) * A.nsplit;
     float o[HD / 64];
-    const float L = kv_join<HD>(A.po, A.pml, n, [&](int k) { return row + k; }, wts[col], acc[col], sub, lane, o);
+    const float L = kv_join<HD, 4>(A.po, A.pml, n, [&](int k) { return row + k; }, wts[col], acc[col], sub, lane, o);
     if (sub || cc != col0 + c) return;
     const int tok = cc / G;
 #pragma unroll
@@ -735,13 +850,13 @@ __global__ __launch_bounds__(1024) void kv_tile_join_kernel(const KvTile A, int 
 /* -------------------------------------------------------------------- host */
 
 struct KvPlan {
-    int flat;                 /* the few-column kernel */
+    int flat;                 /* the few-column kernel: 1 shares, 2 whole kv heads */
     int groups, least;        /* its workgroups and least share */
     int wq, tiles, nsplit;    /* the many-column kernel's */
     size_t pre, po, pml, bytes;
 };
 
-KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads) {
+KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads, int window) {
     KvPlan p = {};
     const int G = heads / c->kv_heads, max_q = b->qstart ? (b->max_q < b->ntok ? b->max_q : b->ntok) : 1;
     const long cols = (long) (max_q > 0 ? max_q : 1) * G, hd = c->head_dim;
@@ -750,7 +865,9 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += (bytes + 255) & ~(size_t) 255; return o; };
     if (cols <= 4) {
-        p.flat = 1;
+        /* up to kKvWhole pages a sequence: a workgroup each, nothing to join */
+        const long seen = window > 0 && (window + kKvPage - 2) / kKvPage + 1 < pages ? (window + kKvPage - 2) / kKvPage + 1 : pages;
+        p.flat = seen <= kKvWhole ? 2 : 1;
         const long most = 2 * cu_count() < kKvFlatMost ? 2 * cu_count() : kKvFlatMost, all = pages * b->nseq * c->kv_heads;
         p.groups = (int) (all < 1 ? 1 : (all < most ? all : most));
         p.least = 1;
@@ -786,7 +903,7 @@ extern "C" {
 size_t sparkmv_kv_attend_work(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, int heads) {
     if (kv_check_cache(cache) || kv_check_batch(batch) || heads < 1 || heads % cache->kv_heads) return 0;
     if (batch->nseq == 0 || batch->ntok == 0) return 0;
-    return kv_plan(cache, batch, heads).bytes;
+    return kv_plan(cache, batch, heads, 0).bytes;
 }
 
 int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_query * query,
@@ -815,7 +932,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
                   cache->kv_heads);
         return -1;
     }
-    const KvPlan p = kv_plan(cache, batch, q.heads);
+    const KvPlan p = kv_plan(cache, batch, q.heads, q.window);
     if (p.bytes && (!q.work || !kv_aligned(q.work, 256) || q.work_bytes < p.bytes)) {
         set_error("attention needs %zu bytes of 256-byte aligned workspace, not %zu", p.bytes, q.work ? q.work_bytes : 0);
         return -1;
@@ -829,17 +946,29 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
         f.b.max_q = max_q;
         f.least = p.least;
         f.pre = (int *) (mem + p.pre); f.po = (float *) (mem + p.po); f.pml = (float *) (mem + p.pml);
-        const dim3 grid((unsigned) p.groups), join((unsigned) batch->nseq, (unsigned) cache->kv_heads);
-        const uint32_t lds = ((uint32_t) batch->nseq + 1) * 4;
+        const dim3 join((unsigned) batch->nseq, (unsigned) cache->kv_heads, (unsigned) (max_q * (q.heads / cache->kv_heads)));
+        const uint32_t pre = batch->nseq > 64 ? ((uint32_t) batch->nseq + 1) * 4 : 0;
+#define KV_FLAT_N(H, W, GRID, LDS)                                                                                   \
+    do {                                                                                                             \
+        static LdsAllowed allowed;                                                                                   \
+        if (lds_allow(allowed, (const void *) kv_flat_kernel<H, W>, LDS + 1024, "LDS opt-in for the kv attention"))  \
+            return -1;                                                                                               \
+        hipLaunchKernelGGL((kv_flat_kernel<H, W>), dim3((unsigned) (GRID)), dim3(64 * W), LDS, s, f);                \
+    } while (0)
 #define KV_FLAT(H)                                                                                                   \
     do {                                                                                                             \
-        hipLaunchKernelGGL(kv_flat_kernel<H>, grid, dim3(256), lds, s, f);                                           \
-        hipLaunchKernelGGL(kv_flat_join_kernel<H>, join, dim3(1024), 0, s, f);                                       \
+        if (p.flat == 2) {                                                                                           \
+            KV_FLAT_N(H, 8, batch->nseq * cache->kv_heads, kv_flat_lds(H, 8));                                       \
+        } else {                                                                                                     \
+            KV_FLAT_N(H, 4, p.groups, kv_flat_lds(H, 4) + pre);                                                      \
+            hipLaunchKernelGGL(kv_flat_join_kernel<H>, join, dim3(512), 0, s, f);                                    \
+        }                                                                                                            \
     } while (0)
         if (hd == 64) KV_FLAT(64);
         else if (hd == 128) KV_FLAT(128);
         else KV_FLAT(256);
 #undef KV_FLAT
+#undef KV_FLAT_N
         return kv_check_launch("kv attention launch");
     }
     KvTile t;
