@@ -47,6 +47,18 @@ template <int CTRL>
 __device__ __forceinline__ float kv_quad(float v) { return __int_as_float(kv_quad<CTRL>(__float_as_int(v))); }
 constexpr int kKvXor1 = 0xb1, kKvXor2 = 0x4e;   /* quad permutations: lanes 1 0 3 2, 2 3 0 1 */
 
+/* the largest of a wave, in each lane */
+__device__ __forceinline__ uint32_t kv_wave_max(uint32_t v) {
+    v = max(v, (uint32_t) kv_quad<kKvXor1>((int) v));
+    v = max(v, (uint32_t) kv_quad<kKvXor2>((int) v));
+    v = max(v, (uint32_t) kv_quad<0x141>((int) v));   /* lane 7 - i of eight */
+    v = max(v, (uint32_t) kv_quad<0x140>((int) v));   /* lane 15 - i of sixteen */
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t) a[0], (uint32_t) a[1]);
+    a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t) a[0], (uint32_t) a[1]);
+}
+
 /* the largest, or the sum, of the four lanes 16 apart, in each of them */
 __device__ __forceinline__ float kv_rows_max(float v) {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -102,14 +114,25 @@ __device__ __forceinline__ int kv_q_exponent(const float (&x)[NC][16], bool & ba
     return ex;
 }
 
-/* out[row][head][d] = o / l, gated; no weight at all gives 0 */
-__device__ __forceinline__ void kv_write(const sparkmv_kv_query & q, int row, int head, int hd, int d, float o, float l) {
+/* out[row][head][d ..] = o / l, gated, N neighbours; no weight at all gives 0 */
+template <int N>
+__device__ __forceinline__ void kv_write(const sparkmv_kv_query & q, int row, int head, int hd, int d, const float * o, float l) {
+    typedef float fn __attribute__((ext_vector_type(N)));
+    typedef uint16_t hn __attribute__((ext_vector_type(N)));
     float f = l == 0.0f ? 0.0f : 1.0f / l;
     if (q.gate) f *= 1.0f / (1.0f + expf(-q.gate[(size_t) row * q.ldg + head]));
-    const float v = l == 0.0f ? 0.0f : o * f;
     const size_t at = (size_t) row * q.ldo + (size_t) head * hd + d;
-    if (q.out_dtype == SPARKMV_X_F32) ((float *) q.out)[at] = v;
-    else ((uint16_t *) q.out)[at] = kv_bf16(v);
+    fn v;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = l == 0.0f ? 0.0f : o[i] * f;
+    if (q.out_dtype == SPARKMV_X_F32) {
+        *(fn *) ((float *) q.out + at) = v;
+    } else {
+        hn w;
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = kv_bf16(v[i]);
+        *(hn *) ((uint16_t *) q.out + at) = w;
+    }
 }
 
 /* ------------------------------------------------------------- few columns
@@ -153,6 +176,7 @@ constexpr int kv_flat_lds(int hd, int waves) { return waves * 16 * (hd + 4) * 4 
 template <int HD, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void kv_flat_kernel(const KvFlat A) {
     constexpr int NC = HD / 64, ND = HD / 16, NT = 64 * WAVES, E = HD / 64, LO = HD + 4;
+    constexpr int V = WAVES == 8 ? 2 : 4;   /* elements a thread at the end */
     constexpr bool WHOLE = WAVES == 8;
     extern __shared__ __attribute__((aligned(16))) uint8_t ldyn[];
     float * lo = (float *) ldyn;                      /* [WAVES][16][LO]: a wave's output, digit by digit */
@@ -335,8 +359,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_flat_kernel(const KvFlat A) 
 #pragma unroll
             for (int e = 0; e < E; e++) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
             /* non-negative floats, a NaN above the infinities, order as integers do */
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) big = max(big, (uint32_t) __shfl_xor((int) big, o, 64));
+            big = kv_wave_max(big);
             const bool bad = big >= 0x7f800000u;
             int ex = 0;
             (void) frexpf(__uint_as_float(bad ? 0u : big), &ex);
@@ -469,24 +492,31 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_flat_kernel(const KvFlat A) 
         __syncthreads();
         const bool whole = WHOLE || seg == n;
         const size_t at = 2 * (size_t) blockIdx.x + (off == 0 ? 1 : 0);
-        for (int k = tid; k < ncol * HD; k += NT) {
-            const int cc = k / HD, d = k - cc * HD;
-            float M = lm[0][cc];
+        for (int k = tid; k < ncol * (HD / V); k += NT) {
+            const int cc = k / (HD / V), d = V * (k % (HD / V));
+            float M = lm[0][cc], L = 0.0f, v[V];
 #pragma unroll
             for (int w = 1; w < WAVES; w++) M = fmaxf(M, lm[w][cc]);
-            float L = 0.0f, v = 0.0f;
-#pragma unroll 1
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] = 0.0f;
+#pragma unroll 4
             for (int w = 0; w < WAVES; w++) {
-                const float * p = lo + (w * 16 + 4 * cc) * LO + d;
+                typedef float fv __attribute__((ext_vector_type(V)));
+                fv p[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[i] = *(const fv *) (lo + (w * 16 + 4 * cc + i) * LO + d);
                 const float r = lm[w][cc] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[w][cc] - M);
                 L += lm[w][cc] == -INFINITY ? ll[w][cc] : r * ll[w][cc];
                 /* digits 2^24 .. 2^0, over the weight's 2^30 */
-                v += r * (((p[3 * LO] * 0x1p-30f + p[2 * LO] * 0x1p-22f) + p[LO] * 0x1p-14f) + p[0] * 0x1p-6f);
+#pragma unroll
+                for (int e = 0; e < V; e++) v[e] += r * (((p[3][e] * 0x1p-30f + p[2][e] * 0x1p-22f) + p[1][e] * 0x1p-14f) + p[0][e] * 0x1p-6f);
             }
             if (whole) {
-                kv_write(A.q, s.row + cc / G, h * G + cc % G, HD, d, v, L);
+                kv_write<V>(A.q, s.row + cc / G, h * G + cc % G, HD, d, v, L);
             } else {
-                A.po[(at * 4 + cc) * HD + d] = v;
+                float * to = A.po + (at * 4 + cc) * HD + d;
+#pragma unroll
+                for (int e = 0; e < V; e++) to[e] = v[e];
                 if (d == 0) {
                     A.pml[(at * 4 + cc) * 2] = M;
                     A.pml[(at * 4 + cc) * 2 + 1] = L;
@@ -556,8 +586,7 @@ __global__ __launch_bounds__(512) void kv_flat_join_kernel(const KvFlat A) {
     const float L = kv_join<HD, 8>(A.po, A.pml, w1 - w0 + 1, [&](int k) { return (2 * (size_t) (w0 + k) + (k == 0)) * 4 + c; },
                                    wts, acc, wave, lane, o);
     if (wave) return;
-#pragma unroll
-    for (int e = 0; e < HD / 64; e++) kv_write(A.q, s.row + c / G, h * G + c % G, HD, HD / 64 * lane + e, o[e], L);
+    kv_write<HD / 64>(A.q, s.row + c / G, h * G + c % G, HD, HD / 64 * lane, o, L);
 }
 
 /* -------------------------------------------------------------- many columns
@@ -806,9 +835,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
     if (wfirst + c16 >= ncol) return;
     if (A.nsplit == 1) {
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) kv_write(A.q, s.row + tok, head, HD, 16 * (ND * wd + d) + 4 * g + e, o[d][e], l);
+        for (int d = 0; d < ND; d++) {
+            const float v[4] = {o[d][0], o[d][1], o[d][2], o[d][3]};
+            kv_write<4>(A.q, s.row + tok, head, HD, 16 * (ND * wd + d) + 4 * g, v, l);
+        }
         return;
     }
     const size_t at = (((size_t) blockIdx.x * kvh + h) * (16 * WQ) + 16 * wq + c16) * A.nsplit + blockIdx.z;
@@ -843,8 +873,7 @@ __global__ __launch_bounds__(1024) void kv_tile_join_kernel(const KvTile A, int 
     const float L = kv_join<HD, 4>(A.po, A.pml, n, [&](int k) { return row + k; }, wts[col], acc[col], sub, lane, o);
     if (sub || cc != col0 + c) return;
     const int tok = cc / G;
-#pragma unroll
-    for (int e = 0; e < HD / 64; e++) kv_write(A.q, s.row + tok, h * G + cc - tok * G, HD, HD / 64 * lane + e, o[e], L);
+    kv_write<HD / 64>(A.q, s.row + tok, h * G + cc - tok * G, HD, HD / 64 * lane, o, L);
 }
 
 /* -------------------------------------------------------------------- host */
