@@ -337,6 +337,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_flat_kernel(const KvFlat A) 
             }
             there = __ballot(have);
             fetch_k(0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto begin_v = [&]() {
             const auto p = page_at(A.c.v, 0);
 #pragma unroll
             for (int d = 0; d < ND; d++) vr[d] = (kv_i4) __builtin_amdgcn_raw_buffer_load_b128(p, vlane, d * 256, 0);
@@ -381,6 +384,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_flat_kernel(const KvFlat A) 
                 lbad[wave] = bad ? __uint_as_float(0x7fc00000u) : 0.0f;
             }
         }
+        if (wave < seg) begin_v();
         __syncthreads();
         const float cs = lcs[col];
         float m = -INFINITY, l = 0.0f;
@@ -388,7 +392,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_flat_kernel(const KvFlat A) 
 #pragma unroll
         for (int d = 0; d < ND; d++) o[d] = kv_f4{0.f, 0.f, 0.f, 0.f};
         for (int base = wave; base < seg; base += 64 * WAVES) {
-            if (base > wave) begin(base);
+            if (base > wave) {
+                begin(base);
+                begin_v();
+            }
             for (int j = 0; j < count; j++) {
                 const int nx = min(j + 1, count - 1);
                 float a[4][4];
