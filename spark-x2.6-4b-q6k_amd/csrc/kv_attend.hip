@@ -857,14 +857,18 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
     }
 }
 
-/* Joins the splits of a tile: four waves a column, four columns at a time. */
+/* Joins the splits of a tile, a wave `each` columns one after another: lane k holds
+ * split k's m and l, and eight rows of HD elements are in flight. With four waves
+ * a column, as above, a chunk of 512 tokens in four splits took 36 us, not 12: most
+ * waves had one row. One column a wave where that gives fewer than eight
+ * workgroups a CU (three blocks of 8 tokens: 6.1 us, with four 12.7), else four. */
 constexpr int kKvSplits = 64;
 template <int HD>
-__global__ __launch_bounds__(1024) void kv_tile_join_kernel(const KvTile A, int cols) {
-    __shared__ float wts[4][kKvSplits];
-    __shared__ __attribute__((aligned(16))) float acc[4][3 * HD];
-    __shared__ int lfind[20];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = wave >> 2, sub = wave & 3;
+__global__ __launch_bounds__(256) void kv_tile_join_kernel(const KvTile A, int cols, int each) {
+    constexpr int E = HD / 64;
+    typedef float fe __attribute__((ext_vector_type(E)));
+    __shared__ int lfind[8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     const int kvh = A.c.kv_heads, G = A.q.heads / kvh, h = blockIdx.y;
     KvSeq s;
     int place;
@@ -872,15 +876,41 @@ __global__ __launch_bounds__(1024) void kv_tile_join_kernel(const KvTile A, int 
     const int ncol = s.count * G, col0 = place * cols, t0 = col0 / G, t1 = min(col0 + cols - 1, ncol - 1) / G + 1;
     int first;
     const int npages = kv_span(s, t0, t1, A.q.window, first), per = (npages + A.nsplit - 1) / A.nsplit, n = (npages + per - 1) / per;
-    const int c = 4 * (int) blockIdx.z + col;
-    if (col0 + 4 * (int) blockIdx.z >= ncol) return;
-    const int cc = min(col0 + c, ncol - 1);
-    const size_t row = (((size_t) blockIdx.x * kvh + h) * cols + (cc - col0)) * A.nsplit;
-    float o[HD / 64];
-    const float L = kv_join<HD, 4>(A.po, A.pml, n, [&](int k) { return row + k; }, wts[col], acc[col], sub, lane, o);
-    if (sub || cc != col0 + c) return;
-    const int tok = cc / G;
-    kv_write<HD / 64>(A.q, s.row + tok, h * G + cc - tok * G, HD, HD / 64 * lane, o, L);
+    for (int u = 0; u < each; u++) {
+        const int c = 4 * each * (int) blockIdx.z + each * wave + u, cc = col0 + c;
+        if (cc >= ncol) return;
+        const size_t row = (((size_t) blockIdx.x * kvh + h) * cols + c) * A.nsplit;
+        float m = -INFINITY, l = 0.0f;
+        if (lane < n) {
+            m = A.pml[2 * (row + lane)];
+            l = A.pml[2 * (row + lane) + 1];
+        }
+        const float * p = A.po + row * HD + E * lane;
+        fe v[8], sum = (fe) 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = *(const fe *) (p + (size_t) min(j, n - 1) * HD);
+        float M = m;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+        float L = m == -INFINITY ? l : f * l;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+        for (int k0 = 0; k0 < n; k0 += 8) {
+            if (k0) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = *(const fe *) (p + (size_t) min(k0 + j, n - 1) * HD);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (k0 + j < n) sum += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), k0 + j)) * v[j];
+        }
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = sum[e];
+        const int tok = cc / G;
+        kv_write<E>(A.q, s.row + tok, h * G + cc - tok * G, HD, E * lane, o, L);
+    }
 }
 
 /* -------------------------------------------------------------------- host */
@@ -1014,6 +1044,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     t.po = (float *) (mem + p.po); t.pml = (float *) (mem + p.pml);
     const dim3 grid((unsigned) p.tiles, (unsigned) cache->kv_heads, (unsigned) p.nsplit);
     const uint32_t lds = 4 * kKvPage * (uint32_t) hd;
+    const int each = (long) grid.x * grid.y * 4 * p.wq < 8 * cu_count() ? 1 : 4;
 #define KV_TILE(H, D, W)                                                                                             \
     do {                                                                                                             \
         static LdsAllowed allowed;                                                                                   \
@@ -1032,7 +1063,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
         else if (p.wq == 2) KV_TILE_D(H, 2);                                                                         \
         else KV_TILE_D(H, 4);                                                                                        \
         if (p.nsplit > 1)                                                                                            \
-            hipLaunchKernelGGL(kv_tile_join_kernel<H>, dim3(grid.x, grid.y, 4 * p.wq), dim3(1024), 0, s, t, 16 * p.wq); \
+            hipLaunchKernelGGL(kv_tile_join_kernel<H>, dim3(grid.x, grid.y, 4 * p.wq / each), dim3(256), 0, s, t, 16 * p.wq, each); \
     } while (0)
     if (hd == 64) KV_TILE_W(64);
     else if (hd == 128) KV_TILE_W(128);
