@@ -622,6 +622,32 @@ size_t sparkmv_kv_attend_work(const sparkmv_kv_cache * cache, const sparkmv_kv_b
 int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_query * query,
                       void * stream);
 
+/* ---- the forward over the paged cache: several sequences, one read of the weights ----
+ * A model's paged cache beside its f32 one (which stays as it is): npages pages
+ * in each layer's pools, one page table of nslots x max_pages (at most 131072
+ * positions a slot) for all layers. Made once. */
+int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages);
+/* Slot's pages: entry j for positions 64 j .. 64 j + 63, the n given ones, -1
+ * for none and in the rest. The host array is read before the call returns (it
+ * waits for the stream's earlier work). */
+int sparkmv_model_set_pages(void * model, int slot, const int * pages, int n, void * stream);
+/* Layer's cache, for sparkmv_kv_read and inspection. */
+int sparkmv_model_paged_cache(void * model, int layer, sparkmv_kv_cache * out);
+/* One step of up to 16 sequences in different slots: count[i] tokens at positions
+ * pos[i] .. of slot[i], tokens in the order of the sequences, at most 512 in all
+ * (one each: a decode step; more: prompt chunks, verified blocks). Each matrix is
+ * read once for all of them: up to 16 tokens through the batched GEMV, more
+ * through the prefill GEMM, as sparkmv_model_forward_batch. Keys and values enter
+ * the paged cache (sparkmv_kv_append) and attention runs over it
+ * (sparkmv_kv_attend); the caller keeps the lengths and may go back to an earlier
+ * position at any time. logits, when non-null: with every 0 a row [vocab] for
+ * each sequence's last token, else one for each token (at most 16). Host arrays
+ * are read before the call returns. A step larger than those before it
+ * (re)allocates buffers after a device synchronization. Layer-input capture and
+ * the cached length are of the f32 cache and not touched. */
+int sparkmv_model_paged_step(void * model, const uint32_t * tokens, int nseq, const int * slot, const int * pos,
+                             const int * count, int every, float * logits, void * stream);
+
 /* ---- log probabilities ----
  * Beside sparkmv_argmax: for each of `rows` rows of n logits (x_dtype, row
  * stride ld), with lse = log sum e^x: logprob[r] = x[tokens[r]] - lse,

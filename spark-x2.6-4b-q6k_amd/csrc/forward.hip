@@ -34,6 +34,7 @@
  */
 #include "act.h"
 #include "kq.h"
+#include "kv.h"
 #include "model.h"
 #include "prefill.h"
 #include "vq.h"
@@ -708,6 +709,12 @@ __global__ void fw_q8_0_rows_dev_kernel(const uint8_t * blocks, int cols, const 
     _Float16 d;
     __builtin_memcpy(&d, b, 2);
     out[(size_t) t * cols + i] = (float) d * (float) (int8_t) b[2 + (i & 31)];
+}
+
+/* Rows of a paged step that get logits: out row i = h row idx[i] (device). */
+__global__ void fw_pick_rows_kernel(const float * h, const int * idx, int n, float * out) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) out[(size_t) blockIdx.y * n + i] = h[(size_t) idx[blockIdx.y] * n + i];
 }
 
 /* Attention of token t = blockIdx.y (query rotated in qkv, every key of its
@@ -1520,6 +1527,16 @@ struct Model {
     std::vector<int> cap_slot;
     int cap_n = 0;
     float * cap = nullptr;
+    /* the paged cache of several sequences (sparkmv_model_paged), one
+     * allocation: each layer's pools, one page table, rope tables, and a step's
+     * tokens, slots, positions, row starts and picked rows */
+    void * pmem = nullptr;
+    std::vector<sparkmv_kv_cache> paged;
+    int * ptable = nullptr, * pstep = nullptr;
+    float * prope[2] = {nullptr, nullptr};   /* full, sliding */
+    /* attention's workspace, grown by a step that needs more */
+    void * pwork = nullptr;
+    size_t pwork_bytes = 0;
 };
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t) 255; }
@@ -1772,6 +1789,8 @@ void sparkmv_model_destroy(void * model) {
     if (m->mem) (void) hipFree(m->mem);
     if (m->vmem) (void) hipFree(m->vmem);
     if (m->cap) (void) hipFree(m->cap);
+    if (m->pmem) (void) hipFree(m->pmem);
+    if (m->pwork) (void) hipFree(m->pwork);
     for (void * p : m->owned) (void) hipFree(p);
     delete m;
 }
@@ -2213,9 +2232,238 @@ int prompt(Model * m, int N, int pos, float * logits, hipStream_t s) {
     return kq_gemv_launch(8, m->head_blocks, c.vocab, c.hidden, xin, b16 ? 0 : 1, c.hidden, 1, logits, c.vocab, 0, s);
 }
 
+constexpr int kPagedSeq = kMaxCols;   /* sequences, and rows of logits, of a paged step */
+
+/* A paged step: b.ntok tokens (in m->vtok) of b.nseq sequences through every
+ * layer, their keys and values into the paged cache and attention over it; then
+ * the final norm and the head of the nrow rows whose numbers are at pick. */
+int paged_step(Model * m, const sparkmv_kv_batch & b, const int * pick, int nrow, float * logits, hipStream_t s) {
+    const sparkmv_model_cfg & c = m->c;
+    const bool b16 = c.x_dtype == SPARKMV_X_BF16;
+    const int qd = c.heads * c.head_dim, kvd = c.kv_heads * c.head_dim, hd = c.head_dim, ldq = qd + 2 * kvd, N = b.ntok;
+    if (m->head_kind == 0) {
+        hipLaunchKernelGGL(fw_fill_kernel, dim3((N * c.hidden + 255) / 256), dim3(256), 0, s, m->vh, N * c.hidden, 0.0f);
+        if (check_launch("fill launch")) return -1;
+        const Layout L = make_layout(c.dim, c.nc, c.vocab, c.hidden, c.v3);
+        for (int st = 0; st < c.nstages; st++)
+            if (vq_row_dequant_dev_launch(m->head_stages[st], L, m->vtok, m->vh, s, N, (size_t) c.hidden)) return -1;
+    } else {
+        hipLaunchKernelGGL(fw_q8_0_rows_dev_kernel, dim3((c.hidden + 255) / 256, N), dim3(256), 0, s,
+                           (const uint8_t *) m->head_blocks, c.hidden, (const int *) m->vtok, m->vh);
+        if (check_launch("embedding launch")) return -1;
+    }
+    const void * xin = b16 ? (const void *) m->vxn16 : (const void *) m->vxn;
+    for (int li = 0; li < c.layers; li++) {
+        const sparkmv_model_layer & L = m->layers[li];
+        const bool full = L.full != 0;
+        if (rmsnorm(*m, m->vh, L.in_norm, s, N, m->vxn, m->vxn16)) return -1;
+        if (N <= kMaxCols) {
+            if (gemv2(*m, L.qkv, ldq, m->vqkv, L.attn_gate, c.heads, m->vg, c.hidden, xin, s, N, ldq)) return -1;
+        } else {
+            if (mat_n(*m, L.qkv, ldq, c.hidden, xin, m->vqkv, 0, s, N, ldq)) return -1;
+            if (mat_n(*m, L.attn_gate, c.heads, c.hidden, xin, m->vg, 0, s, N, ldq)) return -1;
+        }
+        sparkmv_kv_new kn;
+        memset(&kn, 0, sizeof kn);
+        kn.q = m->vqkv; kn.k = m->vqkv + qd; kn.v = m->vqkv + qd + kvd; kn.q_out = m->vqkv;
+        kn.ldq = kn.ldk = kn.ldv = kn.ldqo = ldq;
+        kn.x_dtype = SPARKMV_X_F32; kn.heads = c.heads;
+        kn.rope_dim = rope_dim(hd, full ? c.rope_full_partial : c.rope_slide_partial);
+        kn.rope = kn.rope_dim ? m->prope[full ? 0 : 1] : nullptr;
+        kn.rope_rows = m->paged[li].max_pages * kKvPage;
+        if (sparkmv_kv_append(&m->paged[li], &b, &kn, s)) return -1;
+        sparkmv_kv_query q;
+        memset(&q, 0, sizeof q);
+        q.q = m->vqkv; q.ldq = ldq; q.q_dtype = SPARKMV_X_F32; q.heads = c.heads;
+        q.scale = 1.0f / sqrtf((float) hd); q.window = full ? 0 : c.sliding_window;
+        q.gate = m->vg; q.ldg = ldq;
+        q.out = b16 ? (void *) m->vattn16 : (void *) m->vattn; q.ldo = qd;
+        q.out_dtype = b16 ? SPARKMV_X_BF16 : SPARKMV_X_F32;
+        q.work = m->pwork; q.work_bytes = m->pwork_bytes;
+        if (sparkmv_kv_attend(&m->paged[li], &b, &q, s)) return -1;
+        if (mat_n(*m, L.out, c.hidden, qd, b16 ? (const void *) m->vattn16 : (const void *) m->vattn, m->vh, 1, s, N, c.hidden))
+            return -1;
+        if (rmsnorm(*m, m->vh, L.post_norm, s, N, m->vxn, m->vxn16)) return -1;
+        if (N <= kMaxCols) {
+            if (gate_up_act_n(*m, L.gate, L.up, c.intermediate, c.hidden, xin, m->vmg, m->vmu, m->vact,
+                              b16 ? m->vact16 : nullptr, s, N))
+                return -1;
+        } else {
+            if (mat_n(*m, L.gate, c.intermediate, c.hidden, xin, m->vmg, 0, s, N, c.intermediate)) return -1;
+            if (mat_n(*m, L.up, c.intermediate, c.hidden, xin, m->vmu, 0, s, N, c.intermediate)) return -1;
+            hipLaunchKernelGGL(fw_gelu_mul_kernel, dim3((N * c.intermediate / 4 + 255) / 256 + 1), dim3(256), 0, s,
+                               m->vmg, m->vmu, b16 ? nullptr : m->vact, b16 ? m->vact16 : nullptr, N * c.intermediate);
+            if (check_launch("gelu launch")) return -1;
+        }
+        if (mat_n(*m, L.down, c.hidden, c.intermediate, b16 ? (const void *) m->vact16 : (const void *) m->vact, m->vh, 1, s, N,
+                  c.hidden))
+            return -1;
+    }
+    if (!logits) return 0;
+    /* the picked rows, normalised where they are put */
+    hipLaunchKernelGGL(fw_pick_rows_kernel, dim3((c.hidden + 255) / 256, nrow), dim3(256), 0, s, m->vh, pick, c.hidden, m->vxn);
+    if (check_launch("row pick launch")) return -1;
+    if (rmsnorm(*m, m->vxn, m->final_norm, s, nrow, m->vxn, m->vxn16)) return -1;
+    if (m->head_kind == 0) return gemv(*m, m->head_stages, c.vocab, c.hidden, xin, logits, 0, s, nrow, c.vocab);
+    return kq_gemv_launch(8, m->head_blocks, c.vocab, c.hidden, xin, b16 ? 0 : 1, c.hidden, nrow, logits, c.vocab, 0, s);
+}
+
 }  // namespace
 
 extern "C" {
+
+int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
+    Model * m = (Model *) model;
+    if (!m) { set_error("model is null"); return -1; }
+    if (npages < 1 || nslots < 1 || max_pages < 1) {
+        set_error("a paged cache of %d pages, %d slots of %d pages", npages, nslots, max_pages);
+        return -1;
+    }
+    if (m->pmem) { set_error("the model's paged cache is there already"); return -1; }
+    const sparkmv_model_cfg & c = m->c;
+    /* the interface's limit on positions, as for max_ctx */
+    if (max_pages > 131072 / kKvPage) { set_error("%d pages of %d positions are above 131072", max_pages, kKvPage); return -1; }
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t o = off; off += align256(bytes); return o; };
+    const size_t codes = (size_t) npages * c.kv_heads * kKvPage * c.head_dim, scales = (size_t) npages * c.kv_heads * 4;
+    std::vector<size_t> at((size_t) c.layers * 4);
+    for (int li = 0; li < c.layers; li++) {
+        at[4 * li] = take(codes);
+        at[4 * li + 1] = take(codes);
+        at[4 * li + 2] = take(scales);
+        at[4 * li + 3] = take(scales);
+    }
+    const size_t o_table = take((size_t) nslots * max_pages * 4), o_step = take((3 * kPagedSeq + 1 + kPagedSeq) * 4);
+    const int dims[2] = {rope_dim(c.head_dim, c.rope_full_partial), rope_dim(c.head_dim, c.rope_slide_partial)};
+    for (int d : dims)
+        if (d % 2) { set_error("a paged cache takes an even rotated width, not %d", d); return -1; }
+    const double theta[2] = {c.rope_full_theta, c.rope_slide_theta};
+    size_t o_rope[2];
+    for (int r = 0; r < 2; r++) o_rope[r] = take((size_t) max_pages * kKvPage * dims[r] * 4);
+    void * mem = nullptr;
+    hipError_t e = hipMalloc(&mem, off);
+    if (e != hipSuccess) return fail_hip("paged cache", e);
+    uint8_t * b = (uint8_t *) mem;
+    /* no slot has a page yet; pages' codes and scales are written before they are read */
+    e = hipMemset(b + o_table, 0xff, (size_t) nslots * max_pages * 4);
+    int rc = e == hipSuccess ? 0 : fail_hip("page table", e);
+    for (int r = 0; r < 2 && !rc; r++)
+        if (dims[r]) rc = sparkmv_rope_table((float *) (b + o_rope[r]), max_pages * kKvPage, dims[r], theta[r], nullptr);
+    if (!rc) {
+        e = hipDeviceSynchronize();
+        if (e != hipSuccess) rc = fail_hip("paged cache", e);
+    }
+    if (rc) {
+        (void) hipFree(mem);
+        return -1;
+    }
+    m->pmem = mem;
+    m->ptable = (int *) (b + o_table);
+    m->pstep = (int *) (b + o_step);
+    for (int r = 0; r < 2; r++) m->prope[r] = (float *) (b + o_rope[r]);
+    m->paged.resize((size_t) c.layers);
+    for (int li = 0; li < c.layers; li++) {
+        sparkmv_kv_cache & k = m->paged[li];
+        memset(&k, 0, sizeof k);
+        k.kv_heads = c.kv_heads; k.head_dim = c.head_dim; k.npages = npages; k.nslots = nslots; k.max_pages = max_pages;
+        k.k = (int8_t *) (b + at[4 * li]); k.v = (int8_t *) (b + at[4 * li + 1]);
+        k.k_scale = (float *) (b + at[4 * li + 2]); k.v_scale = (float *) (b + at[4 * li + 3]);
+        k.pages = m->ptable;
+    }
+    return 0;
+}
+
+int sparkmv_model_set_pages(void * model, int slot, const int * pages, int n, void * stream) {
+    Model * m = (Model *) model;
+    if (!m || (n > 0 && !pages)) { set_error("model or pages is null"); return -1; }
+    if (!m->pmem) { set_error("the model has no paged cache: call sparkmv_model_paged first"); return -1; }
+    const sparkmv_kv_cache & k = m->paged[0];
+    if (slot < 0 || slot >= k.nslots) { set_error("slot %d is outside 0..%d", slot, k.nslots - 1); return -1; }
+    if (n < 0 || n > k.max_pages) { set_error("%d pages are outside 0..%d", n, k.max_pages); return -1; }
+    std::vector<int> row((size_t) k.max_pages, -1);
+    for (int j = 0; j < n; j++) {
+        if (pages[j] < -1 || pages[j] >= k.npages) { set_error("page %d is outside 0..%d", pages[j], k.npages - 1); return -1; }
+        row[(size_t) j] = pages[j];
+    }
+    hipStream_t s = (hipStream_t) stream;
+    hipError_t e = hipMemcpyAsync(m->ptable + (size_t) slot * k.max_pages, row.data(), row.size() * 4, hipMemcpyHostToDevice, s);
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    return e == hipSuccess ? 0 : fail_hip("page table upload", e);
+}
+
+int sparkmv_model_paged_cache(void * model, int layer, sparkmv_kv_cache * out) {
+    Model * m = (Model *) model;
+    if (!m || !out) { set_error("model or output is null"); return -1; }
+    if (!m->pmem) { set_error("the model has no paged cache: call sparkmv_model_paged first"); return -1; }
+    if (layer < 0 || layer >= m->c.layers) { set_error("layer %d is outside 0..%d", layer, m->c.layers - 1); return -1; }
+    *out = m->paged[(size_t) layer];
+    return 0;
+}
+
+int sparkmv_model_paged_step(void * model, const uint32_t * tokens, int nseq, const int * slot, const int * pos,
+                             const int * count, int every, float * logits, void * stream) {
+    Model * m = (Model *) model;
+    if (!m || !tokens || !slot || !pos || !count) { set_error("model, tokens, slots, positions or counts is null"); return -1; }
+    if (!m->pmem) { set_error("the model has no paged cache: call sparkmv_model_paged first"); return -1; }
+    if (nseq < 1 || nseq > kPagedSeq) { set_error("a paged step holds 1..%d sequences, not %d", kPagedSeq, nseq); return -1; }
+    const sparkmv_kv_cache & k = m->paged[0];
+    int step[4 * kPagedSeq + 1], * sl = step, * ps = sl + kPagedSeq, * qs = ps + kPagedSeq, * pick = qs + kPagedSeq + 1;
+    int ntok = 0, max_q = 0, max_len = 0;
+    memset(step, 0, sizeof step);
+    for (int i = 0; i < nseq; i++) {
+        if (slot[i] < 0 || slot[i] >= k.nslots) { set_error("slot %d is outside 0..%d", slot[i], k.nslots - 1); return -1; }
+        for (int j = 0; j < i; j++)
+            if (slot[j] == slot[i]) { set_error("slot %d is in the step twice", slot[i]); return -1; }
+        if (count[i] < 1 || count[i] > kPromptMax - ntok) {
+            set_error("a paged step holds 1..%d tokens, each sequence one at least", kPromptMax);
+            return -1;
+        }
+        if (pos[i] < 0 || (long) pos[i] + count[i] > (long) k.max_pages * kKvPage) {
+            set_error("positions %d..%ld exceed the slot's %ld", pos[i], (long) pos[i] + count[i] - 1, (long) k.max_pages * kKvPage);
+            return -1;
+        }
+        sl[i] = slot[i];
+        ps[i] = pos[i];
+        qs[i] = ntok;
+        ntok += count[i];
+        qs[i + 1] = ntok;
+        if (!every) pick[i] = ntok - 1;
+        max_q = count[i] > max_q ? count[i] : max_q;
+        max_len = pos[i] + count[i] > max_len ? pos[i] + count[i] : max_len;
+    }
+    if (every && logits && ntok > kPagedSeq) { set_error("logits of every token take 1..%d tokens, not %d", kPagedSeq, ntok); return -1; }
+    if (every)
+        for (int t = 0; t < ntok && t < kPagedSeq; t++) pick[t] = t;
+    for (int t = 0; t < ntok; t++)
+        if ((long) tokens[t] >= m->c.vocab) { set_error("token %u is outside the vocabulary", tokens[t]); return -1; }
+    if (ready(m)) return -1;
+    sparkmv_kv_batch b;
+    memset(&b, 0, sizeof b);
+    b.nseq = nseq; b.ntok = ntok; b.max_q = max_q; b.max_len = max_len;
+    b.slot = m->pstep; b.pos = m->pstep + kPagedSeq; b.qstart = m->pstep + 2 * kPagedSeq;
+    const size_t need = sparkmv_kv_attend_work(&k, &b, m->c.heads);
+    if (!m->vmem || ntok > m->vcap || need > m->pwork_bytes) {
+        if (m->vmem || m->pwork) {
+            hipError_t e = hipDeviceSynchronize();
+            if (e != hipSuccess) return fail_hip("synchronize before larger buffers", e);
+        }
+        if (alloc_block(m, ntok)) return -1;
+        if (need > m->pwork_bytes) {
+            void * w = nullptr;
+            hipError_t e = hipMalloc(&w, need);
+            if (e != hipSuccess) return fail_hip("attention workspace", e);
+            if (m->pwork) (void) hipFree(m->pwork);
+            m->pwork = w;
+            m->pwork_bytes = need;
+        }
+    }
+    hipStream_t s = (hipStream_t) stream;
+    hipError_t e = hipMemcpyAsync(m->vtok, tokens, (size_t) ntok * sizeof(int), hipMemcpyHostToDevice, s);
+    if (e == hipSuccess) e = hipMemcpyAsync(m->pstep, step, sizeof step, hipMemcpyHostToDevice, s);
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    if (e != hipSuccess) return fail_hip("step upload", e);
+    return paged_step(m, b, m->pstep + 3 * kPagedSeq + 1, every ? ntok : nseq, logits, s);
+}
 
 int sparkmv_model_forward(void * model, uint32_t token, int pos, float * logits, void * stream) {
     Model * m = (Model *) model;

@@ -212,6 +212,11 @@ SIGNATURES = {
     "sparkmv_model_captured": (_I, [_P, _I, _PP]),
     "sparkmv_model_embed_row": (_I, [_P, ctypes.c_uint32, _P, _P]),
     "sparkmv_argmax": (_I, [_P, _I, _P, _P]),
+    "sparkmv_model_paged": (_I, [_P, _I, _I, _I]),
+    "sparkmv_model_set_pages": (_I, [_P, _I, ctypes.POINTER(_I), _I, _P]),
+    "sparkmv_model_paged_cache": (_I, [_P, _I, ctypes.POINTER(KvCache)]),
+    "sparkmv_model_paged_step": (_I, [_P, ctypes.POINTER(ctypes.c_uint32), _I, ctypes.POINTER(_I), ctypes.POINTER(_I),
+                                      ctypes.POINTER(_I), _I, _P, _P]),
     "sparkmv_rope_table": (_I, [_P, _I, _I, ctypes.c_double, _P]),
     "sparkmv_kv_append": (_I, [_P, _P, _P, _P]),
     "sparkmv_kv_read": (_I, [_P, _I, _P, _P, _I, _P, _P, _I, _P]),
@@ -733,6 +738,47 @@ class Model:
 
     def __len__(self):
         return lib().sparkmv_model_len(self.h)
+
+    def paged(self, npages, nslots, max_pages):
+        """Make the paged 8-bit cache of several sequences (sparkmv_model_paged),
+        beside the f32 cache of forward and verify."""
+        check(lib().sparkmv_model_paged(self.h, int(npages), int(nslots), int(max_pages)), "model paged")
+
+    def set_pages(self, slot, pages, stream=None):
+        """The slot's pages, in the order of their positions (64 each)."""
+        arr = (_I * max(1, len(pages)))(*[int(p) for p in pages])
+        check(lib().sparkmv_model_set_pages(self.h, int(slot), arr, len(pages), _stream_ptr(stream)), "model pages")
+
+    def paged_step(self, tokens, slots, pos, logits=None, every=False, stream=None):
+        """One step of several sequences: tokens[i] (a list) at positions pos[i] ..
+        of slots[i]. logits: device f32 [len(slots), vocab] for each sequence's
+        last token, or with every [tokens in all, vocab] (at most 16 rows)."""
+        flat = [int(t) for seq in tokens for t in seq]
+        n = len(slots)
+        if len(tokens) != n or len(pos) != n:
+            raise SparkmvError(f"model paged step: {len(tokens)} token lists and {len(pos)} positions for {n} slots")
+        if logits is not None:
+            torch = _torch()
+            _kv_flat("paged step logits", logits, (torch.float32,), (len(flat) if every else n, self.cfg["vocab"]), None)
+        ints = lambda v: (_I * max(1, len(v)))(*[int(x) for x in v])  # noqa: E731
+        check(lib().sparkmv_model_paged_step(self.h, (ctypes.c_uint32 * max(1, len(flat)))(*flat), n, ints(slots), ints(pos),
+                                             ints([len(t) for t in tokens]), int(bool(every)), _ptr(logits),
+                                             _stream_ptr(stream)), "model paged step")
+
+    def paged_read(self, layer, start, k_out, v_out, slot=None, stream=None):
+        """Cached positions of a layer as PagedKV.read gives them: start and slot
+        device int32, k_out and v_out [nseq, n, kv_heads, head_dim]."""
+        torch = _torch()
+        c = KvCache()
+        check(lib().sparkmv_model_paged_cache(self.h, int(layer), ctypes.byref(c)), "model paged cache")
+        _kv_flat("paged read start", start, (torch.int32,), (None,), None)
+        for t in (k_out, v_out):
+            _kv_flat("paged read", t, (k_out.dtype,), (start.shape[0], k_out.shape[1], c.kv_heads, c.head_dim), start.device)
+        if slot is not None:
+            _kv_flat("paged read slots", slot, (torch.int32,), (start.shape[0],), start.device)
+        check(lib().sparkmv_kv_read(ctypes.byref(c), start.shape[0], _ptr(slot), start.data_ptr(), k_out.shape[1],
+                                    k_out.data_ptr(), v_out.data_ptr(), X_F32 if k_out.dtype == torch.float32 else X_BF16,
+                                    _stream_ptr(stream)), "model paged read")
 
     def apply_profile(self, profile, artifact, gpu):
         n = lib().sparkmv_model_apply_profile(self.h, profile.h, artifact, gpu.encode())
