@@ -688,6 +688,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         }
         __syncthreads();
     };
+    /* a kilobyte of keys, 16 positions x 64 bytes, enters LDS as the matrix
+     * instruction's lanes take it (lane 16 g + position: 16 bytes): as it lies,
+     * sixteen lanes would read at a stride of 64 bytes, from a quarter of the banks */
+    const uint32_t klane = c16 * 64 + 16 * g;
     auto fetch = [&](int j, int b) {
         const size_t at = ((size_t) max(__builtin_amdgcn_readfirstlane(lid[j & (kKvIds - 1)]), 0) * kvh + h) * (size_t) HALF;
         const int8_t * kc = A.c.k + at, * vc = A.c.v + at;
@@ -695,7 +699,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
 #pragma unroll
         for (int k = 0; k < HALF / 4096; k++) {
             const int o = (4 * k + wave) * 1024;
-            __builtin_amdgcn_global_load_lds((const void *) (kc + o + 16 * lane), (lds_void *) (to + o), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const void *) (kc + o + klane), (lds_void *) (to + o), 16, 0, 0);
             __builtin_amdgcn_global_load_lds((const void *) (vc + o + 16 * lane), (lds_void *) (to + HALF + o), 16, 0, 0);
         }
     };
@@ -719,13 +723,15 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         for (int c = 0; c < NC; c++) kv_load16(A.q, at + 64 * c, x[c]);
         const int ex = kv_q_exponent<NC>(x, qbad);
         constexpr int B = D == 2 ? 14 : 30;
+        /* a negative scale turns the queries, so that scores grow with their sums */
+        const float sign = A.q.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 uint32_t y[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (uint32_t) (int) rintf(ldexpf(qbad ? 0.0f : x[c][4 * w + e], B - ex)) + BIAS;
+                for (int e = 0; e < 4; e++) y[e] = (uint32_t) (int) rintf(ldexpf(qbad ? 0.0f : x[c][4 * w + e] * sign, B - ex)) + BIAS;
 #pragma unroll
                 for (int d = 0; d < D; d++) {
                     const uint32_t b = D - 1 - d, sel = b | (b + 4) << 8 | 0x0c0c0000u;
@@ -733,7 +739,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
                     qd[d][c][w] = (int) ((lo2 | hi2 << 16) ^ (d ? 0x80808080u : 0u));
                 }
             }
-        cs = ldexpf(A.q.scale * kKvLog2e, ex - B);
+        cs = ldexpf(fabsf(A.q.scale) * kKvLog2e, ex - B);
     }
     /* the value of a product's digit sums */
     auto value = [&](const kv_i4 * a, int e) -> float {
@@ -756,10 +762,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         }
         const int p0 = (first + j) * kKvPage;
         if (!live || id < 0 || p0 > wpos_hi || p0 + kKvPage - 1 < wbeg_lo) continue;   /* uniform in the wave */
-        const uint8_t * kp = lbuf + (size_t) (j & 1) * 2 * HALF + 16 * g + 64 * c16;
+        const uint8_t * kp = lbuf + (size_t) (j & 1) * 2 * HALF + 16 * lane;
         const uint8_t * vp = lbuf + (size_t) (j & 1) * 2 * HALF + HALF + (g * HD + 16 * ND * wd + c16) * 16;
         float x[4][4];
-        const float f = cs * kscale;
+        float f = cs * kscale;   /* of the sums; a scale is not negative */
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             kv_i4 acc[D];
@@ -772,7 +778,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
                 for (int d = 0; d < D; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qd[d][c], acc[d], 0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[t][e] = value(acc, e) * f;
+            for (int e = 0; e < 4; e++) x[t][e] = value(acc, e);
         }
         if (p0 < wbeg_hi || p0 + kKvPage - 1 > wpos_lo || kscale != kscale) {
             bool any = false;
@@ -783,8 +789,9 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
                     const int p = p0 + 16 * t + 4 * g + e;
                     const bool seen = p >= beg_c && p <= pos_c;
                     any = any || seen;
-                    x[t][e] = seen && kscale == kscale ? x[t][e] : -INFINITY;
+                    x[t][e] = seen && kscale == kscale ? x[t][e] * f : -INFINITY;
                 }
+            f = 1.0f;
             if (any && kscale != kscale) l = kscale;   /* NaN to the end for a column that sees some of it */
         }
         float mp = -INFINITY;
@@ -792,7 +799,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) mp = fmaxf(mp, x[t][e]);
-        mp = kv_rows_max(mp);
+        mp = kv_rows_max(mp) * f;
         if (__any(mp > m + kKvLag)) {
             const float mn = fmaxf(m, mp);
             const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -809,9 +816,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
             uint32_t y[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float p = __builtin_amdgcn_exp2f(x[t][e] - mref);
+                const float p = __builtin_amdgcn_exp2f(fmaf(x[t][e], f, -mref));
                 sum += p;
-                y[e] = (uint32_t) (int) (D == 2 ? p * PMAX + 0.5f : p * PMAX) + BIAS;
+                /* rounded, and the digits' bias: 32768.5 is exact in f32, 2^30 + 0x808080 is not */
+                y[e] = D == 2 ? (uint32_t) (int) (p * PMAX + (0.5f + BIAS)) : (uint32_t) (int) (p * PMAX) + BIAS;
             }
 #pragma unroll
             for (int d = 0; d < D; d++) {
