@@ -521,8 +521,8 @@ int sparkmv_argmax(const float * logits, int n, int * out, void * stream);
 /* ---- several sequences: a paged cache that holds keys and values in 8 bits ----
  * No counterpart in the reference, which serves one sequence from f32 rows.
  * A page holds SPARKMV_KV_PAGE positions of every kv head; a page and kv head
- * have one scale for the keys and one for the values, and a cached value is
- * its code (-127..127) times the scale. A sequence is a slot: a row of the
+ * have one scale for the keys and one for the values, not negative, and a cached
+ * value is its code (-127..127) times the scale. A sequence is a slot: a row of the
  * page table, entry j naming the page of positions 64 j .. 64 j + 63. The
  * caller owns every array, hands out pages and keeps the lengths; several
  * slots may name one page as long as none appends to it. Codes of a page's
@@ -581,9 +581,10 @@ int sparkmv_rope_table(float * table, int rows, int rope_dim, double theta, void
  * their pages. A page opened here (its first position is new), or whose scale
  * no longer covers its new values, takes the scale
  *   f32(largest |new value| * h / 127),  h = 1 if the page is full after the call, else 1.25
- * and its older codes are rounded anew to it; a code is the value over the
- * scale, rounded to nearest even. The headroom h makes a later growth rare and
- * keeps the sum of all roundings under 2.5 steps however often it happens. A
+ * (2^-126 at least) and its older codes are rounded anew to it; a code is the
+ * value over the scale, rounded to nearest even. The headroom h makes a later
+ * growth rare, and a value is off by at most 3 steps however often it happens:
+ * half a step at each, the steps growing by 1.25 but for the last. A
  * value that is not finite makes the scale NaN, and the page's head reads as
  * NaN until its first position is appended again. A sequence may be cut back
  * to any length (append again at a smaller pos): a page keeps its scale then. A slot may appear

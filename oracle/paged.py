@@ -78,12 +78,14 @@ def append(cache, q, k, v, rope, pos, qstart=None, slot=None, max_q=1 << 30):
                         codes[here[held:held + hi - lo]] = 0
                         continue
                     now = was
-                    if not held or need > 127.0 * was:
-                        now = float(np.float32(need * (1.0 if full else 1.25) / 127.0))
+                    if not was > 0 or need > 127.0 * was:
+                        now = max(float(np.float32(need * (1.0 if full else 1.25) / 127.0)), 2.0 ** -126)
                         scales[page, h] = now
                         old = codes[here[:held]].astype(np.float64)
-                        codes[here[:held]] = np.rint(old * was / now) if now > 0 else 0
-                    codes[here[held:held + hi - lo]] = np.rint(rows[:, h] / now) if now > 0 else 0
+                        codes[here[:held]] = np.rint(old * was / now)
+                    new = np.rint(rows[:, h] / now)
+                    assert np.abs(new).max() <= 127
+                    codes[here[held:held + hi - lo]] = new
     return q_out
 
 

@@ -44,6 +44,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <exception>
 #include <map>
 #include <vector>
 
@@ -2323,10 +2324,17 @@ int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
     const sparkmv_model_cfg & c = m->c;
     /* the interface's limit on positions, as for max_ctx */
     if (max_pages > 131072 / kKvPage) { set_error("%d pages of %d positions are above 131072", max_pages, kKvPage); return -1; }
+    std::vector<size_t> at;
+    try {
+        at.resize((size_t) c.layers * 4);
+        m->paged.resize((size_t) c.layers);
+    } catch (const std::exception &) {
+        set_error("paged cache: out of host memory");
+        return -1;
+    }
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += align256(bytes); return o; };
     const size_t codes = (size_t) npages * c.kv_heads * kKvPage * c.head_dim, scales = (size_t) npages * c.kv_heads * 4;
-    std::vector<size_t> at((size_t) c.layers * 4);
     for (int li = 0; li < c.layers; li++) {
         at[4 * li] = take(codes);
         at[4 * li + 1] = take(codes);
@@ -2361,7 +2369,6 @@ int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
     m->ptable = (int *) (b + o_table);
     m->pstep = (int *) (b + o_step);
     for (int r = 0; r < 2; r++) m->prope[r] = (float *) (b + o_rope[r]);
-    m->paged.resize((size_t) c.layers);
     for (int li = 0; li < c.layers; li++) {
         sparkmv_kv_cache & k = m->paged[li];
         memset(&k, 0, sizeof k);
@@ -2380,13 +2387,14 @@ int sparkmv_model_set_pages(void * model, int slot, const int * pages, int n, vo
     const sparkmv_kv_cache & k = m->paged[0];
     if (slot < 0 || slot >= k.nslots) { set_error("slot %d is outside 0..%d", slot, k.nslots - 1); return -1; }
     if (n < 0 || n > k.max_pages) { set_error("%d pages are outside 0..%d", n, k.max_pages); return -1; }
-    std::vector<int> row((size_t) k.max_pages, -1);
+    int row[131072 / kKvPage];   /* max_pages, at most */
+    for (int j = 0; j < k.max_pages; j++) row[j] = -1;
     for (int j = 0; j < n; j++) {
         if (pages[j] < -1 || pages[j] >= k.npages) { set_error("page %d is outside 0..%d", pages[j], k.npages - 1); return -1; }
-        row[(size_t) j] = pages[j];
+        row[j] = pages[j];
     }
     hipStream_t s = (hipStream_t) stream;
-    hipError_t e = hipMemcpyAsync(m->ptable + (size_t) slot * k.max_pages, row.data(), row.size() * 4, hipMemcpyHostToDevice, s);
+    hipError_t e = hipMemcpyAsync(m->ptable + (size_t) slot * k.max_pages, row, (size_t) k.max_pages * 4, hipMemcpyHostToDevice, s);
     if (e == hipSuccess) e = hipStreamSynchronize(s);
     return e == hipSuccess ? 0 : fail_hip("page table upload", e);
 }

@@ -54,7 +54,8 @@ __global__ __launch_bounds__(256) void kv_rope_table_kernel(float * tab, int row
  * there), the scale from 64 bits, the code as the nearest integer of the exact
  * quotient. That one is found in f32: n0 = rint(x * (1 / s)) is off by one at
  * most, and x - s n0, one fma, is exact (its bits lie between the last place
- * of s or x and s), so comparing it with s / 2 settles the rounding. */
+ * of s or x and s, and s is not below 2^-126), so comparing it with s / 2
+ * settles the rounding. */
 struct KvAppend {
     sparkmv_kv_cache c;
     sparkmv_kv_batch b;
@@ -231,17 +232,13 @@ __global__ __launch_bounds__(NT, NT == 256 ? 1 : 8) void kv_append_kernel(const 
     for (int k = 0; k < NT / 64; k++) big = max(big, lmax[k]);
     const double need = (double) __uint_as_float(big);
     const bool bad = big >= 0x7f800000u || was != was;
-    const bool keep = held && need <= 127.0 * (double) was;
+    const bool keep = held && was > 0.0f && need <= 127.0 * (double) was;
     const float now = bad ? __uint_as_float(0x7fc00000u)
-                          : (keep ? was : (float) (need * (hi == p0 + kKvPage ? 1.0 : 1.25) / 127.0));
+                          : (keep ? was : fmaxf((float) (need * (hi == p0 + kKvPage ? 1.0 : 1.25) / 127.0), 1.17549435e-38f));
     if ((!keep || bad) && tid == 0) *scale = now;
-    /* a scale below 2^-100 and what it divides go up by 2^100, exactly, so that
-     * the reciprocal and the remainders stay in f32's range */
-    const bool none = bad || !(now > 0.0f);
-    const float up = now < 7.888609e-31f ? 1.2676506e30f : 1.0f, div = now * up, inv = none ? 0.0f : 1.0f / div;
+    const float inv = 1.0f / now;
     const bool again = held && !keep && !bad;   /* older codes rounded anew */
-    const double was_up = (double) was * (double) up;
-    auto old_code = [&](int c) -> int8_t { return none ? 0 : (int8_t) kv_code((double) c * was_up, (double) div, inv); };
+    auto old_code = [&](int c) -> int8_t { return (int8_t) kv_code((double) c * (double) was, (double) now, inv); };
     /* codes to LDS: keys by row, values as they lie in a page */
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -250,7 +247,7 @@ __global__ __launch_bounds__(NT, NT == 256 ? 1 : 8) void kv_append_kernel(const 
         if (k >= np) continue;
         int e1;
         const int e0 = kv_pair(k & (pairs - 1), half, e1);
-        const int a = none ? 0 : kv_code(x[u] * up, div, inv), b = none ? 0 : kv_code(y[u] * up, div, inv);
+        const int a = bad ? 0 : kv_code(x[u], now, inv), b = bad ? 0 : kv_code(y[u], now, inv);
         lcode[which ? kv_value_at(held + r, e0, hd) : r * hd + e0] = (int8_t) a;
         lcode[which ? kv_value_at(held + r, e1, hd) : r * hd + e1] = (int8_t) b;
     }
@@ -470,6 +467,10 @@ int sparkmv_kv_append(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
         return -1;
     }
     if (batch->nseq == 0 || batch->ntok == 0) return 0;
+    if (n.heads && n.q == n.q_out && n.ldq != n.ldqo && batch->ntok > 1) {
+        set_error("queries rotated in place with two row strides, %d and %d", n.ldq, n.ldqo);
+        return -1;
+    }
     const long kvd = (long) cache->kv_heads * hd, qd = (long) n.heads * hd;
     if (kv_check_rows("keys", n.k, n.ldk, kvd, n.x_dtype, batch->ntok) ||
         kv_check_rows("values", n.v, n.ldv, kvd, n.x_dtype, batch->ntok))

@@ -952,9 +952,10 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
         p.wq = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
         p.tiles = (int) ((long) b->ntok * G / (16 * p.wq) + b->nseq);
         const long busy = ((long) b->ntok * G + 16 * p.wq - 1) / (16 * p.wq) * c->kv_heads;
-        /* two workgroups a CU, eight pages a split */
+        /* two workgroups a CU, three pages a split at least (three blocks of 8 tokens
+         * at 6001, the call: 8 pages 35 us, 4 27.4, 3 25.5, 2 29.5) */
         long n = (2 * cu_count() + busy - 1) / busy;
-        if (n > pages / 8) n = pages / 8;
+        if (n > pages / 3) n = pages / 3;
         p.nsplit = (int) (n < 1 ? 1 : (n > kKvSplits ? kKvSplits : n));
         if (p.nsplit > 1) {
             const size_t rows = (size_t) p.tiles * c->kv_heads * 16 * p.wq * p.nsplit;

@@ -124,6 +124,27 @@ def test_append_one_by_one_and_cut_back(sm, dev):
             c.same()
 
 
+def test_append_many_sequences(sm, dev):
+    """More sequences than a workgroup has threads, each with a few tokens."""
+    import torch
+    n, kvh, hd = 300, 1, 64
+    c = Case(sm, dev, kvh, hd, n, 1, 83, fill=False)
+    counts = c.rng.integers(0, 4, n)
+    pos = c.rng.integers(-1, 60, n)
+    qstart = np.concatenate([[0], np.cumsum(counts)])
+    ntok = int(qstart[-1])
+    q, qf = rows(dev, c.rng.standard_normal((ntok, 3, hd)), torch.bfloat16)
+    k, kf = rows(dev, c.rng.standard_normal((ntok, kvh, hd)), torch.bfloat16)
+    table = sm.rope_table(64, 32, 1e4, dev)
+    q_out = torch.full_like(q, 5.0)
+    c.kv.append(c.batch(pos, ntok, qstart), q, k, k, table, q_out)
+    want = paged.append(c.host, qf, kf, kf, table.cpu().numpy(), pos, qstart)
+    c.same()
+    got, none = q_out.double().cpu().numpy(), np.isnan(want)
+    assert np.all(got[none] == 5.0)
+    assert np.all(np.abs(got - want)[~none] <= 2.0 ** -8 * np.abs(want[~none]) * (1 + 1e-9))
+
+
 @pytest.mark.parametrize("what", ["nan", "inf", "zero", "tiny", "denormal", "huge", "ties", "f32 to bf16"])
 def test_append_of_unusual_values(sm, dev, what):
     import torch
@@ -348,6 +369,38 @@ def test_attend_bad_queries(sm, dev):
         assert np.array_equal(got, good)
 
 
+@pytest.mark.parametrize("counts", [None, [3, 1, 2], [40, 3, 70]])
+def test_attend_longer_than_said(sm, dev, counts):
+    """max_len only shapes launches: sequences far past it, and far below, are
+    served in full; so are more sequences than a wave has lanes."""
+    import torch
+    c = Case(sm, dev, 2, 64, 3, 60, 73)
+    pos = [3500, 1, 2000]
+    qstart = None if counts is None else np.concatenate([[0], np.cumsum(counts)])
+    ntok = 3 if counts is None else int(qstart[-1])
+    q, qf = rows(dev, c.rng.standard_normal((ntok, 8, 64)), torch.float32)
+    for max_len in (1, 0, 1 << 20):
+        out = torch.full((ntok, 8, 64), 7.0, device=dev)
+        c.kv.attend(c.batch(pos, ntok, qstart, max_len=max_len), q, out)
+        check_attention(c, q, qf, out, 0.125, 0, None, pos, qstart, None, note=f"max_len {max_len}")
+
+
+def test_attend_many_sequences(sm, dev):
+    """More sequences than a wave has lanes, idle ones among them, over shared
+    pages: decode steps short and long, and ragged blocks."""
+    c = Case(sm, dev, 2, 64, 6, 40, 79)
+    rng = np.random.default_rng(8)
+    for n in (65, 300):
+        slot = rng.integers(0, 6, n)
+        for most in (200, 2400):
+            pos = rng.integers(0, most, n)
+            pos[rng.random(n) < 0.2] = -1
+            attend(c, list(pos), None, list(slot), 4, note=f"{n} sequences up to {most}")
+        counts = rng.integers(0, 4, n)
+        pos = rng.integers(0, 600, n)
+        attend(c, list(pos), np.concatenate([[0], np.cumsum(counts)]), list(slot), 4, "f32", "bf16", note=f"{n} ragged")
+
+
 @pytest.mark.parametrize("form", ["one", "many", "block", "chunk"])
 def test_attend_long(sm, dev, form):
     """Work split over a long axis and joined."""
@@ -458,8 +511,8 @@ def test_one_conversation(sm, dev):
             for p in range(len(kept[s])):
                 kc, vc = paged.read(c.host, s, p, hd)
                 page = c.host["pages"][s, p // 64]
-                assert np.all(np.abs(kc - kept[s][p][0]) <= 2.5 * c.host["k_scale"][page][:, None] * (1 + 1e-6))
-                assert np.all(np.abs(vc - kept[s][p][1]) <= 2.5 * c.host["v_scale"][page][:, None] * (1 + 1e-6))
+                assert np.all(np.abs(kc - kept[s][p][0]) <= 3 * c.host["k_scale"][page][:, None] * (1 + 1e-6))
+                assert np.all(np.abs(vc - kept[s][p][1]) <= 3 * c.host["v_scale"][page][:, None] * (1 + 1e-6))
             lens[s] += counts[s]
 
 

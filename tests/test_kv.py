@@ -75,7 +75,7 @@ def test_bad_batches(sm, bad, text):
     ({"rope_dim": 66}, "rope_dim 66"), ({"rope_dim": -2}, "rope_dim -2"), ({"rope": None}, "rope table is null"),
     ({"rope_rows": 127}, "does not cover 128"), ({"k": None}, "keys is null"), ({"v": None}, "values is null"),
     ({"ldk": 127}, "holds no 128"), ({"ldv": 130}, "16-byte aligned"), ({"v": P + 4}, "16-byte aligned"),
-    ({"ldq": 255}, "holds no 256"), ({"ldqo": 258}, "16-byte aligned"), ({"q_out": P + 2}, "16-byte aligned")])
+    ({"ldqo": 260}, "two row strides"), ({"ldq": 255, "q": 2 * P}, "holds no 256"), ({"ldqo": 258, "q": 2 * P}, "16-byte aligned"), ({"q_out": P + 2}, "16-byte aligned")])
 def test_bad_new_rows(sm, bad, text):
     refused(sm, sm.lib().sparkmv_kv_append(ref(cache(sm)), ref(batch(sm)), ref(new(sm, **bad)), None), text)
 
@@ -159,9 +159,9 @@ def test_layout_is_a_permutation():
 
 def test_oracle_rounding_bound():
     """Appended one at a time with magnitudes that keep growing, every value
-    stays within 2.5 steps of the page's last scale: each growth multiplies
-    the scale by 1.25 at least, so the half steps of all roundings add up to
-    at most s / 2 / (1 - 1 / 1.25)."""
+    stays within 3 steps of the page's last scale: each growth but the one
+    that fills the page multiplies the scale by 1.25 at least, so the half steps
+    of all roundings add up to at most s / 2 / (1 - 1 / 1.25) + s / 2."""
     rng = np.random.default_rng(3)
     hd = 64
     c = {"k": np.zeros((1, 1, 64 * hd), np.int8), "v": np.zeros((1, 1, 64 * hd), np.int8),
@@ -171,5 +171,5 @@ def test_oracle_rounding_bound():
         paged.append(c, None, x[p:p + 1], x[p:p + 1], None, [p])
     for p in range(64):
         k, v = paged.read(c, 0, p, hd)
-        assert np.abs(k - x[p]).max() <= 2.5 * c["k_scale"][0, 0] * (1 + 1e-6)
+        assert np.abs(k - x[p]).max() <= 3 * c["k_scale"][0, 0] * (1 + 1e-6)
         assert np.array_equal(k, v)
