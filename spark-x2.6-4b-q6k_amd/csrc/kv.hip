@@ -139,13 +139,17 @@ __global__ __launch_bounds__(NT, NT == 256 ? 1 : 8) void kv_append_kernel(const 
         const int w = (int) blockIdx.x - A.nkv, t0 = w / A.qparts * A.qtok, per = A.n.heads << sh;
         const int first = w % A.qparts * (NT * kKvPairs);   /* 0 where a workgroup takes whole tokens */
         const int n = A.qparts > 1 ? min(per, first + NT * kKvPairs) : min(A.qtok, A.b.ntok - t0) * per;
+#pragma unroll 1
         for (int i = tid; i < A.qtok; i += NT) lpos[i] = -1;
         __syncthreads();
+#pragma unroll 1
         for (int i = tid; i < A.b.nseq; i += NT) {
             const KvSeq s = kv_seq(A.b, i, A.c.nslots, A.c.max_pages);
+#pragma unroll 1
             for (int t = max(s.row, t0); t < min(s.row + s.count, t0 + A.qtok); t++) lpos[t - t0] = s.pos + t - s.row;
         }
         __syncthreads();
+#pragma unroll 1
         for (int j0 = first; j0 < n; j0 += NT * kKvPairs) {
             const int i0 = j0 + tid, live = (n - j0 + NT - 1) / NT;
             double a[kKvPairs], b[kKvPairs];
@@ -254,11 +258,13 @@ __global__ __launch_bounds__(NT, NT == 256 ? 1 : 8) void kv_append_kernel(const 
     __syncthreads();
     if (!which) {
         const int per = hd / 16;   /* pieces of a position */
+#pragma unroll 1
         for (int k = tid; k < rows * per; k += NT) {
             const int r = k >> (sh - 3), d = 16 * (k & (per - 1));
             *(int4 *) (codes + kv_key_at(held + r, d)) = *(const int4 *) (lcode + r * hd + d);
         }
         if (again)
+#pragma unroll 1
             for (int k = tid; k < held * per; k += NT) {
                 Piece q;
                 int4 * at = (int4 *) (codes + kv_key_at(k >> (sh - 3), 16 * (k & (per - 1))));
@@ -272,6 +278,7 @@ __global__ __launch_bounds__(NT, NT == 256 ? 1 : 8) void kv_append_kernel(const 
     /* positions from .. upto - 1 of a page come from LDS, the others stay */
     const int from = again ? 0 : held;
     if (again) {
+#pragma unroll 1
         for (int k = tid; k < 4 * hd; k += NT) {
             Piece q;
             q.v = *(const int4 *) (codes + (size_t) k * 16);

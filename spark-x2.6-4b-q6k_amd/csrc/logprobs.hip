@@ -177,12 +177,13 @@ __device__ __forceinline__ float lp_value(uint64_t key) {
 __device__ __forceinline__ int lp_place(uint64_t key) { return (int) ~(uint32_t) key; }
 
 /* how many of the n keys are larger; zeros follow the list up to a multiple of
- * kLpPad, whose reads are in flight together (one at a time they cost 5 us for
- * 256 keys, so 1.4) */
+ * kLpPad, whose reads are in flight together (the join of one row of 131072:
+ * 10.4 us with one read at a time, 8.7 so, 7.6 with waves ranking first) */
 constexpr int kLpPad = 16;
 __device__ __forceinline__ int lp_rank(const uint64_t * keys, int n, uint64_t mine) {
     typedef uint64_t u2 __attribute__((ext_vector_type(2)));
     int c = 0;
+#pragma unroll 1
     for (int i = 0; i < n; i += kLpPad) {
         u2 v[kLpPad / 2];
 #pragma unroll
@@ -204,31 +205,35 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     __shared__ __attribute__((aligned(16))) uint64_t lseg[kLpList + kLpPad];
     __shared__ uint64_t lpick[kLpMaxK], lleast;
     __shared__ float red[3][4];
-    __shared__ int count[2];
+    __shared__ __attribute__((aligned(16))) uint64_t lcand[4 * kLpMaxK + kLpPad];
+    __shared__ int count[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x, k = A.k;
     const X * row = (const X *) A.x + (size_t) r * A.ld;
-    if (tid < 2) count[tid] = 0;
+    if (tid < 3) count[tid] = 0;
+    if (tid < 4 * kLpMaxK + kLpPad) lcand[tid] = 0;
     const int tok = A.tokens ? A.tokens[r] : -1;
     const float given = tok >= 0 && tok < A.n ? lp_one(row + tok) : 0.0f;
+    /* this thread's segments, requested before anything is waited for */
+    const float * seg = A.seg + (size_t) r * A.nseg;
+    const int nseg = k ? A.nseg : 0;
+    float held[kLpHeld];
+#pragma unroll
+    for (int j = 0; j < kLpHeld; j++) held[j] = tid + 256 * j < nseg ? seg[tid + 256 * j] : NAN;
     /* the row's M, z and e */
     float M = -INFINITY, z = 0.0f, e = 0.0f;
     const lp_f4 * parts = A.parts + (size_t) r * A.nparts;
+#pragma unroll 1
     for (int i = tid; i < A.nparts; i += 256) M = fmaxf(M, parts[i][0]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
     if (lane == 0) red[0][wave] = M;
-    /* this thread's segments */
-    const float * seg = A.seg + (size_t) r * A.nseg;
-    const int nseg = k ? A.nseg : 0;
     uint64_t best = 0;
-    float held[kLpHeld];
-#pragma unroll
-    for (int j = 0; j < kLpHeld; j++) held[j] = tid + 256 * j < nseg ? seg[tid + 256 * j] : NAN;
 #pragma unroll
     for (int j = 0; j < kLpHeld; j++) {
         const uint64_t key = lp_key(held[j], tid + 256 * j);
         best = key > best ? key : best;
     }
+#pragma unroll 1
     for (int i = tid + 256 * kLpHeld; i < nseg; i += 256) {
         const uint64_t key = lp_key(seg[i], i);
         best = key > best ? key : best;
@@ -237,6 +242,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     lkey[tid] = best;
     __syncthreads();
     M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+#pragma unroll 1
     for (int i = tid; i < A.nparts; i += 256) {
         const lp_f4 p = parts[i];
         const float d = p[0] == -INFINITY ? 0.0f : fmaxf(p[0] - M, -1.0e30f), f = p[0] == -INFINITY ? 1.0f : expf(d);
@@ -254,8 +260,16 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     }
     /* the k best segments are among those of the k threads whose best is best,
      * and none of them is below the last of these threads' best */
-    const int place = k && best ? lp_rank(lkey, 256, best) : k;
-    if (place == k - 1) lleast = best;
+    int place = k;
+    if (k) {
+        /* first among its wave's, then among the waves' k best: all 256 at once read
+         * four times the LDS and took 2.8 us of the launch, this 0.9 */
+        if (best) place = lp_rank(lkey + 64 * wave, 64, best);
+        if (place < k) lcand[atomicAdd(&count[2], 1)] = best;
+        __syncthreads();
+        if (place < k) place = lp_rank(lcand, count[2], best);
+        if (place == k - 1) lleast = best;
+    }
     __syncthreads();
     if (place < k) {
         const uint64_t least = lleast;
@@ -264,6 +278,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
             const uint64_t key = lp_key(held[j], tid + 256 * j);
             if (key >= least) lseg[atomicAdd(&count[0], 1)] = key;
         }
+#pragma unroll 1
         for (int i = tid + 256 * kLpHeld; i < nseg; i += 256) {
             const uint64_t key = lp_key(seg[i], i);
             if (key >= least) lseg[atomicAdd(&count[0], 1)] = key;
@@ -284,6 +299,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     if (tid < kLpPad) lseg[nc + tid] = 0;
     if (tid < kLpMaxK) lpick[tid] = 0;
     __syncthreads();
+#pragma unroll 1
     for (int i = tid; i < nc; i += 256) {
         const int rank = lp_rank(lseg, nc, lseg[i]);
         if (rank < k) lpick[rank] = lseg[i];
@@ -294,6 +310,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     const float floor_ = nk == k ? lp_value(lpick[k - 1]) : -INFINITY;
     uint64_t * list = lseg;   /* nk * 32 <= 1024 keys */
     static_assert(kLpList >= kLpMaxK * kLpSeg, "the list holds every logit of the picked segments");
+#pragma unroll 1
     for (int i = tid; i < nk * kLpSeg; i += 256) {
         const int at = lp_place(lpick[i / kLpSeg]) * kLpSeg + i % kLpSeg;
         if (at >= A.n) continue;
@@ -304,6 +321,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     const int nl = count[1];
     if (tid < kLpPad) list[nl + tid] = 0;
     __syncthreads();
+#pragma unroll 1
     for (int i = tid; i < nl; i += 256) {
         const uint64_t key = list[i];
         const int rank = lp_rank(list, nl, key);
@@ -312,6 +330,7 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
             A.top_lp[(size_t) r * k + rank] = lp(lp_value(key));
         }
     }
+#pragma unroll 1
     for (int i = nl + tid; i < k; i += 256) {
         A.top_id[(size_t) r * k + i] = -1;
         A.top_lp[(size_t) r * k + i] = bad ? NAN : -INFINITY;
