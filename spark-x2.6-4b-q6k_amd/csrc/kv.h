@@ -46,11 +46,14 @@ __device__ __forceinline__ KvSeq kv_seq(const sparkmv_kv_batch & b, int i, int n
 
 __device__ __forceinline__ float kv_load(const float * p) { return *p; }
 __device__ __forceinline__ float kv_load(const uint16_t * p) { return __uint_as_float((uint32_t) *p << 16); }
-__device__ __forceinline__ uint16_t kv_bf16(float f) {
-    uint32_t u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t) ((u >> 16) | 0x40u);
-    return (uint16_t) ((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+/* to nearest even, a NaN stays one: one instruction for two (in integer
+ * arithmetic fourteen, which a call that runs them once also has to fetch) */
+__device__ __forceinline__ uint32_t kv_bf16x2(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
 }
+__device__ __forceinline__ uint16_t kv_bf16(float f) { return (uint16_t) kv_bf16x2(f, f); }
 __device__ __forceinline__ void kv_store(float * p, float v) { *p = v; }
 __device__ __forceinline__ void kv_store(uint16_t * p, float v) { *p = kv_bf16(v); }
 

@@ -118,7 +118,6 @@ __device__ __forceinline__ int kv_q_exponent(const float (&x)[NC][16], bool & ba
 template <int N>
 __device__ __forceinline__ void kv_write(const sparkmv_kv_query & q, int row, int head, int hd, int d, const float * o, float l) {
     typedef float fn __attribute__((ext_vector_type(N)));
-    typedef uint16_t hn __attribute__((ext_vector_type(N)));
     float f = l == 0.0f ? 0.0f : 1.0f / l;
     if (q.gate) f *= 1.0f / (1.0f + expf(-q.gate[(size_t) row * q.ldg + head]));
     const size_t at = (size_t) row * q.ldo + (size_t) head * hd + d;
@@ -128,10 +127,15 @@ __device__ __forceinline__ void kv_write(const sparkmv_kv_query & q, int row, in
     if (q.out_dtype == SPARKMV_X_F32) {
         *(fn *) ((float *) q.out + at) = v;
     } else {
-        hn w;
+        if constexpr (N == 1) {
+            ((uint16_t *) q.out)[at] = kv_bf16(v[0]);
+        } else {
+            typedef uint32_t un __attribute__((ext_vector_type(N / 2)));
+            un w;
 #pragma unroll
-        for (int i = 0; i < N; i++) w[i] = kv_bf16(v[i]);
-        *(hn *) ((uint16_t *) q.out + at) = w;
+            for (int i = 0; i < N / 2; i++) w[i] = kv_bf16x2(v[2 * i], v[2 * i + 1]);
+            *(un *) ((uint16_t *) q.out + at) = w;
+        }
     }
 }
 
