@@ -15,13 +15,11 @@ namespace {
 __device__ __forceinline__ void kv_store_wide(float * p, double v) { *p = (float) v; }
 __device__ __forceinline__ void kv_store_wide(uint16_t * p, double v) {
     const float f = (float) v;
-    uint32_t u = __float_as_uint(f);
     const double back = (double) f;
-    if (back != v && __builtin_isfinite(f)) {
-        if (fabs(back) > fabs(v)) u--;   /* rounded away from zero: step back */
-        u |= 1u;
-    }
-    *p = kv_bf16(__uint_as_float(u));
+    const uint32_t off = (uint32_t) (back != v) & (uint32_t) (fabsf(f) < INFINITY);
+    /* one step back where it was rounded away from zero */
+    const uint32_t u = __float_as_uint(f) - (off & (uint32_t) (fabs(back) > fabs(v)));
+    *p = kv_bf16(__uint_as_float(u | off));
 }
 
 /* ---------------------------------------------------------------- rope table */
@@ -77,27 +75,32 @@ __device__ __forceinline__ int kv_pair(int j, int half, int & second) {
 }
 
 /* up to four pairs and their turns, requested together and then turned: at(u, row,
- * tab) gives the u-th pair's place in its head, its row and its table row (NULL:
- * not turned). Only `live` of them, a uniform count, are there: a call of one
- * token steps over the others' instructions, which it would otherwise fetch */
+ * tab) gives the u-th pair's place in its head, its row and its table row (used
+ * with rot, a uniform truth, only). Only `live` of them, a uniform count, are
+ * there: a call of one token steps over the others' instructions, which it would
+ * otherwise fetch */
 constexpr int kKvPairs = 4;
 template <typename X, typename At>
-__device__ __forceinline__ void kv_turn(At at, int live, int half, double * a, double * b) {
+__device__ __forceinline__ void kv_turn(At at, int live, bool rot, int half, double * a, double * b) {
     float x[kKvPairs], y[kKvPairs], c[kKvPairs], s[kKvPairs];
     bool turn[kKvPairs];
 #pragma unroll
     for (int u = 0; u < kKvPairs; u++) {
         if (u >= live) break;
         const X * row;
-        const float * tab;
+        const float * tab = nullptr;
         const int j = at(u, row, tab);
         int e1;
         const int e0 = kv_pair(j, half, e1);
         x[u] = kv_load(row + e0);
         y[u] = kv_load(row + e1);
-        turn[u] = j < half && tab;
-        c[u] = turn[u] ? tab[j] : 1.0f;
-        s[u] = turn[u] ? tab[half + j] : 0.0f;
+        turn[u] = rot & (j < half);
+        c[u] = 1.0f;
+        s[u] = 0.0f;
+        if (rot) {
+            c[u] = tab[min(j, half - 1)];
+            s[u] = tab[half + min(j, half - 1)];
+        }
     }
 #pragma unroll
     for (int u = 0; u < kKvPairs; u++) {
@@ -108,19 +111,18 @@ __device__ __forceinline__ void kv_turn(At at, int live, int half, double * a, d
     }
 }
 
-/* nearest integer of x / s (ties to even), |x / s| <= 127.5; r is f32(1 / s) */
+/* nearest integer of x / s (ties to even), |x / s| <= 127.5; r is f32(1 / s). Without
+ * branches: sixteen of them a thread were half of the kernel's instructions */
 __device__ __forceinline__ int kv_code(float x, float s, float r) {
-    float n = rintf(x * r);
-    const float e = fmaf(-s, n, x), e2 = 2.0f * fabsf(e);
-    if (e2 > s || (e2 == s && ((int) n & 1))) n += e > 0.0f ? 1.0f : -1.0f;
-    return (int) n;
+    const float n = rintf(x * r), e = fmaf(-s, n, x), e2 = 2.0f * fabsf(e);
+    const int i = (int) n, off = (int) (e2 > s) | ((int) (e2 == s) & i);
+    return i + (off & 1) * (e > 0.0f ? 1 : -1);
 }
 /* the same of a product of a code and its old scale, exact in 64 bits */
 __device__ __forceinline__ int kv_code(double x, double s, float r) {
-    double n = rint(x * (double) r);
-    const double e = fma(-s, n, x), e2 = 2.0 * fabs(e);
-    if (e2 > s || (e2 == s && ((int) n & 1))) n += e > 0.0 ? 1.0 : -1.0;
-    return (int) n;
+    const double n = rint(x * (double) r), e = fma(-s, n, x), e2 = 2.0 * fabs(e);
+    const int i = (int) n, off = (int) (e2 > s) | ((int) (e2 == s) & i);
+    return i + (off & 1) * (e > 0.0 ? 1 : -1);
 }
 
 constexpr int kv_append_rows(int nt) { return nt == 256 ? 8 : kKvPage; }   /* new rows of a page, at most */
@@ -156,9 +158,9 @@ __global__ __launch_bounds__(NT, NT == 256 ? 1 : 8) void kv_append_kernel(const 
             kv_turn<X>([&](int u, const X *& row, const float *& tab) {
                 const int k = min(i0 + u * NT, n - 1), t = A.qparts > 1 ? 0 : k / per, e = k - t * per, pos = lpos[t];
                 row = (const X *) A.n.q + (size_t) (t0 + t) * A.n.ldq + (size_t) (e >> sh) * hd;
-                tab = half && pos >= 0 ? A.n.rope + (size_t) pos * 2 * half : nullptr;
+                tab = A.n.rope + (size_t) max(pos, 0) * 2 * half;
                 return e & (pairs - 1);
-            }, live, half, a, b);
+            }, live, half > 0, half, a, b);
 #pragma unroll
             for (int u = 0; u < kKvPairs; u++) {
                 if (u >= live) break;
@@ -200,9 +202,9 @@ __global__ __launch_bounds__(NT, NT == 256 ? 1 : 8) void kv_append_kernel(const 
         kv_turn<X>([&](int u, const X *& row, const float *& tab) {
             const int k = min(tid + (v + u) * NT, np - 1), r = k >> sh;
             row = src + (size_t) (s.row + lo + r - s.pos) * ld;
-            tab = which || !half ? nullptr : A.n.rope + (size_t) (lo + r) * 2 * half;
+            tab = A.n.rope + (size_t) (lo + r) * 2 * half;
             return k & (pairs - 1);
-        }, live - v, half, a, b);
+        }, live - v, !which && half > 0, half, a, b);
 #pragma unroll
         for (int u = 0; u < kKvPairs; u++) {
             if (v + u >= live) break;
