@@ -158,10 +158,17 @@ __device__ __forceinline__ void kv_write(const sparkmv_kv_query & q, int row, in
  * A short call is bound by its chain of reads (positions, page numbers, codes)
  * and by fetching instructions that run once, about 0.5 us a kilobyte: so the
  * codes are requested before the queries are looked at, and what runs once is
- * kept in loops. */
-constexpr int kKvItem = 8;
+ * kept in loops.
+ *
+ * 16 query and 4 kv heads of 256: one token at position 131071 55.4 us (4.85 TB/s)
+ * and 7.2 for the join, 48 at up to 12000 66.6 (4.8 TB/s) and 6.6, one at 1003 (one
+ * launch) 12.1, 24 in windows of 512 11.6. */
+constexpr int kKvItem = 8;          /* 48 sequences of up to 12000: 83 us, without it 184 */
 constexpr int kKvFlatMost = 1024;   /* workgroups, at most */
-constexpr int kKvWhole = 24;        /* pages of a sequence that one workgroup takes alone */
+/* pages of a sequence that one workgroup takes alone: three turns of its eight
+ * waves, about what a join and its launch cost (16 pages: 12.1 us, in shares
+ * 16.4) */
+constexpr int kKvWhole = 24;
 
 struct KvFlat {
     sparkmv_kv_cache c;
@@ -608,7 +615,13 @@ __global__ __launch_bounds__(512) void kv_flat_join_kernel(const KvFlat A) {
  * WQ < 4 the other waves work on the same columns and take a part of the
  * elements in the product with the values (and repeat the scores). Each digit is
  * an instruction of its own here, on the same codes. Work that is split over the
- * pages is joined by a second launch. */
+ * pages is joined by a second launch.
+ *
+ * A chunk of 512 tokens at 16384 (16 query, 4 kv heads of 256, bf16 out): 200 us for
+ * 140 GFLOP, bound by the vector instructions around the products (414 a wave and
+ * page, half of them the values' sums from i32; VALU 62 % busy, MFMA 31). Six waves
+ * a workgroup, for three a SIMD, took 294: they do not fill the SIMDs evenly. Three
+ * blocks of 8 at 6001 (f32 out): 18.8 us and 6.9 for the join. */
 struct KvTile {
     sparkmv_kv_cache c;
     sparkmv_kv_batch b;
@@ -693,8 +706,8 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         __syncthreads();
     };
     /* a kilobyte of keys, 16 positions x 64 bytes, enters LDS as the matrix
-     * instruction's lanes take it (lane 16 g + position: 16 bytes): as it lies,
-     * sixteen lanes would read at a stride of 64 bytes, from a quarter of the banks */
+     * instruction's lanes take it (lane 16 g + position: 16 bytes), so that reads
+     * are contiguous: as it lies, sixteen lanes would read at a stride of 64 bytes */
     const uint32_t klane = c16 * 64 + 16 * g;
     auto fetch = [&](int j, int b) {
         const size_t at = ((size_t) max(__builtin_amdgcn_readfirstlane(lid[j & (kKvIds - 1)]), 0) * kvh + h) * (size_t) HALF;
