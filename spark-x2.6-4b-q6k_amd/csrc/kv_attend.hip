@@ -165,10 +165,12 @@ __device__ __forceinline__ void kv_write(const sparkmv_kv_query & q, int row, in
  * launch) 12.1, 24 in windows of 512 11.6. */
 constexpr int kKvItem = 8;          /* 48 sequences of up to 12000: 83 us, without it 184 */
 constexpr int kKvFlatMost = 1024;   /* workgroups, at most */
-/* pages of a sequence that one workgroup takes alone: three turns of its eight
- * waves, about what a join and its launch cost (16 pages: 12.1 us, in shares
- * 16.4) */
-constexpr int kKvWhole = 24;
+/* Pages of a sequence that one workgroup takes alone, in turns of its eight waves;
+ * above, shares and a join. us alone and in shares, 4 kv heads of 256: one sequence of
+ * 8 pages 9.6 and 11.9, 16 12.1 and 12.2, 24 15.0 and 12.3; 8 sequences of 24 pages
+ * 16.7 and 17.3, 32 19.8 and 18.2; 24 of 24 17.9 and 26.9, 32 31.0 and 31.3. So 16, or
+ * 24 from 32 workgroups on. */
+int kv_whole(long items) { return items < 32 ? 16 : 24; }
 
 struct KvFlat {
     sparkmv_kv_cache c;
@@ -634,7 +636,8 @@ struct KvTile {
 constexpr int kKvIds = 256;   /* page numbers held at a time */
 
 /* tile number `tile` of the batch, tiles of `cols` columns: its sequence and its
- * place there; false past the last one. Every thread of the workgroup calls it. */
+ * place there, a sequence's last (longest) first: the other way 4096 tokens from
+ * position 0 took 237 us, not 200; false past the last one. Every thread of the workgroup calls it. */
 __device__ __forceinline__ bool kv_find_tile(const sparkmv_kv_batch & b, const sparkmv_kv_cache & c, int G, int cols, int tile,
                                              int * lds, KvSeq & s, int & place) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
@@ -660,7 +663,7 @@ __device__ __forceinline__ bool kv_find_tile(const sparkmv_kv_batch & b, const s
         }
         if (tile >= at && tile < at + n) {
             lds[0] = i0 + tid;
-            lds[1] = tile - at;
+            lds[1] = n - 1 - (tile - at);
         }
         if (tile < before) break;
     }
@@ -682,14 +685,17 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
     __shared__ int lid[kKvIds];
     __shared__ float lks[kKvIds], lvs[kKvIds];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c16 = lane & 15;
-    const int wq = wave % WQ, wd = wave / WQ, kvh = A.c.kv_heads, G = A.q.heads / kvh, h = blockIdx.y;
+    const int wq = wave % WQ, wd = wave / WQ, kvh = A.c.kv_heads, G = A.q.heads / kvh;
+    /* splits next to each other, then kv heads, then tiles: the tiles that the batch
+     * does not fill are no XCD's alone, and an XCD sees few (split, kv head) */
+    const int split = (int) blockIdx.x % A.nsplit, th = (int) blockIdx.x / A.nsplit, h = th % kvh, tile = th / kvh;
     KvSeq s;
     int place;
-    if (!kv_find_tile(A.b, A.c, G, 16 * WQ, blockIdx.x, lfind, s, place)) return;
+    if (!kv_find_tile(A.b, A.c, G, 16 * WQ, tile, lfind, s, place)) return;
     const int ncol = s.count * G, col0 = place * 16 * WQ, t0 = col0 / G, t1 = min(col0 + 16 * WQ - 1, ncol - 1) / G + 1;
     int first;
     const int npages = kv_span(s, t0, t1, A.q.window, first), per = (npages + A.nsplit - 1) / A.nsplit;
-    const int jbeg = (int) blockIdx.z * per, jend = min(npages, jbeg + per);
+    const int jbeg = split * per, jend = min(npages, jbeg + per);
     if (jbeg >= jend) return;
     first += jbeg;
     const int n = jend - jbeg;
@@ -873,7 +879,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         }
         return;
     }
-    const size_t at = (((size_t) blockIdx.x * kvh + h) * (16 * WQ) + 16 * wq + c16) * A.nsplit + blockIdx.z;
+    const size_t at = (((size_t) tile * kvh + h) * (16 * WQ) + 16 * wq + c16) * A.nsplit + split;
 #pragma unroll
     for (int d = 0; d < ND; d++) *(kv_f4 *) (A.po + at * HD + 16 * (ND * wd + d) + 4 * g) = o[d];
     if (wd == 0 && g == 0) {
@@ -894,17 +900,18 @@ __global__ __launch_bounds__(256) void kv_tile_join_kernel(const KvTile A, int c
     typedef float fe __attribute__((ext_vector_type(E)));
     __shared__ int lfind[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
-    const int kvh = A.c.kv_heads, G = A.q.heads / kvh, h = blockIdx.y;
+    const int kvh = A.c.kv_heads, G = A.q.heads / kvh;
+    const int parts = cols / (4 * each), part = (int) blockIdx.x % parts, th = (int) blockIdx.x / parts, h = th % kvh, tile = th / kvh;
     KvSeq s;
     int place;
-    if (!kv_find_tile(A.b, A.c, G, cols, blockIdx.x, lfind, s, place)) return;
+    if (!kv_find_tile(A.b, A.c, G, cols, tile, lfind, s, place)) return;
     const int ncol = s.count * G, col0 = place * cols, t0 = col0 / G, t1 = min(col0 + cols - 1, ncol - 1) / G + 1;
     int first;
     const int npages = kv_span(s, t0, t1, A.q.window, first), per = (npages + A.nsplit - 1) / A.nsplit, n = (npages + per - 1) / per;
     for (int u = 0; u < each; u++) {
-        const int c = 4 * each * (int) blockIdx.z + each * wave + u, cc = col0 + c;
+        const int c = 4 * each * part + each * wave + u, cc = col0 + c;
         if (cc >= ncol) return;
-        const size_t row = (((size_t) blockIdx.x * kvh + h) * cols + c) * A.nsplit;
+        const size_t row = (((size_t) tile * kvh + h) * cols + c) * A.nsplit;
         float m = -INFINITY, l = 0.0f;
         if (lane < n) {
             m = A.pml[2 * (row + lane)];
@@ -943,7 +950,8 @@ __global__ __launch_bounds__(256) void kv_tile_join_kernel(const KvTile A, int c
 struct KvPlan {
     int flat;                 /* the few-column kernel: 1 shares, 2 whole kv heads */
     int groups, least;        /* its workgroups and least share */
-    int wq, tiles, nsplit;    /* the many-column kernel's */
+    long tiles;
+    int wq, nsplit;           /* the many-column kernel's */
     size_t pre, po, pml, bytes;
 };
 
@@ -956,9 +964,9 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += (bytes + 255) & ~(size_t) 255; return o; };
     if (cols <= 4) {
-        /* up to kKvWhole pages a sequence: a workgroup each, nothing to join */
+        /* up to kv_whole() pages a sequence: a workgroup each, nothing to join */
         const long seen = window > 0 && (window + kKvPage - 2) / kKvPage + 1 < pages ? (window + kKvPage - 2) / kKvPage + 1 : pages;
-        p.flat = seen <= kKvWhole ? 2 : 1;
+        p.flat = seen <= kv_whole((long) b->nseq * c->kv_heads) ? 2 : 1;
         const long most = 2 * cu_count() < kKvFlatMost ? 2 * cu_count() : kKvFlatMost, all = pages * b->nseq * c->kv_heads;
         p.groups = (int) (all < 1 ? 1 : (all < most ? all : most));
         p.least = 1;
@@ -967,7 +975,7 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
         p.pml = take((size_t) p.groups * 2 * 4 * 2 * 4);
     } else {
         p.wq = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
-        p.tiles = (int) ((long) b->ntok * G / (16 * p.wq) + b->nseq);
+        p.tiles = (long) b->ntok * G / (16 * p.wq) + b->nseq;
         const long busy = ((long) b->ntok * G + 16 * p.wq - 1) / (16 * p.wq) * c->kv_heads;
         /* two workgroups a CU, three pages a split at least (three blocks of 8 tokens
          * at 6001, the call: 8 pages 35 us, 4 27.4, 3 25.5, 2 29.5) */
@@ -1068,9 +1076,11 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     t.b.max_q = max_q;
     t.nsplit = p.nsplit;
     t.po = (float *) (mem + p.po); t.pml = (float *) (mem + p.pml);
-    const dim3 grid((unsigned) p.tiles, (unsigned) cache->kv_heads, (unsigned) p.nsplit);
+    const long th = p.tiles * cache->kv_heads;
+    if (th > 0xffffff / p.nsplit) { set_error("attention over %ld tiles of tokens is too much for one call", th); return -1; }
+    const dim3 grid((unsigned) (th * p.nsplit));
     const uint32_t lds = 4 * kKvPage * (uint32_t) hd;
-    const int each = (long) grid.x * grid.y * 4 * p.wq < 8 * cu_count() ? 1 : 4;
+    const int each = th * 4 * p.wq < 8 * cu_count() ? 1 : 4;
 #define KV_TILE(H, D, W)                                                                                             \
     do {                                                                                                             \
         static LdsAllowed allowed;                                                                                   \
@@ -1089,7 +1099,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
         else if (p.wq == 2) KV_TILE_D(H, 2);                                                                         \
         else KV_TILE_D(H, 4);                                                                                        \
         if (p.nsplit > 1)                                                                                            \
-            hipLaunchKernelGGL(kv_tile_join_kernel<H>, dim3(grid.x, grid.y, 4 * p.wq / each), dim3(256), 0, s, t, 16 * p.wq, each); \
+            hipLaunchKernelGGL(kv_tile_join_kernel<H>, dim3((unsigned) (th * 4 * p.wq / each)), dim3(256), 0, s, t, 16 * p.wq, each); \
     } while (0)
     if (hd == 64) KV_TILE_W(64);
     else if (hd == 128) KV_TILE_W(128);
