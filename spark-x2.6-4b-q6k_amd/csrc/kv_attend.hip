@@ -894,6 +894,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
  * waves had one row. One column a wave where that gives fewer than eight
  * workgroups a CU (three blocks of 8 tokens: 6.1 us, with four 12.7), else four. */
 constexpr int kKvSplits = 64;
+constexpr int kKvAlone = 8;   /* pages that take about as long as a join and its launch */
 template <int HD>
 __global__ __launch_bounds__(256) void kv_tile_join_kernel(const KvTile A, int cols, int each) {
     constexpr int E = HD / 64;
@@ -974,14 +975,21 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
         p.po = take((size_t) p.groups * 2 * 4 * hd * 4);
         p.pml = take((size_t) p.groups * 2 * 4 * 2 * 4);
     } else {
+        /* columns a workgroup: as a sequence's tokens give (16 sequences at 6000 of 4
+         * tokens with 1, 2 and 4: 52, 81 and 85 us, of 8: 70, 58 and 70, of 16: 111, 81 and
+         * 70), fewer where that leaves half of the CUs idle however it is split (one of 32
+         * tokens at 1000: 20.2, 21.1 and 23.6) */
+        const long most = pages <= kKvAlone ? 1 : (pages / 3 < kKvSplits ? pages / 3 : kKvSplits);
+        auto busy = [&]() { return ((long) b->ntok * G + 16 * p.wq - 1) / (16 * p.wq) * c->kv_heads; };
         p.wq = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
+        while (p.wq > 1 && 2 * busy() * most <= cu_count()) p.wq /= 2;
         p.tiles = (long) b->ntok * G / (16 * p.wq) + b->nseq;
-        const long busy = ((long) b->ntok * G + 16 * p.wq - 1) / (16 * p.wq) * c->kv_heads;
-        /* two workgroups a CU, three pages a split at least (three blocks of 8 tokens
-         * at 6001, the call: 8 pages 35 us, 4 27.4, 3 25.5, 2 29.5) */
-        long n = (2 * cu_count() + busy - 1) / busy;
-        if (n > pages / 3) n = pages / 3;
-        p.nsplit = (int) (n < 1 ? 1 : (n > kKvSplits ? kKvSplits : n));
+        /* as many as two workgroups a CU hold, three pages a split at least (three
+         * blocks of 8 tokens at 6001, the call: 8 pages 35 us, 4 27.4, 3 25.5, 2 29.5); one
+         * if that spares no more pages than the join costs */
+        long n = 2 * cu_count() / busy();
+        n = n < 1 ? 1 : (n < most ? n : most);
+        p.nsplit = pages - pages / n <= kKvAlone ? 1 : (int) n;
         if (p.nsplit > 1) {
             const size_t rows = (size_t) p.tiles * c->kv_heads * 16 * p.wq * p.nsplit;
             p.po = take(rows * hd * 4);
