@@ -984,11 +984,14 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
         p.wq = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
         while (p.wq > 1 && 2 * busy() * most <= cu_count()) p.wq /= 2;
         p.tiles = (long) b->ntok * G / (16 * p.wq) + b->nseq;
-        /* as many as two workgroups a CU hold, three pages a split at least (three
-         * blocks of 8 tokens at 6001, the call: 8 pages 35 us, 4 27.4, 3 25.5, 2 29.5); one
-         * if that spares no more pages than the join costs */
+        /* as many as two workgroups a CU hold, four pages a split about (three blocks of
+         * 8 tokens at 6001, the call: 8 pages 35 us, 4 25.5, 3 27.3, 2 29.5); one if that
+         * spares no more pages than the join costs */
         long n = 2 * cu_count() / busy();
         n = n < 1 ? 1 : (n < most ? n : most);
+        /* halves of half again as many workgroups fill the last turn better (three
+         * blocks of 512 at 6000: 243 us, whole 274; at 3000 147 and 155) */
+        if (n == 1 && most > 1 && busy() > cu_count() && 2 * busy() <= 3 * cu_count() && pages >= 48) n = 2;
         p.nsplit = pages - pages / n <= kKvAlone ? 1 : (int) n;
         if (p.nsplit > 1) {
             const size_t rows = (size_t) p.tiles * c->kv_heads * 16 * p.wq * p.nsplit;
