@@ -303,6 +303,30 @@ def test_attend_several_tokens(sm, dev, kvh, group, hd, counts, x, o):
     attend(c, [0, 190, 130], qstart, None, kvh * group, x, o, note=f"{counts} kvh {kvh} group {group} hd {hd} {x}")
 
 
+@pytest.mark.parametrize("x,o", [("f32", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("kvh,group,hd,most,longest", [
+    (2, 8, 64, 13, 700), (2, 8, 128, 13, 700), (2, 8, 256, 13, 700),     # up to 104 columns a sequence, split
+    (4, 4, 64, 8, 700), (4, 4, 128, 8, 700), (4, 4, 256, 8, 700),        # up to 32
+    (8, 8, 64, 17, 300), (8, 8, 128, 17, 300), (8, 4, 256, 8, 300)])     # short: whole
+def test_attend_blocks_that_fill_the_card(sm, dev, kvh, group, hd, most, longest, x, o):
+    """Enough tokens that a workgroup takes as many columns as a sequence gives;
+    fewer tokens are taken in smaller tiles."""
+    n = 16 if longest > 512 else 20
+    c = Case(sm, dev, kvh, hd, n, longest // 64 + 2, 51 + hd + kvh)
+    counts = [most - i % 4 for i in range(n)]
+    counts[3], counts[7] = 0, 1
+    pos = c.rng.integers(0, longest + 1, n).tolist()
+    pos[0], pos[1] = longest, 0
+    qstart = np.concatenate([[1], 1 + np.cumsum(counts)])
+    attend(c, pos, qstart, None, kvh * group, x, o, note=f"kvh {kvh} group {group} hd {hd} blocks of up to {most}")
+
+
+def test_attend_prompt_of_many_tiles(sm, dev):
+    """A prompt from its first position: tiles of one page up to all."""
+    c = Case(sm, dev, 2, 64, 2, 18, 57)
+    attend(c, [0, 5], [0, 1100, 1117], None, 16, "bf16", "bf16", note="a prompt of 1100")
+
+
 @pytest.mark.parametrize("o", ["f32", "bf16"])
 @pytest.mark.parametrize("counts", [None, [4, 9, 40]])
 def test_attend_sharp_and_flat(sm, dev, counts, o):
