@@ -619,7 +619,7 @@ __global__ __launch_bounds__(512) void kv_flat_join_kernel(const KvFlat A) {
  * an instruction of its own here, on the same codes. Work that is split over the
  * pages is joined by a second launch.
  *
- * A chunk of 512 tokens at 16384 (16 query, 4 kv heads of 256, bf16 out): 200 us for
+ * A chunk of 512 tokens at 16384 (16 query, 4 kv heads of 256, bf16 out): 193 us for
  * 140 GFLOP, bound by the vector instructions around the products (414 a wave and
  * page, half of them the values' sums from i32; VALU 62 % busy, MFMA 31). Six waves
  * a workgroup, for three a SIMD, took 294: they do not fill the SIMDs evenly. Three
