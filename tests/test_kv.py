@@ -106,6 +106,13 @@ def test_workspace(sm):
             "too many for one call")
 
 
+def test_more_tiles_than_a_launch_holds(sm):
+    """2^30 tokens of 64 x 16 heads: 2^28 tiles of 64 columns, each on 64 kv heads."""
+    rows = query(sm, heads=1024, ldq=1 << 16, ldo=1 << 16)
+    refused(sm, sm.lib().sparkmv_kv_attend(ref(cache(sm, kv_heads=64)), ref(batch(sm, ntok=1 << 30, qstart=P, max_q=64)), ref(rows), None),
+            "too much for one call")
+
+
 def test_null_structures_and_empty_calls(sm):
     L = sm.lib()
     c, b, n, q = cache(sm), batch(sm), new(sm), query(sm)
