@@ -144,6 +144,72 @@ def attend(cache, q, hd, scale, window, gate, pos, qstart=None, slot=None, max_q
     return out, size
 
 
+def seen_rows(cache, hd, window, pos, qstart=None, slot=None, max_q=1 << 30, ntok=None):
+    """(row, kv head, keys, values) of every token of a call and kv head: what it
+    sees, [positions, hd] in f64."""
+    npages, kvh, _ = cache["k"].shape
+    off = offsets(hd)
+    for s, p0, row, n in sequences(cache, pos, qstart, slot, ntok, max_q if qstart is not None else 1):
+        for j in range(n):
+            p = p0 + j
+            at = np.arange(max(0, p + 1 - window) if window else 0, p + 1)
+            page = cache["pages"][s, at // PAGE].astype(int)
+            at, page = at[(page >= 0) & (page < npages)], page[(page >= 0) & (page < npages)]
+            for h in range(kvh):
+                yield (row + j, h) + tuple(
+                    np.take_along_axis(cache[m][page, h], off[w][at % PAGE], 1).astype(np.float64)
+                    * cache[m + "_scale"][page, h].astype(np.float64)[:, None] for w, m in enumerate("kv"))
+
+
+def attend_one(q, k, v, scale):
+    """(out, weights, scores) of one query [hd] over keys and values [n, hd]."""
+    s = k @ q * scale
+    w = np.exp(s - s.max())
+    w /= w.sum()
+    return w @ v, w, s
+
+
+def attend_digits(q, k, v, scale, q_bits, w_bits, of_sum):
+    """attend_one with the query and the weights as integers: q_bits below the
+    power of two over the largest element; w_bits of each 64 positions' largest
+    weight or, with of_sum, of their sum. Everything else in 64 bits."""
+    ex = np.frexp(np.abs(q).max())[1]
+    s = k @ np.rint(np.ldexp(q, q_bits - ex)) * np.ldexp(scale, int(ex) - q_bits)
+    o, l, M = 0.0, 0.0, s.max()
+    for a in range(0, len(s), PAGE):
+        m = s[a:a + PAGE].max()
+        p = np.exp(s[a:a + PAGE] - m)
+        unit = 2.0 ** -w_bits * (p.sum() if of_sum else 1.0)
+        o = o + np.exp(m - M) * (np.rint(p / unit) * unit @ v[a:a + PAGE])
+        l = l + np.exp(m - M) * p.sum()
+    return o / l
+
+
+def attend_bound(q, k, v, scale, bf16):
+    """How far an element of attend_one may be off, from the roundings that the
+    call makes, u = 2^-24. With S the largest |score|, Q = largest |q| times the
+    largest sum |k|, scaled, W the weighted sum of |v|, V the largest |v|, n positions:
+      scores: the query's integer 2^-30 Q; three sums of digits' products, which
+      are |score| and Q / 31 at most; five roundings of factors; the reference's
+      and the difference's, 3 S; in the exponents of a page's, a share's and the
+      join's factors 3 S each; each exponential 2 u: (21 S + Q / 8 + 10) u in all.
+      A weight is off by that, relative to it, and so is their sum;
+      sums over positions: two roundings a page in each of the two sums, and as
+      many in a join, n / 16, and 32 for lanes, factors, division and gate;
+      weights: 2^-30 of the largest of 64, u V.
+    With bf16 outputs the query may be held to 2^-22 of its largest element, a
+    weight to half of 2^-22.9 of its 64 positions' sum, 2^-17 V of all 64, and the
+    output is rounded to half a step, 2^-8."""
+    out, w, s = attend_one(q, k, v, scale)
+    S, W, V = np.abs(s).max(), w @ np.abs(v), np.abs(v).max(0)
+    Q = np.abs(q).max() * np.abs(k).sum(1).max() * abs(scale)
+    b = 2.0 ** -24 * (W * (2 * (21 * S + Q / 8 + 10) + len(s) / 16 + 32) + V)
+    if bf16:
+        b = b + 2 * 2.0 ** -22 * Q * W + 2.0 ** -17 * V
+        b = b + 2.0 ** -8 * (np.abs(out) + b)
+    return b
+
+
 def logprobs(x, tokens, k):
     """Rows of logits (f64): log probabilities of tokens, entropies, and the k
     largest logits' ids and log probabilities."""

@@ -9,17 +9,22 @@
  * (256 * 127 * 128 < 2^23), and D digits' sums make the product.
  *
  *   A query element is an integer at a power of two that the head's largest
- *   element sets: 31 bits with four digits, more than f32 holds; 15 with two.
+ *   element sets: 31 bits with four digits, more than f32 holds; 23 with three,
+ *   f32's own 24 bits of the largest element to within one.
  *
  *   A weight e^(s - m) takes as m the largest score of its own page, so its
- *   integer (31 or 15 bits) is fine against the page's largest weight whatever
- *   the rest of the sequence holds. The page's sum enters the f32 output times
- *   value scale * e^(m - M), where M, a running reference, moves only when a
- *   page passes it by 2^kKvLag.
+ *   integer is fine against the page's weights whatever the rest of the sequence
+ *   holds: with four digits 31 bits of the page's largest, with three 23 bits of
+ *   the page's sum. The page's sum enters the f32 output times value scale *
+ *   e^(m - M), where M, a running reference, moves only when a page passes it by
+ *   2^kKvLag.
  *
- * Four digits serve f32 outputs; two (2^-15, under bf16's half step of 2^-9
- * even where 64 weights add up) serve bf16 ones, except where four cost
- * nothing. Scores, weights' sums and outputs are f32. */
+ * Four digits serve f32 outputs; three serve bf16 ones, except where four cost
+ * nothing. Two would be enough only for rows without outliers: with one query
+ * element 100 times the others 15 bits of it leave their scores off by 1 %, and
+ * where the first position has nearly all the weight (and next to no value)
+ * those of the others are a few steps of 2^-15 each. Scores, weights' sums and
+ * outputs are f32. */
 #include "kv.h"
 
 #include <math.h>
@@ -619,11 +624,11 @@ __global__ __launch_bounds__(512) void kv_flat_join_kernel(const KvFlat A) {
  * an instruction of its own here, on the same codes. Work that is split over the
  * pages is joined by a second launch.
  *
- * A chunk of 512 tokens at 16384 (16 query, 4 kv heads of 256, bf16 out): 193 us for
- * 140 GFLOP, bound by the vector instructions around the products (414 a wave and
- * page, half of them the values' sums from i32; VALU 62 % busy, MFMA 31). Six waves
- * a workgroup, for three a SIMD, took 294: they do not fill the SIMDs evenly. Three
- * blocks of 8 at 6001 (f32 out): 18.8 us and 6.9 for the join. */
+ * A chunk of 512 tokens at 16384 (16 query, 4 kv heads of 256, bf16 out): the call
+ * takes 235 us for 140 GFLOP, 298 with f32 outputs and their four digits; bound by the
+ * vector instructions around the products, half of them the values' sums from i32.
+ * Six waves a workgroup, for three a SIMD, took half as long again: they do not fill
+ * the SIMDs evenly. Three blocks of 8 at 6001 (f32 out): 18.8 us and 6.9 for the join. */
 struct KvTile {
     sparkmv_kv_cache c;
     sparkmv_kv_batch b;
@@ -677,8 +682,10 @@ __device__ __forceinline__ bool kv_find_tile(const sparkmv_kv_batch & b, const s
 template <int HD, int D, int WQ>
 __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
     constexpr int NC = HD / 64, WD = 4 / WQ, ND = HD / 16 / WD, HALF = kKvPage * HD;
-    constexpr float PMAX = D == 2 ? 32512.0f : 1073741824.0f;   /* a weight of 1: 127 * 256, or 2^30 */
-    constexpr uint32_t BIAS = D == 2 ? 0x80u : 0x808080u;
+    /* what a weight of 1, or all of a page's weights together, becomes: 2^30; below
+     * 0x7f7f7f by what the f32 roundings may add, so that three digits hold it */
+    constexpr float PMAX = D == 3 ? 8355584.0f : 1073741824.0f;
+    constexpr uint32_t BIAS = D == 3 ? 0x8080u : 0x808080u;
     typedef __attribute__((address_space(3))) void lds_void;
     extern __shared__ __attribute__((aligned(16))) uint8_t lbuf[];   /* [2][keys, values] */
     __shared__ int lfind[8];
@@ -745,7 +752,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
 #pragma unroll
         for (int c = 0; c < NC; c++) kv_load16(A.q, at + 64 * c, x[c]);
         const int ex = kv_q_exponent<NC>(x, qbad);
-        constexpr int B = D == 2 ? 14 : 30;
+        constexpr int B = D == 3 ? 22 : 30;
         /* a negative scale turns the queries, so that scores grow with their sums */
         const float sign = A.q.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
@@ -764,10 +771,20 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
             }
         cs = ldexpf(fabsf(A.q.scale) * kKvLog2e, ex - B);
     }
-    /* the value of a product's digit sums */
-    auto value = [&](const kv_i4 * a, int e) -> float {
-        if constexpr (D == 2) return (float) (a[0][e] * 256 + a[1][e]);
+    /* the value of a product's digit sums: of a score; of a page's output, which
+     * with three digits is below 127 * 2^23 */
+    auto score = [&](const kv_i4 * a, int e) -> float {
+        if constexpr (D == 3) return fmaf((float) (a[0][e] * 256 + a[1][e]), 256.0f, (float) a[2][e]);
         else return fmaf((float) (a[0][e] * 256 + a[1][e]), 65536.0f, (float) (a[2][e] * 256 + a[3][e]));
+    };
+    auto value = [&](const kv_i4 * a, int e) -> float {
+        if constexpr (D == 3) {
+            int hi = a[0][e] * 256 + a[1][e];
+            asm("" : "+v"(hi));   /* two shifted adds: as one sum it takes three instructions */
+            return (float) (hi * 256 + a[2][e]);
+        } else {
+            return score(a, e);
+        }
     };
     float m = -INFINITY, l = 0.0f;
     kv_f4 o[ND];
@@ -801,7 +818,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
                 for (int d = 0; d < D; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qd[d][c], acc[d], 0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[t][e] = value(acc, e);
+            for (int e = 0; e < 4; e++) x[t][e] = score(acc, e);
         }
         if (p0 < wbeg_hi || p0 + kKvPage - 1 > wpos_lo || kscale != kscale) {
             bool any = false;
@@ -835,15 +852,28 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         kv_i4 P[D];
         float sum = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            uint32_t y[4];
+        for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(x[t][e], f, -mref));
-                sum += p;
-                /* rounded, and the digits' bias: 32768.5 is exact in f32, 2^30 + 0x808080 is not */
-                y[e] = D == 2 ? (uint32_t) (int) (p * PMAX + (0.5f + BIAS)) : (uint32_t) (int) (p * PMAX) + BIAS;
+                x[t][e] = __builtin_amdgcn_exp2f(fmaf(x[t][e], f, -mref));
+                sum += x[t][e];
             }
+        /* the integer of a weight of 1, and back: with three digits what makes the
+         * page's weights PMAX together */
+        float up = PMAX, down = 1.0f / PMAX;
+        if constexpr (D == 3) {
+            const float all = kv_rows_sum(sum);
+            up = all > 0.0f ? PMAX * __builtin_amdgcn_rcpf(all) : 0.0f;
+            down *= all;
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            uint32_t y[4];
+            /* with the digits' bias. Three: 2^23 more leaves the nearest integer in the
+             * lower bits of the f32; 2^30 + 0x808080 would not be exact */
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                y[e] = D == 3 ? __float_as_uint(fmaf(x[t][e], up, 8388608.0f + BIAS)) : (uint32_t) (int) (x[t][e] * up) + BIAS;
 #pragma unroll
             for (int d = 0; d < D; d++) {
                 const uint32_t b = D - 1 - d, sel = b | (b + 4) << 8 | 0x0c0c0000u;
@@ -853,7 +883,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
         }
         const float step = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - m);
         l += sum * step;
-        const float w = mp == -INFINITY ? 0.0f : step * vscale * (1.0f / PMAX);
+        const float w = mp == -INFINITY ? 0.0f : step * vscale * down;
         if (vscale == vscale) {
 #pragma unroll
             for (int d = 0; d < ND; d++) {
@@ -1102,7 +1132,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
 #define KV_TILE_D(H, W)                                                                                              \
     do {                                                                                                             \
         if (q.out_dtype == SPARKMV_X_F32) KV_TILE(H, 4, W);                                                          \
-        else KV_TILE(H, 2, W);                                                                                       \
+        else KV_TILE(H, 3, W);                                                                                       \
     } while (0)
 #define KV_TILE_W(H)                                                                                                 \
     do {                                                                                                             \
