@@ -840,6 +840,15 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
 #pragma unroll
             for (int e = 0; e < 4; e++) mp = fmaxf(mp, x[t][e]);
         mp = kv_rows_max(mp) * f;
+        /* a large score times f, not rounded, may lie above the reference by more than a
+         * digit holds: 2^-9 at 2^16, 1 at 2^25 */
+        if (D == 4 && __any(fabsf(mp) >= 0x1p16f)) {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[t][e] *= f;
+            f = 1.0f;
+        }
         if (__any(mp > m + kKvLag)) {
             const float mn = fmaxf(m, mp);
             const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);

@@ -44,3 +44,29 @@ def test_outliers_and_sinks(sm, dev, kind, form, kvh, group, hd, x, o):
             most = max(most, (np.abs(got[row, g] - want) / paged.attend_bound(qf[row, g], k, v, hd ** -0.5, o == "bf16")).max())
     print(f"{kind} {form} kvh {kvh} group {group} hd {hd} {x} {o}: {most:.3f} of the bound")
     assert most <= 1
+
+
+@pytest.mark.parametrize("size", [3.0e5, 3.0e8])
+@pytest.mark.parametrize("x,o", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("kvh,group,hd", [(2, 4, 256), (1, 16, 64), (8, 4, 128)])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_very_large_scores(sm, dev, form, kvh, group, hd, x, o, size):
+    """Each query is a multiple of the key at one of its positions, with a score
+    of `size` there: that position has all the weight, the others' scores being
+    lower by a tenth of it at least, and the output is its value. Off by the
+    weight's integer, 2^-23, the division and the gate, a few 2^-24, and a bf16
+    output's half step."""
+    pos, qstart = FORMS[form]
+    c, q = scene("outlier", kvh, group, hd, 7 * hd + kvh, qstart or [0, 1, 2, 3])
+    rng, want = np.random.default_rng(3), np.zeros(q.shape)
+    for row, h, k, v in paged.seen_rows(c, hd, 0, pos, qstart, ntok=len(q)):
+        for g in range(h * group, (h + 1) * group):
+            at = rng.integers(len(k))
+            unit = k[at] / (k[at] @ k[at] * hd ** -0.5)
+            at = np.argmax(k @ unit)     # a longer key may score more
+            q[row, g], want[row, g] = unit * size, v[at]
+            s = np.sort(k @ unit)
+            assert len(s) == 1 or s[-2] < s[-1] - 0.01
+    got, _ = run(sm, dev, c, q, hd, pos, qstart, x, o)
+    err = np.abs(got - want)
+    assert np.all(err <= np.abs(want) * (8 * 2.0 ** -24 + 2.0 ** -22 + (2.0 ** -8 if o == "bf16" else 0.0))), float(err.max())
