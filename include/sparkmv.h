@@ -549,7 +549,8 @@ typedef struct {
 
 /* The sequences of one call: sequence i is slot[i] (NULL: slot i), its new
  * tokens are rows qstart[i] .. qstart[i + 1] - 1 of the call's ntok rows (NULL:
- * row i alone) at positions pos[i] .. A negative pos leaves the sequence out.
+ * row i alone) at positions pos[i] .. A negative pos, or rows that end before
+ * they begin, leave the sequence out; no row is in two sequences.
  * Rows of no sequence are left as they were. max_q bounds the new tokens of
  * one sequence (further ones are left out); max_len is the longest length
  * after the call as far as the host knows: it shapes launches only, and a

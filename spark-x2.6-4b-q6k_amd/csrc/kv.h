@@ -27,8 +27,8 @@ __host__ __device__ inline int kv_value_at(int pos, int d, int hd) {
 /* One sequence of a batch as a kernel reads it: its slot, the position of its
  * first new token and its rows of the call's tokens. count is 0 for a
  * sequence that the call leaves out: a negative position, a slot outside the
- * table, rows outside the call's. Tokens past max_q are left out, and so are
- * positions past the page table. */
+ * table, rows outside the call's, or that end before they begin. Tokens past max_q
+ * are left out, and so are positions past the page table. */
 struct KvSeq {
     int slot, pos, row, count;
 };
@@ -39,7 +39,8 @@ __device__ __forceinline__ KvSeq kv_seq(const sparkmv_kv_batch & b, int i, int n
     s.pos = b.pos[i];
     s.row = b.qstart ? b.qstart[i] : i;
     int end = b.qstart ? b.qstart[i + 1] : i + 1;
-    if (s.slot < 0 || s.slot >= nslots || s.pos < 0 || s.row < 0 || end > b.ntok) end = s.row;
+    /* the last test keeps the difference below from wrapping */
+    if (s.slot < 0 || s.slot >= nslots || s.pos < 0 || s.row < 0 || end > b.ntok || end < s.row) end = s.row;
     s.count = max(0, min(min(end - s.row, b.max_q), max_pages * kKvPage - s.pos));
     return s;
 }
