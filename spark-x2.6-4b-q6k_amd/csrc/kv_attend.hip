@@ -988,6 +988,7 @@ __global__ __launch_bounds__(256) void kv_tile_join_kernel(const KvTile A, int c
 /* -------------------------------------------------------------------- host */
 
 struct KvPlan {
+    int max_q;                /* the batch's, at most its rows */
     int flat;                 /* the few-column kernel: 1 shares, 2 whole kv heads */
     int groups, least;        /* its workgroups and least share */
     long tiles;
@@ -997,8 +998,9 @@ struct KvPlan {
 
 KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads, int window) {
     KvPlan p = {};
-    const int G = heads / c->kv_heads, max_q = b->qstart ? (b->max_q < b->ntok ? b->max_q : b->ntok) : 1;
-    const long cols = (long) (max_q > 0 ? max_q : 1) * G, hd = c->head_dim;
+    const int G = heads / c->kv_heads;
+    p.max_q = b->qstart ? (b->max_q < b->ntok ? b->max_q : b->ntok) : 1;
+    const long cols = (long) p.max_q * G, hd = c->head_dim;
     long len = b->max_len > 0 ? b->max_len : (long) c->max_pages * kKvPage;
     const long pages = (len + kKvPage - 1) / kKvPage;
     size_t off = 0;
@@ -1089,14 +1091,14 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     }
     hipStream_t s = (hipStream_t) stream;
     uint8_t * mem = (uint8_t *) q.work;
-    const int max_q = batch->qstart ? batch->max_q : 1, hd = cache->head_dim;
+    const int hd = cache->head_dim;
     if (p.flat) {
         KvFlat f;
         f.c = *cache; f.b = *batch; f.q = q;
-        f.b.max_q = max_q;
+        f.b.max_q = p.max_q;
         f.least = p.least;
         f.pre = (int *) (mem + p.pre); f.po = (float *) (mem + p.po); f.pml = (float *) (mem + p.pml);
-        const dim3 join((unsigned) batch->nseq, (unsigned) cache->kv_heads, (unsigned) (max_q * (q.heads / cache->kv_heads)));
+        const dim3 join((unsigned) batch->nseq, (unsigned) cache->kv_heads, (unsigned) (p.max_q * (q.heads / cache->kv_heads)));
         const uint32_t pre = batch->nseq > 64 ? ((uint32_t) batch->nseq + 1) * 4 : 0;
 #define KV_FLAT_N(H, W, GRID, LDS)                                                                                   \
     do {                                                                                                             \
@@ -1123,7 +1125,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     }
     KvTile t;
     t.c = *cache; t.b = *batch; t.q = q;
-    t.b.max_q = max_q;
+    t.b.max_q = p.max_q;
     t.nsplit = p.nsplit;
     t.po = (float *) (mem + p.po); t.pml = (float *) (mem + p.pml);
     const long th = p.tiles * cache->kv_heads;

@@ -34,3 +34,26 @@ def test_row_starts_that_fall(sm, dev, group, max_q):
     assert np.array_equal(got, np.where(np.isnan(want), 7.0, want).astype(np.float32).astype(np.float64))
     c.kv.attend(b, q, out)
     check_attention(c, q, qf, out, 0.125, 0, None, pos, qstart, None, most, f"group {group} max_q {max_q}")
+
+
+@pytest.mark.parametrize("max_q", [5, 512, 20000, 1 << 30, (1 << 31) - 1])
+@pytest.mark.parametrize("counts,group", [([1], 4), ([2], 2), ([1, 2, 1], 1), ([0, 1], 4), ([5, 9], 4)])
+def test_max_q_far_above_the_rows(sm, dev, counts, group, max_q):
+    """max_q only bounds: a context long enough to be split among workgroups
+    and joined, with bounds that no launch could take for a size."""
+    import torch
+    kvh, hd = 2, 64
+    n = len(counts)
+    c = Case(sm, dev, kvh, hd, n, 50, 97)
+    qstart = np.concatenate([[0], np.cumsum(counts)])
+    ntok = int(qstart[-1])
+    pos = [3000, 40, 2900][:n]
+    q, qf = rows(dev, c.rng.standard_normal((ntok, kvh * group, hd)), torch.float32)
+    k, kf = rows(dev, c.rng.standard_normal((ntok, kvh, hd)), torch.float32)
+    b = c.batch(pos, ntok, qstart, max_q=max_q, max_len=3100)
+    c.kv.append(b, None, k, k)
+    paged.append(c.host, None, kf, kf, None, pos, qstart, None, max_q)
+    c.same()
+    out = torch.full_like(q, 7.0)
+    c.kv.attend(b, q, out)
+    check_attention(c, q, qf, out, 0.125, 0, None, pos, qstart, None, max_q, f"{counts} group {group} max_q {max_q}")
