@@ -645,6 +645,8 @@ class Model:
     a device uint8 tensor of Q8_0 blocks; final_norm a device f32 tensor.
     The model keeps references to everything it was given."""
 
+    paged_device = None   # of the paged cache, once there is one
+
     def __init__(self, cfg, layers, head, final_norm):
         c = ModelCfg(**cfg)
         self.cfg = dict(cfg)
@@ -742,7 +744,9 @@ class Model:
     def paged(self, npages, nslots, max_pages):
         """Make the paged 8-bit cache of several sequences (sparkmv_model_paged),
         beside the f32 cache of forward and verify."""
+        torch = _torch()
         check(lib().sparkmv_model_paged(self.h, int(npages), int(nslots), int(max_pages)), "model paged")
+        self.paged_device = torch.device("cuda", torch.cuda.current_device())
 
     def set_pages(self, slot, pages, stream=None):
         """The slot's pages, in the order of their positions (64 each)."""
@@ -759,7 +763,8 @@ class Model:
             raise SparkmvError(f"model paged step: {len(tokens)} token lists and {len(pos)} positions for {n} slots")
         if logits is not None:
             torch = _torch()
-            _kv_flat("paged step logits", logits, (torch.float32,), (len(flat) if every else n, self.cfg["vocab"]), None)
+            _kv_flat("paged step logits", logits, (torch.float32,), (len(flat) if every else n, self.cfg["vocab"]),
+                     self.paged_device)
         ints = lambda v: (_I * max(1, len(v)))(*[int(x) for x in v])  # noqa: E731
         check(lib().sparkmv_model_paged_step(self.h, (ctypes.c_uint32 * max(1, len(flat)))(*flat), n, ints(slots), ints(pos),
                                              ints([len(t) for t in tokens]), int(bool(every)), _ptr(logits),
@@ -767,18 +772,11 @@ class Model:
 
     def paged_read(self, layer, start, k_out, v_out, slot=None, stream=None):
         """Cached positions of a layer as PagedKV.read gives them: start and slot
-        device int32, k_out and v_out [nseq, n, kv_heads, head_dim]."""
-        torch = _torch()
+        device int32, k_out and v_out [nseq, n, kv_heads, head_dim], f32 or bf16
+        (either may be None)."""
         c = KvCache()
         check(lib().sparkmv_model_paged_cache(self.h, int(layer), ctypes.byref(c)), "model paged cache")
-        _kv_flat("paged read start", start, (torch.int32,), (None,), None)
-        for t in (k_out, v_out):
-            _kv_flat("paged read", t, (k_out.dtype,), (start.shape[0], k_out.shape[1], c.kv_heads, c.head_dim), start.device)
-        if slot is not None:
-            _kv_flat("paged read slots", slot, (torch.int32,), (start.shape[0],), start.device)
-        check(lib().sparkmv_kv_read(ctypes.byref(c), start.shape[0], _ptr(slot), start.data_ptr(), k_out.shape[1],
-                                    k_out.data_ptr(), v_out.data_ptr(), X_F32 if k_out.dtype == torch.float32 else X_BF16,
-                                    _stream_ptr(stream)), "model paged read")
+        _kv_read_call(c, start, k_out, v_out, slot, self.paged_device, "model paged read", ())(stream)
 
     def apply_profile(self, profile, artifact, gpu):
         n = lib().sparkmv_model_apply_profile(self.h, profile.h, artifact, gpu.encode())
@@ -897,6 +895,27 @@ def _kv_rows(what, t, dtypes, heads, head_dim, device):
     return t.shape[0], t.stride(0) if t.shape[0] > 1 else heads * head_dim
 
 
+def _kv_read_call(c, start, k_out, v_out, slot, device, what, keep):
+    """The call that reads positions of the cache c (a KvCache) on a device, or
+    where start is, into the outputs that are given."""
+    torch = _torch()
+    i32, ft = (torch.int32,), (torch.float32, torch.bfloat16)
+    outs = [t for t in (k_out, v_out) if t is not None]
+    if not outs:
+        raise SparkmvError(what + ": nothing to read into")
+    _kv_flat(what + " start", start, i32, (None,), device)
+    n = outs[0].shape[1] if outs[0].dim() == 4 else None
+    for t in outs:
+        _kv_flat(what, t, ft, (start.shape[0], n, c.kv_heads, c.head_dim), start.device)
+        if t.dtype != outs[0].dtype:
+            raise SparkmvError(what + ": keys and values of two types")
+    if slot is not None:
+        _kv_flat(what + " slots", slot, i32, (start.shape[0],), start.device)
+    return _Call(lib().sparkmv_kv_read,
+                 (ctypes.addressof(c), start.shape[0], _ptr(slot), start.data_ptr(), n, _ptr(k_out), _ptr(v_out),
+                  X_F32 if outs[0].dtype == torch.float32 else X_BF16), start.device, what, (keep, c, start, k_out, v_out, slot))
+
+
 def rope_table(rows, rope_dim, theta, device="cuda", stream=None):
     """[rows, rope_dim] f32: cos then sin of position * theta^(-2 i / rope_dim)
     (sparkmv_rope_table, the model's own expressions)."""
@@ -1004,22 +1023,7 @@ class PagedKV:
     def read_op(self, start, k_out=None, v_out=None, slot=None):
         """The call that reads positions start[i] .. of slot[i] (None: slot i) into
         k_out and v_out ([nseq, n, kv_heads, head_dim], f32 or bf16)."""
-        torch = _torch()
-        i32, ft = (torch.int32,), (torch.float32, torch.bfloat16)
-        outs = [t for t in (k_out, v_out) if t is not None]
-        if not outs:
-            raise SparkmvError("kv read: nothing to read into")
-        _kv_flat("kv read start", start, i32, (None,), self.device)
-        for t in outs:
-            _kv_flat("kv read", t, ft, (start.shape[0], outs[0].shape[1], self.kv_heads, self.head_dim), self.device)
-            if t.dtype != outs[0].dtype:
-                raise SparkmvError("kv read: keys and values of two types")
-        if slot is not None:
-            _kv_flat("kv read slots", slot, i32, (start.shape[0],), self.device)
-        return _Call(lib().sparkmv_kv_read,
-                     (ctypes.addressof(self.c), start.shape[0], _ptr(slot), start.data_ptr(), outs[0].shape[1],
-                      _ptr(k_out), _ptr(v_out), X_F32 if outs[0].dtype == torch.float32 else X_BF16),
-                     self.device, "kv read", (self, start, k_out, v_out, slot))
+        return _kv_read_call(self.c, start, k_out, v_out, slot, self.device, "kv read", self)
 
     def read(self, start, k_out=None, v_out=None, slot=None, stream=None):
         self.read_op(start, k_out, v_out, slot)(stream)
