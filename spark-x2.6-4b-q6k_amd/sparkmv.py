@@ -18,6 +18,7 @@ Interface mirror (the reference's Rust surface this stands beside):
   Model.forward            tools/vq-runtime/src/model.rs:441-591 (Model::forward),
                            as the GPU runtime runs it, tools/vq/gpu/vq-model-gpu.cu:776-835
 """
+import contextlib
 import ctypes
 import os
 
@@ -859,13 +860,20 @@ class _Call:
             raise SparkmvError(f"{self.what}: {last_error()}")
 
 
-def _used_on(stream, *tensors):
-    """Tensors made here on the current stream and used on the caller's: their
-    memory is not handed out again before that stream's work is done"""
+def _made_on(stream):
+    """Tensors made inside belong to the stream (None: the current one) that a
+    call will use: their memory waits for no other stream's earlier work, and is
+    not handed out again before the call is done"""
+    return contextlib.nullcontext() if stream is None else _torch().cuda.stream(stream)
+
+
+def _returned(stream, device, *tensors):
+    """Tensors that were made on the given stream and will be read on the current
+    one: their memory is not handed out again before that is done"""
     if stream is not None:
         for t in tensors:
             if t is not None:
-                t.record_stream(stream)
+                t.record_stream(_torch().cuda.current_stream(device))
 
 
 def _kv_tensor(what, t, dtypes, shape, device):
@@ -920,9 +928,11 @@ def rope_table(rows, rope_dim, theta, device="cuda", stream=None):
     """[rows, rope_dim] f32: cos then sin of position * theta^(-2 i / rope_dim)
     (sparkmv_rope_table, the model's own expressions)."""
     torch = _torch()
-    out = torch.empty((rows, rope_dim), dtype=torch.float32, device=device)
+    with _made_on(stream):
+        out = torch.empty((rows, rope_dim), dtype=torch.float32, device=device)
     with torch.cuda.device(out.device):
         check(lib().sparkmv_rope_table(out.data_ptr(), rows, rope_dim, float(theta), _stream_ptr(stream)), "rope table")
+    _returned(stream, out.device, out)
     return out
 
 
@@ -1064,9 +1074,9 @@ class PagedKV:
                      self.device, "kv attend", (self, batch, q, out, gate, work, n))
 
     def attend(self, batch, q, out, scale=None, window=0, gate=None, work=None, stream=None):
-        op = self.attend_op(batch, q, out, scale, window, gate, work)
+        with _made_on(stream):
+            op = self.attend_op(batch, q, out, scale, window, gate, work)
         op(stream)
-        _used_on(stream, op.keep[5])
 
 
 def logprobs_op(logits, tokens=None, logprob=None, entropy=None, top_id=None, top_logprob=None, work=None):
@@ -1108,11 +1118,12 @@ def logprobs(logits, tokens=None, k=0, stream=None):
     torch = _torch()
     rows, dev = logits.shape[0], logits.device
     f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
-    lp = f(rows) if tokens is not None else None
-    ent, ids, tops = f(rows), torch.empty((rows, k), dtype=torch.int32, device=dev), f(rows, k)
-    op = logprobs_op(logits, tokens, lp, ent, ids, tops)
+    with _made_on(stream):
+        lp = f(rows) if tokens is not None else None
+        ent, ids, tops = f(rows), torch.empty((rows, k), dtype=torch.int32, device=dev), f(rows, k)
+        op = logprobs_op(logits, tokens, lp, ent, ids, tops)
     op(stream)
-    _used_on(stream, lp, ent, ids, tops, op.keep[6])
+    _returned(stream, dev, lp, ent, ids, tops)
     return lp, ent, ids, tops
 
 

@@ -57,3 +57,72 @@ def test_max_q_far_above_the_rows(sm, dev, counts, group, max_q):
     out = torch.full_like(q, 7.0)
     c.kv.attend(b, q, out)
     check_attention(c, q, qf, out, 0.125, 0, None, pos, qstart, None, max_q, f"{counts} group {group} max_q {max_q}")
+
+
+class Busy:
+    """A block of memory that work queued on the current stream reads late, and
+    that was handed back before: whoever gets it has to come after that work."""
+
+    def __init__(self, dev, nbytes):
+        import torch
+        a = torch.ones(4096, 4096, device=dev)
+        block = torch.full((nbytes,), 5, dtype=torch.uint8, device=dev)
+        a @ a
+        torch.cuda.synchronize()
+        for _ in range(20):     # some milliseconds
+            a = a @ a * 1e-4
+        self.read = block.clone()
+
+    def check(self):
+        import torch
+        torch.cuda.synchronize()
+        assert torch.all(self.read == 5)
+
+
+def operators(sm, dev):
+    """(name, workspace bytes, one-shot call, its op, check) of the calls that make a workspace."""
+    import torch
+    c = Case(sm, dev, 2, 128, 2, 40, 101)
+    pos, heads = [2500, 2400], 8
+    q, qf = rows(dev, c.rng.standard_normal((2, heads, 128)), torch.float32)
+    out = torch.full((2, heads, 128), 7.0, device=dev)
+    b = c.batch(pos, max_len=2501)
+    x = torch.from_numpy(c.rng.standard_normal((64, 20000)).astype(np.float32)).to(dev)
+    want = torch.log_softmax(x.double().cpu(), 1)
+    tok = torch.zeros(64, dtype=torch.int32, device=dev)
+    lp, ent = torch.zeros(64, device=dev), torch.zeros(64, device=dev)
+    ids, tops = torch.zeros(64, 5, dtype=torch.int32, device=dev), torch.zeros(64, 5, device=dev)
+
+    def attended():
+        check_attention(c, q, qf, out, 128 ** -0.5, 0, None, pos, None, None, note="attention")
+        out.fill_(7.0)
+
+    def answered(got):
+        assert float((got[0].double().cpu() - want[:, 0]).abs().max()) <= 1e-4     # as tests/test_gpu_paged_model.py
+        assert torch.equal(got[2][:, 0].cpu().long(), want.argmax(1))
+
+    need = sm.lib().sparkmv_kv_attend_work(sm.ctypes.addressof(c.kv.c), sm.ctypes.addressof(b.c), heads)
+    yield ("attend", need, lambda s: c.kv.attend(b, q, out, stream=s), lambda: c.kv.attend_op(b, q, out), lambda got: attended())
+    yield ("logprobs", sm.lib().sparkmv_logprobs_work(64, 20000, 5), lambda s: sm.logprobs(x, tok, 5, stream=s),
+           lambda: sm.logprobs_op(x, tok, lp, ent, ids, tops), lambda got: answered(got or (lp, ent, ids, tops)))
+
+
+def test_calls_on_another_stream_make_their_memory_there(sm, dev):
+    """A call on a given stream takes no memory that the current stream's earlier
+    work is still reading; what it returns may be read on the current stream."""
+    import torch
+    s = torch.cuda.Stream(device=dev)
+    for name, need, call, _, check in operators(sm, dev):
+        s.wait_stream(torch.cuda.current_stream())
+        call(s)     # loaded and warm
+        torch.cuda.synchronize()
+        busy = Busy(dev, need)
+        got = call(s)
+        torch.cuda.current_stream().wait_stream(s)
+        busy.check()
+        check(got)
+    busy = Busy(dev, 1 << 20)
+    table = sm.rope_table(4096, 64, 1e4, dev, stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    busy.check()
+    assert torch.equal(table, sm.rope_table(4096, 64, 1e4, dev))
