@@ -841,9 +841,11 @@ def argmax(logits, stream=None):
 class _Call:
     """One operator's call with its arguments laid out once: call it (on the
     current stream, or the given one) as often as the tensors it holds change
-    their values. It runs on the device of its tensors."""
+    their values. It runs on the device of its tensors. A workspace made with it
+    (`made`) may be used on any stream, but not by two at once; keep the call as
+    long as a graph that recorded it is replayed."""
 
-    def __init__(self, fn, args, device, what, keep):
+    def __init__(self, fn, args, device, what, keep, made=None):
         torch = _torch()
         self.fn, self.args, self.what, self.keep = fn, args, what, keep
         self.device = device.index if device.index is not None else torch.cuda.current_device()
@@ -851,12 +853,37 @@ class _Call:
         self.raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda d: torch.cuda.current_stream(d).cuda_stream)
         self.current = torch.cuda.current_device
+        self.made = made
+        if made is not None:
+            home = torch.cuda.current_stream(self.device)
+            self.used, self.ready = {home.cuda_stream}, None
+            with torch.cuda.device(self.device):
+                if not torch.cuda.is_current_stream_capturing():
+                    self.ready = home.record_event()
+
+    def _first_use(self, raw, stream):
+        """The workspace's memory may still be read by earlier work of the stream it
+        was made on, and may not be handed out again before this one's is done. A
+        stream that records a graph runs nothing yet: its graph's replays come
+        after that work as everything else the graph reads does."""
+        torch = _torch()
+        stream = torch.cuda.current_stream(self.device) if stream is None else stream
+        with torch.cuda.stream(stream):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        if self.ready is not None:
+            stream.wait_event(self.ready)
+        self.made.record_stream(stream)
+        self.used.add(raw)
 
     def __call__(self, stream=None):
         if self.current() != self.device:
             with _torch().cuda.device(self.device):
                 return self(stream)
-        if self.fn(*self.args, self.raw(self.device) if stream is None else stream.cuda_stream) != 0:
+        raw = self.raw(self.device) if stream is None else stream.cuda_stream
+        if self.made is not None and raw not in self.used:
+            self._first_use(raw, stream)
+        if self.fn(*self.args, raw) != 0:
             raise SparkmvError(f"{self.what}: {last_error()}")
 
 
@@ -1045,6 +1072,10 @@ class PagedKV:
         sees, its own included (0: all). gate: f32 [ntok, heads]; a head's output
         times its sigmoid. work: uint8 tensor (None: made here); calls that may
         overlap need one each."""
+        return self._attend_call(batch, q, out, scale, window, gate, work, True)
+
+    def _attend_call(self, batch, q, out, scale, window, gate, work, again):
+        """again: the call may be used more than once, on other streams too"""
         torch = _torch()
         self._same(batch)
         ft = (torch.float32, torch.bfloat16)
@@ -1065,17 +1096,18 @@ class PagedKV:
             n.gate, n.ldg = gate.data_ptr(), gate.stride(0) if gate.shape[0] > 1 else heads
         with torch.cuda.device(self.device):
             need = lib().sparkmv_kv_attend_work(ctypes.addressof(self.c), ctypes.addressof(batch.c), heads)
+        made = None
         if work is None and need:
-            work = torch.empty(need, dtype=torch.uint8, device=self.device)
+            work = made = torch.empty(need, dtype=torch.uint8, device=self.device)
         if work is not None:
             _kv_flat("kv attend work", work, (torch.uint8,), (None,), self.device)
             n.work, n.work_bytes = work.data_ptr(), work.numel()
         return _Call(lib().sparkmv_kv_attend, (ctypes.addressof(self.c), ctypes.addressof(batch.c), ctypes.addressof(n)),
-                     self.device, "kv attend", (self, batch, q, out, gate, work, n))
+                     self.device, "kv attend", (self, batch, q, out, gate, work, n), made if again else None)
 
     def attend(self, batch, q, out, scale=None, window=0, gate=None, work=None, stream=None):
         with _made_on(stream):
-            op = self.attend_op(batch, q, out, scale, window, gate, work)
+            op = self._attend_call(batch, q, out, scale, window, gate, work, False)
         op(stream)
 
 
@@ -1084,6 +1116,10 @@ def logprobs_op(logits, tokens=None, logprob=None, entropy=None, top_id=None, to
     log probability of tokens[row] (int32), the entropy, and the top_id.shape[1]
     <= 32 largest logits' ids (int32) and log probabilities (sparkmv_logprobs);
     outputs that are None are left out."""
+    return _logprobs_call(logits, tokens, logprob, entropy, top_id, top_logprob, work, True)
+
+
+def _logprobs_call(logits, tokens, logprob, entropy, top_id, top_logprob, work, again):
     torch = _torch()
     _kv_tensor("logits", logits, (torch.float32, torch.bfloat16), (None, None), None)
     dev, (rows, n) = logits.device, logits.shape
@@ -1100,8 +1136,9 @@ def logprobs_op(logits, tokens=None, logprob=None, entropy=None, top_id=None, to
             _kv_flat("logprobs " + what, t, dt, shape, dev)
     with torch.cuda.device(dev):
         need = lib().sparkmv_logprobs_work(rows, n, k)
+    made = None
     if work is None and need:
-        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        work = made = torch.empty(need, dtype=torch.uint8, device=dev)
     if work is not None:
         _kv_flat("logprobs work", work, (torch.uint8,), (None,), dev)
     return _Call(lib().sparkmv_logprobs,
@@ -1109,7 +1146,7 @@ def logprobs_op(logits, tokens=None, logprob=None, entropy=None, top_id=None, to
                   logits.stride(0) if rows > 1 else n, _ptr(tokens), k, _ptr(logprob), _ptr(entropy),
                   _ptr(top_id) if k else None, _ptr(top_logprob) if k else None, _ptr(work),
                   0 if work is None else work.numel()),
-                 dev, "logprobs", (logits, tokens, logprob, entropy, top_id, top_logprob, work))
+                 dev, "logprobs", (logits, tokens, logprob, entropy, top_id, top_logprob, work), made if again else None)
 
 
 def logprobs(logits, tokens=None, k=0, stream=None):
@@ -1121,7 +1158,7 @@ def logprobs(logits, tokens=None, k=0, stream=None):
     with _made_on(stream):
         lp = f(rows) if tokens is not None else None
         ent, ids, tops = f(rows), torch.empty((rows, k), dtype=torch.int32, device=dev), f(rows, k)
-        op = logprobs_op(logits, tokens, lp, ent, ids, tops)
+        op = _logprobs_call(logits, tokens, lp, ent, ids, tops, None, False)
     op(stream)
     _returned(stream, dev, lp, ent, ids, tops)
     return lp, ent, ids, tops

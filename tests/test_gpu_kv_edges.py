@@ -126,3 +126,62 @@ def test_calls_on_another_stream_make_their_memory_there(sm, dev):
     torch.cuda.current_stream().wait_stream(s)
     busy.check()
     assert torch.equal(table, sm.rope_table(4096, 64, 1e4, dev))
+
+
+@pytest.mark.parametrize("how", ["given", "current"])
+def test_an_op_used_on_another_stream_than_it_was_made_on(sm, dev, how):
+    """The workspace waits for the work that had its memory before, and is not
+    handed out again while a stream that the call ran on is not done with it."""
+    import torch
+    s = torch.cuda.Stream(device=dev)
+
+    def use(op):
+        if how == "given":
+            op(s)
+        else:
+            with torch.cuda.stream(s):
+                op()
+
+    for name, need, _, make, check in operators(sm, dev):
+        s.wait_stream(torch.cuda.current_stream())
+        use(make())
+        torch.cuda.synchronize()
+        busy = Busy(dev, need)
+        op = make()
+        use(op)
+        torch.cuda.current_stream().wait_stream(s)
+        busy.check()
+        check(None)
+        # dropped while its stream still runs it: the memory's next owner keeps its values
+        op = make()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            Busy(dev, 1024)
+        use(op)
+        del op
+        after = torch.full((need,), 9, dtype=torch.uint8, device=dev)
+        torch.cuda.synchronize()
+        assert torch.all(after == 9), name
+        check(None)
+
+
+def test_ops_in_graphs_and_on_streams_by_turns(sm, dev):
+    """An op recorded on one stream, replayed, called on another and on the
+    current one: the same outputs each time."""
+    import torch
+    for name, need, _, make, check in operators(sm, dev):
+        s = torch.cuda.Stream(device=dev)
+        op = make()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            op()
+        for turn in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            check(None)
+            op(s)
+            torch.cuda.synchronize()
+            check(None)
+            op()
+            torch.cuda.synchronize()
+            check(None)
