@@ -584,8 +584,10 @@ int sparkmv_rope_table(float * table, int rows, int rope_dim, double theta, void
  *   f32(largest |new value| * h / 127),  h = 1 if the page is full after the call, else 1.25
  * (2^-126 at least) and its older codes are rounded anew to it; a code is the
  * value over the scale, rounded to nearest even. The headroom h makes a later
- * growth rare, and a value is off by at most 3 steps however often it happens:
- * half a step at each, the steps growing by 1.25 but for the last. A
+ * growth rare, and a value is off by at most 3 steps however often it happens
+ * until the page is full: half a step at each, the steps growing by 1.25 but for
+ * the last. Each further time that the page is cut back, filled again and its
+ * scale grows by that, however little, may add half a step. A
  * value that is not finite makes the scale NaN, and the page's head reads as
  * NaN until its first position is appended again. A sequence may be cut back
  * to any length (append again at a smaller pos): a page keeps its scale then. A slot may appear

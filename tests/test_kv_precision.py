@@ -78,3 +78,36 @@ def test_narrower_queries_are_seen(shape):
 def test_narrower_weights_are_seen(shape):
     assert worst("sink", shape, False, 30, 15, False) > 1
     assert worst("sink", shape, True, 22, 15, False) > 1
+
+
+@pytest.mark.parametrize("refills", [1, 5, 20, 60])
+def test_a_page_cut_back_and_filled_again(refills):
+    """Drafted tokens that end a page, rejected and drafted again with slightly
+    larger values each time: the older values are rounded anew each time. After
+    the first filling a value is off by 3 steps at most (tests/test_kv.py); each
+    refill adds half a step and no step is smaller than those before it. The bound
+    of a page that is filled once does not hold here."""
+    rng = np.random.default_rng(5)
+    hd = 64
+    c = {"k": np.zeros((1, 1, 64 * hd), np.int8), "v": np.zeros((1, 1, 64 * hd), np.int8),
+         "k_scale": np.zeros((1, 1), np.float32), "v_scale": np.zeros((1, 1), np.float32), "pages": np.zeros((1, 1), np.int32)}
+    x = rng.standard_normal((64, 1, hd)).astype(np.float32).astype(np.float64)
+    for p in range(60):
+        paged.append(c, None, x[p:p + 1], x[p:p + 1], None, [p])
+    most = 0.0
+    for n in range(refills + 1):
+        new = rng.uniform(-1, 1, (4, 1, hd)) * 6.0 * 1.01 ** n
+        new[0, 0, 0] = 6.0 * 1.01 ** n
+        new = new.astype(np.float32).astype(np.float64)
+        before = c["k_scale"][0, 0]
+        paged.append(c, None, new, new, None, [60], [0, 4])
+        assert c["k_scale"][0, 0] > before
+        x[60:] = new
+        for p in range(64):
+            k, v = paged.read(c, 0, p, hd)
+            err = np.abs(k - x[p]).max() / c["k_scale"][0, 0]
+            assert err <= (3 + n / 2) * (1 + 1e-6)
+            assert np.array_equal(k, v)
+            most = max(most, err)
+    if refills >= 20:
+        assert most > 3
