@@ -1079,7 +1079,8 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
         set_error("gate: a row stride of %d holds no %d heads", q.ldg, q.heads);
         return -1;
     }
-    if ((long) batch->nseq * (cache->max_pages + kKvItem) * cache->kv_heads > 0x7fffffffl) {
+    /* the few-column kernel's count of pages, and where its last shares would end */
+    if ((long) batch->nseq * (cache->max_pages + kKvItem) * cache->kv_heads > 0x7fffffffl - kKvFlatMost) {
         set_error("%d sequences of up to %d pages and %d kv heads are too many for one call", batch->nseq, cache->max_pages,
                   cache->kv_heads);
         return -1;
