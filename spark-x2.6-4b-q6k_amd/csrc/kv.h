@@ -12,6 +12,7 @@ namespace sparkmv {
 constexpr int kKvPage = SPARKMV_KV_PAGE;
 constexpr int kKvMaxSeq = 4096;      /* sequences of one call */
 constexpr int kKvMaxGroup = 16;      /* query heads per kv head */
+constexpr long kKvThreads = 0xffffffffl;   /* threads of a launch along one axis */
 
 /* A page's codes of one kv head. Keys: [head_dim / 64][position][64 bytes], so
  * that a wave's 16-byte loads of 16 positions (lane = position + 16 * quarter)

@@ -457,7 +457,7 @@ int sparkmv_rope_table(float * table, int rows, int rope_dim, double theta, void
     }
     if (!(theta > 0.0)) { set_error("theta must be positive"); return -1; }
     const size_t n = (size_t) rows * (rope_dim / 2), wg = (n + 255) / 256;
-    if (wg > 0x7fffffffu) { set_error("rope table of %d rows and %d values is too large", rows, rope_dim); return -1; }
+    if (wg > kKvThreads / 256) { set_error("rope table of %d rows and %d values is too large", rows, rope_dim); return -1; }
     hipLaunchKernelGGL(kv_rope_table_kernel, dim3((unsigned) wg), dim3(256), 0, (hipStream_t) stream, table, rows,
                        rope_dim / 2, (float) theta);
     return kv_check_launch("rope table launch");
@@ -501,8 +501,8 @@ int sparkmv_kv_append(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     a.c = *cache; a.b = *batch; a.n = n;
     a.b.max_q = batch->qstart ? max_q : 1;
     a.half = n.rope_dim / 2;
-    a.nb = (a.b.max_q + kKvPage - 2) / kKvPage + 1;
-    if (a.nb > cache->max_pages) a.nb = cache->max_pages;
+    const long nb = ((long) a.b.max_q + kKvPage - 2) / kKvPage + 1;
+    a.nb = (int) (nb < cache->max_pages ? nb : cache->max_pages);
     /* 256 threads hold eight rows of a page, 512 all 64 of up to 128 elements, 1024
      * of 256: with 256 threads the rows of a chunk of 512 tokens came in 32 turns, 33
      * us, with 1024 it takes 13.6; one row gives no more than 128 threads a pair (64
@@ -512,8 +512,8 @@ int sparkmv_kv_append(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     a.qtok = per && per <= qpairs ? qpairs / per : 1;
     a.qparts = per > qpairs ? (per + qpairs - 1) / qpairs : 1;
     const long nkv = (long) batch->nseq * a.nb * cache->kv_heads * 2;
-    const long wgs = nkv + (n.heads ? (long) ((batch->ntok + a.qtok - 1) / a.qtok) * a.qparts : 0);
-    if (wgs > 0x7fffffffl) { set_error("an append of %ld workgroups", wgs); return -1; }
+    const long wgs = nkv + (n.heads ? ((long) batch->ntok + a.qtok - 1) / a.qtok * a.qparts : 0);
+    if (wgs > kKvThreads / nt) { set_error("an append of %ld workgroups is too much for one call", wgs); return -1; }
     a.nkv = (int) nkv;
     const dim3 grid((unsigned) wgs), block((unsigned) nt);
     hipStream_t s = (hipStream_t) stream;
@@ -539,8 +539,8 @@ int sparkmv_kv_read(const sparkmv_kv_cache * cache, int nseq, const int * slot, 
     if (nseq == 0 || n == 0 || (!k_out && !v_out)) return 0;
     if (!from) { set_error("kv read has no positions"); return -1; }
     if (!kv_aligned(k_out, 16) || !kv_aligned(v_out, 16)) { set_error("kv read: rows do not start 16-byte aligned"); return -1; }
-    const long nb = (n + kKvPage - 2) / kKvPage + 1, wgs = (long) nseq * nb;
-    if (wgs > 0x7fffffffl) { set_error("a read of %ld pages", wgs); return -1; }
+    const long nb = ((long) n + kKvPage - 2) / kKvPage + 1, wgs = (long) nseq * nb;
+    if (wgs > kKvThreads / 256) { set_error("a read of %ld pages is too much for one call", wgs); return -1; }
     const dim3 grid((unsigned) wgs, (unsigned) cache->kv_heads, 2), block(256);
     hipStream_t s = (hipStream_t) stream;
     if (out_dtype == SPARKMV_X_F32)

@@ -1007,7 +1007,7 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
     auto take = [&](size_t bytes) { const size_t o = off; off += (bytes + 255) & ~(size_t) 255; return o; };
     if (cols <= 4) {
         /* up to kv_whole() pages a sequence: a workgroup each, nothing to join */
-        const long seen = window > 0 && (window + kKvPage - 2) / kKvPage + 1 < pages ? (window + kKvPage - 2) / kKvPage + 1 : pages;
+        const long in_window = ((long) window + kKvPage - 2) / kKvPage + 1, seen = window > 0 && in_window < pages ? in_window : pages;
         p.flat = seen <= kv_whole((long) b->nseq * c->kv_heads) ? 2 : 1;
         const long most = 2 * cu_count() < kKvFlatMost ? 2 * cu_count() : kKvFlatMost, all = pages * b->nseq * c->kv_heads;
         p.groups = (int) (all < 1 ? 1 : (all < most ? all : most));
@@ -1130,7 +1130,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     t.nsplit = p.nsplit;
     t.po = (float *) (mem + p.po); t.pml = (float *) (mem + p.pml);
     const long th = p.tiles * cache->kv_heads;
-    if (th > 0xffffff / p.nsplit) { set_error("attention over %ld tiles of tokens is too much for one call", th); return -1; }
+    if (th > kKvThreads / 256 / p.nsplit) { set_error("attention over %ld tiles of tokens is too much for one call", th); return -1; }
     const dim3 grid((unsigned) (th * p.nsplit));
     const uint32_t lds = 4 * kKvPage * (uint32_t) hd;
     const int each = th * 4 * p.wq < 8 * cu_count() ? 1 : 4;

@@ -185,3 +185,15 @@ def test_ops_in_graphs_and_on_streams_by_turns(sm, dev):
             op()
             torch.cuda.synchronize()
             check(None)
+
+
+def test_the_largest_window(sm, dev):
+    """A window that no position leaves is no window: the same launches, the same bits."""
+    import torch
+    c = Case(sm, dev, 2, 64, 2, 100, 103)
+    q = torch.randn(2, 8, 64, device=dev)
+    b = c.batch([6000, 5000], max_len=6001)
+    out = [torch.full_like(q, 7.0) for _ in range(4)]
+    for o, w in zip(out, (0, (1 << 31) - 1, (1 << 31) - 64, 1 << 30)):
+        c.kv.attend(b, q, o, window=w)
+    assert all(torch.equal(out[0], o) for o in out[1:])
