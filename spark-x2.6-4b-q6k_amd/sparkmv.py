@@ -966,8 +966,8 @@ def rope_table(rows, rope_dim, theta, device="cuda", stream=None):
 class KVBatch:
     """The sequences of one call over a PagedKV (sparkmv_kv_batch). pos: device
     int32 [nseq], each sequence's first new position (negative: left out).
-    qstart: device int32 [nseq + 1], the rows of its new tokens among ntok (None:
-    row i is sequence i's one token). slot: device int32 [nseq] (None: slot i).
+    qstart: device int32 [nseq + 1], the rows of its new tokens among the call's
+    ntok rows, which is given with it (None: row i is sequence i's one token). slot: device int32 [nseq] (None: slot i).
     max_q bounds a sequence's new tokens, max_len is the longest length the
     host expects (it shapes launches only). The tensors' values are read when
     a call runs."""
@@ -978,6 +978,8 @@ class KVBatch:
         nseq = pos.shape[0]
         self.keep = [_kv_flat("kv batch positions", pos, i32, (None,), None)]
         if qstart is not None:
+            if ntok is None:   # its last entry, on the device: rows past a guess would be left out
+                raise SparkmvError("kv batch: row starts without the number of rows")
             self.keep.append(_kv_flat("kv batch rows", qstart, i32, (nseq + 1,), self.device))
         if slot is not None:
             self.keep.append(_kv_flat("kv batch slots", slot, i32, (nseq,), self.device))

@@ -64,3 +64,10 @@ def test_paged_read_of_other_shapes_types_and_devices(sm, model):
             model.paged_read(0, *args)
     with pytest.raises(sm.SparkmvError, match="on cuda:1"):
         model.paged_step([[1]], [0], [0], Fake((1, 10), torch.float32, "cuda:1"))
+
+
+def test_row_starts_need_their_number_of_rows(sm):
+    pos, starts = Fake((2,), torch.int32), Fake((3,), torch.int32)
+    with pytest.raises(sm.SparkmvError, match="without the number of rows"):
+        sm.KVBatch(pos, qstart=starts)
+    assert sm.KVBatch(pos, 9, starts).c.max_q == 9 and sm.KVBatch(pos).c.ntok == 2
