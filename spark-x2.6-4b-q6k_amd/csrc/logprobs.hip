@@ -291,10 +291,14 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     z = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     e = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
     const bool bad = z != z;
-    const float lz = logf(z);
-    auto lp = [&](float v) -> float { return bad ? NAN : (v == -INFINITY ? -INFINITY : v - M - lz); };
+    /* log z = exponent * log 2 + log of 1 .. 2, and what follows, in 64 bits: in f32 the
+     * three roundings of a result were more than the sums' own */
+    int ex = 0;
+    const float part = frexpf(z, &ex);
+    const double lz = (double) (ex - 1) * 0.693147180559945309417 + (double) logf(2.0f * part);
+    auto lp = [&](float v) -> float { return bad ? NAN : (v == -INFINITY ? -INFINITY : (float) ((double) v - (double) M - lz)); };
     if (tid == 0) {
-        if (A.entropy) A.entropy[r] = bad ? NAN : (M == -INFINITY ? 0.0f : lz - e / z);
+        if (A.entropy) A.entropy[r] = bad ? NAN : (M == -INFINITY ? 0.0f : (float) (lz - (double) e / (double) z));
         if (A.tokens) A.logprob[r] = tok >= 0 && tok < A.n ? lp(given) : NAN;
     }
     if (!k) return;
