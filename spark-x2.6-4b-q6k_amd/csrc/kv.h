@@ -56,8 +56,6 @@ __device__ __forceinline__ uint32_t kv_bf16x2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
 }
 __device__ __forceinline__ uint16_t kv_bf16(float f) { return (uint16_t) kv_bf16x2(f, f); }
-__device__ __forceinline__ void kv_store(float * p, float v) { *p = v; }
-__device__ __forceinline__ void kv_store(uint16_t * p, float v) { *p = kv_bf16(v); }
 
 /* the host's checks: 0, or -1 with the message set. kv_check_rows: nrows rows of
  * n values at stride ld, each starting 16-byte aligned */

@@ -1,6 +1,7 @@
 /* kv.hip — the paged 8-bit cache: the append with the position rotation on the
- * way, reading positions back, and attention over it (include/sparkmv.h has
- * the cache's layout and its rules; kv.h the offsets of a code). */
+ * way, reading positions back, and the checks of its calls (include/sparkmv.h
+ * has the cache's layout and its rules; kv.h the offsets of a code; kv_attend.hip
+ * attention over it). */
 #include "kv.h"
 
 #include <math.h>

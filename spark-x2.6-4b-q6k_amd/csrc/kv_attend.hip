@@ -181,7 +181,6 @@ struct KvFlat {
     sparkmv_kv_cache c;
     sparkmv_kv_batch b;
     sparkmv_kv_query q;
-    int least;       /* pages of a share, at least */
     int * pre;       /* [nseq + 2]: what one kv head of the sequences before counts; the share */
     float * po;      /* [workgroups][2][4][HD] */
     float * pml;     /* [workgroups][2][4][2] */
@@ -249,7 +248,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_flat_kernel(const KvFlat A) 
             __syncthreads();
             total = __builtin_amdgcn_readfirstlane(lpre[nseq]);
         }
-        const int share = max((total * kvh + (int) gridDim.x - 1) / (int) gridDim.x, A.least);
+        const int share = max((total * kvh + (int) gridDim.x - 1) / (int) gridDim.x, 1);
         if (blockIdx.x == 0) {
             if (few) {
                 if (tid < nseq) A.pre[tid] = before;
@@ -990,7 +989,7 @@ __global__ __launch_bounds__(256) void kv_tile_join_kernel(const KvTile A, int c
 struct KvPlan {
     int max_q;                /* the batch's, at most its rows */
     int flat;                 /* the few-column kernel: 1 shares, 2 whole kv heads */
-    int groups, least;        /* its workgroups and least share */
+    int groups;               /* its workgroups */
     long tiles;
     int wq, nsplit;           /* the many-column kernel's */
     size_t pre, po, pml, bytes;
@@ -1011,7 +1010,6 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
         p.flat = seen <= kv_whole((long) b->nseq * c->kv_heads) ? 2 : 1;
         const long most = 2 * cu_count() < kKvFlatMost ? 2 * cu_count() : kKvFlatMost, all = pages * b->nseq * c->kv_heads;
         p.groups = (int) (all < 1 ? 1 : (all < most ? all : most));
-        p.least = 1;
         p.pre = take(((size_t) b->nseq + 2) * 4);
         p.po = take((size_t) p.groups * 2 * 4 * hd * 4);
         p.pml = take((size_t) p.groups * 2 * 4 * 2 * 4);
@@ -1097,7 +1095,6 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
         KvFlat f;
         f.c = *cache; f.b = *batch; f.q = q;
         f.b.max_q = p.max_q;
-        f.least = p.least;
         f.pre = (int *) (mem + p.pre); f.po = (float *) (mem + p.po); f.pml = (float *) (mem + p.pml);
         const dim3 join((unsigned) batch->nseq, (unsigned) cache->kv_heads, (unsigned) (p.max_q * (q.heads / cache->kv_heads)));
         const uint32_t pre = batch->nseq > 64 ? ((uint32_t) batch->nseq + 1) * 4 : 0;

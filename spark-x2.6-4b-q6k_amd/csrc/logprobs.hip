@@ -345,12 +345,12 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
 }
 
 struct LpPlan {
-    int loads, nparts, nseg;
+    int nseg;
     size_t parts, seg, bytes;
 };
 
-/* Parts of 2 loads a lane where there are few rows, else of 8; sized for the
- * shorter of the two types' loads, so that a plan does not depend on the type */
+/* A row's parts are 512 logits at least (two loads of one), so that the size does
+ * not depend on type and alignment */
 LpPlan lp_plan(int rows, int n, int k) {
     LpPlan p = {};
     p.nseg = (n + kLpSeg - 1) / kLpSeg;
