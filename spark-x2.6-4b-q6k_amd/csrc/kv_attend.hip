@@ -1028,8 +1028,11 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
          * spares no more pages than the join costs */
         long n = 2 * cu_count() / busy();
         n = n < 1 ? 1 : (n < most ? n : most);
-        /* halves of half again as many workgroups fill the last turn better (three
-         * blocks of 512 at 6000: 243 us, whole 274; at 3000 147 and 155) */
+        /* one and a half turns of the CUs in halves are three shorter ones. us in halves and
+         * whole, bf16 outputs: three blocks of 512 at 2500 161 and 170, 3000 165 and 182,
+         * 6000 279 and 325, 12000 516 and 613; one of 1100 at 2500 143 and 152, 12000 501 and
+         * 604; f32 3000 202 and 234. Of fewer pages halves gain less and from about 30 on lose:
+         * three at 1700 115 and 120, 1200 104 and 98, 700 89 and 77 */
         if (n == 1 && most > 1 && busy() > cu_count() && 2 * busy() <= 3 * cu_count() && pages >= 48) n = 2;
         p.nsplit = pages - pages / n <= kKvAlone ? 1 : (int) n;
         if (p.nsplit > 1) {
