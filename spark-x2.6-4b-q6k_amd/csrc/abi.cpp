@@ -36,6 +36,8 @@ void set_error(const char * fmt, ...) {
 
 int fail_hip(const char * what, hipError_t e) {
     set_error("%s: %s", what, hipGetErrorString(e));
+    /* reported: the next launch's check is not to find it again */
+    (void) hipGetLastError();
     return -1;
 }
 
