@@ -647,7 +647,8 @@ int sparkmv_model_paged_cache(void * model, int layer, sparkmv_kv_cache * out);
  * through the prefill GEMM, as sparkmv_model_forward_batch. Keys and values enter
  * the paged cache (sparkmv_kv_append) and attention runs over it
  * (sparkmv_kv_attend); the caller keeps the lengths and may go back to an earlier
- * position at any time. logits, when non-null: with every 0 a row [vocab] for
+ * position at any time. Every new token's page has to be there, and no page may take
+ * tokens of two places. logits, when non-null: with every 0 a row [vocab] for
  * each sequence's last token, else one for each token (at most 16). Host arrays
  * are read before the call returns. A step larger than those before it
  * (re)allocates buffers after a device synchronization. Layer-input capture and

@@ -1534,6 +1534,7 @@ struct Model {
     void * pmem = nullptr;
     std::vector<sparkmv_kv_cache> paged;
     int * ptable = nullptr, * pstep = nullptr;
+    std::vector<int> ptable_host;            /* the page table as it was last set */
     float * prope[2] = {nullptr, nullptr};   /* full, sliding */
     /* attention's workspace, grown by a step that needs more */
     void * pwork = nullptr;
@@ -2328,6 +2329,7 @@ int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
     try {
         at.resize((size_t) c.layers * 4);
         m->paged.resize((size_t) c.layers);
+        m->ptable_host.assign((size_t) nslots * max_pages, -1);
     } catch (const std::exception &) {
         set_error("paged cache: out of host memory");
         return -1;
@@ -2396,7 +2398,9 @@ int sparkmv_model_set_pages(void * model, int slot, const int * pages, int n, vo
     hipStream_t s = (hipStream_t) stream;
     hipError_t e = hipMemcpyAsync(m->ptable + (size_t) slot * k.max_pages, row, (size_t) k.max_pages * 4, hipMemcpyHostToDevice, s);
     if (e == hipSuccess) e = hipStreamSynchronize(s);
-    return e == hipSuccess ? 0 : fail_hip("page table upload", e);
+    if (e != hipSuccess) return fail_hip("page table upload", e);
+    memcpy(m->ptable_host.data() + (size_t) slot * k.max_pages, row, (size_t) k.max_pages * 4);
+    return 0;
 }
 
 int sparkmv_model_paged_cache(void * model, int layer, sparkmv_kv_cache * out) {
@@ -2439,6 +2443,16 @@ int sparkmv_model_paged_step(void * model, const uint32_t * tokens, int nseq, co
         max_q = count[i] > max_q ? count[i] : max_q;
         max_len = pos[i] + count[i] > max_len ? pos[i] + count[i] : max_len;
     }
+    /* the pages that the new tokens enter: there, and no two sequences' */
+    int entered[kPromptMax + kPagedSeq], ne = 0;
+    for (int i = 0; i < nseq; i++)
+        for (int j = pos[i] / kKvPage; j <= (pos[i] + count[i] - 1) / kKvPage; j++) {
+            const int page = m->ptable_host[(size_t) slot[i] * k.max_pages + j];
+            if (page < 0) { set_error("slot %d has no page for position %d", slot[i], j * kKvPage > pos[i] ? j * kKvPage : pos[i]); return -1; }
+            for (int u = 0; u < ne; u++)
+                if (entered[u] == page) { set_error("page %d would take tokens of two places", page); return -1; }
+            entered[ne++] = page;
+        }
     if (every && logits && ntok > kPagedSeq) { set_error("logits of every token take 1..%d tokens, not %d", kPagedSeq, ntok); return -1; }
     if (every)
         for (int t = 0; t < ntok && t < kPagedSeq; t++) pick[t] = t;
