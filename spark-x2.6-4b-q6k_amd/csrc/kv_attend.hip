@@ -624,10 +624,11 @@ __global__ __launch_bounds__(512) void kv_flat_join_kernel(const KvFlat A) {
  * pages is joined by a second launch.
  *
  * A chunk of 512 tokens at 16384 (16 query, 4 kv heads of 256, bf16 out): the call
- * takes 235 us for 140 GFLOP, 298 with f32 outputs and their four digits; bound by the
- * vector instructions around the products, half of them the values' sums from i32.
- * Six waves a workgroup, for three a SIMD, took half as long again: they do not fill
- * the SIMDs evenly. Three blocks of 8 at 6001 (f32 out): 18.8 us and 6.9 for the join. */
+ * with its join takes 233 us for 140 GFLOP, 300 with f32 outputs and their four
+ * digits; bound by the vector instructions around the products (535 a wave and page,
+ * half of them the values' sums from i32; VALU 67 % busy, MFMA 40). Six waves a
+ * workgroup, for three a SIMD, took half as long again: they do not fill the SIMDs
+ * evenly. Three blocks of 8 at 6001 (f32 out): 19 us and 6.9 for the join. */
 struct KvTile {
     sparkmv_kv_cache c;
     sparkmv_kv_batch b;
@@ -641,7 +642,7 @@ constexpr int kKvIds = 256;   /* page numbers held at a time */
 
 /* tile number `tile` of the batch, tiles of `cols` columns: its sequence and its
  * place there, a sequence's last (longest) first: the other way 4096 tokens from
- * position 0 took 237 us, not 200; false past the last one. Every thread of the workgroup calls it. */
+ * position 0 took 278 us, not 238; false past the last one. Every thread of the workgroup calls it. */
 __device__ __forceinline__ bool kv_find_tile(const sparkmv_kv_batch & b, const sparkmv_kv_cache & c, int G, int cols, int tile,
                                              int * lds, KvSeq & s, int & place) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
@@ -930,7 +931,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
  * split k's m and l, and eight rows of HD elements are in flight. With four waves
  * a column, as above, a chunk of 512 tokens in four splits took 36 us, not 12: most
  * waves had one row. One column a wave where that gives fewer than eight
- * workgroups a CU (three blocks of 8 tokens: 6.1 us, with four 12.7), else four. */
+ * workgroups a CU (three blocks of 8 tokens: 6.9 us, with four 12.7), else four. */
 constexpr int kKvSplits = 64;
 constexpr int kKvAlone = 8;   /* pages that take about as long as a join and its launch */
 template <int HD>
@@ -1015,9 +1016,9 @@ KvPlan kv_plan(const sparkmv_kv_cache * c, const sparkmv_kv_batch * b, int heads
         p.pml = take((size_t) p.groups * 2 * 4 * 2 * 4);
     } else {
         /* columns a workgroup: as a sequence's tokens give (16 sequences at 6000 of 4
-         * tokens with 1, 2 and 4: 52, 81 and 85 us, of 8: 70, 58 and 70, of 16: 111, 81 and
-         * 70), fewer where that leaves half of the CUs idle however it is split (one of 32
-         * tokens at 1000: 20.2, 21.1 and 23.6) */
+         * tokens with 1, 2 and 4, bf16 out: 57, 67 and 90 us, of 8: 79, 62 and 74, of 16: 129,
+         * 91 and 77; f32 60, 67, 100, 95, 69, 82, 161, 111, 87), fewer where that leaves half
+         * of the CUs idle however it is split (one of 32 tokens at 1000: 19.6, 22.1 and 23.6) */
         const long most = pages <= kKvAlone ? 1 : (pages / 3 < kKvSplits ? pages / 3 : kKvSplits);
         auto busy = [&]() { return ((long) b->ntok * G + 16 * p.wq - 1) / (16 * p.wq) * c->kv_heads; };
         p.wq = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);

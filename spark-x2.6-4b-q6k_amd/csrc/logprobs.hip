@@ -201,7 +201,7 @@ constexpr int kLpList = kLpMaxK * (kLpMaxN / kLpSeg / 256);   /* segments of k t
 constexpr int kLpHeld = 20;
 
 /* Bound by its chain, two reads and three rankings: one row of 131072 with 8
- * alternatives 7.7 us, 512 rows with 20 14.1. */
+ * alternatives 7.7 us, 512 rows with 20 13.2. */
 template <typename X>
 __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs A) {
     __shared__ __attribute__((aligned(16))) uint64_t lkey[256];
