@@ -840,9 +840,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvTile A) {
 #pragma unroll
             for (int e = 0; e < 4; e++) mp = fmaxf(mp, x[t][e]);
         mp = kv_rows_max(mp) * f;
-        /* a large score times f, not rounded, may lie above the reference by more than a
-         * digit holds: 2^-9 at 2^16, 1 at 2^25 */
-        if (D == 4 && __any(fabsf(mp) >= 0x1p16f)) {
+        /* a large score times f, not rounded, lies above or below the reference by up to
+         * 2^-9 at 2^16, by 1 at 2^25, where four digits no longer hold the weight, and by 128
+         * at 2^32, where no f32 does */
+        if (__any(fabsf(mp) >= 0x1p16f)) {
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll

@@ -47,11 +47,7 @@ def test_outliers_and_sinks(sm, dev, kind, form, kvh, group, hd, x, o):
     assert most <= 1
 
 
-@pytest.mark.parametrize("size", [3.0e5, 3.0e8])
-@pytest.mark.parametrize("x,o", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
-@pytest.mark.parametrize("kvh,group,hd", [(2, 4, 256), (1, 16, 64), (8, 4, 128)])
-@pytest.mark.parametrize("form", list(FORMS))
-def test_very_large_scores(sm, dev, form, kvh, group, hd, x, o, size):
+def check_one_position(sm, dev, form, kvh, group, hd, x, o, size):
     """Each query is a multiple of the key at one of its positions, with a score
     of `size` there: that position has all the weight, the others' scores being
     lower by a tenth of it at least, and the output is its value. Off by the
@@ -71,3 +67,22 @@ def test_very_large_scores(sm, dev, form, kvh, group, hd, x, o, size):
     got, _ = run(sm, dev, c, q, hd, pos, qstart, x, o)
     err = np.abs(got - want)
     assert np.all(err <= np.abs(want) * (8 * 2.0 ** -24 + 2.0 ** -22 + (2.0 ** -8 if o == "bf16" else 0.0))), float(err.max())
+
+
+SHAPES = [(2, 4, 256), (1, 16, 64), (8, 4, 128)]
+
+
+@pytest.mark.parametrize("size", [3.0e5, 3.0e8])
+@pytest.mark.parametrize("x,o", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("kvh,group,hd", SHAPES)
+@pytest.mark.parametrize("form", list(FORMS))
+def test_very_large_scores(sm, dev, form, kvh, group, hd, x, o, size):
+    check_one_position(sm, dev, form, kvh, group, hd, x, o, size)
+
+
+@pytest.mark.parametrize("size", [1.0e10, 3.0e12, 1.0e25])
+@pytest.mark.parametrize("x,o", [("f32", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("kvh,group,hd", SHAPES)
+@pytest.mark.parametrize("form", list(FORMS))
+def test_scores_whose_last_place_is_more_than_an_exponent(sm, dev, form, kvh, group, hd, x, o, size):
+    check_one_position(sm, dev, form, kvh, group, hd, x, o, size)
