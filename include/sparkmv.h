@@ -622,11 +622,11 @@ size_t sparkmv_kv_attend_work(const sparkmv_kv_cache * cache, const sparkmv_kv_b
 /* Attention over the cache after the append: token j of a sequence, at
  * position pos + j, sees positions up to its own (the last `window` of them).
  * Scores, softmax statistics and sums are f32, and scores have to lie within its
- * range. A token none of whose positions has a
- * page gives zeros. Queries and outputs may be f32 or bf16 apart. A query element is
- * held to 2^-30 of the largest of its token and head, a weight to 2^-30 of the
- * largest of its page; with bf16 outputs it may be 2^-22 and, of the sum of its
- * page's weights, 2^-23. */
+ * range. A token none of whose positions has a page gives zeros. Queries and
+ * outputs may be f32 or bf16 apart. A query element is held to 2^-30 of the largest
+ * of its token and head, a weight to 2^-30 of the largest of its page; with bf16
+ * outputs a query element may be held to 2^-22, a weight to 2^-23 of the sum of its
+ * page's. */
 int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_query * query,
                       void * stream);
 
