@@ -630,6 +630,133 @@ size_t sparkmv_kv_attend_work(const sparkmv_kv_cache * cache, const sparkmv_kv_b
 int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_query * query,
                       void * stream);
 
+/* ---- rotary tables for long contexts ----
+ * Beside sparkmv_rope_table, in the same layout: row p holds a cos(p f_i), then
+ * a sin(p f_i), i < rope_dim / 2, computed in 64 bits and rounded once, with
+ * f0_i = theta^(-2 i / rope_dim) and
+ *   NONE    f = f0
+ *   LINEAR  f = f0 / factor
+ *   NTK     theta factor^(d / (d - 2)) in place of theta (d = rope_dim, above 2)
+ *   YARN    c(r) = d ln(original / (2 pi r)) / (2 ln theta), lo = max(floor c(beta_fast), 0),
+ *           hi = min(ceil c(beta_slow), d - 1), t = clamp((i - lo) / max(hi - lo, 0.001), 0, 1):
+ *           f = f0 (1 - t) + f0 t / factor
+ *   BANDS   w = original f0 / (2 pi) turns: f0 above `high`, f0 / factor below `low`, between
+ *           them f0 ((1 - s) / factor + s), s = (w - low) / (high - low)
+ * (position interpolation, NTK-aware interpolation, YaRN and interpolation by
+ * wavelength, as published). a is `attention`, or where that is 0: 0.1 ln(factor) + 1
+ * for YARN, else 1. factor is 1 or more; scaling NULL is NONE. rope_dim is at most 256. */
+#define SPARKMV_ROPE_NONE   0
+#define SPARKMV_ROPE_LINEAR 1
+#define SPARKMV_ROPE_NTK    2
+#define SPARKMV_ROPE_YARN   3
+#define SPARKMV_ROPE_BANDS  4
+typedef struct {
+    int kind;
+    double factor, original;       /* original: positions the model was trained on */
+    double beta_fast, beta_slow;   /* YARN: turns over `original` */
+    double low, high;              /* BANDS */
+    double attention;
+} sparkmv_rope_scaling;
+int sparkmv_rope_table_scaled(float * table, int rows, int rope_dim, double theta, const sparkmv_rope_scaling * scaling,
+                              void * stream);
+
+/* ---- norm and rotation of query and key heads in one pass ----
+ * A head x becomes x / sqrt(mean x^2 + eps) * w where a norm's weights w are given,
+ * and then its first rope_dim elements turn by a row of the table: e with
+ * e + rope_dim / 2, interleaved 2 e with 2 e + 1: (a, b) -> (a c - b s, b c + a s).
+ * In 64 bits, rounded once to the output. */
+typedef struct {
+    const float * rope;              /* [rope_rows][rope_dim]: cosines, then sines; NULL with rope_dim 0 */
+    int rope_rows, rope_dim;
+    int interleaved;
+    const float * q_norm, * k_norm;  /* [head_dim]; NULL: no norm */
+    float eps;                       /* positive where there is a norm */
+} sparkmv_head_turn;
+
+/* Rows of ntok tokens, heads x head_dim (queries) and kv_heads x head_dim (keys)
+ * values each; either may be absent (NULL and no heads). Outputs may be the inputs
+ * themselves, with the same stride. head_dim is a multiple of 4, at most 256; rows
+ * start 16-byte aligned. */
+typedef struct {
+    const void * q, * k;
+    void * q_out, * k_out;
+    int ldq, ldk, ldqo, ldko, x_dtype;
+    int heads, kv_heads, head_dim, ntok;
+    const int * pos;                 /* [ntok], device; not read without a table */
+} sparkmv_qk_rows;
+
+/* Asynchronous on its stream, allocates nothing; positions are read from device
+ * memory. A token at a position outside the table is left as it was. */
+int sparkmv_qk_rope(const sparkmv_qk_rows * rows, const sparkmv_head_turn * turn, void * stream);
+
+/* ---- the paged cache in 4 bits ----
+ * As the 8-bit cache in everything but what a page holds, at 4.25 bits a value: 32
+ * neighbouring elements of a position's kv head share a power of two, and a cached
+ * value is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, times it (the
+ * Microscaling formats' E2M1 elements with E8M0 scales). The scale is the smallest
+ * 2^e with |value| <= 7 * 2^e for all 32, -120 <= e <= 125; a value becomes the
+ * nearest, of two as near the one with the even code (0 .. 7 in the order above), so
+ * that it is off by at most 1 * 2^e. 32 elements one of which is not finite read as
+ * NaN. Positions share nothing: no append changes another position, and what a
+ * position holds depends on its own rows only.
+ *
+ * data is [npages][kv_heads][68 * head_dim] bytes, 16-byte aligned
+ * (sparkmv_kv4_bytes): key codes, value codes (32 * head_dim bytes each), key scales,
+ * value scales (2 * head_dim each; 127 + e, above 252 for NaN). Where in them (the even
+ * element of a pair is the low half of its byte), for element d of position p, with
+ * t = p / 16, c = p % 16, u = p / 32, a = p / 16 % 2, g = p / 4 % 4, b = p % 4,
+ * n = head_dim / 16, block = d / 32:
+ *   key code     head_dim 64: ((t 4 + d / 16) 16 + c) 8 + d % 16 / 2; else
+ *                (((t head_dim / 128 + block / 4) 4 + block % 4) 16 + c) 16 + d % 32 / 2
+ *   value code   y = (4 a + b) n / 2 + d % n / 2: (((u n / 4 + y / 16) 4 + g) 16 + d / n) 16 + y % 16
+ *   key scale    head_dim 64: (block 16 + c) 4 + t; else
+ *                ((block % 4 16 + c) 4 + t) head_dim / 128 + block / 4
+ *   value scale  (g head_dim / 32 + block) 16 + 8 u + 4 a + b
+ *
+ * Calls are asynchronous, allocate nothing, clear nothing with a memset and check what
+ * device memory says, as those of the 8-bit cache. */
+typedef struct {
+    int kv_heads, head_dim;        /* head_dim 64, 128 or 256 */
+    int npages;                    /* pages of the pool */
+    int nslots, max_pages;         /* the page table's rows and entries per row */
+    uint8_t * data;
+    const int * pages;             /* [nslots][max_pages], device */
+} sparkmv_kv4_cache;
+
+/* Bytes of a pool of npages pages. */
+size_t sparkmv_kv4_bytes(int kv_heads, int head_dim, int npages);
+
+/* The new tokens' rows, as sparkmv_kv_new, and how their heads turn; the table must
+ * cover 64 * max_pages positions. */
+typedef struct {
+    const void * q, * k, * v;      /* q NULL (and heads 0): no queries to turn */
+    int ldq, ldk, ldv, x_dtype, heads;
+    void * q_out;                  /* [ntok][ldqo], x_dtype; may be q itself */
+    int ldqo;
+    sparkmv_head_turn turn;
+} sparkmv_kv4_new;
+
+/* Append: queries and keys are normed and turned (sparkmv_qk_rope; a query is rounded
+ * to x_dtype, a key to f32), then keys and values enter their pages. A slot may appear
+ * once in an append. Rows of no sequence are left as they were. */
+int sparkmv_kv4_append(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv4_new * rows,
+                       void * stream);
+
+/* Cached positions as values, as sparkmv_kv_read. Both types hold them exactly. */
+int sparkmv_kv4_read(const sparkmv_kv4_cache * cache, int nseq, const int * slot, const int * from, int n, void * k_out,
+                     void * v_out, int out_dtype, void * stream);
+
+/* Attention over the cache after the append, as sparkmv_kv_attend: causal within the
+ * window, gated, zeros for a token none of whose positions has a page. f32 query
+ * elements enter whole, and so does a weight for f32 outputs; for bf16 ones it is held
+ * to 2^-17 of itself. Scores, statistics and sums are f32, and scores have to lie
+ * within its range. A position that reads as NaN, in any element of its key or value,
+ * makes the tokens that see it NaN and no others. work: sparkmv_kv4_attend_work bytes
+ * on the current device. */
+size_t sparkmv_kv4_attend_work(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch * batch, int heads);
+int sparkmv_kv4_attend(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_query * query,
+                       void * stream);
+
 /* ---- the forward over the paged cache: several sequences, one read of the weights ----
  * A model's paged cache beside its f32 one (which stays as it is): npages pages
  * in each layer's pools, one page table of nslots x max_pages (at most 131072

@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <math.h>
+
 #include "../../include/sparkmv.h"
 #include "common.h"
 
@@ -56,6 +58,26 @@ __device__ __forceinline__ uint32_t kv_bf16x2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
 }
 __device__ __forceinline__ uint16_t kv_bf16(float f) { return (uint16_t) kv_bf16x2(f, f); }
+
+/* 64 bits to f32 toward zero with the lost bits kept in the last one: an odd value
+ * cannot lie between two bf16 values, so that the next rounding is the only one */
+__device__ __forceinline__ float kv_odd(double v) {
+    const float f = (float) v;
+    const double back = (double) f;
+    const uint32_t off = (uint32_t) (back != v) & (uint32_t) (fabsf(f) < INFINITY);
+    /* one step back where it was rounded away from zero */
+    const uint32_t u = __float_as_uint(f) - (off & (uint32_t) (fabs(back) > fabs(v)));
+    return __uint_as_float(u | off);
+}
+__device__ __forceinline__ void kv_store_wide(float * p, double v) { *p = (float) v; }
+__device__ __forceinline__ void kv_store_wide(uint16_t * p, double v) { *p = kv_bf16(kv_odd(v)); }
+/* four neighbours, aligned to four of them */
+__device__ __forceinline__ void kv_store_wide4(float * p, const double * v) {
+    *(float4 *) p = float4{(float) v[0], (float) v[1], (float) v[2], (float) v[3]};
+}
+__device__ __forceinline__ void kv_store_wide4(uint16_t * p, const double * v) {
+    *(uint2 *) p = uint2{kv_bf16x2(kv_odd(v[0]), kv_odd(v[1])), kv_bf16x2(kv_odd(v[2]), kv_odd(v[3]))};
+}
 
 /* the host's checks: 0, or -1 with the message set. kv_check_rows: nrows rows of
  * n values at stride ld, each starting 16-byte aligned */

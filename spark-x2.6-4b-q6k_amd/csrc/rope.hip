@@ -1,0 +1,225 @@
+/* rope.hip — rotary tables scaled for long contexts, and the norm and rotation of
+ * query and key heads in one pass (include/sparkmv.h). */
+#include "heads.h"
+
+#include <math.h>
+
+namespace sparkmv {
+
+namespace {
+
+/* ---------------------------------------------------------------- the table
+ * A thread owns one frequency and walks kRopeRun positions. */
+constexpr int kRopeRun = 64;
+
+struct RopeTable {
+    float * table;
+    int rows, half;
+    double freq[kHeadMax / 2];
+    double attention;
+};
+
+__global__ __launch_bounds__(256) void rope_table_kernel(const RopeTable A) {
+    const size_t n = (size_t) blockIdx.x * 256 + threadIdx.x;
+    const int j = (int) (n % A.half);
+    const long p0 = (long) (n / A.half) * kRopeRun;
+    const double f = A.freq[j];
+    for (long p = p0; p < p0 + kRopeRun && p < A.rows; p++) {
+        double s, c;
+        sincos((double) p * f, &s, &c);
+        float * row = A.table + (size_t) p * 2 * A.half;
+        row[j] = (float) (c * A.attention);
+        row[A.half + j] = (float) (s * A.attention);
+    }
+}
+
+/* ------------------------------------------------------- norm and rotation
+ * A wave takes up to U * (64 / lanes) heads of one token, queries or keys, whose
+ * cosines, sines and weights it reads once. Bound by the rows in and out. */
+struct QkRope {
+    sparkmv_qk_rows r;
+    sparkmv_head_turn t;
+    int sh;              /* lanes of a head, as a shift */
+    int qparts, parts;   /* waves of a token's queries, and of the token */
+};
+
+template <typename X, int U>
+__global__ __launch_bounds__(256) void qk_rope_kernel(const QkRope A) {
+    const long w = ((long) blockIdx.x * 256 + threadIdx.x) >> 6;
+    const long tok = w / A.parts;
+    if (tok >= A.r.ntok) return;
+    const int lane = threadIdx.x & 63, lanes = 1 << A.sh, l = lane & (lanes - 1), per = 64 >> A.sh;
+    int part = (int) (w - tok * A.parts);
+    const bool key = part >= A.qparts;
+    if (key) part -= A.qparts;
+    const int hd = A.r.head_dim, half = A.t.rope_dim / 2, nh = key ? A.r.kv_heads : A.r.heads;
+    const X * in = (const X *) (key ? A.r.k : A.r.q) + (size_t) tok * (key ? A.r.ldk : A.r.ldq);
+    X * out = (X *) (key ? A.r.k_out : A.r.q_out) + (size_t) tok * (key ? A.r.ldko : A.r.ldqo);
+    const float * weight = key ? A.t.k_norm : A.t.q_norm;
+    const float * row = nullptr;
+    HeadLane h;
+    head_pairs(h, 4 * l, half, A.t.interleaved);
+    const int h0 = part * U * per + (lane >> A.sh);
+    float x[U][4], y[U][4];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        head_fetch(h, in + (size_t) min(h0 + u * per, nh - 1) * hd, hd, half, A.t.interleaved, x[u], y[u]);
+    if (half) {
+        const int p = A.r.pos[tok];
+        if (p < 0 || p >= A.t.rope_rows) return;
+        row = A.t.rope + (size_t) p * A.t.rope_dim;
+    }
+    head_angles(h, row, half, A.t.interleaved);
+    head_weights(h, weight, hd);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        double o[4];
+        head_turn(h, x[u], y[u], weight != nullptr, A.t.eps, hd, lanes, o);
+        if (h0 + u * per >= nh || h.e0 >= hd) continue;
+        kv_store_wide4(out + (size_t) (h0 + u * per) * hd + h.e0, o);
+    }
+}
+
+}  // namespace
+
+int check_turn(const char * what, const sparkmv_head_turn * t, int hd, long nrow) {
+    if (t->rope_dim < 0 || t->rope_dim % 2 || t->rope_dim > hd) {
+        set_error("%s: rope_dim %d is not even within 0..%d", what, t->rope_dim, hd);
+        return -1;
+    }
+    if (t->rope_dim && !t->rope) { set_error("%s: rope table is null", what); return -1; }
+    if (t->rope_dim && t->rope_rows < nrow) {
+        set_error("%s: a rope table of %d rows does not cover %ld positions", what, t->rope_rows, nrow);
+        return -1;
+    }
+    if ((t->q_norm || t->k_norm) && !(t->eps > 0.0f && t->eps < INFINITY)) {
+        set_error("%s: a norm's eps must be positive", what);
+        return -1;
+    }
+    return 0;
+}
+
+}  // namespace sparkmv
+
+using namespace sparkmv;
+
+extern "C" {
+
+int sparkmv_rope_table_scaled(float * table, int rows, int rope_dim, double theta, const sparkmv_rope_scaling * scaling,
+                              void * stream) {
+    if (!table) { set_error("rope table is null"); return -1; }
+    if (rows < 1 || rope_dim < 2 || rope_dim % 2 || rope_dim > kHeadMax) {
+        set_error("rope table of %d rows and %d values", rows, rope_dim);
+        return -1;
+    }
+    if (!(theta > 0.0 && theta < INFINITY)) { set_error("theta must be positive"); return -1; }
+    RopeTable a;
+    a.table = table; a.rows = rows; a.half = rope_dim / 2;
+    sparkmv_rope_scaling z = {};
+    if (scaling) z = *scaling;
+    if (z.kind < SPARKMV_ROPE_NONE || z.kind > SPARKMV_ROPE_BANDS) { set_error("unknown rope scaling %d", z.kind); return -1; }
+    if (z.kind != SPARKMV_ROPE_NONE && !(z.factor >= 1.0 && z.factor < INFINITY)) {
+        set_error("a rope scaling's factor must be 1 or more");
+        return -1;
+    }
+    if ((z.kind == SPARKMV_ROPE_YARN || z.kind == SPARKMV_ROPE_BANDS) && !(z.original > 0.0 && z.original < INFINITY)) {
+        set_error("a rope scaling by wavelength needs the original context");
+        return -1;
+    }
+    if (!(z.attention >= 0.0 && z.attention < INFINITY)) { set_error("a rope scaling's attention factor is negative"); return -1; }
+    if (z.kind == SPARKMV_ROPE_YARN && !(z.beta_slow > 0.0 && z.beta_fast >= z.beta_slow && z.beta_fast < INFINITY)) {
+        set_error("yarn needs 0 < beta_slow <= beta_fast");
+        return -1;
+    }
+    if (z.kind == SPARKMV_ROPE_YARN && theta <= 1.0) { set_error("yarn needs a theta above 1"); return -1; }
+    if (z.kind == SPARKMV_ROPE_BANDS && !(z.low > 0.0 && z.high > z.low && z.high < INFINITY)) {
+        set_error("bands need 0 < low < high");
+        return -1;
+    }
+    const double pi = 3.14159265358979323846, d = (double) rope_dim;
+    double lo = 0.0, hi = 0.0;
+    if (z.kind == SPARKMV_ROPE_YARN) {
+        auto at = [&](double turns) { return d * log(z.original / (2.0 * pi * turns)) / (2.0 * log(theta)); };
+        lo = fmax(floor(at(z.beta_fast)), 0.0);
+        hi = fmin(ceil(at(z.beta_slow)), d - 1.0);
+    }
+    const double base = z.kind == SPARKMV_ROPE_NTK && rope_dim > 2 ? theta * pow(z.factor, d / (d - 2.0)) : theta;
+    for (int i = 0; i < a.half; i++) {
+        double f = pow(base, -2.0 * i / d);
+        if (z.kind == SPARKMV_ROPE_LINEAR) {
+            f /= z.factor;
+        } else if (z.kind == SPARKMV_ROPE_YARN) {
+            const double t = fmin(fmax(((double) i - lo) / fmax(hi - lo, 0.001), 0.0), 1.0);
+            f = f * (1.0 - t) + f / z.factor * t;
+        } else if (z.kind == SPARKMV_ROPE_BANDS) {
+            const double turns = z.original * f / (2.0 * pi), t = (turns - z.low) / (z.high - z.low);
+            if (turns < z.low) f /= z.factor;
+            else if (turns <= z.high) f *= (1.0 - t) / z.factor + t;
+        }
+        a.freq[i] = f;
+    }
+    a.attention = z.attention > 0.0 ? z.attention : (z.kind == SPARKMV_ROPE_YARN ? 0.1 * log(z.factor) + 1.0 : 1.0);
+    const size_t n = (((size_t) rows + kRopeRun - 1) / kRopeRun) * a.half, wg = (n + 255) / 256;
+    hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned) wg), dim3(256), 0, (hipStream_t) stream, a);
+    return kv_check_launch("rope table launch");
+}
+
+int sparkmv_qk_rope(const sparkmv_qk_rows * rows, const sparkmv_head_turn * turn, void * stream) {
+    if (!rows || !turn) { set_error("qk rope: rows or turn is null"); return -1; }
+    const sparkmv_qk_rows & r = *rows;
+    if (kv_check_dtype("qk rope", r.x_dtype)) return -1;
+    if (r.head_dim < 4 || r.head_dim > kHeadMax || r.head_dim % 4) {
+        set_error("qk rope: head_dim %d is not a multiple of 4 within 4..%d", r.head_dim, kHeadMax);
+        return -1;
+    }
+    if (r.ntok < 0) { set_error("%d tokens", r.ntok); return -1; }
+    if (r.heads < 0 || r.kv_heads < 0 || r.heads > 65536 || r.kv_heads > 65536) {
+        set_error("qk rope: %d query and %d key heads are outside 0..65536", r.heads, r.kv_heads);
+        return -1;
+    }
+    if ((r.heads > 0) != (r.q != nullptr) || (r.heads > 0) != (r.q_out != nullptr)) {
+        set_error("%d query heads, queries and their output do not agree", r.heads);
+        return -1;
+    }
+    if ((r.kv_heads > 0) != (r.k != nullptr) || (r.kv_heads > 0) != (r.k_out != nullptr)) {
+        set_error("%d key heads, keys and their output do not agree", r.kv_heads);
+        return -1;
+    }
+    if (check_turn("qk rope", turn, r.head_dim, 1)) return -1;
+    if (r.ntok == 0 || (r.heads == 0 && r.kv_heads == 0)) return 0;
+    if (turn->rope_dim && !r.pos) { set_error("qk rope has no positions"); return -1; }
+    const long qd = (long) r.heads * r.head_dim, kd = (long) r.kv_heads * r.head_dim;
+    if (r.heads && (kv_check_rows("queries", r.q, r.ldq, qd, r.x_dtype, r.ntok) ||
+                    kv_check_rows("turned queries", r.q_out, r.ldqo, qd, r.x_dtype, r.ntok)))
+        return -1;
+    if (r.kv_heads && (kv_check_rows("keys", r.k, r.ldk, kd, r.x_dtype, r.ntok) ||
+                       kv_check_rows("turned keys", r.k_out, r.ldko, kd, r.x_dtype, r.ntok)))
+        return -1;
+    if (r.ntok > 1 && ((r.heads && r.q == r.q_out && r.ldq != r.ldqo) || (r.kv_heads && r.k == r.k_out && r.ldk != r.ldko))) {
+        set_error("rows turned in place with two row strides");
+        return -1;
+    }
+    QkRope a;
+    a.r = r; a.t = *turn;
+    a.sh = head_lane_shift(r.head_dim);
+    const int per = 64 >> a.sh;
+    auto waves = [&](int heads, int u) { return (heads + u * per - 1) / (u * per); };
+    const long all = (long) r.ntok * (waves(r.heads, 1) + waves(r.kv_heads, 1));
+    const int u = all > 16 * cu_count() ? 4 : 1;
+    a.qparts = waves(r.heads, u);
+    a.parts = a.qparts + waves(r.kv_heads, u);
+    const long wg = ((long) r.ntok * a.parts + 3) / 4;
+    if (wg > kKvThreads / 256) { set_error("qk rope of %d tokens is too much for one call", r.ntok); return -1; }
+    const dim3 grid((unsigned) wg), block(256);
+    hipStream_t s = (hipStream_t) stream;
+    if (r.x_dtype == SPARKMV_X_F32) {
+        if (u == 4) hipLaunchKernelGGL((qk_rope_kernel<float, 4>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((qk_rope_kernel<float, 1>), grid, block, 0, s, a);
+    } else {
+        if (u == 4) hipLaunchKernelGGL((qk_rope_kernel<uint16_t, 4>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((qk_rope_kernel<uint16_t, 1>), grid, block, 0, s, a);
+    }
+    return kv_check_launch("qk rope launch");
+}
+
+}  // extern "C"

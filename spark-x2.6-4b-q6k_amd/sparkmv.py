@@ -106,6 +106,37 @@ class KvQuery(ctypes.Structure):
                 ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_size_t)]
 
 
+class RopeScalingC(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_double), ("original", ctypes.c_double),
+                ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double), ("low", ctypes.c_double),
+                ("high", ctypes.c_double), ("attention", ctypes.c_double)]
+
+
+class HeadTurn(ctypes.Structure):
+    _fields_ = [("rope", ctypes.c_void_p), ("rope_rows", ctypes.c_int), ("rope_dim", ctypes.c_int),
+                ("interleaved", ctypes.c_int), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
+                ("eps", ctypes.c_float)]
+
+
+class QkRows(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+                ("ldq", ctypes.c_int), ("ldk", ctypes.c_int), ("ldqo", ctypes.c_int), ("ldko", ctypes.c_int),
+                ("x_dtype", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("ntok", ctypes.c_int), ("pos", ctypes.c_void_p)]
+
+
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("npages", ctypes.c_int),
+                ("nslots", ctypes.c_int), ("max_pages", ctypes.c_int), ("data", ctypes.c_void_p),
+                ("pages", ctypes.c_void_p)]
+
+
+class Kv4New(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ldq", ctypes.c_int),
+                ("ldk", ctypes.c_int), ("ldv", ctypes.c_int), ("x_dtype", ctypes.c_int), ("heads", ctypes.c_int),
+                ("q_out", ctypes.c_void_p), ("ldqo", ctypes.c_int), ("turn", HeadTurn)]
+
+
 # chain op input transforms (sparkmv_chain_add_vq x_mode)
 X_MODE_BF16, X_MODE_F32, X_MODE_NORM = 0, 1, 2
 
@@ -223,6 +254,13 @@ SIGNATURES = {
     "sparkmv_kv_read": (_I, [_P, _I, _P, _P, _I, _P, _P, _I, _P]),
     "sparkmv_kv_attend_work": (_S, [_P, _P, _I]),
     "sparkmv_kv_attend": (_I, [_P, _P, _P, _P]),
+    "sparkmv_rope_table_scaled": (_I, [_P, _I, _I, ctypes.c_double, _P, _P]),
+    "sparkmv_qk_rope": (_I, [_P, _P, _P]),
+    "sparkmv_kv4_bytes": (_S, [_I] * 3),
+    "sparkmv_kv4_append": (_I, [_P, _P, _P, _P]),
+    "sparkmv_kv4_read": (_I, [_P, _I, _P, _P, _I, _P, _P, _I, _P]),
+    "sparkmv_kv4_attend_work": (_S, [_P, _P, _I]),
+    "sparkmv_kv4_attend": (_I, [_P, _P, _P, _P]),
     "sparkmv_logprobs_work": (_S, [_I] * 3),
     "sparkmv_logprobs": (_I, [_P, _I, _I, _I, _S, _P, _I, _P, _P, _P, _P, _P, _S, _P]),
     "sparkmv_config_load": (_I, [ctypes.c_char_p, ctypes.POINTER(ModelCfg), ctypes.POINTER(_I), _I]),
@@ -931,8 +969,8 @@ def _kv_rows(what, t, dtypes, heads, head_dim, device):
 
 
 def _kv_read_call(c, start, k_out, v_out, slot, device, what, keep):
-    """The call that reads positions of the cache c (a KvCache) on a device, or
-    where start is, into the outputs that are given."""
+    """The call that reads positions of the cache c (a KvCache or Kv4Cache) on a
+    device, or where start is, into the outputs that are given."""
     torch = _torch()
     i32, ft = (torch.int32,), (torch.float32, torch.bfloat16)
     outs = [t for t in (k_out, v_out) if t is not None]
@@ -946,21 +984,109 @@ def _kv_read_call(c, start, k_out, v_out, slot, device, what, keep):
             raise SparkmvError(what + ": keys and values of two types")
     if slot is not None:
         _kv_flat(what + " slots", slot, i32, (start.shape[0],), start.device)
-    return _Call(lib().sparkmv_kv_read,
+    return _Call(lib().sparkmv_kv4_read if isinstance(c, Kv4Cache) else lib().sparkmv_kv_read,
                  (ctypes.addressof(c), start.shape[0], _ptr(slot), start.data_ptr(), n, _ptr(k_out), _ptr(v_out),
                   X_F32 if outs[0].dtype == torch.float32 else X_BF16), start.device, what, (keep, c, start, k_out, v_out, slot))
 
 
-def rope_table(rows, rope_dim, theta, device="cuda", stream=None):
+def rope_table(rows, rope_dim, theta, device="cuda", stream=None, scaling=None):
     """[rows, rope_dim] f32: cos then sin of position * theta^(-2 i / rope_dim)
-    (sparkmv_rope_table, the model's own expressions)."""
+    (sparkmv_rope_table, the model's own expressions); with a RopeScaling the
+    scaled frequencies, in 64 bits (sparkmv_rope_table_scaled)."""
     torch = _torch()
     with _made_on(stream):
         out = torch.empty((rows, rope_dim), dtype=torch.float32, device=device)
-    with torch.cuda.device(out.device):
-        check(lib().sparkmv_rope_table(out.data_ptr(), rows, rope_dim, float(theta), _stream_ptr(stream)), "rope table")
+    if scaling is not None:
+        rope_table_op(out, theta, scaling)(stream)
+    else:
+        with torch.cuda.device(out.device):
+            check(lib().sparkmv_rope_table(out.data_ptr(), rows, rope_dim, float(theta), _stream_ptr(stream)), "rope table")
     _returned(stream, out.device, out)
     return out
+
+
+class RopeScaling:
+    """How a rotary table's frequencies are scaled for a long context
+    (sparkmv_rope_scaling): kind "none", "linear", "ntk", "yarn" or "bands"; factor
+    1 or more; original: the positions that the model was trained on (yarn, bands);
+    beta_fast and beta_slow: yarn's turns; low and high: the bands' turns;
+    attention: what cosines and sines are multiplied by (None: yarn's own, else 1)."""
+
+    KINDS = ("none", "linear", "ntk", "yarn", "bands")
+
+    def __init__(self, kind="none", factor=1.0, original=0, beta_fast=32.0, beta_slow=1.0, low=1.0, high=4.0, attention=None):
+        if kind not in self.KINDS:
+            raise SparkmvError(f"rope scaling: {kind!r} is none of {', '.join(self.KINDS)}")
+        if attention is not None and not attention > 0:
+            raise SparkmvError("rope scaling: the attention factor is not positive")
+        self.c = RopeScalingC(self.KINDS.index(kind), float(factor), float(original), float(beta_fast), float(beta_slow),
+                              float(low), float(high), 0.0 if attention is None else float(attention))
+
+
+def rope_table_op(table, theta, scaling=None):
+    """The call that fills table ([rows, rope_dim] f32) with the cosines and sines of
+    the scaled frequencies, in 64 bits (sparkmv_rope_table_scaled)."""
+    _kv_flat("rope table", table, (_torch().float32,), (None, None), None)
+    if scaling is not None and not isinstance(scaling, RopeScaling):
+        raise SparkmvError("rope table: the scaling is no RopeScaling")
+    return _Call(lib().sparkmv_rope_table_scaled,
+                 (table.data_ptr(), table.shape[0], table.shape[1], float(theta),
+                  ctypes.addressof(scaling.c) if scaling is not None else None),
+                 table.device, "rope table", (table, scaling))
+
+
+def _head_turn(turn, what, rope, interleaved, q_norm, k_norm, eps, head_dim, device):
+    """Fills a HeadTurn from checked tensors on device."""
+    f32 = (_torch().float32,)
+    if rope is not None:
+        _kv_flat(what + " rope", rope, f32, (None, None), device)
+        turn.rope, turn.rope_rows, turn.rope_dim = rope.data_ptr(), rope.shape[0], rope.shape[1]
+    turn.interleaved, turn.eps = int(bool(interleaved)), float(eps)
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is not None:
+            _kv_flat(what + " " + name, t, f32, (head_dim,), device)
+            setattr(turn, name, t.data_ptr())
+
+
+def qk_rope_op(pos, q=None, q_out=None, k=None, k_out=None, rope=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
+    """The call that norms and turns query and key heads in one pass (sparkmv_qk_rope):
+    q and k [ntok, heads, head_dim], f32 or bf16 (either may be None), into q_out and
+    k_out (the inputs themselves, or others of the same shape and type). pos: device
+    int32 [ntok] (None without a rope); rope: a table [rows, rope_dim]; interleaved:
+    neighbours turn together, not halves; q_norm and k_norm: f32 [head_dim]."""
+    torch = _torch()
+    given = [t for t in (q, k) if t is not None]
+    if not given or (q is None) != (q_out is None) or (k is None) != (k_out is None):
+        raise SparkmvError("qk rope: queries or keys and their outputs do not agree")
+    if any(t.dim() != 3 for t in given):
+        raise SparkmvError("qk rope: [tokens, heads, head_dim] is needed")
+    first = given[0]
+    ntok, head_dim, dev = first.shape[0], first.shape[2], first.device
+    xt = (first.dtype,) if first.dtype in (torch.float32, torch.bfloat16) else (torch.float32, torch.bfloat16)
+    r, turn = QkRows(x_dtype=X_F32 if first.dtype == torch.float32 else X_BF16, head_dim=head_dim, ntok=ntok), HeadTurn()
+    for name, t, out, heads in (("q", q, q_out, "heads"), ("k", k, k_out, "kv_heads")):
+        if t is None:
+            continue
+        setattr(r, heads, t.shape[1])
+        for n, x in ((name, t), (name + "_out", out)):
+            if x.shape[0] != ntok:
+                raise SparkmvError(f"qk rope {n}: {x.shape[0]} rows for {ntok} tokens")
+            ld = _kv_rows("qk rope " + n, x, xt, t.shape[1], head_dim, dev)[1]
+            setattr(r, n, x.data_ptr())
+            setattr(r, "ld" + name + ("o" if n != name else ""), ld)
+    if rope is not None and pos is None:
+        raise SparkmvError("qk rope: a table without positions")
+    if pos is not None:
+        _kv_flat("qk rope positions", pos, (torch.int32,), (ntok,), dev)
+        r.pos = pos.data_ptr()
+    _head_turn(turn, "qk rope", rope, interleaved, q_norm, k_norm, eps, head_dim, dev)
+    return _Call(lib().sparkmv_qk_rope, (ctypes.addressof(r), ctypes.addressof(turn)), dev, "qk rope",
+                 (pos, q, q_out, k, k_out, rope, q_norm, k_norm, r, turn))
+
+
+def qk_rope(pos, q=None, q_out=None, k=None, k_out=None, rope=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6,
+            stream=None):
+    qk_rope_op(pos, q, q_out, k, k_out, rope, interleaved, q_norm, k_norm, eps)(stream)
 
 
 class KVBatch:
@@ -998,6 +1124,7 @@ class PagedKV:
     The caller hands out pages and keeps the lengths."""
 
     PAGE = 64
+    _CALLS = "sparkmv_kv"
 
     def __init__(self, kv_heads, head_dim, npages, nslots, max_pages, pages=None, k=None, v=None, k_scale=None,
                  v_scale=None, device="cuda"):
@@ -1026,14 +1153,12 @@ class PagedKV:
         if batch.device != self.device:
             raise SparkmvError(f"kv batch: on {batch.device}, not on {self.device}")
 
-    def append_op(self, batch, q, k, v, rope=None, q_out=None):
-        """The call that rotates q into q_out and k by the table, and appends k
-        and v ([ntok, heads, head_dim] or flat rows, f32 or bf16). q None: keys
-        and values only."""
+    def _new_rows(self, n, batch, q, k, v, q_out):
+        """Fills the rows of a KvNew or Kv4New."""
         torch = _torch()
         self._same(batch)
         xt = (k.dtype,) if k.dtype in (torch.float32, torch.bfloat16) else (torch.float32, torch.bfloat16)
-        n = KvNew(x_dtype=X_F32 if k.dtype == torch.float32 else X_BF16)
+        n.x_dtype = X_F32 if k.dtype == torch.float32 else X_BF16
         for name, t in (("k", k), ("v", v)):
             rows, ld = _kv_rows("kv append " + name, t, xt, self.kv_heads, self.head_dim, self.device)
             if rows < batch.ntok:
@@ -1050,8 +1175,15 @@ class PagedKV:
                     raise SparkmvError(f"kv append {name}: {rows} rows for {batch.ntok} tokens")
                 setattr(n, name, t.data_ptr())
                 setattr(n, ldn, ld)
+
+    def append_op(self, batch, q, k, v, rope=None, q_out=None):
+        """The call that rotates q into q_out and k by the table, and appends k
+        and v ([ntok, heads, head_dim] or flat rows, f32 or bf16). q None: keys
+        and values only."""
+        n = KvNew()
+        self._new_rows(n, batch, q, k, v, q_out)
         if rope is not None:
-            _kv_flat("kv append rope", rope, (torch.float32,), (None, None), self.device)
+            _kv_flat("kv append rope", rope, (_torch().float32,), (None, None), self.device)
             n.rope, n.rope_rows, n.rope_dim = rope.data_ptr(), rope.shape[0], rope.shape[1]
         return _Call(lib().sparkmv_kv_append, (ctypes.addressof(self.c), ctypes.addressof(batch.c), ctypes.addressof(n)),
                      self.device, "kv append", (self, batch, q, k, v, rope, q_out, n))
@@ -1097,20 +1229,59 @@ class PagedKV:
                 raise SparkmvError("kv attend gate: rows of heads side by side, one a token, are needed")
             n.gate, n.ldg = gate.data_ptr(), gate.stride(0) if gate.shape[0] > 1 else heads
         with torch.cuda.device(self.device):
-            need = lib().sparkmv_kv_attend_work(ctypes.addressof(self.c), ctypes.addressof(batch.c), heads)
+            need = getattr(lib(), self._CALLS + "_attend_work")(ctypes.addressof(self.c), ctypes.addressof(batch.c), heads)
         made = None
         if work is None and need:
             work = made = torch.empty(need, dtype=torch.uint8, device=self.device)
         if work is not None:
             _kv_flat("kv attend work", work, (torch.uint8,), (None,), self.device)
             n.work, n.work_bytes = work.data_ptr(), work.numel()
-        return _Call(lib().sparkmv_kv_attend, (ctypes.addressof(self.c), ctypes.addressof(batch.c), ctypes.addressof(n)),
+        return _Call(getattr(lib(), self._CALLS + "_attend"), (ctypes.addressof(self.c), ctypes.addressof(batch.c), ctypes.addressof(n)),
                      self.device, "kv attend", (self, batch, q, out, gate, work, n), made if again else None)
 
     def attend(self, batch, q, out, scale=None, window=0, gate=None, work=None, stream=None):
         with _made_on(stream):
             op = self._attend_call(batch, q, out, scale, window, gate, work, False)
         op(stream)
+
+
+class PagedKV4(PagedKV):
+    """Keys and values of several sequences in 4 bits, 4.25 with the scales, in pages
+    of 64 positions (sparkmv_kv4_*). pages: the page table, device int32 [nslots,
+    max_pages], -1 where a slot has no page; data: uint8 [npages, kv_heads, 68 *
+    head_dim]; both are made here unless given (layers share a table). The caller
+    hands out pages and keeps the lengths. read and attend are those of PagedKV."""
+
+    _CALLS = "sparkmv_kv4"
+
+    def __init__(self, kv_heads, head_dim, npages, nslots, max_pages, pages=None, data=None, device="cuda"):
+        torch = _torch()
+        self.kv_heads, self.head_dim = int(kv_heads), int(head_dim)
+        self.npages, self.nslots, self.max_pages = int(npages), int(nslots), int(max_pages)
+        given = [t for t in (pages, data) if t is not None]
+        dev = given[0].device if given else torch.empty(0, device=device).device
+        shape = (self.npages, self.kv_heads, 68 * self.head_dim)
+        self.pages = torch.full((self.nslots, self.max_pages), -1, dtype=torch.int32, device=dev) if pages is None else pages
+        self.data = torch.zeros(shape, dtype=torch.uint8, device=dev) if data is None else data
+        _kv_flat("kv pages", self.pages, (torch.int32,), (self.nslots, self.max_pages), dev)
+        _kv_flat("kv4 data", self.data, (torch.uint8,), shape, dev)
+        self.device = dev
+        self.c = Kv4Cache(kv_heads=self.kv_heads, head_dim=self.head_dim, npages=self.npages, nslots=self.nslots,
+                          max_pages=self.max_pages, data=self.data.data_ptr(), pages=self.pages.data_ptr())
+
+    def append_op(self, batch, q, k, v, rope=None, q_out=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
+        """The call that norms (q_norm, k_norm: f32 [head_dim], or None) and turns q
+        into q_out and k by the table, and appends k and v ([ntok, heads, head_dim] or
+        flat rows, f32 or bf16). q None: keys and values only. interleaved:
+        neighbouring elements turn together, not halves."""
+        n = Kv4New()
+        self._new_rows(n, batch, q, k, v, q_out)
+        _head_turn(n.turn, "kv append", rope, interleaved, q_norm, k_norm, eps, self.head_dim, self.device)
+        return _Call(lib().sparkmv_kv4_append, (ctypes.addressof(self.c), ctypes.addressof(batch.c), ctypes.addressof(n)),
+                     self.device, "kv append", (self, batch, q, k, v, rope, q_out, q_norm, k_norm, n))
+
+    def append(self, batch, q, k, v, rope=None, q_out=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6, stream=None):
+        self.append_op(batch, q, k, v, rope, q_out, interleaved, q_norm, k_norm, eps)(stream)
 
 
 def logprobs_op(logits, tokens=None, logprob=None, entropy=None, top_id=None, top_logprob=None, work=None):
