@@ -762,12 +762,16 @@ int sparkmv_kv4_attend(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
  * in each layer's pools, one page table of nslots x max_pages (at most 131072
  * positions a slot) for all layers. Made once. */
 int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages);
+/* The same with caches of 4 bits (sparkmv_kv4_append, sparkmv_kv4_attend in the step). A
+ * model has one of the two. */
+int sparkmv_model_paged4(void * model, int npages, int nslots, int max_pages);
 /* Slot's pages: entry j for positions 64 j .. 64 j + 63, the n given ones, -1
  * for none and in the rest. The host array is read before the call returns (it
  * waits for the stream's earlier work). */
 int sparkmv_model_set_pages(void * model, int slot, const int * pages, int n, void * stream);
-/* Layer's cache, for sparkmv_kv_read and inspection. */
+/* Layer's cache, for sparkmv_kv_read or sparkmv_kv4_read and inspection. */
 int sparkmv_model_paged_cache(void * model, int layer, sparkmv_kv_cache * out);
+int sparkmv_model_paged4_cache(void * model, int layer, sparkmv_kv4_cache * out);
 /* One step of up to 16 sequences in different slots: count[i] tokens at positions
  * pos[i] .. of slot[i], tokens in the order of the sequences, at most 512 in all
  * (one each: a decode step; more: prompt chunks, verified blocks). Each matrix is

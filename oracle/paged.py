@@ -240,13 +240,14 @@ def logprobs(x, tokens, k):
     return lp, ent, ids, tops
 
 
-def model_step(f, caches, tables, tokens, slot, pos, qstart, after_append=None):
+def model_step(f, caches, tables, tokens, slot, pos, qstart, after_append=None, of=None):
     """One paged step of a forward.Forward f (its weights and arithmetic; its f32
     cache is not touched): the final residual's logits of every token. caches:
     per layer, as append() takes them; tables: rope tables (full, sliding).
     after_append(li), when given, may put other codes into caches[li] before
-    attention reads them."""
+    attention reads them. of: a module with another cache's append() and attend()."""
     import forward as fw
+    put, look = (append, attend) if of is None else (of.append, of.attend)
     c = f.c
     hd, heads, kvh = c["head_dim"], c["heads"], c["kv_heads"]
     qd, kvd, n = heads * hd, kvh * hd, len(tokens)
@@ -256,11 +257,11 @@ def model_step(f, caches, tables, tokens, slot, pos, qstart, after_append=None):
         xn = np.stack([f.q(fw.rms_norm(x, L["in_norm"], c["eps"])) for x in h])
         qkv = np.stack([(L["qkv"] @ x).astype(np.float32) for x in xn]).astype(np.float64)
         gate = np.stack([(L["attn_gate"] @ x).astype(np.float32) for x in xn])
-        q = append(caches[li], qkv[:, :qd].reshape(n, heads, hd), qkv[:, qd:qd + kvd].reshape(n, kvh, hd),
+        q = put(caches[li], qkv[:, :qd].reshape(n, heads, hd), qkv[:, qd:qd + kvd].reshape(n, kvh, hd),
                    qkv[:, qd + kvd:].reshape(n, kvh, hd), tables[0 if full else 1], pos, qstart, slot)
         if after_append:
             after_append(li)
-        out, _ = attend(caches[li], q.astype(np.float32).astype(np.float64), hd, float(np.float32(1.0) / np.sqrt(np.float32(hd))),
+        out, _ = look(caches[li], q.astype(np.float32).astype(np.float64), hd, float(np.float32(1.0) / np.sqrt(np.float32(hd))),
                         0 if full else c["sliding_window"], gate.astype(np.float64), pos, qstart, slot)
         for t in range(n):
             a = out[t].reshape(qd).astype(np.float32)

@@ -1532,7 +1532,8 @@ struct Model {
      * allocation: each layer's pools, one page table, rope tables, and a step's
      * tokens, slots, positions, row starts and picked rows */
     void * pmem = nullptr;
-    std::vector<sparkmv_kv_cache> paged;
+    std::vector<sparkmv_kv_cache> paged;     /* of 4 bits: all but the arrays of codes and scales */
+    std::vector<sparkmv_kv4_cache> paged4;   /* empty with 8 bits */
     int * ptable = nullptr, * pstep = nullptr;
     std::vector<int> ptable_host;            /* the page table as it was last set */
     float * prope[2] = {nullptr, nullptr};   /* full, sliding */
@@ -2273,7 +2274,17 @@ int paged_step(Model * m, const sparkmv_kv_batch & b, const int * pick, int nrow
         kn.rope_dim = rope_dim(hd, full ? c.rope_full_partial : c.rope_slide_partial);
         kn.rope = kn.rope_dim ? m->prope[full ? 0 : 1] : nullptr;
         kn.rope_rows = m->paged[li].max_pages * kKvPage;
-        if (sparkmv_kv_append(&m->paged[li], &b, &kn, s)) return -1;
+        if (m->paged4.empty()) {
+            if (sparkmv_kv_append(&m->paged[li], &b, &kn, s)) return -1;
+        } else {
+            sparkmv_kv4_new k4;
+            memset(&k4, 0, sizeof k4);
+            k4.q = kn.q; k4.k = kn.k; k4.v = kn.v; k4.q_out = kn.q_out;
+            k4.ldq = kn.ldq; k4.ldk = kn.ldk; k4.ldv = kn.ldv; k4.ldqo = kn.ldqo;
+            k4.x_dtype = kn.x_dtype; k4.heads = kn.heads;
+            k4.turn.rope = kn.rope; k4.turn.rope_rows = kn.rope_rows; k4.turn.rope_dim = kn.rope_dim;
+            if (sparkmv_kv4_append(&m->paged4[li], &b, &k4, s)) return -1;
+        }
         sparkmv_kv_query q;
         memset(&q, 0, sizeof q);
         q.q = m->vqkv; q.ldq = ldq; q.q_dtype = SPARKMV_X_F32; q.heads = c.heads;
@@ -2282,7 +2293,7 @@ int paged_step(Model * m, const sparkmv_kv_batch & b, const int * pick, int nrow
         q.out = b16 ? (void *) m->vattn16 : (void *) m->vattn; q.ldo = qd;
         q.out_dtype = b16 ? SPARKMV_X_BF16 : SPARKMV_X_F32;
         q.work = m->pwork; q.work_bytes = m->pwork_bytes;
-        if (sparkmv_kv_attend(&m->paged[li], &b, &q, s)) return -1;
+        if (m->paged4.empty() ? sparkmv_kv_attend(&m->paged[li], &b, &q, s) : sparkmv_kv4_attend(&m->paged4[li], &b, &q, s)) return -1;
         if (mat_n(*m, L.out, c.hidden, qd, b16 ? (const void *) m->vattn16 : (const void *) m->vattn, m->vh, 1, s, N, c.hidden))
             return -1;
         if (rmsnorm(*m, m->vh, L.post_norm, s, N, m->vxn, m->vxn16)) return -1;
@@ -2310,12 +2321,8 @@ int paged_step(Model * m, const sparkmv_kv_batch & b, const int * pick, int nrow
     return kq_gemv_launch(8, m->head_blocks, c.vocab, c.hidden, xin, b16 ? 0 : 1, c.hidden, nrow, logits, c.vocab, 0, s);
 }
 
-}  // namespace
-
-extern "C" {
-
-int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
-    Model * m = (Model *) model;
+/* The model's paged cache of 8 or 4 bits. */
+int make_paged(Model * m, int npages, int nslots, int max_pages, int bits) {
     if (!m) { set_error("model is null"); return -1; }
     if (npages < 1 || nslots < 1 || max_pages < 1) {
         set_error("a paged cache of %d pages, %d slots of %d pages", npages, nslots, max_pages);
@@ -2329,6 +2336,7 @@ int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
     try {
         at.resize((size_t) c.layers * 4);
         m->paged.resize((size_t) c.layers);
+        m->paged4.resize(bits == 4 ? (size_t) c.layers : 0);
         m->ptable_host.assign((size_t) nslots * max_pages, -1);
     } catch (const std::exception &) {
         set_error("paged cache: out of host memory");
@@ -2338,6 +2346,10 @@ int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
     auto take = [&](size_t bytes) { const size_t o = off; off += align256(bytes); return o; };
     const size_t codes = (size_t) npages * c.kv_heads * kKvPage * c.head_dim, scales = (size_t) npages * c.kv_heads * 4;
     for (int li = 0; li < c.layers; li++) {
+        if (bits == 4) {
+            at[4 * li] = take(sparkmv_kv4_bytes(c.kv_heads, c.head_dim, npages));
+            continue;
+        }
         at[4 * li] = take(codes);
         at[4 * li + 1] = take(codes);
         at[4 * li + 2] = take(scales);
@@ -2375,11 +2387,27 @@ int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
         sparkmv_kv_cache & k = m->paged[li];
         memset(&k, 0, sizeof k);
         k.kv_heads = c.kv_heads; k.head_dim = c.head_dim; k.npages = npages; k.nslots = nslots; k.max_pages = max_pages;
+        k.pages = m->ptable;
+        if (bits == 4) {
+            m->paged4[li] = {c.kv_heads, c.head_dim, npages, nslots, max_pages, b + at[4 * li], m->ptable};
+            continue;
+        }
         k.k = (int8_t *) (b + at[4 * li]); k.v = (int8_t *) (b + at[4 * li + 1]);
         k.k_scale = (float *) (b + at[4 * li + 2]); k.v_scale = (float *) (b + at[4 * li + 3]);
-        k.pages = m->ptable;
     }
     return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sparkmv_model_paged(void * model, int npages, int nslots, int max_pages) {
+    return make_paged((Model *) model, npages, nslots, max_pages, 8);
+}
+
+int sparkmv_model_paged4(void * model, int npages, int nslots, int max_pages) {
+    return make_paged((Model *) model, npages, nslots, max_pages, 4);
 }
 
 int sparkmv_model_set_pages(void * model, int slot, const int * pages, int n, void * stream) {
@@ -2408,7 +2436,18 @@ int sparkmv_model_paged_cache(void * model, int layer, sparkmv_kv_cache * out) {
     if (!m || !out) { set_error("model or output is null"); return -1; }
     if (!m->pmem) { set_error("the model has no paged cache: call sparkmv_model_paged first"); return -1; }
     if (layer < 0 || layer >= m->c.layers) { set_error("layer %d is outside 0..%d", layer, m->c.layers - 1); return -1; }
+    if (!m->paged4.empty()) { set_error("the model's paged cache is one of 4 bits"); return -1; }
     *out = m->paged[(size_t) layer];
+    return 0;
+}
+
+int sparkmv_model_paged4_cache(void * model, int layer, sparkmv_kv4_cache * out) {
+    Model * m = (Model *) model;
+    if (!m || !out) { set_error("model or output is null"); return -1; }
+    if (!m->pmem) { set_error("the model has no paged cache: call sparkmv_model_paged4 first"); return -1; }
+    if (layer < 0 || layer >= m->c.layers) { set_error("layer %d is outside 0..%d", layer, m->c.layers - 1); return -1; }
+    if (m->paged4.empty()) { set_error("the model's paged cache is one of 8 bits"); return -1; }
+    *out = m->paged4[(size_t) layer];
     return 0;
 }
 
@@ -2463,7 +2502,8 @@ int sparkmv_model_paged_step(void * model, const uint32_t * tokens, int nseq, co
     memset(&b, 0, sizeof b);
     b.nseq = nseq; b.ntok = ntok; b.max_q = max_q; b.max_len = max_len;
     b.slot = m->pstep; b.pos = m->pstep + kPagedSeq; b.qstart = m->pstep + 2 * kPagedSeq;
-    const size_t need = sparkmv_kv_attend_work(&k, &b, m->c.heads);
+    const size_t need = m->paged4.empty() ? sparkmv_kv_attend_work(&k, &b, m->c.heads)
+                                          : sparkmv_kv4_attend_work(&m->paged4[0], &b, m->c.heads);
     if (!m->vmem || ntok > m->vcap || need > m->pwork_bytes) {
         if (m->vmem || m->pwork) {
             hipError_t e = hipDeviceSynchronize();

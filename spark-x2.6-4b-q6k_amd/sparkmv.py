@@ -245,6 +245,8 @@ SIGNATURES = {
     "sparkmv_model_embed_row": (_I, [_P, ctypes.c_uint32, _P, _P]),
     "sparkmv_argmax": (_I, [_P, _I, _P, _P]),
     "sparkmv_model_paged": (_I, [_P, _I, _I, _I]),
+    "sparkmv_model_paged4": (_I, [_P, _I, _I, _I]),
+    "sparkmv_model_paged4_cache": (_I, [_P, _I, ctypes.POINTER(Kv4Cache)]),
     "sparkmv_model_set_pages": (_I, [_P, _I, ctypes.POINTER(_I), _I, _P]),
     "sparkmv_model_paged_cache": (_I, [_P, _I, ctypes.POINTER(KvCache)]),
     "sparkmv_model_paged_step": (_I, [_P, ctypes.POINTER(ctypes.c_uint32), _I, ctypes.POINTER(_I), ctypes.POINTER(_I),
@@ -780,11 +782,17 @@ class Model:
     def __len__(self):
         return lib().sparkmv_model_len(self.h)
 
-    def paged(self, npages, nslots, max_pages):
-        """Make the paged 8-bit cache of several sequences (sparkmv_model_paged),
-        beside the f32 cache of forward and verify."""
+    paged_bits = 8
+
+    def paged(self, npages, nslots, max_pages, bits=8):
+        """Make the paged cache of several sequences, of 8 or 4 bits
+        (sparkmv_model_paged, _paged4), beside the f32 cache of forward and verify."""
         torch = _torch()
-        check(lib().sparkmv_model_paged(self.h, int(npages), int(nslots), int(max_pages)), "model paged")
+        if bits not in (8, 4):
+            raise SparkmvError(f"model paged: a cache of {bits} bits is none of 8 and 4")
+        make = lib().sparkmv_model_paged if bits == 8 else lib().sparkmv_model_paged4
+        check(make(self.h, int(npages), int(nslots), int(max_pages)), "model paged")
+        self.paged_bits = bits
         self.paged_device = torch.device("cuda", torch.cuda.current_device())
 
     def set_pages(self, slot, pages, stream=None):
@@ -813,8 +821,9 @@ class Model:
         """Cached positions of a layer as PagedKV.read gives them: start and slot
         device int32, k_out and v_out [nseq, n, kv_heads, head_dim], f32 or bf16
         (either may be None)."""
-        c = KvCache()
-        check(lib().sparkmv_model_paged_cache(self.h, int(layer), ctypes.byref(c)), "model paged cache")
+        c = KvCache() if self.paged_bits == 8 else Kv4Cache()
+        of = lib().sparkmv_model_paged_cache if self.paged_bits == 8 else lib().sparkmv_model_paged4_cache
+        check(of(self.h, int(layer), ctypes.byref(c)), "model paged cache")
         _kv_read_call(c, start, k_out, v_out, slot, self.paged_device, "model paged read", ())(stream)
 
     def apply_profile(self, profile, artifact, gpu):
