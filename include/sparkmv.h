@@ -747,9 +747,12 @@ int sparkmv_kv4_read(const sparkmv_kv4_cache * cache, int nseq, const int * slot
                      void * v_out, int out_dtype, void * stream);
 
 /* Attention over the cache after the append, as sparkmv_kv_attend: causal within the
- * window, gated, zeros for a token none of whose positions has a page. f32 query
- * elements enter whole, and so does a weight for f32 outputs; for bf16 ones it is held
- * to 2^-17 of itself. Scores, statistics and sums are f32, and scores have to lie
+ * window, gated, zeros for a token none of whose positions has a page. Query elements
+ * enter whole in a call of up to 32 columns (max_q tokens times query heads per kv head);
+ * of more, an f32 element is held to 2^-24 of the largest of its 32 neighbours (those
+ * that share a scale of the keys), a bf16 one whole down to 2^-13 of that and to 2^-21
+ * below. A weight enters whole for f32 outputs; for bf16 ones it is held to 2^-17 of
+ * itself. Scores, statistics and sums are f32, and scores have to lie
  * within its range. A position that reads as NaN, in any element of its key or value,
  * makes the tokens that see it NaN and no others. work: sparkmv_kv4_attend_work bytes
  * on the current device. */

@@ -621,12 +621,14 @@ __global__ __launch_bounds__(512) void kv4_flat_join_kernel(const Kv4Flat A) {
  * operands that they become, converted once for all waves.
  *
  * The scores use the instruction that multiplies 4-bit codes as they are, 16 x 16 x 128
- * with a power of two for every 32 elements, four times as fast a product as bf16's. A
- * query element enters it as DQ numbers of 6 bits (E2M3): 32 neighbours share a power of
- * two s with |x| < 4 s, each part is the nearest number of what the ones before left out,
- * and is off by s / 8 at most, 1 / 32 of what the one before was. So an element is held
- * to 2^-24 of the largest of its 32 neighbours with five parts (bf16 queries need four
- * for their 8 bits down to 2^-11 of it).
+ * with a power of two for every 32 elements. A query element enters it as a sum of
+ * parts, each the nearest small number to what the ones before left out; 32 neighbours
+ * share a power of two:
+ *   bf16 queries as two numbers of 8 bits (E4M3), which is all of an element down to
+ *     2^-13 of the largest of the 32, and below that all but 2^-21 of the largest;
+ *   f32 queries as five numbers of 6 bits (E2M3, four times as fast a product as
+ *     bf16's), below 4 in magnitude and off by 1 / 8 at most: 2^-24 of the largest of the
+ *     32 is what may be lost. Six for head_dim 64, where an instruction takes two parts.
  *
  * Weights times values as in the flat kernels. */
 constexpr int kKv4Tile = 128;       /* columns of a workgroup */
@@ -645,7 +647,9 @@ struct Kv4Tile {
     float * pml;     /* [workgroups][2][128][2] */
 };
 
-constexpr int kv4_tile_lds(int hd) { return 2 * (32 + 128) * hd; }
+/* instructions' parts of the queries that wait in LDS: all of them leave too few registers */
+constexpr int kv4_tile_far(int hd, int dq) { return hd == 256 && dq > 2 ? 2 : 0; }
+constexpr int kv4_tile_lds(int hd, int dq) { return 2 * (32 + 128) * hd + kv4_tile_far(hd, dq) * (hd / 128) * 8 * 1536; }
 
 /* the sequence and the place within it of tile number j, from the tiles before each sequence */
 __device__ __forceinline__ KvSeq kv4_tile_seq(const sparkmv_kv_batch & b, const sparkmv_kv4_cache & c, const int * lseq, int j, int & place) {
@@ -722,9 +726,13 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
     constexpr int ND = HD / 16, NB = HD / 32, BUF = (32 + 128) * HD;
     constexpr int NJ = HD >= 128 ? HD / 128 : 1;         /* instructions of 128 elements a head */
     constexpr int NM = HD == 64 ? DQ / 2 : DQ;           /* instructions a score tile and 128 elements */
+    constexpr bool F8 = DQ == 2;                         /* parts of 8 bits, else of 6 */
+    constexpr int PW = F8 ? 8 : 6, NR = NM - kv4_tile_far(HD, DQ);   /* words of a part; instructions' parts in registers */
+    constexpr int PB = F8 ? 4 : 5;                       /* a part is held to 2^-PB of what the one before was */
     typedef __attribute__((address_space(3))) void lds_void;
     extern __shared__ __attribute__((aligned(16))) uint8_t lbuf[];   /* [2][keys' codes, values' operands] */
-    int * lseq = (int *) (lbuf + 2 * BUF), * lpre = lseq + A.b.nseq;
+    uint8_t * lfar = lbuf + 2 * BUF;                      /* [wave][part][NJ][64 lanes' 16 bytes, 64 lanes' 8] */
+    int * lseq = (int *) (lbuf + kv4_tile_lds(HD, DQ)), * lpre = lseq + A.b.nseq;
     __shared__ int lid[kKv4Ids], lsum[10];
     __shared__ uint32_t lnan[2][2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c16 = lane & 15;
@@ -793,31 +801,36 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
         const int vu = wave & 1, vk = wave >> 1;
         const bool converts = HD > 64 || wave < 4;
         uint32_t vr[8], vsc[2], ks[NJ];
+        /* buffer loads: a page's base is uniform, so its addresses are three registers a lane */
+        const uint32_t lane16 = 16 * lane, kslane = ((HD == 64 ? g & 1 : g) * 16 + c16) * 4 * NJ, vslane = (g * NB + (c16 * ND) / 32) * 16;
         auto fetch = [&](int j, int b) {
-            const uint8_t * page = A.c.data + ((size_t) max(__builtin_amdgcn_readfirstlane(lid[j & (kKv4Ids - 1)]), 0) * kvh + h) * (size_t) (68 * HD);
-            uint8_t * to = lbuf + (size_t) b * BUF;
-            if (wave < HD / 32) __builtin_amdgcn_global_load_lds((const void *) (page + wave * 1024 + 16 * lane), (lds_void *) (to + wave * 1024), 16, 0, 0);
-            const uint8_t * kp = page + 64 * HD + ((HD == 64 ? g & 1 : g) * 16 + c16) * 4 * NJ;
-#pragma unroll
-            for (int w = 0; w < NJ; w++) ks[w] = *(const uint32_t *) (kp + 4 * w);
+            const uint64_t at = (uint64_t) A.c.data + ((uint64_t) (uint32_t) max(__builtin_amdgcn_readfirstlane(lid[j & (kKv4Ids - 1)]), 0) * (uint32_t) kvh + (uint32_t) h) * (68 * HD);
+            const uint64_t lo32 = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) at), hi32 = (uint32_t) __builtin_amdgcn_readfirstlane((int) (at >> 32));
+            const auto page = __builtin_amdgcn_make_buffer_rsrc((void *) (hi32 << 32 | lo32), 0, 68 * HD, 0x00027000);
+            if (wave < HD / 32)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(page, (lds_void *) (lbuf + (size_t) b * BUF + wave * 1024), 16, lane16, wave * 1024, 0, 0);
+            if constexpr (NJ == 2) {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b64(page, kslane, 64 * HD, 0);
+                ks[0] = v[0];
+                ks[1] = v[1];
+            } else {
+                ks[0] = __builtin_amdgcn_raw_buffer_load_b32(page, kslane, 64 * HD, 0);
+            }
             if (converts) {
-                const uint8_t * vp = page + 32 * HD + (vu * (ND / 4) * 64 + lane) * 16;
+                const int vp = 32 * HD + vu * (ND / 4) * 1024;
                 if constexpr (HD == 256) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) vr[e] = *(const uint32_t *) (vp + (e >> 1) * 1024 + (e & 1) * 8 + (vk >> 1) * 4);
-                } else if constexpr (HD == 128) {
+                    for (int e = 0; e < 8; e++)
+                        vr[e] = __builtin_amdgcn_raw_buffer_load_b32(page, lane16 + (e & 1) * 8, vp + (e >> 1) * 1024 + (vk >> 1) * 4, 0);
+                } else {
 #pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        const kv4_u4 v = *(const kv4_u4 *) (vp + w * 1024);
+                    for (int w = 0; w < HD / 64; w++) {
+                        const kv4_u4 v = (kv4_u4) __builtin_amdgcn_raw_buffer_load_b128(page, lane16, vp + w * 1024, 0);
 #pragma unroll
                         for (int e = 0; e < 4; e++) vr[4 * w + e] = v[e];
                     }
-                } else {
-                    const kv4_u4 v = *(const kv4_u4 *) vp;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) vr[e] = v[e];
                 }
-                const kv4_u2 v = *(const kv4_u2 *) (page + 66 * HD + (g * NB + (c16 * ND) / 32) * 16 + 8 * vu);
+                const auto v = __builtin_amdgcn_raw_buffer_load_b64(page, vslane + 8 * vu, 66 * HD, 0);
                 vsc[0] = v[0];
                 vsc[1] = v[1];
             }
@@ -880,42 +893,48 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
         const int wpos_lo = s.pos + min(wfirst, last) / G, wpos_hi = s.pos + min(wfirst + 15, last) / G;   /* the wave's first and last token */
         const int wbeg_lo = A.q.window > 0 && wpos_lo + 1 > A.q.window ? wpos_lo + 1 - A.q.window : 0;
         const int wbeg_hi = A.q.window > 0 && wpos_hi + 1 > A.q.window ? wpos_hi + 1 - A.q.window : 0;
-        kv4_u6 qd[NM][NJ];
+        uint32_t qd[NR][NJ][PW] = {};
+        uint8_t * far = lfar + wave * (NM - NR) * NJ * 1536;
         uint32_t qs[NJ][2];   /* the parts' scales, a byte each */
         float f;
         {
-            float x[NJ][32];
             int ex[NJ], most = -1000;
             bool bad = false;
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                const size_t at = (size_t) (s.row + tok) * A.q.ldq + (size_t) head * HD + 32 * (HD == 64 ? g & 1 : 4 * j + g);
-                uint32_t big = 0;
-                if (A.q.q_dtype == SPARKMV_X_F32) {
+            float x[32];
+            const size_t row = (size_t) (s.row + tok) * A.q.ldq + (size_t) head * HD;
+            auto load = [&](int at0, int at1) {   /* 16 elements each */
+                if (!F8) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const kv_f4 v = *(const kv_f4 *) ((const float *) A.q.q + at + 4 * e);
+                        const kv_f4 v = *(const kv_f4 *) ((const float *) A.q.q + row + (e < 4 ? at0 : at1) + 4 * (e & 3));
 #pragma unroll
-                        for (int i = 0; i < 4; i++) x[j][4 * e + i] = v[i];
+                        for (int i = 0; i < 4; i++) x[4 * e + i] = v[i];
                     }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const kv4_u4 v = *(const kv4_u4 *) ((const uint16_t *) A.q.q + at + 8 * e);
+                        const kv4_u4 v = *(const kv4_u4 *) ((const uint16_t *) A.q.q + row + (e < 2 ? at0 : at1) + 8 * (e & 1));
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            x[j][8 * e + 2 * i] = __uint_as_float(v[i] << 16);
-                            x[j][8 * e + 2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+                            x[8 * e + 2 * i] = __uint_as_float(v[i] << 16);
+                            x[8 * e + 2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
                         }
                     }
                 }
+            };
 #pragma unroll
-                for (int e = 0; e < 32; e++) big = max(big, __float_as_uint(x[j][e]) & 0x7fffffffu);
+            for (int j = 0; j < NJ; j++) {
+                const int at = 32 * (HD == 64 ? g & 1 : 4 * j + g);
+                load(at, at + 16);
+                uint32_t big = 0;
+#pragma unroll
+                for (int e = 0; e < 32; e++) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
                 bad = bad || big >= 0x7f800000u;
                 int e2 = 0;
                 (void) frexpf(__uint_as_float(big >= 0x7f800000u ? 0u : big), &e2);
                 ex[j] = big ? e2 : -1000;
                 most = max(most, ex[j]);
+                __builtin_amdgcn_sched_barrier(0);
             }
             /* the column's exponent; blocks far below it count as nothing */
             most = max(most, __shfl_xor(most, 16, 64));
@@ -928,40 +947,72 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
             const float sign = A.q.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                const int low = max(ex[j] - most, -90);
-                const bool none = any || ex[j] - most < -90;
-                /* x / 2^(ex - 2) < 4 in magnitude; part d in steps of 2^(-5 d) of that */
+                /* this lane's elements: its block; or with 8 bits, where a lane holds two times 16
+                 * of the instruction's, halves of blocks g / 2 and 2 + g / 2 (64 elements: of g / 2) */
+                const int low = max(ex[j] - most, -90), at = 32 * (HD == 64 ? g & 1 : 4 * j + g);
+                const int at0 = F8 ? 32 * (4 * j + (g >> 1)) + 16 * (g & 1) : at, at1 = F8 ? at0 + (HD == 64 ? 0 : 64) : at + 16;
+                const int ex0 = F8 ? __shfl(ex[j], 16 * (g >> 1) + c16, 64) : ex[j];
+                const int ex1 = F8 && HD >= 128 ? __shfl(ex[j], 32 + 16 * (g >> 1) + c16, 64) : ex0;
+                const bool none0 = any || ex0 - most < -90, none1 = any || ex1 - most < -90;
+                /* below 4 in magnitude, or 256 with 8 bits; part d in steps of 2^(-PB d) of that.
+                 * Read again: all blocks at once would not fit the registers */
+                load(at0, at1);
+                constexpr int top = F8 ? 8 : 2;
 #pragma unroll
-                for (int e = 0; e < 32; e++) x[j][e] = none ? 0.0f : ldexpf(x[j][e] * sign, 2 - ex[j]);
+                for (int e = 0; e < 32; e++) x[e] = (e < 16 ? none0 : none1) ? 0.0f : ldexpf(x[e] * sign, top - (e < 16 ? ex0 : ex1));
                 qs[j][0] = qs[j][1] = 0;
 #pragma unroll
                 for (int d = 0; d < DQ; d++) {
-                    kv4_f16 ev, od;
+                    uint32_t part[PW];
+                    if constexpr (F8) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        ev[e] = x[j][2 * e];
-                        od[e] = x[j][2 * e + 1];
+                        for (int e = 0; e < 8; e++) {
+                            int v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * e], x[4 * e + 1], 0, false);
+                            v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * e + 2], x[4 * e + 3], v, true);
+                            part[e] = (uint32_t) v;
+                            const auto lo2 = __builtin_amdgcn_cvt_pk_f32_fp8(v, false), hi2 = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
+                            x[4 * e] = (x[4 * e] - lo2[0]) * 16.0f;
+                            x[4 * e + 1] = (x[4 * e + 1] - lo2[1]) * 16.0f;
+                            x[4 * e + 2] = (x[4 * e + 2] - hi2[0]) * 16.0f;
+                            x[4 * e + 3] = (x[4 * e + 3] - hi2[1]) * 16.0f;
+                        }
+                    } else {
+                        kv4_f16 ev, od;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            ev[e] = x[2 * e];
+                            od[e] = x[2 * e + 1];
+                        }
+                        const kv4_u6 six = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev, od, 1.0f);
+                        const kv4_f32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(six, 1.0f);
+#pragma unroll
+                        for (int e = 0; e < 6; e++) part[e] = six[e];
+#pragma unroll
+                        for (int e = 0; e < 32; e++) x[e] = (x[e] - back[e]) * 32.0f;
                     }
-                    const kv4_u6 part = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev, od, 1.0f);
-                    const kv4_f32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(part, 1.0f);
-#pragma unroll
-                    for (int e = 0; e < 32; e++) x[j][e] = (x[j][e] - back[e]) * 32.0f;
-                    const uint32_t sb = (uint32_t) (127 + low - 2 - 5 * d);
+                    const uint32_t sb = (uint32_t) (127 + low - top - PB * d);
                     if constexpr (HD == 64) {
-                        /* two parts an instruction: lanes of blocks 2 and 3 take the second one */
+                        /* two parts an instruction: the second one in the place of blocks 2 and 3 */
                         const bool mine = (g >> 1) == (d & 1);
-                        if (d & 1) {
 #pragma unroll
-                            for (int e = 0; e < 6; e++) qd[d / 2][j][e] = mine ? part[e] : qd[d / 2][j][e];
-                        } else {
-                            qd[d / 2][j] = part;
+                        for (int e = 0; e < PW; e++) {
+                            if constexpr (F8) qd[d / 2][j][e] = (e < 4) == !(d & 1) ? part[e] : qd[d / 2][j][e];
+                            else qd[d / 2][j][e] = mine || !(d & 1) ? part[e] : qd[d / 2][j][e];
                         }
                         if (mine) qs[j][0] |= sb << (8 * (d / 2));
                     } else {
-                        qd[d][j] = part;
+                        if (d < NR) {
+#pragma unroll
+                            for (int e = 0; e < PW; e++) qd[d % NR][j][e] = part[e];
+                        } else {
+                            uint8_t * to = far + ((d - NR) * NJ + j) * 1536;
+                            *(kv4_u4 *) (to + 16 * lane) = kv4_u4{part[0], part[1], part[2], part[3]};
+                            *(kv4_u2 *) (to + 1024 + 8 * lane) = kv4_u2{part[4], part[5]};
+                        }
                         qs[j][d / 4] |= sb << (8 * (d % 4));
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         convert(0);
@@ -969,47 +1020,67 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
         kv_f4 o[ND];
 #pragma unroll
         for (int d = 0; d < ND; d++) o[d] = kv_f4{0.f, 0.f, 0.f, 0.f};
+        int idn = lid[0];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   /* this wave's part of page 0 */
         for (int j = 0; j < seg; j++) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   /* this wave's part of page j */
-            __syncthreads();                                    /* everyone's, and everyone is done with the other buffer */
-            const int b = j & 1, id = lid[j & (kKv4Ids - 1)];
+            __syncthreads();   /* everyone's part of page j, and everyone is done with the other buffer */
+            const int b = j & 1, id = idn, p0 = (first + j) * kKvPage;
             uint32_t ksj[NJ];
 #pragma unroll
             for (int w = 0; w < NJ; w++) ksj[w] = ks[w];
             if (j + 1 < seg) {
-                if ((j & (kKv4Ids - 1)) == kKv4Ids - 1) ids(j + 1);
+                if (((j + 1) & (kKv4Ids - 1)) == 0) ids(j + 1);
+                idn = lid[(j + 1) & (kKv4Ids - 1)];
                 fetch(j + 1, b ^ 1);
             }
-            const int p0 = (first + j) * kKvPage;
+            const uint8_t * kp = lbuf + (size_t) b * BUF, * vp = kp + 32 * HD + 16 * lane;
             if (live && id >= 0 && p0 <= wpos_hi && p0 + kKvPage - 1 >= wbeg_lo) {   /* uniform in the wave */
-                const uint8_t * kp = lbuf + (size_t) b * BUF, * vp = kp + 32 * HD + 16 * lane;
-                /* scores: tile t's positions 4 g + e of this lane's column */
-                float x[4][4];
+                /* scores: tile t's positions 4 g + e of this lane's column. Four tiles at a time,
+                 * so that no product waits for the sum before it */
+                kv_f4 x[4];
+                kv_i4 kf[4];
+                auto keys = [&](int jj) {
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    kv_f4 acc = kv_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int jj = 0; jj < NJ; jj++) {
-                        kv4_i8 kf = {0, 0, 0, 0, 0, 0, 0, 0};
+                    for (int t = 0; t < 4; t++) {
                         if constexpr (HD >= 128) {
-                            const kv_i4 v = *(const kv_i4 *) (kp + ((t * NJ + jj) * 64 + lane) * 16);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) kf[e] = v[e];
+                            kf[t] = *(const kv_i4 *) (kp + ((t * NJ + jj) * 64 + lane) * 16);
                         } else {
 #pragma unroll
                             for (int w = 0; w < 2; w++) {
                                 const kv4_u2 v = *(const kv4_u2 *) (kp + ((t * 4 + 2 * (g & 1) + w) * 16 + c16) * 8);
-                                kf[2 * w] = (int) v[0];
-                                kf[2 * w + 1] = (int) v[1];
+                                kf[t][2 * w] = (int) v[0];
+                                kf[t][2 * w + 1] = (int) v[1];
                             }
                         }
-                        const int k = t * NJ + jj;   /* its scale: byte k of ksj */
+                    }
+                };
 #pragma unroll
-                        for (int d = NM - 1; d >= 0; d--) {
-                            kv4_i8 qf = {0, 0, 0, 0, 0, 0, 0, 0};
+                for (int t = 0; t < 4; t++) x[t] = kv_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                            for (int e = 0; e < 6; e++) qf[e] = (int) qd[d][jj][e];
-#define KV4_SCORE(KB, QB) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf, acc, 4, 2, KB, (int) ksj[k / 4], QB, (int) qs[jj][d / 4])
+                for (int jj = 0; jj < NJ; jj++) {
+                    keys(jj);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int d = NM - 1; d >= 0; d--) {
+                        kv4_i8 qf = {0, 0, 0, 0, 0, 0, 0, 0};
+                        if (d < NR) {
+#pragma unroll
+                            for (int e = 0; e < PW; e++) qf[e] = (int) qd[d % NR][jj][e];
+                        } else {
+                            const uint8_t * from = far + ((d - NR) * NJ + jj) * 1536;
+                            const kv4_u4 v4 = *(const kv4_u4 *) (from + 16 * lane);
+                            const kv4_u2 v2 = *(const kv4_u2 *) (from + 1024 + 8 * lane);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) qf[e] = (int) v4[e];
+                            qf[4] = (int) v2[0];
+                            qf[5] = (int) v2[1];
+                        }
+#pragma unroll
+                        for (int t = 0; t < 4; t++) {
+                            const kv_i4 v = kf[t];
+                            const kv4_i8 k8 = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
+                            const int k = t * NJ + jj;   /* its scale: byte k of ksj */
+#define KV4_SCORE(KB, QB) x[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k8, qf, x[t], 4, F8 ? 0 : 2, KB, (int) ksj[k / 4], QB, (int) qs[jj][d / 4])
 #define KV4_SCORE_Q(QB)                                                                                              \
     do {                                                                                                             \
         if (k % 4 == 0) KV4_SCORE(0, QB);                                                                            \
@@ -1025,8 +1096,6 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
 #undef KV4_SCORE
                         }
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[t][e] = acc[e];
                 }
                 /* positions that are not numbers: bits 0 .. 63 */
                 uint64_t nan = (uint64_t) __builtin_amdgcn_readfirstlane((int) lnan[b][1]) << 32 | (uint32_t) __builtin_amdgcn_readfirstlane((int) lnan[b][0]);
@@ -1046,12 +1115,13 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
                 }
                 float ff = f;
                 if (p0 < wbeg_hi || p0 + kKvPage - 1 > wpos_lo || nan) {
+                    const uint32_t nan_lo = (uint32_t) nan >> (4 * g), nan_hi = (uint32_t) (nan >> 32) >> (4 * g);
 #pragma unroll
                     for (int t = 0; t < 4; t++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int p = p0 + 16 * t + 4 * g + e;
-                            const bool seen = p >= beg_c && p <= pos_c, num = !(nan >> (16 * t + 4 * g + e) & 1);
+                            const bool seen = p >= beg_c && p <= pos_c, num = !((t < 2 ? nan_lo : nan_hi) >> (16 * (t & 1) + e) & 1);
                             x[t][e] = seen && num ? x[t][e] * f : -INFINITY;
                             if (seen && !num) l = __uint_as_float(0x7fc00000u);
                         }
@@ -1079,29 +1149,45 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
                         x[t][e] = __builtin_amdgcn_exp2f(fmaf(x[t][e], ff, -mref));
                         l += x[t][e];
                     }
+                /* the weights' parts, pairs of positions */
+                kv4_u4 P[2][DP];
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    kv4_u4 P[DP];
+                for (int w = 0; w < 2; w++)
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         float y = x[2 * w + (k >> 1)][2 * (k & 1)], z = x[2 * w + (k >> 1)][2 * (k & 1) + 1];
 #pragma unroll
                         for (int d = 0; d < DP; d++) {
-                            P[d][k] = kv_bf16x2(y, z);
-                            y -= __uint_as_float(P[d][k] << 16);
-                            z -= __uint_as_float(P[d][k] & 0xffff0000u);
+                            P[w][d][k] = kv_bf16x2(y, z);
+                            y -= __uint_as_float(P[w][d][k] << 16);
+                            z -= __uint_as_float(P[w][d][k] & 0xffff0000u);
                         }
                     }
+                /* the values' operands, VG at a time, one group ahead of the products */
+                constexpr int VG = F8 ? 4 : 2;
+                kv4_b8 vf[2][VG];
+                auto values = [&](int n4) {
 #pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        const kv4_b8 vf = *(const kv4_b8 *) (vp + (w * ND + d) * 1024);
+                    for (int e = 0; e < VG; e++) vf[n4 & 1][e] = *(const kv4_b8 *) (vp + (VG * n4 + e) * 1024);
+                };
+                values(0);
 #pragma unroll
-                        for (int i = DP - 1; i >= 0; i--)
-                            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(kv4_b8, P[i]), o[d], 0, 0, 0);
-                    }
+                for (int n4 = 0; n4 < 2 * ND / VG; n4++) {
+                    if (n4 + 1 < 2 * ND / VG) values(n4 + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int w = n4 / (ND / VG), d0 = VG * (n4 % (ND / VG));
+#pragma unroll
+                    for (int i = DP - 1; i >= 0; i--)
+#pragma unroll
+                        for (int e = 0; e < VG; e++)
+                            o[d0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[n4 & 1][e], __builtin_bit_cast(kv4_b8, P[w][i]), o[d0 + e], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (j + 1 < seg) convert(b ^ 1);
+            if (j + 1 < seg) {
+                convert(b ^ 1);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   /* this wave's part of page j + 1 */
+            }
         }
         l = kv_rows_sum(l);
         if (f != f) l = f;
@@ -1130,7 +1216,6 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
         }
         if (!A.share) return;
         u += seg;
-        __syncthreads();   /* the buffers and page numbers are free */
     }
 }
 
@@ -1313,10 +1398,10 @@ int sparkmv_kv4_attend(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
 #define KV4_TILE(H, DQ, DP)                                                                                          \
     do {                                                                                                             \
         static LdsAllowed allowed;                                                                                   \
-        if (lds_allow(allowed, (const void *) kv4_tile_kernel<H, DQ, DP>, kv4_tile_lds(H) + lists + 2048,            \
+        if (lds_allow(allowed, (const void *) kv4_tile_kernel<H, DQ, DP>, kv4_tile_lds(H, DQ) + lists + 2048,            \
                       "LDS opt-in for the kv4 attention"))                                                           \
             return -1;                                                                                               \
-        hipLaunchKernelGGL((kv4_tile_kernel<H, DQ, DP>), grid, dim3(512), kv4_tile_lds(H) + lists, s, t);            \
+        hipLaunchKernelGGL((kv4_tile_kernel<H, DQ, DP>), grid, dim3(512), kv4_tile_lds(H, DQ) + lists, s, t);            \
     } while (0)
 #define KV4_TILE_D(H)                                                                                                \
     do {                                                                                                             \
@@ -1325,8 +1410,8 @@ int sparkmv_kv4_attend(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
             if (q.out_dtype == SPARKMV_X_F32) KV4_TILE(H, five, 3);                                                  \
             else KV4_TILE(H, five, 2);                                                                               \
         } else {                                                                                                     \
-            if (q.out_dtype == SPARKMV_X_F32) KV4_TILE(H, 4, 3);                                                     \
-            else KV4_TILE(H, 4, 2);                                                                                  \
+            if (q.out_dtype == SPARKMV_X_F32) KV4_TILE(H, 2, 3);                                                     \
+            else KV4_TILE(H, 2, 2);                                                                                  \
         }                                                                                                            \
         if (p.groups)                                                                                                \
             hipLaunchKernelGGL(kv4_tile_join_kernel<H>, join, dim3(256), ((uint32_t) batch->nseq + 1) * 4, s, t, each); \
