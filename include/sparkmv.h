@@ -664,7 +664,8 @@ int sparkmv_rope_table_scaled(float * table, int rows, int rope_dim, double thet
  * A head x becomes x / sqrt(mean x^2 + eps) * w where a norm's weights w are given,
  * and then its first rope_dim elements turn by a row of the table: e with
  * e + rope_dim / 2, interleaved 2 e with 2 e + 1: (a, b) -> (a c - b s, b c + a s).
- * In 64 bits, rounded once to the output. */
+ * Sums and roots in 64 bits; products in 64 bits for an f32 output, rounded once, and
+ * in f32 for a bf16 one, off by half a step and 2^-20 of the head's largest element. */
 typedef struct {
     const float * rope;              /* [rope_rows][rope_dim]: cosines, then sines; NULL with rope_dim 0 */
     int rope_rows, rope_dim;

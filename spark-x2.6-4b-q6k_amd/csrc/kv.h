@@ -71,14 +71,6 @@ __device__ __forceinline__ float kv_odd(double v) {
 }
 __device__ __forceinline__ void kv_store_wide(float * p, double v) { *p = (float) v; }
 __device__ __forceinline__ void kv_store_wide(uint16_t * p, double v) { *p = kv_bf16(kv_odd(v)); }
-/* four neighbours, aligned to four of them */
-__device__ __forceinline__ void kv_store_wide4(float * p, const double * v) {
-    *(float4 *) p = float4{(float) v[0], (float) v[1], (float) v[2], (float) v[3]};
-}
-__device__ __forceinline__ void kv_store_wide4(uint16_t * p, const double * v) {
-    *(uint2 *) p = uint2{kv_bf16x2(kv_odd(v[0]), kv_odd(v[1])), kv_bf16x2(kv_odd(v[2]), kv_odd(v[3]))};
-}
-
 /* the host's checks: 0, or -1 with the message set. kv_check_rows: nrows rows of
  * n values at stride ld, each starting 16-byte aligned */
 bool kv_aligned(const void * p, size_t n);

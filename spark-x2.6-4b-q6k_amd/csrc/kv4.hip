@@ -22,6 +22,8 @@ struct Kv4Append {
     sparkmv_kv4_cache c;
     sparkmv_kv_batch b;
     sparkmv_kv4_new n;
+    HeadVec vec;
+    double inv_hd;
     int sh;                       /* lanes of a head, as a shift */
     int qparts, kparts, parts;    /* waves of a token's queries, of its keys (and of its values), of the token */
 };
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4Append A) {
     const long w = ((long) blockIdx.x * 256 + threadIdx.x) >> 6;
     const int tok = __builtin_amdgcn_readfirstlane((int) (w / A.parts));
     if (tok >= A.b.ntok) return;
-    const int lane = threadIdx.x & 63, lanes = 1 << A.sh, l = lane & (lanes - 1), per = 64 >> A.sh;
+    const int lane = threadIdx.x & 63, l = lane & ((1 << A.sh) - 1), e0 = 4 * l, per = 64 >> A.sh;
     int part = __builtin_amdgcn_readfirstlane((int) (w - (long) tok * A.parts));
     const int which = part < A.qparts ? 0 : (part < A.qparts + A.kparts ? 1 : 2);   /* queries, keys, values */
     part -= which == 0 ? 0 : (which == 1 ? A.qparts : A.qparts + A.kparts);
@@ -86,40 +88,48 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4Append A) {
     const X * in = (const X *) (which == 0 ? A.n.q : (which == 1 ? A.n.k : A.n.v)) +
                    (size_t) tok * (which == 0 ? A.n.ldq : (which == 1 ? A.n.ldk : A.n.ldv));
     const float * weight = which == 0 ? A.n.turn.q_norm : (which == 1 ? A.n.turn.k_norm : nullptr);
-    HeadLane h;
-    head_pairs(h, 4 * l, half, inter);
     const int h0 = part * U * per + (lane >> A.sh);
     float x[U][4], y[U][4];
 #pragma unroll
-    for (int u = 0; u < U; u++) head_fetch(h, in + (size_t) min(h0 + u * per, nh - 1) * hd, hd, half, inter, x[u], y[u]);
+    for (int u = 0; u < U; u++) head_fetch<4>(in + (size_t) min(h0 + u * per, nh - 1) * hd, e0, hd, half, inter, A.vec, x[u], y[u]);
     int slot, pos;
     if (!kv4_find_row(A, tok, lane, slot, pos)) return;
-    int page = 0;
-    if (which) {
-        page = A.c.pages[(size_t) slot * A.c.max_pages + pos / kKvPage];
-        if (page < 0 || page >= A.c.npages) return;
+    const float * row = half ? A.n.turn.rope + (size_t) pos * A.n.turn.rope_dim : nullptr;
+    if (which == 0) {
+        typedef typename HeadArith<X>::T T;
+        T C[4], S[4];
+        head_coef<4>(C, S, e0, hd, row, half, inter, weight, A.vec);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            T o[4];
+            const double r = head_norm<4>(x[u], weight != nullptr, A.n.turn.eps, A.inv_hd, A.sh);
+            head_turn<4>(C, S, x[u], y[u], r, o);
+            if (h0 + u * per < nh) head_store<4>((X *) A.n.q_out + (size_t) tok * A.n.ldqo + (size_t) (h0 + u * per) * hd + e0, o);
+        }
+        return;
     }
-    head_angles(h, half ? A.n.turn.rope + (size_t) pos * A.n.turn.rope_dim : nullptr, half, inter);
-    head_weights(h, weight, hd);
+    const int page = A.c.pages[(size_t) slot * A.c.max_pages + pos / kKvPage], p = pos & (kKvPage - 1);
+    if (page < 0 || page >= A.c.npages) return;
+    const int code_at = which == 1 ? kv4_key_at(p, e0, hd) : kv4_value_at(p, e0, hd);
+    const int scale_at = which == 1 ? kv4_key_scale_at(p, e0, hd) : kv4_value_scale_at(p, e0, hd);
+    double C[4], S[4];
+    if (which == 1) head_coef<4>(C, S, e0, hd, row, half, inter, weight, A.vec);
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        double o[4];
-        head_turn(h, x[u], y[u], weight != nullptr, A.n.turn.eps, hd, lanes, o);
-        const int head = h0 + u * per;
-        if (which == 0) {
-            if (head < nh) kv_store_wide4((X *) A.n.q_out + (size_t) tok * A.n.ldqo + (size_t) head * hd + h.e0, o);
-            continue;
-        }
-        float f[4];
+        if (which == 1) {
+            double o[4];
+            const double r = head_norm<4>(x[u], weight != nullptr, A.n.turn.eps, A.inv_hd, A.sh);
+            head_turn<4>(C, S, x[u], y[u], r, o);
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = (float) o[i];
+            for (int i = 0; i < 4; i++) x[u][i] = (float) o[i];
+        }
         uint32_t byte;
-        uint32_t code = kv4_code(f, byte);
+        const uint32_t code = kv4_code(x[u], byte);
+        const int head = h0 + u * per;
         if (head >= nh) continue;
         uint8_t * to = A.c.data + ((size_t) page * kvh + head) * (size_t) kv4_head_bytes(hd);
-        const int p = pos & (kKvPage - 1);
-        *(uint16_t *) (to + (which == 1 ? kv4_key_at(p, h.e0, hd) : kv4_value_at(p, h.e0, hd))) = (uint16_t) code;
-        if ((l & 7) == 0) to[which == 1 ? kv4_key_scale_at(p, h.e0, hd) : kv4_value_scale_at(p, h.e0, hd)] = (uint8_t) byte;
+        *(uint16_t *) (to + code_at) = (uint16_t) code;
+        if ((l & 7) == 0) to[scale_at] = (uint8_t) byte;
     }
 }
 
@@ -234,7 +244,9 @@ int sparkmv_kv4_append(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
     Kv4Append a;
     a.c = *cache; a.b = *batch; a.n = n;
     a.b.max_q = batch->qstart ? batch->max_q : 1;
-    a.sh = head_lane_shift(hd);
+    a.vec = head_vec(n.turn, 4);
+    a.inv_hd = 1.0 / hd;
+    a.sh = head_lane_shift(hd, 4);
     const int per = 64 >> a.sh;
     auto waves = [&](int heads, int u) { return (heads + u * per - 1) / (u * per); };
     const long all = (long) batch->ntok * (waves(n.heads, 1) + 2 * waves(cache->kv_heads, 1));

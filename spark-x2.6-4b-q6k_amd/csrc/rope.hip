@@ -9,12 +9,12 @@ namespace sparkmv {
 namespace {
 
 /* ---------------------------------------------------------------- the table
- * A thread owns one frequency and walks kRopeRun positions. */
-constexpr int kRopeRun = 64;
-
+ * A thread owns one frequency and walks `run` positions from its first: the sine and
+ * cosine there, and from one to the next a rotation by the frequency's own, each off by
+ * some 2^-52, which 32 of them do not bring near f32's 2^-24. Bound by the stores. */
 struct RopeTable {
     float * table;
-    int rows, half;
+    int rows, half, run;
     double freq[kHeadMax / 2];
     double attention;
 };
@@ -22,61 +22,68 @@ struct RopeTable {
 __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTable A) {
     const size_t n = (size_t) blockIdx.x * 256 + threadIdx.x;
     const int j = (int) (n % A.half);
-    const long p0 = (long) (n / A.half) * kRopeRun;
+    const long p0 = (long) (n / A.half) * A.run, p1 = min(p0 + A.run, (long) A.rows);
+    if (p0 >= p1) return;
     const double f = A.freq[j];
-    for (long p = p0; p < p0 + kRopeRun && p < A.rows; p++) {
-        double s, c;
-        sincos((double) p * f, &s, &c);
-        float * row = A.table + (size_t) p * 2 * A.half;
-        row[j] = (float) (c * A.attention);
-        row[A.half + j] = (float) (s * A.attention);
+    double s, c, sf, cf;
+    sincos((double) p0 * f, &s, &c);
+    sincos(f, &sf, &cf);
+    s *= A.attention;
+    c *= A.attention;
+    float * row = A.table + (size_t) p0 * 2 * A.half + j;
+    for (long p = p0; p < p1; p++, row += 2 * A.half) {
+        row[0] = (float) c;
+        row[A.half] = (float) s;
+        const double t = fma(c, cf, -(s * sf));
+        s = fma(s, cf, c * sf);
+        c = t;
     }
 }
 
 /* ------------------------------------------------------- norm and rotation
- * A wave takes up to U * (64 / lanes) heads of one token, queries or keys, whose
- * cosines, sines and weights it reads once. Bound by the rows in and out. */
+ * A wave takes up to U * (64 / lanes) heads of one token, queries or keys, whose C and S
+ * (heads.h) it works out once. Bound by the rows in and out. */
 struct QkRope {
     sparkmv_qk_rows r;
     sparkmv_head_turn t;
+    HeadVec vec;
+    double inv_hd;
     int sh;              /* lanes of a head, as a shift */
     int qparts, parts;   /* waves of a token's queries, and of the token */
 };
 
-template <typename X, int U>
+template <typename X, int EL, int U>
 __global__ __launch_bounds__(256) void qk_rope_kernel(const QkRope A) {
+    typedef typename HeadArith<X>::T T;
     const long w = ((long) blockIdx.x * 256 + threadIdx.x) >> 6;
-    const long tok = w / A.parts;
+    const int tok = __builtin_amdgcn_readfirstlane((int) (w / A.parts));
     if (tok >= A.r.ntok) return;
-    const int lane = threadIdx.x & 63, lanes = 1 << A.sh, l = lane & (lanes - 1), per = 64 >> A.sh;
-    int part = (int) (w - tok * A.parts);
+    const int lane = threadIdx.x & 63, e0 = EL * (lane & ((1 << A.sh) - 1)), per = 64 >> A.sh;
+    int part = __builtin_amdgcn_readfirstlane((int) (w - (long) tok * A.parts));
     const bool key = part >= A.qparts;
     if (key) part -= A.qparts;
-    const int hd = A.r.head_dim, half = A.t.rope_dim / 2, nh = key ? A.r.kv_heads : A.r.heads;
+    const int hd = A.r.head_dim, half = A.t.rope_dim / 2, inter = A.t.interleaved, nh = key ? A.r.kv_heads : A.r.heads;
     const X * in = (const X *) (key ? A.r.k : A.r.q) + (size_t) tok * (key ? A.r.ldk : A.r.ldq);
     X * out = (X *) (key ? A.r.k_out : A.r.q_out) + (size_t) tok * (key ? A.r.ldko : A.r.ldqo);
     const float * weight = key ? A.t.k_norm : A.t.q_norm;
-    const float * row = nullptr;
-    HeadLane h;
-    head_pairs(h, 4 * l, half, A.t.interleaved);
     const int h0 = part * U * per + (lane >> A.sh);
-    float x[U][4], y[U][4];
+    float x[U][EL], y[U][EL];
 #pragma unroll
-    for (int u = 0; u < U; u++)
-        head_fetch(h, in + (size_t) min(h0 + u * per, nh - 1) * hd, hd, half, A.t.interleaved, x[u], y[u]);
+    for (int u = 0; u < U; u++) head_fetch<EL>(in + (size_t) min(h0 + u * per, nh - 1) * hd, e0, hd, half, inter, A.vec, x[u], y[u]);
+    const float * row = nullptr;
     if (half) {
         const int p = A.r.pos[tok];
         if (p < 0 || p >= A.t.rope_rows) return;
         row = A.t.rope + (size_t) p * A.t.rope_dim;
     }
-    head_angles(h, row, half, A.t.interleaved);
-    head_weights(h, weight, hd);
+    T C[EL], S[EL];
+    head_coef<EL>(C, S, e0, hd, row, half, inter, weight, A.vec);
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        double o[4];
-        head_turn(h, x[u], y[u], weight != nullptr, A.t.eps, hd, lanes, o);
-        if (h0 + u * per >= nh || h.e0 >= hd) continue;
-        kv_store_wide4(out + (size_t) (h0 + u * per) * hd + h.e0, o);
+        T o[EL];
+        const double r = head_norm<EL>(x[u], weight != nullptr, A.t.eps, A.inv_hd, A.sh);
+        head_turn<EL>(C, S, x[u], y[u], r, o);
+        if (h0 + u * per < nh && e0 < hd) head_store<EL>(out + (size_t) (h0 + u * per) * hd + e0, o);
     }
 }
 
@@ -159,7 +166,13 @@ int sparkmv_rope_table_scaled(float * table, int rows, int rope_dim, double thet
         a.freq[i] = f;
     }
     a.attention = z.attention > 0.0 ? z.attention : (z.kind == SPARKMV_ROPE_YARN ? 0.1 * log(z.factor) + 1.0 : 1.0);
-    const size_t n = (((size_t) rows + kRopeRun - 1) / kRopeRun) * a.half, wg = (n + 255) / 256;
+    /* few rows: shorter walks, for eight waves a CU (4096 rows of 64 %RUNFIG%) */
+    const long most = 512l * cu_count();
+    a.run = 32;
+    auto threads = [&]() { return ((long) rows + a.run - 1) / a.run * a.half; };
+    while (a.run > 4 && threads() < most) a.run /= 2;
+    const long wg = (threads() + 255) / 256;
+    if (wg > kKvThreads / 256) { set_error("rope table of %d rows and %d values is too large", rows, rope_dim); return -1; }
     hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned) wg), dim3(256), 0, (hipStream_t) stream, a);
     return kv_check_launch("rope table launch");
 }
@@ -201,7 +214,11 @@ int sparkmv_qk_rope(const sparkmv_qk_rows * rows, const sparkmv_head_turn * turn
     }
     QkRope a;
     a.r = r; a.t = *turn;
-    a.sh = head_lane_shift(r.head_dim);
+    /* 16 bytes a lane where heads and halves allow */
+    const int el = r.x_dtype == SPARKMV_X_BF16 && r.head_dim % 8 == 0 && head_vec(*turn, 8).table ? 8 : 4;
+    a.vec = head_vec(*turn, el);
+    a.inv_hd = 1.0 / r.head_dim;
+    a.sh = head_lane_shift(r.head_dim, el);
     const int per = 64 >> a.sh;
     auto waves = [&](int heads, int u) { return (heads + u * per - 1) / (u * per); };
     const long all = (long) r.ntok * (waves(r.heads, 1) + waves(r.kv_heads, 1));
@@ -212,13 +229,15 @@ int sparkmv_qk_rope(const sparkmv_qk_rows * rows, const sparkmv_head_turn * turn
     if (wg > kKvThreads / 256) { set_error("qk rope of %d tokens is too much for one call", r.ntok); return -1; }
     const dim3 grid((unsigned) wg), block(256);
     hipStream_t s = (hipStream_t) stream;
-    if (r.x_dtype == SPARKMV_X_F32) {
-        if (u == 4) hipLaunchKernelGGL((qk_rope_kernel<float, 4>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((qk_rope_kernel<float, 1>), grid, block, 0, s, a);
-    } else {
-        if (u == 4) hipLaunchKernelGGL((qk_rope_kernel<uint16_t, 4>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((qk_rope_kernel<uint16_t, 1>), grid, block, 0, s, a);
-    }
+#define QK_ROPE(X, EL)                                                                                               \
+    do {                                                                                                             \
+        if (u == 4) hipLaunchKernelGGL((qk_rope_kernel<X, EL, 4>), grid, block, 0, s, a);                            \
+        else hipLaunchKernelGGL((qk_rope_kernel<X, EL, 1>), grid, block, 0, s, a);                                   \
+    } while (0)
+    if (r.x_dtype == SPARKMV_X_F32) QK_ROPE(float, 4);
+    else if (el == 8) QK_ROPE(uint16_t, 8);
+    else QK_ROPE(uint16_t, 4);
+#undef QK_ROPE
     return kv_check_launch("qk rope launch");
 }
 

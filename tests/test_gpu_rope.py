@@ -1,7 +1,11 @@
 """GPU tests of scaled rotary tables and of head norms with the rotation, against
-their definitions in 64 bits (oracle/paged4.py). Both are computed in 64 bits and
-rounded once: half a step of the output's type, and 1e-6 of that for what the 64-bit
-sums and roots may be off."""
+their definitions in 64 bits (oracle/paged4.py). Tables and f32 outputs are computed
+in 64 bits and rounded once: half a step of the output's type, and 1e-6 of that for
+what the 64-bit sums and roots may be off (where a sum cancels, 2^-49 of its terms).
+bf16 outputs are computed in f32: the two products' factors (weight times cosine or
+sine) are rounded, then one product, their sum, the root and its product, 6 roundings
+of 2^-24 of the terms' magnitudes, which are two elements at most: 2^-20 of the
+largest normed element of the head beside the half step."""
 import numpy as np
 import pytest
 
@@ -57,19 +61,20 @@ def test_qk_rope(sm, dev, heads, kvh, hd, rope, n, inter, x):
         w = [rows(dev, 1 + 0.3 * rng.standard_normal(hd), torch.float32) if on else (None, None) for on in (qn, kn)]
         want = [np.stack([paged4.turn(f[t], tab[at[t]] if rope else None, inter, wf, eps) for t in range(n)])
                 for f, (_, wf) in zip((qf, kf), w)]
+        size = [np.stack([np.abs(paged4.turn(f[t], None, inter, wf, eps)).max(-1, keepdims=True) for t in range(n)])
+                for f, (_, wf) in zip((qf, kf), w)]
 
-        def check(got, exact):
+        def check(got, exact, most):
             got = got.double().cpu().numpy()
-            # where a sum cancels, what its terms' 64-bit roundings leave
-            assert np.all(np.abs(got - exact) <= half * np.abs(exact) * (1 + 1e-6) + 2.0 ** -49 * np.abs(exact).max())
+            assert np.all(np.abs(got - exact) <= half * np.abs(exact) * (1 + 1e-6) + (2.0 ** -49 if x == "f32" else 2.0 ** -20) * most)
 
         def room(h):    # rows that start 16-byte aligned
             return torch.full((n, 8 * ((h * hd + 7) // 8)), 7.0, dtype=dt, device=dev)[:, :h * hd].unflatten(1, (h, hd))
 
         qo, ko = room(heads), room(kvh)
         sm.qk_rope(pos, q, qo, k, ko, table, inter, w[0][0], w[1][0], eps)
-        check(qo, want[0])
-        check(ko, want[1])
+        check(qo, want[0], size[0])
+        check(ko, want[1], size[1])
         q2, k2 = room(heads).copy_(q), room(kvh).copy_(k)
         sm.qk_rope(pos, q2, q2, None, None, table, inter, w[0][0], None, eps)
         sm.qk_rope(pos, None, None, k2, k2, table, inter, None, w[1][0], eps)
@@ -125,6 +130,22 @@ def test_unusual_values(sm, dev):
     for h in (0, 1, 2, 5):
         assert np.all(np.abs(got[h] - want[h]) <= 2.0 ** -24 * np.abs(want[h]) * (1 + 1e-6) + 2.0 ** -149)
     assert np.isnan(got[3]).all() and np.isnan(got[4, 5]) and np.all(got[4, np.arange(64) != 5] == 0)
+
+
+def test_unusual_bf16_values(sm, dev):
+    """Heads of any magnitude that bf16 holds, under a norm, whose squares no f32 does."""
+    import torch
+    rng = np.random.default_rng(9)
+    w, wf = rows(dev, 1 + 0.3 * rng.standard_normal(64), torch.float32)
+    x, f = rows(dev, rng.standard_normal((1, 8, 64)) * np.array([1e38, 1e30, 1e10, 1.0, 1e-10, 1e-20, 1e-30, 0.0])[None, :, None], torch.bfloat16)
+    table, out = sm.rope_table(5, 64, 1e4, dev), torch.empty_like(x)
+    eps = float(np.float32(1e-38))
+    pos = torch.tensor([3], dtype=torch.int32, device=dev)
+    for inter in (False, True):
+        sm.qk_rope(pos, x, out, rope=table, interleaved=inter, q_norm=w, eps=eps)
+        want = paged4.turn(f[0], table.cpu().numpy()[3], inter, wf, eps)
+        size = np.abs(paged4.turn(f[0], None, inter, wf, eps)).max(-1, keepdims=True)
+        assert np.all(np.abs(out[0].double().cpu().numpy() - want) <= 2.0 ** -8 * np.abs(want) * (1 + 1e-6) + 2.0 ** -20 * size)
 
 
 def test_streams_and_capture(sm, dev):
