@@ -5,13 +5,13 @@
  * An element e of the turned part becomes (x_e C_e + x_p S_e) r, p the element it turns
  * with, r the norm's 1 / sqrt(mean x^2 + eps), C and S the cosine and the sine of the
  * pair (the sine with its sign) times the norm's weights of e and p: C and S are the
- * same for all heads of a token. p's value is read from memory again (it was just
- * fetched), which costs one load of cached data and serves any pairing.
+ * same for all heads of a token.
  *
- * The sum of squares and its root are in 64 bits, which no f32 overflows. The rest is in
- * T: 64 bits where the result is an f32 (a product of two f32 is exact there, so the
- * one rounding that counts is the last), f32 where it is a bf16, 2^-21 of the terms
- * beside its half step of 2^-8. */
+ * The arithmetic is in T: 64 bits where the result is an f32 (a product of two f32 is
+ * exact there, and no sum of squares overflows, so the one rounding that counts is the
+ * last), f32 where it is a bf16: 5 roundings of 2^-24 in the root, counting its halving
+ * of those in the sum, and 5 more in the turn, 2^-20 of the head's largest normed element
+ * beside a half step of 2^-8. A head whose squares leave f32's range takes 64 bits. */
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -32,47 +32,24 @@ inline int head_lane_shift(int n, int el) {
 /* 0, or -1 with the message set; nrow: positions that the table has to cover */
 int check_turn(const char * what, const sparkmv_head_turn * t, int head_dim, long nrow);
 
-/* what a launch knows of the alignment of a turn's arrays, for EL elements a lane */
-struct HeadVec {
-    int table, weights;   /* their pieces can be loaded whole */
-};
-inline HeadVec head_vec(const sparkmv_head_turn & t, int el) {
-    HeadVec v;
-    const int half = t.rope_dim / 2;
-    v.table = ((uintptr_t) t.rope & 15) == 0 && half % 4 == 0 && (t.interleaved ? t.rope_dim : half) % el == 0;
-    v.weights = (((uintptr_t) t.q_norm | (uintptr_t) t.k_norm) & 15) == 0;
-    return v;
-}
-
 namespace {
 
-template <int N>
-__device__ __forceinline__ void head_load(const float * p, float * x) {
-    if constexpr (N == 2) {
-        const float2 v = *(const float2 *) p;
-        x[0] = v.x; x[1] = v.y;
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; k += 4) {
-            const float4 v = *(const float4 *) (p + k);
-            x[k] = v.x; x[k + 1] = v.y; x[k + 2] = v.z; x[k + 3] = v.w;
-        }
-    }
+/* EL neighbours as they lie in memory */
+template <typename X, int EL> struct HeadRaw { uint32_t v[EL * sizeof(X) / 4]; };
+
+template <int EL>
+__device__ __forceinline__ void head_load(const float * p, HeadRaw<float, EL> & x) {
+    const uint4 w = *(const uint4 *) p;
+    x.v[0] = w.x; x.v[1] = w.y; x.v[2] = w.z; x.v[3] = w.w;
 }
-template <int N>
-__device__ __forceinline__ void head_load(const uint16_t * p, float * x) {
-    uint32_t v[N / 2];
-    if constexpr (N == 4) {
+template <int EL>
+__device__ __forceinline__ void head_load(const uint16_t * p, HeadRaw<uint16_t, EL> & x) {
+    if constexpr (EL == 4) {
         const uint2 w = *(const uint2 *) p;
-        v[0] = w.x; v[1] = w.y;
+        x.v[0] = w.x; x.v[1] = w.y;
     } else {
         const uint4 w = *(const uint4 *) p;
-        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-    }
-#pragma unroll
-    for (int k = 0; k < N / 2; k++) {
-        x[2 * k] = __uint_as_float(v[k] << 16);
-        x[2 * k + 1] = __uint_as_float(v[k] & 0xffff0000u);
+        x.v[0] = w.x; x.v[1] = w.y; x.v[2] = w.z; x.v[3] = w.w;
     }
 }
 
@@ -81,90 +58,69 @@ __device__ __forceinline__ int head_pair(int e, int half, int inter) {
     return e >= 2 * half ? e : (inter ? e ^ 1 : (e < half ? e + half : e - half));
 }
 
-/* C and S of elements e0 .. of a head of hd. row: the token's row of the table (half
- * 0: nothing turns); w: the norm's weights, or null */
-template <int EL, typename T>
-__device__ __forceinline__ void head_coef(T * C, T * S, int e0, int hd, const float * row, int half, int inter, const float * w,
-                                          const HeadVec & vec) {
-    float c[EL], s[EL], we[EL], wp[EL];
+/* one element's part in a turn: its norm's weight and its partner's, and where its
+ * cosine and sine stand in a row of the table */
+struct HeadFactor {
+    float we, wp;
+    int at;      /* -1: it does not turn */
+    bool first;  /* of its pair */
+};
+/* w: the norm's weights, or null */
+__device__ __forceinline__ HeadFactor head_factor(int e, int half, int inter, const float * w) {
+    const int p = head_pair(e, half, inter);
+    return {w ? w[e] : 1.0f, w ? w[p] : 1.0f, p == e ? -1 : (inter ? e >> 1 : min(e, p)), p > e};
+}
+template <typename T>
+__device__ __forceinline__ void head_coef(const HeadFactor & f, float c, float s, T & C, T & S) {
+    C = f.at < 0 ? (T) f.we : (T) c * (T) f.we;
+    /* -0: with a partner of 0 it adds nothing, and keeps the sign of a zero */
+    S = f.at < 0 ? (T) -0.0 : (T) (f.first ? -s : s) * (T) f.wp;
+}
+
+template <int EL>
+__device__ __forceinline__ void head_widen(const HeadRaw<float, EL> & x, float * a) {
 #pragma unroll
-    for (int i = 0; i < EL; i++) {
-        c[i] = we[i] = wp[i] = 1.0f;
-        s[i] = -0.0f;   /* with y = 0: adds nothing, and keeps the sign of a zero */
-    }
-    if (e0 < hd && w) {
-        if (vec.weights) head_load<EL>(w + e0, we);
-        else
+    for (int i = 0; i < EL; i++) a[i] = __uint_as_float(x.v[i]);
+}
+template <int EL>
+__device__ __forceinline__ void head_widen(const HeadRaw<uint16_t, EL> & x, float * a) {
 #pragma unroll
-            for (int i = 0; i < EL; i++) we[i] = w[min(e0 + i, hd - 1)];
-    }
-    if (e0 < 2 * half) {
-        if (vec.table) {   /* all of the lane's elements turn */
-            if (inter) {
-                float a[EL / 2], b[EL / 2];
-                head_load<EL / 2>(row + e0 / 2, a);
-                head_load<EL / 2>(row + half + e0 / 2, b);
-#pragma unroll
-                for (int i = 0; i < EL; i++) {
-                    c[i] = a[i / 2];
-                    s[i] = i & 1 ? b[i / 2] : -b[i / 2];
-                    wp[i] = we[i ^ 1];
-                }
-            } else {
-                const bool up = e0 >= half;
-                head_load<EL>(row + (up ? e0 - half : e0), c);
-                head_load<EL>(row + half + (up ? e0 - half : e0), s);
-                if (w) {
-                    const float * q = w + (up ? e0 - half : e0 + half);
-                    if (vec.weights) head_load<EL>(q, wp);
-                    else
-#pragma unroll
-                        for (int i = 0; i < EL; i++) wp[i] = q[i];
-                }
-#pragma unroll
-                for (int i = 0; i < EL; i++) s[i] = up ? s[i] : -s[i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < EL; i++) {
-                const int e = e0 + i, p = head_pair(e, half, inter);
-                if (p == e) continue;
-                const int j = inter ? e >> 1 : (e < half ? e : e - half);
-                c[i] = row[j];
-                s[i] = p > e ? -row[half + j] : row[half + j];
-                if (w) wp[i] = w[p];
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < EL; i++) {
-        C[i] = (T) c[i] * (T) we[i];
-        S[i] = (T) s[i] * (T) wp[i];
+    for (int i = 0; i < EL / 2; i++) {
+        a[2 * i] = __uint_as_float(x.v[i] << 16);
+        a[2 * i + 1] = __uint_as_float(x.v[i] & 0xffff0000u);
     }
 }
 
-/* the elements and those they turn with (0 where they do not); a lane past the head gives zeros */
+/* Elements e0 .. (in x) and those that they turn with as f32: a partner in another lane
+ * is asked of that lane, or read from the row where halves are no whole pieces (vec 0).
+ * Zeros where an element does not turn, and in a lane past the head. */
 template <int EL, typename X>
-__device__ __forceinline__ void head_fetch(const X * row, int e0, int hd, int half, int inter, const HeadVec & vec, float * x, float * y) {
+__device__ __forceinline__ void head_wide(const HeadRaw<X, EL> & x, const X * row, int e0, int hd, int half, int inter, int vec,
+                                          float * a, float * b) {
+    head_widen<EL>(x, a);
 #pragma unroll
-    for (int i = 0; i < EL; i++) x[i] = y[i] = 0.0f;
-    if (e0 >= hd) return;
-    head_load<EL>(row + e0, x);
-    if (e0 >= 2 * half) return;
+    for (int i = 0; i < EL; i++) a[i] = e0 < hd ? a[i] : 0.0f;
     if (inter) {
 #pragma unroll
-        for (int i = 0; i < EL; i++) y[i] = e0 + i < 2 * half ? x[i ^ 1] : 0.0f;
-    } else if (vec.table) {
-        head_load<EL>(row + (e0 >= half ? e0 - half : e0 + half), y);
+        for (int i = 0; i < EL; i++) b[i] = a[i ^ 1];
+    } else if (vec) {
+        HeadRaw<X, EL> y;
+        const int other = 4 * ((int) __lane_id() + (e0 < half ? half / EL : -(half / EL)));
+#pragma unroll
+        for (int i = 0; i < (int) (EL * sizeof(X) / 4); i++) y.v[i] = (uint32_t) __builtin_amdgcn_ds_bpermute(other, (int) x.v[i]);
+        head_widen<EL>(y, b);
     } else {
 #pragma unroll
-        for (int i = 0; i < EL; i++) {
-            const int p = head_pair(e0 + i, half, 0);
-            if (p != e0 + i) y[i] = kv_load(row + p);
-        }
+        for (int i = 0; i < EL; i++) b[i] = e0 + i < 2 * half ? kv_load(row + head_pair(e0 + i, half, 0)) : 0.0f;
     }
+#pragma unroll
+    for (int i = 0; i < EL; i++) b[i] = e0 + i < 2 * half ? b[i] : 0.0f;
 }
 
+template <int CTRL>
+__device__ __forceinline__ float head_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 template <int CTRL>
 __device__ __forceinline__ double head_dpp(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
@@ -174,7 +130,8 @@ __device__ __forceinline__ double head_dpp(double v) {
 }
 
 /* the sum over the 1 << sh lanes of a head, in each of them */
-__device__ __forceinline__ double head_sum(double v, int sh) {
+template <typename T>
+__device__ __forceinline__ T head_sum(T v, int sh) {
     if (sh > 0) v += head_dpp<0xb1>(v);    /* lane ^ 1 */
     if (sh > 1) v += head_dpp<0x4e>(v);    /* lane ^ 2 */
     if (sh > 2) v += head_dpp<0x141>(v);   /* lane 7 - i of eight */
@@ -184,15 +141,27 @@ __device__ __forceinline__ double head_sum(double v, int sh) {
     return v;
 }
 
-/* 1 / sqrt(mean x^2 + eps) of a head; 1 without a norm */
-template <int EL>
+/* 1 / sqrt(mean x^2 + eps) of a head, for arithmetic in T; 1 without a norm */
+template <int EL, typename T>
 __device__ __forceinline__ double head_norm(const float * x, bool norm, float eps, double inv_hd, int sh) {
     if (!norm) return 1.0;
+    if constexpr (sizeof(T) == 4) {
+        /* a bf16's square is exact in f32 within its range */
+        float s0 = x[0] * x[0], s1 = x[1] * x[1];
+#pragma unroll
+        for (int i = 2; i < EL; i += 2) {
+            s0 = fmaf(x[i], x[i], s0);
+            s1 = fmaf(x[i + 1], x[i + 1], s1);
+        }
+        const float ss = head_sum(s0 + s1, sh);
+        if (!__any(!(ss > 0x1p-90f && ss < 0x1p120f)))
+            return __builtin_amdgcn_rsq(fma((double) ss, inv_hd, (double) eps));   /* off by 2^-24 or so */
+    }
     double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < EL; i++) ss = fma((double) x[i], (double) x[i], ss);
     const double a = fma(head_sum(ss, sh), inv_hd, (double) eps);
-    /* the instruction is good to 2^-26 or so; two steps of Newton's iteration */
+    /* two steps of Newton's iteration on the instruction's root */
     double r = __builtin_amdgcn_rsq(a);
 #pragma unroll
     for (int k = 0; k < 2; k++) r = fma(0.5 * r, fma(-a * r, r, 1.0), r);

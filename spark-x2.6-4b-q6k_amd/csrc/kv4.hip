@@ -12,7 +12,8 @@ namespace sparkmv {
 namespace {
 
 /* -------------------------------------------------------------------- append
- * A wave takes up to U * (64 / lanes) heads of one token: queries, keys or values.
+ * A wave takes 64 / lanes heads at a time, a workgroup up to 4 * U such groups of one
+ * token: queries, keys and values. C and S (heads.h) are worked out once a workgroup.
  * Positions share nothing, so that no page is read and a token's codes do not
  * depend on what was there. Keys are rounded once to f32 after norm and rotation
  * (heads.h, 64 bits), and the rest is exact: the scale is a power of two from the
@@ -22,10 +23,11 @@ struct Kv4Append {
     sparkmv_kv4_cache c;
     sparkmv_kv_batch b;
     sparkmv_kv4_new n;
-    HeadVec vec;
     double inv_hd;
-    int sh;                       /* lanes of a head, as a shift */
-    int qparts, kparts, parts;    /* waves of a token's queries, of its keys (and of its values), of the token */
+    int vec;                       /* halves are whole pieces of a lane */
+    int sh;                        /* lanes of a head, as a shift */
+    int qgroups, kgroups, groups;  /* groups of a token's queries, of its keys (and of its values), of the token */
+    int parts;                     /* workgroups of a token */
 };
 
 /* the token in row tok: its slot and position; false if it is of no sequence */
@@ -76,60 +78,75 @@ __device__ __forceinline__ uint32_t kv4_code(const float * x, uint32_t & byte) {
 
 template <typename X, int U>
 __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4Append A) {
-    const long w = ((long) blockIdx.x * 256 + threadIdx.x) >> 6;
-    const int tok = __builtin_amdgcn_readfirstlane((int) (w / A.parts));
-    if (tok >= A.b.ntok) return;
-    const int lane = threadIdx.x & 63, l = lane & ((1 << A.sh) - 1), e0 = 4 * l, per = 64 >> A.sh;
-    int part = __builtin_amdgcn_readfirstlane((int) (w - (long) tok * A.parts));
-    const int which = part < A.qparts ? 0 : (part < A.qparts + A.kparts ? 1 : 2);   /* queries, keys, values */
-    part -= which == 0 ? 0 : (which == 1 ? A.qparts : A.qparts + A.kparts);
-    const int hd = A.c.head_dim, kvh = A.c.kv_heads, inter = A.n.turn.interleaved;
-    const int half = which == 2 ? 0 : A.n.turn.rope_dim / 2, nh = which ? kvh : A.n.heads;
-    const X * in = (const X *) (which == 0 ? A.n.q : (which == 1 ? A.n.k : A.n.v)) +
-                   (size_t) tok * (which == 0 ? A.n.ldq : (which == 1 ? A.n.ldk : A.n.ldv));
-    const float * weight = which == 0 ? A.n.turn.q_norm : (which == 1 ? A.n.turn.k_norm : nullptr);
-    const int h0 = part * U * per + (lane >> A.sh);
-    float x[U][4], y[U][4];
-#pragma unroll
-    for (int u = 0; u < U; u++) head_fetch<4>(in + (size_t) min(h0 + u * per, nh - 1) * hd, e0, hd, half, inter, A.vec, x[u], y[u]);
-    int slot, pos;
-    if (!kv4_find_row(A, tok, lane, slot, pos)) return;
-    const float * row = half ? A.n.turn.rope + (size_t) pos * A.n.turn.rope_dim : nullptr;
-    if (which == 0) {
-        typedef typename HeadArith<X>::T T;
-        T C[4], S[4];
-        head_coef<4>(C, S, e0, hd, row, half, inter, weight, A.vec);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            T o[4];
-            const double r = head_norm<4>(x[u], weight != nullptr, A.n.turn.eps, A.inv_hd, A.sh);
-            head_turn<4>(C, S, x[u], y[u], r, o);
-            if (h0 + u * per < nh) head_store<4>((X *) A.n.q_out + (size_t) tok * A.n.ldqo + (size_t) (h0 + u * per) * hd + e0, o);
-        }
-        return;
-    }
-    const int page = A.c.pages[(size_t) slot * A.c.max_pages + pos / kKvPage], p = pos & (kKvPage - 1);
-    if (page < 0 || page >= A.c.npages) return;
-    const int code_at = which == 1 ? kv4_key_at(p, e0, hd) : kv4_value_at(p, e0, hd);
-    const int scale_at = which == 1 ? kv4_key_scale_at(p, e0, hd) : kv4_value_scale_at(p, e0, hd);
-    double C[4], S[4];
-    if (which == 1) head_coef<4>(C, S, e0, hd, row, half, inter, weight, A.vec);
+    typedef typename HeadArith<X>::T T;
+    __shared__ T qc[kHeadMax], qs[kHeadMax];
+    __shared__ double kc[kHeadMax], ks[kHeadMax];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int tok = (int) blockIdx.x / A.parts, g0 = ((int) blockIdx.x - tok * A.parts) * 4 + wave;
+    const int l = lane & ((1 << A.sh) - 1), e0 = 4 * l, per = 64 >> A.sh;
+    const int hd = A.c.head_dim, kvh = A.c.kv_heads, inter = A.n.turn.interleaved, half = A.n.turn.rope_dim / 2;
+    HeadRaw<X, 4> x[U];
+    const X * at[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        if (which == 1) {
-            double o[4];
-            const double r = head_norm<4>(x[u], weight != nullptr, A.n.turn.eps, A.inv_hd, A.sh);
-            head_turn<4>(C, S, x[u], y[u], r, o);
+        int g = g0 + 4 * u * A.parts;
+        if (g >= A.groups) continue;
+        const int which = g < A.qgroups ? 0 : (g < A.qgroups + A.kgroups ? 1 : 2);   /* queries, keys, values */
+        g -= which == 0 ? 0 : (which == 1 ? A.qgroups : A.qgroups + A.kgroups);
+        const int h = min(g * per + (lane >> A.sh), (which ? kvh : A.n.heads) - 1);
+        at[u] = (const X *) (which == 0 ? A.n.q : (which == 1 ? A.n.k : A.n.v)) +
+                (size_t) tok * (which == 0 ? A.n.ldq : (which == 1 ? A.n.ldk : A.n.ldv)) + (size_t) h * hd;
+        head_load<4>(at[u] + e0, x[u]);
+    }
+    int slot, pos;
+    if (!kv4_find_row(A, tok, lane, slot, pos)) return;
+    const int page = A.c.pages[(size_t) slot * A.c.max_pages + pos / kKvPage], p = pos & (kKvPage - 1);
+    if (tid < hd) {
+        const HeadFactor k = head_factor(tid, half, inter, A.n.turn.k_norm);
+        float c = 1.0f, s = 0.0f;
+        if (k.at >= 0) {
+            const float * row = A.n.turn.rope + (size_t) pos * A.n.turn.rope_dim + k.at;
+            c = row[0];
+            s = row[half];
+        }
+        head_coef(k, c, s, kc[tid], ks[tid]);
+        if (A.qgroups) head_coef(head_factor(tid, half, inter, A.n.turn.q_norm), c, s, qc[tid], qs[tid]);
+    }
+    __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[u][i] = (float) o[i];
+    for (int u = 0; u < U; u++) {
+        int g = g0 + 4 * u * A.parts;
+        if (g >= A.groups) return;
+        const int which = g < A.qgroups ? 0 : (g < A.qgroups + A.kgroups ? 1 : 2);
+        g -= which == 0 ? 0 : (which == 1 ? A.qgroups : A.qgroups + A.kgroups);
+        const int h = g * per + (lane >> A.sh);
+        const bool on = h < (which ? kvh : A.n.heads);
+        float a[4], b[4];
+        head_wide<4>(x[u], at[u], e0, hd, which == 2 ? 0 : half, inter, A.vec, a, b);
+        if (which == 0) {
+            T C[4], S[4], o[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { C[i] = qc[e0 + i]; S[i] = qs[e0 + i]; }
+            const double r = head_norm<4, T>(a, A.n.turn.q_norm != nullptr, A.n.turn.eps, A.inv_hd, A.sh);
+            head_turn<4>(C, S, a, b, r, o);
+            if (on) head_store<4>((X *) A.n.q_out + (size_t) tok * A.n.ldqo + (size_t) h * hd + e0, o);
+            continue;
+        }
+        if (which == 1) {
+            double C[4], S[4], o[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { C[i] = kc[e0 + i]; S[i] = ks[e0 + i]; }
+            const double r = head_norm<4, double>(a, A.n.turn.k_norm != nullptr, A.n.turn.eps, A.inv_hd, A.sh);
+            head_turn<4>(C, S, a, b, r, o);
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[i] = (float) o[i];
         }
         uint32_t byte;
-        const uint32_t code = kv4_code(x[u], byte);
-        const int head = h0 + u * per;
-        if (head >= nh) continue;
-        uint8_t * to = A.c.data + ((size_t) page * kvh + head) * (size_t) kv4_head_bytes(hd);
-        *(uint16_t *) (to + code_at) = (uint16_t) code;
-        if ((l & 7) == 0) to[scale_at] = (uint8_t) byte;
+        const uint32_t code = kv4_code(a, byte);
+        if (!on || page < 0 || page >= A.c.npages) continue;
+        uint8_t * to = A.c.data + ((size_t) page * kvh + h) * (size_t) kv4_head_bytes(hd);
+        *(uint16_t *) (to + (which == 1 ? kv4_key_at(p, e0, hd) : kv4_value_at(p, e0, hd))) = (uint16_t) code;
+        if ((l & 7) == 0) to[which == 1 ? kv4_key_scale_at(p, e0, hd) : kv4_value_scale_at(p, e0, hd)] = (uint8_t) byte;
     }
 }
 
@@ -244,17 +261,17 @@ int sparkmv_kv4_append(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
     Kv4Append a;
     a.c = *cache; a.b = *batch; a.n = n;
     a.b.max_q = batch->qstart ? batch->max_q : 1;
-    a.vec = head_vec(n.turn, 4);
+    a.vec = n.turn.rope_dim / 2 % 4 == 0;
     a.inv_hd = 1.0 / hd;
     a.sh = head_lane_shift(hd, 4);
     const int per = 64 >> a.sh;
-    auto waves = [&](int heads, int u) { return (heads + u * per - 1) / (u * per); };
-    const long all = (long) batch->ntok * (waves(n.heads, 1) + 2 * waves(cache->kv_heads, 1));
-    const int u = all > 16 * cu_count() ? 4 : 1;
-    a.qparts = waves(n.heads, u);
-    a.kparts = waves(cache->kv_heads, u);
-    a.parts = a.qparts + 2 * a.kparts;
-    const long wg = ((long) batch->ntok * a.parts + 3) / 4;
+    a.qgroups = (n.heads + per - 1) / per;
+    a.kgroups = (cache->kv_heads + per - 1) / per;
+    a.groups = a.qgroups + 2 * a.kgroups;
+    auto parts = [&](int u) { return (a.groups + 4 * u - 1) / (4 * u); };
+    const int u = (long) batch->ntok * parts(4) >= 4 * cu_count() ? 4 : 1;
+    a.parts = parts(u);
+    const long wg = (long) batch->ntok * a.parts;
     if (wg > kKvThreads / 256) { set_error("an append of %ld workgroups is too much for one call", wg); return -1; }
     const dim3 grid((unsigned) wg), block(256);
     hipStream_t s = (hipStream_t) stream;

@@ -41,49 +41,77 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTable A) {
 }
 
 /* ------------------------------------------------------- norm and rotation
- * A wave takes up to U * (64 / lanes) heads of one token, queries or keys, whose C and S
- * (heads.h) it works out once. Bound by the rows in and out. */
+ * A wave takes 64 / lanes heads at a time, a workgroup up to 4 * U such groups of one
+ * token, queries' and then keys'. C and S (heads.h) are worked out once a workgroup, an
+ * element a thread, and shared through LDS: loaded by every lane from the table and the
+ * weights they are four times the bytes of the heads themselves, and what bounds. Now
+ * the rows in and out do. */
 struct QkRope {
     sparkmv_qk_rows r;
     sparkmv_head_turn t;
-    HeadVec vec;
     double inv_hd;
+    int vec;             /* halves are whole pieces of a lane */
     int sh;              /* lanes of a head, as a shift */
-    int qparts, parts;   /* waves of a token's queries, and of the token */
+    int qgroups, groups; /* groups of a token's queries, and of the token */
+    int parts;           /* workgroups of a token */
 };
 
 template <typename X, int EL, int U>
 __global__ __launch_bounds__(256) void qk_rope_kernel(const QkRope A) {
     typedef typename HeadArith<X>::T T;
-    const long w = ((long) blockIdx.x * 256 + threadIdx.x) >> 6;
-    const int tok = __builtin_amdgcn_readfirstlane((int) (w / A.parts));
-    if (tok >= A.r.ntok) return;
-    const int lane = threadIdx.x & 63, e0 = EL * (lane & ((1 << A.sh) - 1)), per = 64 >> A.sh;
-    int part = __builtin_amdgcn_readfirstlane((int) (w - (long) tok * A.parts));
-    const bool key = part >= A.qparts;
-    if (key) part -= A.qparts;
-    const int hd = A.r.head_dim, half = A.t.rope_dim / 2, inter = A.t.interleaved, nh = key ? A.r.kv_heads : A.r.heads;
-    const X * in = (const X *) (key ? A.r.k : A.r.q) + (size_t) tok * (key ? A.r.ldk : A.r.ldq);
-    X * out = (X *) (key ? A.r.k_out : A.r.q_out) + (size_t) tok * (key ? A.r.ldko : A.r.ldqo);
-    const float * weight = key ? A.t.k_norm : A.t.q_norm;
-    const int h0 = part * U * per + (lane >> A.sh);
-    float x[U][EL], y[U][EL];
-#pragma unroll
-    for (int u = 0; u < U; u++) head_fetch<EL>(in + (size_t) min(h0 + u * per, nh - 1) * hd, e0, hd, half, inter, A.vec, x[u], y[u]);
-    const float * row = nullptr;
-    if (half) {
-        const int p = A.r.pos[tok];
-        if (p < 0 || p >= A.t.rope_rows) return;
-        row = A.t.rope + (size_t) p * A.t.rope_dim;
+    __shared__ T lc[2][kHeadMax], ls[2][kHeadMax];   /* queries', keys' */
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int tok = (int) blockIdx.x / A.parts, g0 = ((int) blockIdx.x - tok * A.parts) * 4 + wave;
+    const int hd = A.r.head_dim, half = A.t.rope_dim / 2, inter = A.t.interleaved;
+    const int e0 = EL * (lane & ((1 << A.sh) - 1)), per = 64 >> A.sh;
+    const int p = half ? A.r.pos[tok] : 0;
+    HeadFactor qf, kf;
+    if (tid < hd) {
+        qf = head_factor(tid, half, inter, A.t.q_norm);
+        kf = head_factor(tid, half, inter, A.t.k_norm);
     }
-    T C[EL], S[EL];
-    head_coef<EL>(C, S, e0, hd, row, half, inter, weight, A.vec);
+    HeadRaw<X, EL> x[U];
+    const X * at[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
+        const int g = g0 + 4 * u * A.parts;
+        if (g >= A.groups) continue;
+        const bool key = g >= A.qgroups;
+        const int h = min((key ? g - A.qgroups : g) * per + (lane >> A.sh), (key ? A.r.kv_heads : A.r.heads) - 1);
+        at[u] = (const X *) (key ? A.r.k : A.r.q) + (size_t) tok * (key ? A.r.ldk : A.r.ldq) + (size_t) h * hd;
+        if (e0 < hd) head_load<EL>(at[u] + e0, x[u]);
+    }
+    if (half && (p < 0 || p >= A.t.rope_rows)) return;
+    if (tid < hd) {
+        float c = 0.0f, s = 0.0f;
+        if (qf.at >= 0) {
+            const float * row = A.t.rope + (size_t) p * A.t.rope_dim + qf.at;
+            c = row[0];
+            s = row[half];
+        }
+        head_coef(qf, c, s, lc[0][tid], ls[0][tid]);
+        head_coef(kf, c, s, lc[1][tid], ls[1][tid]);
+    }
+    __syncthreads();
+    T C[EL], S[EL];
+    int have = -1;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int g = g0 + 4 * u * A.parts;
+        if (g >= A.groups) return;
+        const int key = g >= A.qgroups, h = (key ? g - A.qgroups : g) * per + (lane >> A.sh);
+        if (key != have) {
+#pragma unroll
+            for (int i = 0; i < EL; i++) { C[i] = lc[key][e0 + i]; S[i] = ls[key][e0 + i]; }
+            have = key;
+        }
+        float v[EL], w[EL];
         T o[EL];
-        const double r = head_norm<EL>(x[u], weight != nullptr, A.t.eps, A.inv_hd, A.sh);
-        head_turn<EL>(C, S, x[u], y[u], r, o);
-        if (h0 + u * per < nh && e0 < hd) head_store<EL>(out + (size_t) (h0 + u * per) * hd + e0, o);
+        head_wide<EL>(x[u], at[u], e0, hd, half, inter, A.vec, v, w);
+        const double r = head_norm<EL, T>(v, (key ? A.t.k_norm : A.t.q_norm) != nullptr, A.t.eps, A.inv_hd, A.sh);
+        head_turn<EL>(C, S, v, w, r, o);
+        if (e0 < hd && h < (key ? A.r.kv_heads : A.r.heads))
+            head_store<EL>((X *) (key ? A.r.k_out : A.r.q_out) + (size_t) tok * (key ? A.r.ldko : A.r.ldqo) + (size_t) h * hd + e0, o);
     }
 }
 
@@ -166,7 +194,7 @@ int sparkmv_rope_table_scaled(float * table, int rows, int rope_dim, double thet
         a.freq[i] = f;
     }
     a.attention = z.attention > 0.0 ? z.attention : (z.kind == SPARKMV_ROPE_YARN ? 0.1 * log(z.factor) + 1.0 : 1.0);
-    /* few rows: shorter walks, for eight waves a CU (4096 rows of 64 %RUNFIG%) */
+    /* few rows: shorter walks, for eight waves a CU (4096 rows of 64 17.9 -> 4.5 us) */
     const long most = 512l * cu_count();
     a.run = 32;
     auto threads = [&]() { return ((long) rows + a.run - 1) / a.run * a.half; };
@@ -215,17 +243,18 @@ int sparkmv_qk_rope(const sparkmv_qk_rows * rows, const sparkmv_head_turn * turn
     QkRope a;
     a.r = r; a.t = *turn;
     /* 16 bytes a lane where heads and halves allow */
-    const int el = r.x_dtype == SPARKMV_X_BF16 && r.head_dim % 8 == 0 && head_vec(*turn, 8).table ? 8 : 4;
-    a.vec = head_vec(*turn, el);
+    const int half = turn->rope_dim / 2;
+    const int el = r.x_dtype == SPARKMV_X_BF16 && r.head_dim % 8 == 0 && (turn->interleaved || half % 8 == 0) ? 8 : 4;
+    a.vec = half % el == 0;
     a.inv_hd = 1.0 / r.head_dim;
     a.sh = head_lane_shift(r.head_dim, el);
     const int per = 64 >> a.sh;
-    auto waves = [&](int heads, int u) { return (heads + u * per - 1) / (u * per); };
-    const long all = (long) r.ntok * (waves(r.heads, 1) + waves(r.kv_heads, 1));
-    const int u = all > 16 * cu_count() ? 4 : 1;
-    a.qparts = waves(r.heads, u);
-    a.parts = a.qparts + waves(r.kv_heads, u);
-    const long wg = ((long) r.ntok * a.parts + 3) / 4;
+    a.qgroups = (r.heads + per - 1) / per;
+    a.groups = a.qgroups + (r.kv_heads + per - 1) / per;
+    auto parts = [&](int u) { return (a.groups + 4 * u - 1) / (4 * u); };
+    const int u = (long) r.ntok * parts(4) >= 4 * cu_count() ? 4 : 1;
+    a.parts = parts(u);
+    const long wg = (long) r.ntok * a.parts;
     if (wg > kKvThreads / 256) { set_error("qk rope of %d tokens is too much for one call", r.ntok); return -1; }
     const dim3 grid((unsigned) wg), block(256);
     hipStream_t s = (hipStream_t) stream;
