@@ -664,8 +664,8 @@ int sparkmv_rope_table_scaled(float * table, int rows, int rope_dim, double thet
  * A head x becomes x / sqrt(mean x^2 + eps) * w where a norm's weights w are given,
  * and then its first rope_dim elements turn by a row of the table: e with
  * e + rope_dim / 2, interleaved 2 e with 2 e + 1: (a, b) -> (a c - b s, b c + a s).
- * Sums and roots in 64 bits; products in 64 bits for an f32 output, rounded once, and
- * in f32 for a bf16 one, off by half a step and 2^-20 of the head's largest element. */
+ * For an f32 output in 64 bits, rounded once; for a bf16 one in f32, off by half a step
+ * and 2^-20 of the head's largest normed element. */
 typedef struct {
     const float * rope;              /* [rope_rows][rope_dim]: cosines, then sines; NULL with rope_dim 0 */
     int rope_rows, rope_dim;
@@ -749,7 +749,7 @@ int sparkmv_kv4_read(const sparkmv_kv4_cache * cache, int nseq, const int * slot
 
 /* Attention over the cache after the append, as sparkmv_kv_attend: causal within the
  * window, gated, zeros for a token none of whose positions has a page. Query elements
- * enter whole in a call of up to 32 columns (max_q tokens times query heads per kv head);
+ * enter whole in a call of up to 48 columns (max_q tokens times query heads per kv head);
  * of more, an f32 element is held to 2^-24 of the largest of its 32 neighbours (those
  * that share a scale of the keys), a bf16 one whole down to 2^-13 of that and to 2^-21
  * below. A weight enters whole for f32 outputs; for bf16 ones it is held to 2^-17 of

@@ -58,7 +58,9 @@ __device__ __forceinline__ uint32_t kv4_quad_part(const uint32_t * part, uint32_
 }
 
 constexpr int kKv4Cols = 16;      /* columns (token, query head) of a kv head that the flat kernels take at a time */
-constexpr int kKv4Item = 8;       /* pages that beginning a kv head of a sequence counts */
+/* pages that beginning a kv head of a sequence counts: with 4, 8, 12 and 16, 48 sequences of 12000 positions
+ * take 70.0, 57.7, 54.3 and 54.3 us, 3 of 6000 with 8 tokens each 19.8, 20.2, 20.1 and 21.1 */
+constexpr int kKv4Item = 12;
 constexpr int kKv4Most = 1024;    /* workgroups of shares, at most */
 
 struct Kv4Flat {
@@ -87,8 +89,10 @@ constexpr int kv4_lds(int hd, int dq, int waves, int cmax) {
 
 /* ------------------------------------------------------------- few columns
  *
- * Up to sixteen columns of a kv head: decode steps and short blocks. Bound by reading
- * the codes once.
+ * Sixteen columns of a kv head at a time: decode steps and short blocks. Bound by
+ * reading the codes, 136 bytes a position of 256: with four heads of them, 131072
+ * positions (143 MB) take 43.5 us and 48 sequences of 12000 (314 MB, partly cached from
+ * call to call) 54.1 with the join's 5; one of 1004 takes 11.6, most of it latency.
  *
  * DQ 0, up to four columns: an instruction's sixteen columns are the four columns
  * times the parts of a query element or weight, so that f32's whole precision costs
@@ -620,6 +624,12 @@ __global__ __launch_bounds__(512) void kv4_flat_join_kernel(const Kv4Flat A) {
  * it is worked on: codes of keys as they lie, by direct loads; values as the bf16
  * operands that they become, converted once for all waves.
  *
+ * 512 bf16 tokens of 16 heads of 256 at 16384 take 205 us with the join's 14: 139 GFLOP
+ * as the formula counts them, 0.68 PFLOP/s, where a large bf16 product reaches 1.2. With
+ * any one of the parts left out (scores, exponentials, conversion, the values' product)
+ * a wave's time falls by a tenth at most: the vector and matrix pipes take turns, two
+ * waves a SIMD being all that the registers hold.
+ *
  * The scores use the instruction that multiplies 4-bit codes as they are, 16 x 16 x 128
  * with a power of two for every 32 elements. A query element enters it as a sum of
  * parts, each the nearest small number to what the ones before left out; 32 neighbours
@@ -632,7 +642,9 @@ __global__ __launch_bounds__(512) void kv4_flat_join_kernel(const Kv4Flat A) {
  *
  * Weights times values as in the flat kernels. */
 constexpr int kKv4Tile = 128;       /* columns of a workgroup */
-constexpr int kKv4TileItem = 6;     /* pages that beginning a tile's kv head counts */
+/* pages that beginning a tile's kv head counts: with 2, 6 and 12, 512 tokens at 16384
+ * take 209, 205 and 217 us, at 1000 52.8, 51.6 and 53.2 */
+constexpr int kKv4TileItem = 6;
 constexpr int kKv4Tiles = 2048;     /* tiles that are split among equal shares, at most */
 constexpr int kKv4Ids = 256;        /* page numbers held at a time */
 
@@ -1252,23 +1264,29 @@ __global__ __launch_bounds__(256) void kv4_tile_join_kernel(const Kv4Tile A, int
         const int c = ((int) blockIdx.z * each + r) * 4 + wave;
         if (col0 + c > last) return;
         auto at = [&](int k) { return (2 * (size_t) (w0 + k) + (k == 0)) * kKv4Tile + c; };
-        float M = -INFINITY, L = 0.0f;
-        for (int k = lane; k < np; k += 64) M = fmaxf(M, A.pml[2 * at(k)]);
+        /* the first rows are requested before their weights are known */
+        fe v[8];
+        auto load = [&](int k0) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = *(const fe *) (A.po + at(min(k0 + k, np - 1)) * HD + E * lane);
+        };
+        const float2 first64 = *(const float2 *) (A.pml + 2 * at(min(lane, np - 1)));
+        load(0);
+        float M = first64.x, L = 0.0f;
+        for (int k = lane + 64; k < np; k += 64) M = fmaxf(M, A.pml[2 * at(k)]);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
         fe sum = (fe) 0.0f;
         for (int k0 = 0; k0 < np; k0 += 64) {
             float f = 0.0f;
             if (k0 + lane < np) {
-                const float m = A.pml[2 * at(k0 + lane)], l = A.pml[2 * at(k0 + lane) + 1];
-                f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-                L += m == -INFINITY ? l : f * l;
+                const float2 ml = k0 ? *(const float2 *) (A.pml + 2 * at(k0 + lane)) : first64;
+                f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+                L += ml.x == -INFINITY ? ml.y : f * ml.y;
             }
             const int upto = min(64, np - k0);
             for (int k1 = 0; k1 < upto; k1 += 8) {
-                fe v[8];
-#pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = *(const fe *) (A.po + at(k0 + min(k1 + k, upto - 1)) * HD + E * lane);
+                if (k0 + k1 > 0) load(k0 + k1);
 #pragma unroll
                 for (int k = 0; k < 8; k++)
                     if (k1 + k < upto) sum += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), k1 + k)) * v[k];
@@ -1305,13 +1323,24 @@ Kv4Plan kv4_plan(const sparkmv_kv4_cache * c, const sparkmv_kv_batch * b, int he
     const long in_window = ((long) window + kKvPage - 2) / kKvPage + 1, seen = window > 0 && in_window < pages ? in_window : pages;
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += (bytes + 255) & ~(size_t) 255; return o; };
-    p.flat = cols <= 2 * kKv4Cols;
+    /* few columns read a tile's pages again for each 16; blocks of 12 tokens with 4 heads
+     * each (48 columns) of 3 sequences of 6000 24.4 us, tiles of 128 28.7; of 16 tokens
+     * 32.6 and 32.5, of one sequence of 60000 60.3 and 55.5 */
+    p.flat = cols <= 3 * kKv4Cols;
     if (p.flat) {
         p.quad = cols <= 4;
         p.cmax = (int) (cols < kKv4Cols ? cols : kKv4Cols);
         p.seq_tiles = (int) ((cols + kKv4Cols - 1) / kKv4Cols);
+        /* whole contexts against shares and a join: 16 pages of one sequence 11.6 and 13.3
+         * us, 32 17.4 and 13.4; 9 pages of 24 sequences 10.7 and 19.6 */
         p.whole = cols <= kKv4Cols && seen <= 16;
-        const long most = 2 * cu_count() < kKv4Most ? 2 * cu_count() : kKv4Most, all = pages * p.seq_tiles * b->nseq * c->kv_heads;
+        /* One workgroup a CU has fewer results to join than two, which keep more loads in
+         * flight. Two against one at head_dim 256: 500 pages 17.2 and 14.7 us, 2500 27.4
+         * and 22.0, 8192 45.9 and 44.3, 18000 40.1 and 42.3, 36000 58.3 and 63.3; at 128,
+         * with less to do for a page: 4000 13.1 and 12.4, 8000 15.4 and 16.6. */
+        const long all = seen * p.seq_tiles * b->nseq * c->kv_heads;
+        const long two = all >= (long) cu_count() * (hd == 256 ? 56 : 24) ? 2 : 1;
+        const long most = two * cu_count() < kKv4Most ? two * cu_count() : kKv4Most;
         p.groups = (int) (all < 1 ? 1 : (all < most ? all : most));
         p.pre = take(((size_t) b->nseq + 2) * 4);
         p.po = take((size_t) p.groups * 2 * p.cmax * hd * 4);
@@ -1319,7 +1348,7 @@ Kv4Plan kv4_plan(const sparkmv_kv4_cache * c, const sparkmv_kv_batch * b, int he
     } else {
         p.tiles = (long) b->ntok * G / kKv4Tile + b->nseq;
         /* shares while their counts fit */
-        if (p.tiles <= kKv4Tiles && p.tiles * ((long) c->max_pages + kKv4TileItem) <= 0x7fffffffl) {
+        if (p.tiles <= kKv4Tiles && p.tiles * ((long) c->max_pages + kKv4TileItem) <= 0x7fffffffl / c->kv_heads) {
             const long all = pages * p.tiles * c->kv_heads, most = cu_count();
             p.groups = (int) (all < 1 ? 1 : (all < most ? all : most));
             p.pre = take(((size_t) p.tiles + 2) * 4);
@@ -1393,8 +1422,10 @@ int sparkmv_kv4_attend(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
         t.pre = (int *) (mem + p.pre); t.po = (float *) (mem + p.po); t.pml = (float *) (mem + p.pml);
         const uint32_t lists = p.groups ? ((uint32_t) batch->nseq + (uint32_t) p.tiles + 1) * 4 : 0;
         const dim3 grid((unsigned) (p.groups ? p.groups : p.tiles * cache->kv_heads));
-        constexpr int each = 4;   /* columns a wave of the join */
-        const dim3 join((unsigned) p.tiles, (unsigned) cache->kv_heads, kKv4Tile / 4 / each);
+        /* columns a wave of the join: one or two, with 12 tiles' kv heads 26.2 us for the call
+         * and 29.2, with 68 39.5 and 38.0 */
+        const int each = p.tiles * cache->kv_heads * (kKv4Tile / 4) > 4 * cu_count() ? 2 : 1;
+        const dim3 join((unsigned) p.tiles, (unsigned) cache->kv_heads, (unsigned) (kKv4Tile / 4 / each));
 #define KV4_TILE(H, DQ, DP)                                                                                          \
     do {                                                                                                             \
         static LdsAllowed allowed;                                                                                   \

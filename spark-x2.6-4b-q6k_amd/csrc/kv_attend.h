@@ -92,24 +92,38 @@ __device__ __forceinline__ float kv_join(const float * po, const float * pml, in
                                          int lane, float (&o)[HD / 64]) {
     constexpr int E = HD / 64;
     typedef float fe __attribute__((ext_vector_type(E)));
-    float M = -INFINITY;
-    for (int k = lane; k < n; k += 64) M = fmaxf(M, pml[2 * at(k)]);
+    /* the first results are requested before their weights are known (joining 128 of
+     * each of 16 columns of 256: 6.7 us, now 5.9) */
+    fe v[8];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = *(const fe *) (po + at(min(k0 + W * j, n - 1)) * HD + E * lane);
+    };
+    constexpr int C = 2;
+    float2 ml[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) ml[c] = *(const float2 *) (pml + 2 * at(min(lane + 64 * c, n - 1)));
+    load(wave);
+    float M = fmaxf(ml[0].x, ml[1].x);
+    for (int k = lane + 64 * C; k < n; k += 64) M = fmaxf(M, pml[2 * at(k)]);
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor(M, s, 64));
     float L = 0.0f;
-    for (int k = lane; k < n; k += 64) {
-        const float m = pml[2 * at(k)], l = pml[2 * at(k) + 1], f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+    auto take = [&](int k, float m, float l) {
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
         L += m == -INFINITY ? l : f * l;
         if (wave == 0) wts[k] = f;
-    }
+    };
+#pragma unroll
+    for (int c = 0; c < C; c++)
+        if (lane + 64 * c < n) take(lane + 64 * c, ml[c].x, ml[c].y);
+    for (int k = lane + 64 * C; k < n; k += 64) take(k, pml[2 * at(k)], pml[2 * at(k) + 1]);
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) L += __shfl_xor(L, s, 64);
     __syncthreads();
     fe sum = (fe) 0.0f;
     for (int k0 = wave; k0 < n; k0 += 8 * W) {
-        fe v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = *(const fe *) (po + at(min(k0 + W * j, n - 1)) * HD + E * lane);
+        if (k0 > wave) load(k0);
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (k0 + W * j < n) sum += wts[k0 + W * j] * v[j];

@@ -498,6 +498,54 @@ def test_attend_long(sm, dev, form):
     attend(c, pos, qstart, None, 8, window=3000, note=f"long {form}, window")
 
 
+def test_attend_blocks_of_more_sequences_than_shares_hold(sm, dev):
+    """2100 blocks of three tokens, whose tiles are too many to share out evenly: a
+    workgroup a tile, one of them over more pages than it holds numbers of."""
+    c = Case(sm, dev, 1, 64, 3, 270, 101)
+    c.fill([70, 17000, 200])
+    n = 2100
+    slot, counts = np.zeros(n, int), np.full(n, 3)
+    pos = c.rng.integers(0, 60, n)
+    slot[[7, 2000]], pos[[7, 2000]] = 1, [16990, 9000]
+    slot[5::9], pos[5::9] = 2, c.rng.integers(0, 190, len(pos[5::9]))
+    counts[11::50] = 0
+    attend(c, list(pos), np.concatenate([[0], np.cumsum(counts)]), list(slot), 16, "bf16", "f32", note="2100 blocks", max_len=17000)
+
+
+def test_attend_shares_of_many_pages(sm, dev):
+    """A length said far too small makes few shares, of more pages than a workgroup holds numbers of."""
+    c = Case(sm, dev, 1, 64, 2, 330, 103)
+    pos, qstart = [20900, 300], [0, 100, 140]
+    c.fill(lengths(pos, qstart, None, 2))
+    for x in ("f32", "bf16"):
+        attend(c, pos, qstart, None, 4, x, "f32", note=f"few shares {x}", max_len=1)
+        attend(c, pos, qstart, None, 4, x, "f32", window=19000, note=f"few shares, window {x}", max_len=1)
+
+
+def test_attend_two_at_once(sm, dev):
+    """Two streams, each with a workspace of its own, the same bits as alone."""
+    import torch
+    c = Case(sm, dev, 2, 128, 4, 40, 107)
+    c.fill([2500] * 4)
+    calls = []
+    for counts in (None, [30, 20, 9, 50]):
+        qstart = None if counts is None else np.concatenate([[0], np.cumsum(counts)])
+        n = 4 if counts is None else int(qstart[-1])
+        q, _ = rows(dev, c.rng.standard_normal((n, 8, 128)), torch.float32)
+        out, alone = torch.zeros_like(q), torch.zeros_like(q)
+        b = c.batch([2000, 5, 2300, 700], n, qstart, max_len=2400)
+        c.kv.attend(b, q, alone)
+        calls.append((c.kv.attend_op(b, q, out), torch.cuda.Stream(device=dev), out, alone))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for op, s, out, _ in calls:
+            with torch.cuda.stream(s):
+                out.zero_()
+            op(s)
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, alone) for _, _, out, alone in calls)
+
+
 def test_rows_claimed_twice_stay_in_bounds(sm, dev):
     """Every sequence claims all rows, which the call does not serve as asked: it
     ends, and the rows next to the call's are left alone."""
