@@ -14,6 +14,8 @@ namespace {
 /* -------------------------------------------------------------------- append
  * A wave takes 64 / lanes heads at a time, a workgroup up to 4 * U such groups of one
  * token: queries, keys and values. C and S (heads.h) are worked out once a workgroup.
+ * Bound by the chain of batch, position, table row, LDS, turn and code: 4.0 us for a
+ * token, 9.0 for 512 of 24 bf16 heads of 256, 11 MB.
  * Positions share nothing, so that no page is read and a token's codes do not
  * depend on what was there. Keys are rounded once to f32 after norm and rotation
  * (heads.h, 64 bits), and the rest is exact: the scale is a power of two from the
@@ -152,7 +154,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4Append A) {
 
 /* ---------------------------------------------------------------------- read
  * One workgroup per (sequence, page its positions touch, kv head, keys or values),
- * eight elements a thread at a time. */
+ * eight elements a thread at a time. Bound by latency: 64 single pages all over the pool
+ * 9.8 us, 512 positions of one sequence in bf16 5.8. */
 __device__ __forceinline__ void kv4_store8(uint16_t * to, const uint32_t * v) { *(uint4 *) to = uint4{v[0], v[1], v[2], v[3]}; }
 __device__ __forceinline__ void kv4_store8(float * to, const uint32_t * v) {
 #pragma unroll
@@ -269,6 +272,8 @@ int sparkmv_kv4_append(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
     a.kgroups = (cache->kv_heads + per - 1) / per;
     a.groups = a.qgroups + 2 * a.kgroups;
     auto parts = [&](int u) { return (a.groups + 4 * u - 1) / (4 * u); };
+    /* one group a wave, or up to four: with 24 f32 heads of 256, read back included, 64
+     * tokens of 64 sequences 13.8 and 15.0 us, 512 of one 16.5 and 15.3, 4096 76 and 64 */
     const int u = (long) batch->ntok * parts(4) >= 4 * cu_count() ? 4 : 1;
     a.parts = parts(u);
     const long wg = (long) batch->ntok * a.parts;

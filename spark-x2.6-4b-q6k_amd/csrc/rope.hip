@@ -11,7 +11,8 @@ namespace {
 /* ---------------------------------------------------------------- the table
  * A thread owns one frequency and walks `run` positions from its first: the sine and
  * cosine there, and from one to the next a rotation by the frequency's own, each off by
- * some 2^-52, which 32 of them do not bring near f32's 2^-24. Bound by the stores. */
+ * some 2^-52, which 32 of them do not bring near f32's 2^-24. Bound by the stores: 131072
+ * rows of 256 24.7 us, 5.4 TB/s; with a sine and cosine for each pair 47.6. */
 struct RopeTable {
     float * table;
     int rows, half, run;
@@ -44,8 +45,9 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTable A) {
  * A wave takes 64 / lanes heads at a time, a workgroup up to 4 * U such groups of one
  * token, queries' and then keys'. C and S (heads.h) are worked out once a workgroup, an
  * element a thread, and shared through LDS: loaded by every lane from the table and the
- * weights they are four times the bytes of the heads themselves, and what bounds. Now
- * the rows in and out do. */
+ * weights they are four times the bytes of the heads themselves, and what bounds (8192
+ * tokens of 40 bf16 heads of 128 68.5 us). Now the rows in and out do: 36.9 us, 4.5 TB/s,
+ * where a copy of them takes 33. */
 struct QkRope {
     sparkmv_qk_rows r;
     sparkmv_head_turn t;
@@ -252,6 +254,8 @@ int sparkmv_qk_rope(const sparkmv_qk_rows * rows, const sparkmv_head_turn * turn
     a.qgroups = (r.heads + per - 1) / per;
     a.groups = a.qgroups + (r.kv_heads + per - 1) / per;
     auto parts = [&](int u) { return (a.groups + 4 * u - 1) / (4 * u); };
+    /* one group a wave, or up to four: 20 f32 heads of 256, 256 tokens 5.0 and 5.6 us, 512
+     * 8.2 and 8.2, 4096 49.3 and 41.8 */
     const int u = (long) r.ntok * parts(4) >= 4 * cu_count() ? 4 : 1;
     a.parts = parts(u);
     const long wg = (long) r.ntok * a.parts;
