@@ -196,6 +196,36 @@ def test_append_leaves_bad_entries_out(sm, dev):
     check_rows(q_out, want, "f32")
 
 
+@pytest.mark.parametrize("inter", [False, True])
+def test_append_with_a_table_and_weights_at_any_address(sm, dev, inter):
+    import torch
+    c = Case(sm, dev, 2, 128, 2, 4, 113)
+    n, heads, rope = 9, 4, 128
+    flat = torch.empty(4 * 64 * rope + 1, device=dev)
+    table = flat[1:].view(4 * 64, rope)
+    table.copy_(sm.rope_table(4 * 64, rope, 1e4, dev))
+    w = torch.from_numpy(1 + 0.3 * c.rng.standard_normal(2 * 128 + 3).astype(np.float32)).to(dev)
+    qn, kn = w[1:129], w[130:258]
+    q, qf = rows(dev, c.rng.standard_normal((n, heads, 128)), torch.float32)
+    k, kf = rows(dev, c.rng.standard_normal((n, 2, 128)), torch.float32)
+    out, turned = torch.empty_like(q), torch.empty_like(q)
+    pos, qstart, eps = [5, 70], [0, 4, 9], float(np.float32(1e-5))
+    c.fill(pos)
+    c.kv.append(c.batch(pos, n, qstart), q, k, k, table, out, inter, qn, kn, eps)
+    at = torch.tensor([5, 6, 7, 8, 70, 71, 72, 73, 74], dtype=torch.int32, device=dev)
+    sm.qk_rope(at, q, turned, None, None, table, inter, qn, None, eps)
+    assert torch.equal(out, turned)
+    want = np.stack([paged4.turn(qf[t], table.cpu().numpy()[int(at[t])], inter, qn.double().cpu().numpy(), eps) for t in range(n)])
+    size = np.abs(want).max(-1, keepdims=True)
+    assert np.all(np.abs(out.double().cpu().numpy() - want) <= 2.0 ** -24 * np.abs(want) * (1 + 1e-6) + 2.0 ** -48 * size)
+    aligned = [t.clone() for t in (table, kn)]
+    other = Case(sm, dev, 2, 128, 2, 4, 113)
+    other.host = {n: a.copy() for n, a in c.host.items()}
+    other.put()
+    other.kv.append(other.batch(pos, n, qstart), None, k, k, aligned[0], None, inter, None, aligned[1], eps)
+    assert torch.equal(c.kv.data, other.kv.data) and not np.array_equal(c.kv.data.cpu().numpy(), c.host["data"])
+
+
 def test_append_from_one_matrix_and_in_place(sm, dev):
     """The forward's layout: q, k and v beside each other in a row, the queries turned where they are."""
     import torch
@@ -510,6 +540,18 @@ def test_attend_blocks_of_more_sequences_than_shares_hold(sm, dev):
     slot[5::9], pos[5::9] = 2, c.rng.integers(0, 190, len(pos[5::9]))
     counts[11::50] = 0
     attend(c, list(pos), np.concatenate([[0], np.cumsum(counts)]), list(slot), 16, "bf16", "f32", note="2100 blocks", max_len=17000)
+
+
+@pytest.mark.parametrize("x,o", [("f32", "f32"), ("bf16", "bf16")])
+def test_attend_short_blocks_of_many_sequences(sm, dev, x, o):
+    """More sequences than a wave has lanes, each with up to three tiles of sixteen columns."""
+    c = Case(sm, dev, 1, 128, 5, 20, 109)
+    c.fill([1200] * 5)
+    n = 90
+    slot, counts, pos = c.rng.integers(0, 5, n), c.rng.integers(0, 13, n), c.rng.integers(0, 1100, n)
+    qstart = np.concatenate([[0], np.cumsum(counts)])
+    for window, most in ((0, 1200), (70, 1200), (0, 100)):
+        attend(c, list(pos), qstart, list(slot), 4, x, o, window=window, max_q=12, max_len=most, note=f"window {window} {x}")
 
 
 def test_attend_shares_of_many_pages(sm, dev):

@@ -2,10 +2,11 @@
 their definitions in 64 bits (oracle/paged4.py). Tables and f32 outputs are computed
 in 64 bits and rounded once: half a step of the output's type, and 1e-6 of that for
 what the 64-bit sums and roots may be off (where a sum cancels, 2^-49 of its terms).
-bf16 outputs are computed in f32: the two products' factors (weight times cosine or
-sine) are rounded, then one product, their sum, the root and its product, 6 roundings
-of 2^-24 of the terms' magnitudes, which are two elements at most: 2^-20 of the
-largest normed element of the head beside the half step."""
+bf16 outputs are computed in f32, in roundings of 2^-24: 9 at most in the sum of 256
+squares, which the root halves, 2 in the root and its conversion, 4 in a term (its
+factor, its product, the sum, the norm's product): 10.5 of the two terms' magnitudes,
+which are sqrt 2 of the largest normed element of the head together, less than 2^-20 of
+it beside the half step."""
 import numpy as np
 import pytest
 
