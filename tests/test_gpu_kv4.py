@@ -564,6 +564,41 @@ def test_attend_shares_of_many_pages(sm, dev):
         attend(c, pos, qstart, None, 4, x, "f32", window=19000, note=f"few shares, window {x}", max_len=1)
 
 
+@pytest.mark.parametrize("counts", [None, [3, 9], [20, 40]])
+def test_pages_past_32_bits(sm, dev, counts):
+    """Pages on both sides of 2^31 and 2^32 bytes give the bits that a small pool gives."""
+    import torch
+    kvh, hd, heads, n = 4, 256, 8, 2
+    size = kvh * 68 * hd
+    at = [(1 << 31) // size, (1 << 31) // size + 1, (1 << 32) // size, (1 << 32) // size + 3, (1 << 32) // size - 1, 2]
+    npages = at[3] + 1
+    pos = [100, 70]
+    qstart = None if counts is None else np.concatenate([[0], np.cumsum(counts)])
+    ntok = n if counts is None else int(qstart[-1])
+    g = torch.Generator(device=dev).manual_seed(5)
+    q, k = (torch.randn(ntok, h, hd, generator=g, device=dev) for h in (heads, kvh))
+    data = torch.empty(npages, kvh, 68 * hd, dtype=torch.uint8, device=dev)
+    small = sm.PagedKV4(kvh, hd, 6, n, 3, pages=torch.arange(6, dtype=torch.int32, device=dev).view(n, 3))
+    large = sm.PagedKV4(kvh, hd, npages, n, 3, pages=torch.tensor(at, dtype=torch.int32, device=dev).view(n, 3), data=data)
+    small.data.random_(0, 256, generator=g)
+    for i, p in enumerate(at):
+        data[p].copy_(small.data[i])
+    got, old = [], torch.randn(sum(pos), kvh, hd, generator=g, device=dev)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for kv in (small, large):
+        kv.append(sm.KVBatch(ints([0, 0]), sum(pos), ints([0, pos[0], sum(pos)]), max_q=max(pos), max_len=192), None, old, old)
+        b = sm.KVBatch(torch.tensor(pos, dtype=torch.int32, device=dev), ntok,
+                       None if qstart is None else torch.tensor(qstart, dtype=torch.int32, device=dev), max_q=64, max_len=192)
+        out, rk, rv = torch.empty_like(q), *(torch.empty(n, 64, kvh, hd, device=dev) for _ in range(2))
+        kv.append(b, None, k, k)
+        kv.attend(b, q, out)
+        kv.read(torch.tensor(pos, dtype=torch.int32, device=dev), rk, rv)
+        assert torch.isfinite(out).all() and out.abs().max() > 0.1
+        got.append([t.view(torch.int32) for t in (out, rk, rv)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert all(torch.equal(data[p], small.data[i]) for i, p in enumerate(at))
+
+
 def test_attend_two_at_once(sm, dev):
     """Two streams, each with a workspace of its own, the same bits as alone."""
     import torch
