@@ -9,9 +9,10 @@
  *
  * The arithmetic is in T: 64 bits where the result is an f32 (a product of two f32 is
  * exact there, and no sum of squares overflows, so the one rounding that counts is the
- * last), f32 where it is a bf16: 5 roundings of 2^-24 in the root, counting its halving
- * of those in the sum, and 5 more in the turn, 2^-20 of the head's largest normed element
- * beside a half step of 2^-8. A head whose squares leave f32's range takes 64 bits. */
+ * last), f32 where it is a bf16: 2^-24 of the terms for each of 4 roundings in the turn,
+ * 2 of the root and half of the sum's 9, with two terms of sqrt 2 of the head's largest
+ * normed element together less than 2^-20 of it, beside a half step of 2^-8.
+ * A head whose squares leave f32's range takes 64 bits. */
 #pragma once
 
 #include <hip/hip_runtime.h>
