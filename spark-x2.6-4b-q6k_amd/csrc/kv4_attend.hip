@@ -624,8 +624,8 @@ __global__ __launch_bounds__(512) void kv4_flat_join_kernel(const Kv4Flat A) {
  * it is worked on: codes of keys as they lie, by direct loads; values as the bf16
  * operands that they become, converted once for all waves.
  *
- * 512 bf16 tokens of 16 heads of 256 at 16384 take 205 us with the join's 14: 139 GFLOP
- * as the formula counts them, 0.68 PFLOP/s, where a large bf16 product reaches 1.2. With
+ * 512 bf16 tokens of 16 heads of 256 at 16384 take 226 us with the join's 13: 139 GFLOP
+ * as the formula counts them, 0.62 PFLOP/s, where a large bf16 product reaches 1.2. With
  * any one of the parts left out (scores, exponentials, conversion, the values' product)
  * a wave's time falls by a tenth at most: the vector and matrix pipes take turns, two
  * waves a SIMD being all that the registers hold.
@@ -633,12 +633,14 @@ __global__ __launch_bounds__(512) void kv4_flat_join_kernel(const Kv4Flat A) {
  * The scores use the instruction that multiplies 4-bit codes as they are, 16 x 16 x 128
  * with a power of two for every 32 elements. A query element enters it as a sum of
  * parts, each the nearest small number to what the ones before left out; 32 neighbours
- * share a power of two:
- *   bf16 queries as two numbers of 8 bits (E4M3), which is all of an element down to
- *     2^-13 of the largest of the 32, and below that all but 2^-21 of the largest;
- *   f32 queries as five numbers of 6 bits (E2M3, four times as fast a product as
- *     bf16's), below 4 in magnitude and off by 1 / 8 at most: 2^-24 of the largest of the
- *     32 is what may be lost. Six for head_dim 64, where an instruction takes two parts.
+ * share a power of two. Five parts of 6 bits (E2M3, four times as fast a product as
+ * bf16's), at most 4 in magnitude and off by 1 / 8 at most: 2^-24 of the largest of the 32 is
+ * what may be lost, and nothing of a bf16 element down to 2^-17 of it. Six parts for
+ * head_dim 64, where an instruction takes two.
+ * Two parts of 8 bits (E4M3) would do for bf16 (205 us for the call above), but for the
+ * sum: within 16 elements of a lane the instruction drops what lies below 2^-13 of the
+ * largest product, which left outputs off by 1e-5. Products of a 6-bit part and a code
+ * are multiples of 1 / 16 up to 24, so none of them is cut.
  *
  * Weights times values as in the flat kernels. */
 constexpr int kKv4Tile = 128;       /* columns of a workgroup */
@@ -659,9 +661,11 @@ struct Kv4Tile {
     float * pml;     /* [workgroups][2][128][2] */
 };
 
+/* parts of a query element: an even number where an instruction takes two */
+constexpr int kv4_tile_parts(int hd) { return hd == 64 ? 6 : 5; }
 /* instructions' parts of the queries that wait in LDS: all of them leave too few registers */
-constexpr int kv4_tile_far(int hd, int dq) { return hd == 256 && dq > 2 ? 2 : 0; }
-constexpr int kv4_tile_lds(int hd, int dq) { return 2 * (32 + 128) * hd + kv4_tile_far(hd, dq) * (hd / 128) * 8 * 1536; }
+constexpr int kv4_tile_far(int hd) { return hd == 256 ? 2 : 0; }
+constexpr int kv4_tile_lds(int hd) { return 2 * (32 + 128) * hd + kv4_tile_far(hd) * (hd / 128) * 8 * 1536; }
 
 /* the sequence and the place within it of tile number j, from the tiles before each sequence */
 __device__ __forceinline__ KvSeq kv4_tile_seq(const sparkmv_kv_batch & b, const sparkmv_kv4_cache & c, const int * lseq, int j, int & place) {
@@ -733,18 +737,17 @@ typedef float kv4_f32 __attribute__((ext_vector_type(32)));
 typedef uint32_t kv4_u6 __attribute__((ext_vector_type(6)));
 typedef int kv4_i8 __attribute__((ext_vector_type(8)));
 
-template <int HD, int DQ, int DP>
+template <int HD, int DP>
 __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
     constexpr int ND = HD / 16, NB = HD / 32, BUF = (32 + 128) * HD;
     constexpr int NJ = HD >= 128 ? HD / 128 : 1;         /* instructions of 128 elements a head */
+    constexpr int DQ = kv4_tile_parts(HD);               /* parts of a query element */
     constexpr int NM = HD == 64 ? DQ / 2 : DQ;           /* instructions a score tile and 128 elements */
-    constexpr bool F8 = DQ == 2;                         /* parts of 8 bits, else of 6 */
-    constexpr int PW = F8 ? 8 : 6, NR = NM - kv4_tile_far(HD, DQ);   /* words of a part; instructions' parts in registers */
-    constexpr int PB = F8 ? 4 : 5;                       /* a part is held to 2^-PB of what the one before was */
+    constexpr int PW = 6, NR = NM - kv4_tile_far(HD);    /* words of a part; instructions' parts in registers */
     typedef __attribute__((address_space(3))) void lds_void;
     extern __shared__ __attribute__((aligned(16))) uint8_t lbuf[];   /* [2][keys' codes, values' operands] */
     uint8_t * lfar = lbuf + 2 * BUF;                      /* [wave][part][NJ][64 lanes' 16 bytes, 64 lanes' 8] */
-    int * lseq = (int *) (lbuf + kv4_tile_lds(HD, DQ)), * lpre = lseq + A.b.nseq;
+    int * lseq = (int *) (lbuf + kv4_tile_lds(HD)), * lpre = lseq + A.b.nseq;
     __shared__ int lid[kKv4Ids], lsum[10];
     __shared__ uint32_t lnan[2][2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c16 = lane & 15;
@@ -914,18 +917,18 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
             bool bad = false;
             float x[32];
             const size_t row = (size_t) (s.row + tok) * A.q.ldq + (size_t) head * HD;
-            auto load = [&](int at0, int at1) {   /* 16 elements each */
-                if (!F8) {
+            auto load = [&](int at) {   /* 32 elements */
+                if (A.q.q_dtype == SPARKMV_X_F32) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const kv_f4 v = *(const kv_f4 *) ((const float *) A.q.q + row + (e < 4 ? at0 : at1) + 4 * (e & 3));
+                        const kv_f4 v = *(const kv_f4 *) ((const float *) A.q.q + row + at + 4 * e);
 #pragma unroll
                         for (int i = 0; i < 4; i++) x[4 * e + i] = v[i];
                     }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const kv4_u4 v = *(const kv4_u4 *) ((const uint16_t *) A.q.q + row + (e < 2 ? at0 : at1) + 8 * (e & 1));
+                        const kv4_u4 v = *(const kv4_u4 *) ((const uint16_t *) A.q.q + row + at + 8 * e);
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             x[8 * e + 2 * i] = __uint_as_float(v[i] << 16);
@@ -936,8 +939,7 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
             };
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                const int at = 32 * (HD == 64 ? g & 1 : 4 * j + g);
-                load(at, at + 16);
+                load(32 * (HD == 64 ? g & 1 : 4 * j + g));
                 uint32_t big = 0;
 #pragma unroll
                 for (int e = 0; e < 32; e++) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
@@ -959,58 +961,35 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
             const float sign = A.q.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                /* this lane's elements: its block; or with 8 bits, where a lane holds two times 16
-                 * of the instruction's, halves of blocks g / 2 and 2 + g / 2 (64 elements: of g / 2) */
-                const int low = max(ex[j] - most, -90), at = 32 * (HD == 64 ? g & 1 : 4 * j + g);
-                const int at0 = F8 ? 32 * (4 * j + (g >> 1)) + 16 * (g & 1) : at, at1 = F8 ? at0 + (HD == 64 ? 0 : 64) : at + 16;
-                const int ex0 = F8 ? __shfl(ex[j], 16 * (g >> 1) + c16, 64) : ex[j];
-                const int ex1 = F8 && HD >= 128 ? __shfl(ex[j], 32 + 16 * (g >> 1) + c16, 64) : ex0;
-                const bool none0 = any || ex0 - most < -90, none1 = any || ex1 - most < -90;
-                /* below 4 in magnitude, or 256 with 8 bits; part d in steps of 2^(-PB d) of that.
+                const int low = max(ex[j] - most, -90);
+                const bool none = any || ex[j] - most < -90;
+                /* below 4 in magnitude; part d in steps of 2^(-5 d) of that.
                  * Read again: all blocks at once would not fit the registers */
-                load(at0, at1);
-                constexpr int top = F8 ? 8 : 2;
+                load(32 * (HD == 64 ? g & 1 : 4 * j + g));
 #pragma unroll
-                for (int e = 0; e < 32; e++) x[e] = (e < 16 ? none0 : none1) ? 0.0f : ldexpf(x[e] * sign, top - (e < 16 ? ex0 : ex1));
+                for (int e = 0; e < 32; e++) x[e] = none ? 0.0f : ldexpf(x[e] * sign, 2 - ex[j]);
                 qs[j][0] = qs[j][1] = 0;
 #pragma unroll
                 for (int d = 0; d < DQ; d++) {
                     uint32_t part[PW];
-                    if constexpr (F8) {
+                    kv4_f16 ev, od;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            int v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * e], x[4 * e + 1], 0, false);
-                            v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * e + 2], x[4 * e + 3], v, true);
-                            part[e] = (uint32_t) v;
-                            const auto lo2 = __builtin_amdgcn_cvt_pk_f32_fp8(v, false), hi2 = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
-                            x[4 * e] = (x[4 * e] - lo2[0]) * 16.0f;
-                            x[4 * e + 1] = (x[4 * e + 1] - lo2[1]) * 16.0f;
-                            x[4 * e + 2] = (x[4 * e + 2] - hi2[0]) * 16.0f;
-                            x[4 * e + 3] = (x[4 * e + 3] - hi2[1]) * 16.0f;
-                        }
-                    } else {
-                        kv4_f16 ev, od;
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            ev[e] = x[2 * e];
-                            od[e] = x[2 * e + 1];
-                        }
-                        const kv4_u6 six = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev, od, 1.0f);
-                        const kv4_f32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(six, 1.0f);
-#pragma unroll
-                        for (int e = 0; e < 6; e++) part[e] = six[e];
-#pragma unroll
-                        for (int e = 0; e < 32; e++) x[e] = (x[e] - back[e]) * 32.0f;
+                    for (int e = 0; e < 16; e++) {
+                        ev[e] = x[2 * e];
+                        od[e] = x[2 * e + 1];
                     }
-                    const uint32_t sb = (uint32_t) (127 + low - top - PB * d);
+                    const kv4_u6 six = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev, od, 1.0f);
+                    const kv4_f32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(six, 1.0f);
+#pragma unroll
+                    for (int e = 0; e < 6; e++) part[e] = six[e];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) x[e] = (x[e] - back[e]) * 32.0f;
+                    const uint32_t sb = (uint32_t) (127 + low - 2 - 5 * d);
                     if constexpr (HD == 64) {
                         /* two parts an instruction: the second one in the place of blocks 2 and 3 */
                         const bool mine = (g >> 1) == (d & 1);
 #pragma unroll
-                        for (int e = 0; e < PW; e++) {
-                            if constexpr (F8) qd[d / 2][j][e] = (e < 4) == !(d & 1) ? part[e] : qd[d / 2][j][e];
-                            else qd[d / 2][j][e] = mine || !(d & 1) ? part[e] : qd[d / 2][j][e];
-                        }
+                        for (int e = 0; e < PW; e++) qd[d / 2][j][e] = mine || !(d & 1) ? part[e] : qd[d / 2][j][e];
                         if (mine) qs[j][0] |= sb << (8 * (d / 2));
                     } else {
                         if (d < NR) {
@@ -1092,7 +1071,7 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
                             const kv_i4 v = kf[t];
                             const kv4_i8 k8 = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
                             const int k = t * NJ + jj;   /* its scale: byte k of ksj */
-#define KV4_SCORE(KB, QB) x[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k8, qf, x[t], 4, F8 ? 0 : 2, KB, (int) ksj[k / 4], QB, (int) qs[jj][d / 4])
+#define KV4_SCORE(KB, QB) x[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k8, qf, x[t], 4, 2, KB, (int) ksj[k / 4], QB, (int) qs[jj][d / 4])
 #define KV4_SCORE_Q(QB)                                                                                              \
     do {                                                                                                             \
         if (k % 4 == 0) KV4_SCORE(0, QB);                                                                            \
@@ -1176,7 +1155,7 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
                         }
                     }
                 /* the values' operands, VG at a time, one group ahead of the products */
-                constexpr int VG = F8 ? 4 : 2;
+                constexpr int VG = 2;
                 kv4_b8 vf[2][VG];
                 auto values = [&](int n4) {
 #pragma unroll
@@ -1427,24 +1406,18 @@ int sparkmv_kv4_attend(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
          * and 29.2, with 68 39.5 and 38.0 */
         const int each = p.tiles * cache->kv_heads * (kKv4Tile / 4) > 4 * cu_count() ? 2 : 1;
         const dim3 join((unsigned) p.tiles, (unsigned) cache->kv_heads, (unsigned) (kKv4Tile / 4 / each));
-#define KV4_TILE(H, DQ, DP)                                                                                          \
+#define KV4_TILE(H, DP)                                                                                              \
     do {                                                                                                             \
         static LdsAllowed allowed;                                                                                   \
-        if (lds_allow(allowed, (const void *) kv4_tile_kernel<H, DQ, DP>, kv4_tile_lds(H, DQ) + lists + 2048,            \
+        if (lds_allow(allowed, (const void *) kv4_tile_kernel<H, DP>, kv4_tile_lds(H) + lists + 2048,                \
                       "LDS opt-in for the kv4 attention"))                                                           \
             return -1;                                                                                               \
-        hipLaunchKernelGGL((kv4_tile_kernel<H, DQ, DP>), grid, dim3(512), kv4_tile_lds(H, DQ) + lists, s, t);            \
+        hipLaunchKernelGGL((kv4_tile_kernel<H, DP>), grid, dim3(512), kv4_tile_lds(H) + lists, s, t);                \
     } while (0)
 #define KV4_TILE_D(H)                                                                                                \
     do {                                                                                                             \
-        constexpr int five = H == 64 ? 6 : 5;   /* an even number of parts where an instruction takes two */         \
-        if (q.q_dtype == SPARKMV_X_F32) {                                                                            \
-            if (q.out_dtype == SPARKMV_X_F32) KV4_TILE(H, five, 3);                                                  \
-            else KV4_TILE(H, five, 2);                                                                               \
-        } else {                                                                                                     \
-            if (q.out_dtype == SPARKMV_X_F32) KV4_TILE(H, 2, 3);                                                     \
-            else KV4_TILE(H, 2, 2);                                                                                  \
-        }                                                                                                            \
+        if (q.out_dtype == SPARKMV_X_F32) KV4_TILE(H, 3);                                                            \
+        else KV4_TILE(H, 2);                                                                                         \
         if (p.groups)                                                                                                \
             hipLaunchKernelGGL(kv4_tile_join_kernel<H>, join, dim3(256), ((uint32_t) batch->nseq + 1) * 4, s, t, each); \
     } while (0)

@@ -1,0 +1,88 @@
+"""GPU tests of the 4-bit cache's attention where a score is exact in f32, so that
+what queries lose on their way shows, and of queries and keys of far apart magnitudes.
+
+Queries here are small multiples of a power of two, of at most eight significant bits,
+and keys are codes under one power of two, such that every partial sum of a score is
+a multiple of one power of two g below 2^24 g: exact in f32, in any order. u = 2^-24
+(half a step of f32). The score's factor and its product with it are rounded (2 u s of
+the exponent), and so is the difference to the reference (2 u of the largest score):
+with s the largest score a weight is off by 4 u s of itself, by twice that relative to
+the sum of the weights, the sums of n positions by (n / 2 + 160) u as in test_gpu_kv4.py:
+  |out - exact| <= W (8 s + 160 + n / 2) u, W the weighted sum of |v|;
+bf16 outputs hold a weight to 2^-17 of itself (W 2^-17 more) and are rounded once."""
+import numpy as np
+import pytest
+
+import paged4
+from test_gpu_kv import rows, types
+from test_gpu_kv4 import U, Case, lengths
+
+pytestmark = pytest.mark.gpu
+
+# up to 48 columns of a kv head and sequence, and more
+MAX_Q = {"decode": 1, "block": 7, "chunk": 60}
+FORMS = {"decode": ([200, 3, 129], None), "block": ([200, 3, 129], [0, 5, 6, 13]), "chunk": ([140, 3, 70], [0, 60, 65, 95])}
+
+
+def put_keys(c, length, byte):
+    """Key scale bytes of positions 0 .. length[slot] - 1: byte(block) for each block of 32."""
+    off = paged4.offsets(c.hd)
+    for s, n in enumerate(length):
+        for p in range(n):
+            page = c.host["data"][c.host["pages"][s, p // 64]]
+            for blk in range(c.hd // 32):
+                page[:, off[1, p % 64, 32 * blk]] = byte(blk)
+
+
+def check_exact(c, q, out, scale, pos, qstart):
+    qf = q.double().cpu().numpy()
+    want, size = paged4.attend(c.host, qf, c.hd, scale, 0, None, pos, qstart)
+    got = out.double().cpu().numpy()
+    assert np.isfinite(want).all() and np.isfinite(got).all()
+    s, w, n = largest_score(c, qf, scale, pos, qstart), size[..., 1], max(pos) + len(qf)
+    assert 1.0 < s < 100.0      # scores matter
+    bound = w * (8 * s + 160 + n / 2) * U
+    if str(out.dtype).endswith("bfloat16"):
+        bound = bound + w * 2.0 ** -17 + 2.0 ** -8 * np.abs(want).max(-1)
+    err = np.abs(got - want)
+    print(f"relL2 {np.linalg.norm(err) / np.linalg.norm(want):.2e}, of the bound {(err / bound[..., None]).max():.2f}")
+    assert np.all(err <= bound[..., None])
+
+
+def largest_score(c, qf, scale, pos, qstart):
+    """Of any row and position that it sees."""
+    group, most = qf.shape[1] // c.kvh, 0.0
+    for i, p0 in enumerate(pos):
+        r = range(i, i + 1) if qstart is None else range(qstart[i], qstart[i + 1])
+        n = p0 + len(r)
+        page = c.host["pages"][i, :(n + 63) // 64].astype(int)
+        k = paged4.values(c.host, page, c.hd)[0].transpose(1, 0, 2, 3).reshape(c.kvh, -1, c.hd)[:, :n]
+        for t in r:
+            for g in range(qf.shape[1]):
+                most = max(most, np.abs(k[g // group] @ qf[t, g]).max() * abs(scale))
+    return most
+
+
+@pytest.mark.parametrize("x,o", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f32", "bf16")])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_queries_enter_whole(sm, dev, form, hd, x, o):
+    """Large elements beside small ones, each of which moves the scores: half the
+    elements are 128 .. 255, the others 1 / 8 .. 15 / 8, down to 2^-11 of the largest. Sums
+    are multiples of 1 / 16 below 256 * 255 * 6 < 2^19."""
+    import torch
+    pos, qstart = FORMS[form]
+    c = Case(sm, dev, 2, hd, 3, 5, 201 + hd)
+    length = lengths(pos, qstart, None, 3)
+    c.fill(length)
+    put_keys(c, length, lambda blk: 127)
+    c.put()
+    ntok = 3 if qstart is None else qstart[-1]
+    shape = (ntok, 8, hd)
+    big = c.rng.integers(128, 256, shape) * np.where(c.rng.random(shape) < 0.5, -1, 1)
+    small = c.rng.integers(-15, 16, shape) / 8.0
+    q, qf = rows(dev, np.where(c.rng.random(shape) < 0.5, big, small), types()[x])
+    out = torch.full(shape, 7.0, dtype=types()[o], device=dev)
+    scale = 2.0 ** (-10 if hd == 64 else -11)
+    c.kv.attend(c.batch(pos, ntok, qstart, max_q=MAX_Q[form], max_len=300), q, out, scale)
+    check_exact(c, q, out, scale, pos, qstart)
