@@ -956,13 +956,18 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
             uint32_t any = bad;
             any |= __shfl_xor((int) any, 16, 64);
             any |= __shfl_xor((int) any, 32, 64);
-            most = min(max(most, -100), 100);   /* so that f is a normal number */
-            f = any ? __uint_as_float(0x7fc00000u) : ldexpf(fabsf(A.q.scale) * kKvLog2e, most);
+            /* Scores are summed up with the column's elements below 2^-9, so that 256 products with
+             * codes of up to 6 * 2^125 stay within f32, and f brings them back. Where f would be no
+             * normal number they are larger or smaller than that, and a sum leaves f32 with its score */
+            int es;
+            (void) frexpf(fabsf(A.q.scale), &es);
+            const int up = min(max(most + 9, -120 - es), 120 - es);
+            f = any ? __uint_as_float(0x7fc00000u) : ldexpf(fabsf(A.q.scale) * kKvLog2e, up);
             const float sign = A.q.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                const int low = max(ex[j] - most, -90);
-                const bool none = any || ex[j] - most < -90;
+                const int low = min(max(ex[j] - up, -99), 127);
+                const bool none = any || ex[j] - up < -99;
                 /* below 4 in magnitude; part d in steps of 2^(-5 d) of that.
                  * Read again: all blocks at once would not fit the registers */
                 load(32 * (HD == 64 ? g & 1 : 4 * j + g));

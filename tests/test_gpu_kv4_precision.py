@@ -86,3 +86,36 @@ def test_queries_enter_whole(sm, dev, form, hd, x, o):
     scale = 2.0 ** (-10 if hd == 64 else -11)
     c.kv.attend(c.batch(pos, ntok, qstart, max_q=MAX_Q[form], max_len=300), q, out, scale)
     check_exact(c, q, out, scale, pos, qstart)
+
+
+def apart(sm, dev, form, hd, x, q_exp, key_byte, scale, keep=None, seed=0):
+    """Queries of +-1 .. 15 times 2^q_exp(block) and keys with scale byte key_byte(block)."""
+    import torch
+    pos, qstart = FORMS[form]
+    c = Case(sm, dev, 2, hd, 3, 5, 301 + hd + seed)
+    length = lengths(pos, qstart, None, 3)
+    c.fill(length)
+    put_keys(c, length, key_byte)
+    if keep:
+        off = paged4.offsets(hd)
+        for blk in range(hd // 32):
+            if not keep(blk):
+                c.host["data"][:, :, off[0, :, 32 * blk:32 * blk + 32].ravel()] = 0
+    c.put()
+    ntok = 3 if qstart is None else qstart[-1]
+    shape = (ntok, 8, hd)
+    f = np.array([2.0 ** q_exp(d // 32) for d in range(hd)])
+    q, _ = rows(dev, c.rng.integers(1, 16, shape) * np.where(c.rng.random(shape) < 0.5, -1, 1) * f, types()[x])
+    out = torch.full(shape, 7.0, device=dev)
+    c.kv.attend(c.batch(pos, ntok, qstart, max_q=MAX_Q[form], max_len=300), q, out, scale)
+    check_exact(c, q, out, scale, pos, qstart)
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("q_exp,key_byte,scale_exp", [(-90, 252, -44), (-122, 252, -11), (100, 20, -1), (118, 7, -6), (-20, 127, 12)])
+def test_queries_and_keys_of_any_magnitude(sm, dev, q_exp, key_byte, scale_exp, form, hd, x):
+    """Down to 2^-122 and up to 2^122, under keys that bring the scores near 1: they
+    are multiples of one power of two up to 256 * 15 * 12 of them."""
+    apart(sm, dev, form, hd, x, lambda blk: q_exp, lambda blk: key_byte, 2.0 ** scale_exp)
