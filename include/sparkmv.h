@@ -751,7 +751,8 @@ int sparkmv_kv4_read(const sparkmv_kv4_cache * cache, int nseq, const int * slot
  * window, gated, zeros for a token none of whose positions has a page. Query elements
  * enter whole in a call of up to 48 columns (max_q tokens times query heads per kv head);
  * of more, an element is held to 2^-24 of the largest of its 32 neighbours (those
- * that share a scale of the keys), which is all of a bf16 one down to 2^-17 of that. A weight enters whole for f32 outputs; for bf16 ones it is held to 2^-17 of
+ * that share a scale of the keys), which is all of a bf16 one down to 2^-17 of that, or to
+ * 2^-116 of the head's largest where that is more. A weight enters whole for f32 outputs; for bf16 ones it is held to 2^-17 of
  * itself. Scores, statistics and sums are f32, and scores have to lie
  * within its range. A position that reads as NaN, in any element of its key or value,
  * makes the tokens that see it NaN and no others. work: sparkmv_kv4_attend_work bytes

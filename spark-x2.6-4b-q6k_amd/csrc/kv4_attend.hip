@@ -950,7 +950,7 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
                 most = max(most, ex[j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            /* the column's exponent; blocks far below it count as nothing */
+            /* the column's exponent */
             most = max(most, __shfl_xor(most, 16, 64));
             most = max(most, __shfl_xor(most, 32, 64));
             uint32_t any = bad;
@@ -966,13 +966,12 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
             const float sign = A.q.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                const int low = min(max(ex[j] - up, -99), 127);
-                const bool none = any || ex[j] - up < -99;
+                const int low = min(max(ex[j] - up, -200), 127);
                 /* below 4 in magnitude; part d in steps of 2^(-5 d) of that.
                  * Read again: all blocks at once would not fit the registers */
                 load(32 * (HD == 64 ? g & 1 : 4 * j + g));
 #pragma unroll
-                for (int e = 0; e < 32; e++) x[e] = none ? 0.0f : ldexpf(x[e] * sign, 2 - ex[j]);
+                for (int e = 0; e < 32; e++) x[e] = any ? 0.0f : ldexpf(x[e] * sign, 2 - ex[j]);
                 qs[j][0] = qs[j][1] = 0;
 #pragma unroll
                 for (int d = 0; d < DQ; d++) {
@@ -989,7 +988,11 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
                     for (int e = 0; e < 6; e++) part[e] = six[e];
 #pragma unroll
                     for (int e = 0; e < 32; e++) x[e] = (x[e] - back[e]) * 32.0f;
-                    const uint32_t sb = (uint32_t) (127 + low - 2 - 5 * d);
+                    /* a part that no scale reaches is below 2^-126, 2^-116 of the column's largest element */
+                    const int exp = 127 + low - 2 - 5 * d;
+                    const uint32_t sb = (uint32_t) max(exp, 0);
+#pragma unroll
+                    for (int e = 0; e < PW; e++) part[e] = exp < 0 ? 0u : part[e];
                     if constexpr (HD == 64) {
                         /* two parts an instruction: the second one in the place of blocks 2 and 3 */
                         const bool mine = (g >> 1) == (d & 1);

@@ -119,3 +119,12 @@ def test_queries_and_keys_of_any_magnitude(sm, dev, q_exp, key_byte, scale_exp, 
     """Down to 2^-122 and up to 2^122, under keys that bring the scores near 1: they
     are multiples of one power of two up to 256 * 15 * 12 of them."""
     apart(sm, dev, form, hd, x, lambda blk: q_exp, lambda blk: key_byte, 2.0 ** scale_exp)
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("span", [30, 89, 100, 108])
+def test_blocks_of_queries_far_apart(sm, dev, span, form, hd, x):
+    """32 elements 2^span times the others, under keys that are zero: the others make the scores."""
+    apart(sm, dev, form, hd, x, lambda blk: span - 40 if blk == 0 else -40, lambda blk: 127 + 42, 2.0 ** -8, lambda blk: blk > 0, span)
