@@ -1189,7 +1189,6 @@ __global__ __launch_bounds__(512, 2) void kv4_tile_kernel(const Kv4Tile A) {
             }
         }
         l = kv_rows_sum(l);
-        if (f != f) l = f;
         const bool whole = seg == n && off == 0;
         if (wfirst + c16 <= last) {
             if (whole) {

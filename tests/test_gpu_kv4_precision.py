@@ -128,3 +128,23 @@ def test_queries_and_keys_of_any_magnitude(sm, dev, q_exp, key_byte, scale_exp, 
 def test_blocks_of_queries_far_apart(sm, dev, span, form, hd, x):
     """32 elements 2^span times the others, under keys that are zero: the others make the scores."""
     apart(sm, dev, form, hd, x, lambda blk: span - 40 if blk == 0 else -40, lambda blk: 127 + 42, 2.0 ** -8, lambda blk: blk > 0, span)
+
+
+@pytest.mark.parametrize("o", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_bad_queries_without_pages(sm, dev, form, hd, o):
+    """A token none of whose positions has a page is zeros, whatever its query holds."""
+    import torch
+    pos, qstart = FORMS[form]
+    c = Case(sm, dev, 2, hd, 3, 5, 401)
+    c.fill(lengths(pos, qstart, None, 3))
+    c.host["pages"][1, :] = -1
+    c.put()
+    ntok = 3 if qstart is None else qstart[-1]
+    at = slice(1, 2) if qstart is None else slice(qstart[1], qstart[2])
+    q = torch.randn(ntok, 8, hd, device=dev)
+    q[at, 1, 3], q[at, 2, 40], q[at, 7, 60] = float("nan"), float("inf"), -float("inf")
+    out = torch.full(q.shape, 7.0, dtype=types()[o], device=dev)
+    c.kv.attend(c.batch(pos, ntok, qstart, max_q=MAX_Q[form], max_len=300), q, out)
+    assert torch.all(out[at] == 0.0) and torch.isfinite(out).all() and torch.all(out[0].abs().amax(-1) > 0)
