@@ -15,7 +15,7 @@ import pytest
 
 import paged4
 from test_gpu_kv import rows, types
-from test_gpu_kv4 import U, Case, lengths
+from test_gpu_kv4 import U, Case, attend, lengths
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +148,50 @@ def test_bad_queries_without_pages(sm, dev, form, hd, o):
     out = torch.full(q.shape, 7.0, dtype=types()[o], device=dev)
     c.kv.attend(c.batch(pos, ntok, qstart, max_q=MAX_Q[form], max_len=300), q, out)
     assert torch.all(out[at] == 0.0) and torch.isfinite(out).all() and torch.all(out[0].abs().amax(-1) > 0)
+
+
+@pytest.mark.parametrize("kvh,group,hd", [(2, 4, 256), (1, 1, 64), (2, 2, 128), (1, 3, 256), (1, 16, 64), (2, 5, 128), (1, 16, 256)])
+@pytest.mark.parametrize("counts", [[8, 1, 3], [70, 33, 1], [150, 0, 64]])
+def test_bf16_queries_with_f32_outputs(sm, dev, kvh, group, hd, counts):
+    c = Case(sm, dev, kvh, hd, 3, 6, 501 + hd)
+    qstart = np.concatenate([[1], 1 + np.cumsum(counts)])
+    pos = [0, 190, 130]
+    c.fill(lengths(pos, qstart, None, 3))
+    attend(c, pos, qstart, None, kvh * group, "bf16", "f32", note=f"{counts} kvh {kvh} group {group} hd {hd}")
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_outliers_under_keys_of_zero(sm, dev, form, hd, x):
+    """One element 300 times the others, under keys that are zero, so that the others
+    make the scores. Past 48 columns an element that needs more bits is off by 2^-24 of
+    the largest of its 32 neighbours, a score by the sum of that times its keys, and a
+    weight by twice that relative to the sum; the rest of the bound is
+    test_gpu_kv4.py's."""
+    import torch
+    pos, qstart = FORMS[form]
+    c = Case(sm, dev, 2, hd, 3, 5, 601 + hd)
+    c.fill(lengths(pos, qstart, None, 3))
+    off = paged4.offsets(hd)
+    c.host["data"][:, :, off[0, :, 4:6].ravel()] = 0     # two elements of a byte
+    c.put()
+    ntok = 3 if qstart is None else qstart[-1]
+    x0 = c.rng.standard_normal((ntok, 8, hd)) + 0.3
+    x0[:, :, 5] *= 300.0
+    x0[:, ::2, 7] *= 1e-3
+    q, qf = rows(dev, x0, types()[x])
+    out = torch.full(q.shape, 7.0, device=dev)
+    scale = hd ** -0.5
+    c.kv.attend(c.batch(pos, ntok, qstart, max_q=MAX_Q[form], max_len=300), q, out, scale)
+    want, size = paged4.attend(c.host, qf, hd, scale, 0, None, pos, qstart)
+    off_by = np.zeros(qf.shape)
+    if form == "chunk":
+        most = np.repeat(np.abs(qf).reshape(ntok, 8, -1, 32).max(-1), 32, -1)
+        off_by = np.where((x == "bf16") & (np.abs(qf) >= 2.0 ** -17 * most), 0.0, 2.0 ** -24 * most)
+    _, lost = paged4.attend(c.host, off_by, hd, scale, 0, None, pos, qstart)
+    s, w, n = size[..., 0], size[..., 1], max(pos) + ntok
+    bound = w * ((2 * (hd + 8) * s + 160 + n / 2) * U + 2 * lost[..., 0])
+    err = np.abs(out.double().cpu().numpy() - want)
+    print(f"relL2 {np.linalg.norm(err) / np.linalg.norm(want):.2e}, of the bound {(err / bound[..., None]).max():.2f}")
+    assert np.all(err <= bound[..., None])
