@@ -458,7 +458,9 @@ int sparkmv_kv_append(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
     const sparkmv_kv_new & n = *rows;
     const int hd = cache->head_dim;
     if (kv_check_dtype("kv rows", n.x_dtype)) return -1;
-    if (n.heads < 0 || (n.heads > 0) != (n.q != nullptr) || (n.heads > 0) != (n.q_out != nullptr)) {
+    /* an array of no rows may be null */
+    const bool any = batch->nseq > 0 && batch->ntok > 0;
+    if (n.heads < 0 || (any && ((n.heads > 0) != (n.q != nullptr) || (n.heads > 0) != (n.q_out != nullptr)))) {
         set_error("%d query heads, queries and their output do not agree", n.heads);
         return -1;
     }

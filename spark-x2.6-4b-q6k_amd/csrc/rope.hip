@@ -220,11 +220,12 @@ int sparkmv_qk_rope(const sparkmv_qk_rows * rows, const sparkmv_head_turn * turn
         set_error("qk rope: %d query and %d key heads are outside 0..65536", r.heads, r.kv_heads);
         return -1;
     }
-    if ((r.heads > 0) != (r.q != nullptr) || (r.heads > 0) != (r.q_out != nullptr)) {
+    /* an array of no rows may be null */
+    if (r.ntok > 0 && ((r.heads > 0) != (r.q != nullptr) || (r.heads > 0) != (r.q_out != nullptr))) {
         set_error("%d query heads, queries and their output do not agree", r.heads);
         return -1;
     }
-    if ((r.kv_heads > 0) != (r.k != nullptr) || (r.kv_heads > 0) != (r.k_out != nullptr)) {
+    if (r.ntok > 0 && ((r.kv_heads > 0) != (r.k != nullptr) || (r.kv_heads > 0) != (r.k_out != nullptr))) {
         set_error("%d key heads, keys and their output do not agree", r.kv_heads);
         return -1;
     }
