@@ -169,7 +169,9 @@ __device__ __forceinline__ double head_norm(const float * x, bool norm, float ep
     return a < INFINITY ? r : 1.0 / sqrt(a);
 }
 
-/* x normed and turned, in T; with f32, where that could leave its range, in 64 bits */
+/* x normed and turned, in T. In f32 x takes the norm's factor first, so that no product with
+ * large or small weights leaves f32 where the result does not; a factor that could leave it
+ * takes 64 bits */
 template <int EL>
 __device__ __forceinline__ void head_turn(const double * C, const double * S, const float * x, const float * y, double r, double * out) {
 #pragma unroll
@@ -183,7 +185,7 @@ __device__ __forceinline__ void head_turn(const float * C, const float * S, cons
     } else {
         const float rf = (float) r;
 #pragma unroll
-        for (int i = 0; i < EL; i++) out[i] = fmaf(x[i], C[i], y[i] * S[i]) * rf;
+        for (int i = 0; i < EL; i++) out[i] = fmaf(x[i] * rf, C[i], y[i] * rf * S[i]);
     }
 }
 
