@@ -17,6 +17,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <math.h>
+
 #include "kv.h"
 
 namespace sparkmv {

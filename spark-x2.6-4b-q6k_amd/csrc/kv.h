@@ -4,8 +4,6 @@
 
 #include <hip/hip_runtime.h>
 
-#include <math.h>
-
 #include "../../include/sparkmv.h"
 #include "common.h"
 
@@ -59,18 +57,6 @@ __device__ __forceinline__ uint32_t kv_bf16x2(float a, float b) {
 }
 __device__ __forceinline__ uint16_t kv_bf16(float f) { return (uint16_t) kv_bf16x2(f, f); }
 
-/* 64 bits to f32 toward zero with the lost bits kept in the last one: an odd value
- * cannot lie between two bf16 values, so that the next rounding is the only one */
-__device__ __forceinline__ float kv_odd(double v) {
-    const float f = (float) v;
-    const double back = (double) f;
-    const uint32_t off = (uint32_t) (back != v) & (uint32_t) (fabsf(f) < INFINITY);
-    /* one step back where it was rounded away from zero */
-    const uint32_t u = __float_as_uint(f) - (off & (uint32_t) (fabs(back) > fabs(v)));
-    return __uint_as_float(u | off);
-}
-__device__ __forceinline__ void kv_store_wide(float * p, double v) { *p = (float) v; }
-__device__ __forceinline__ void kv_store_wide(uint16_t * p, double v) { *p = kv_bf16(kv_odd(v)); }
 /* the host's checks: 0, or -1 with the message set. kv_check_rows: nrows rows of
  * n values at stride ld, each starting 16-byte aligned */
 bool kv_aligned(const void * p, size_t n);

@@ -10,6 +10,19 @@ namespace sparkmv {
 
 namespace {
 
+/* 64 bits to bf16 with one rounding: to f32 toward zero with the lost bits kept
+ * in the last one (an odd value cannot lie between two bf16 values), then to
+ * nearest even */
+__device__ __forceinline__ void kv_store_wide(float * p, double v) { *p = (float) v; }
+__device__ __forceinline__ void kv_store_wide(uint16_t * p, double v) {
+    const float f = (float) v;
+    const double back = (double) f;
+    const uint32_t off = (uint32_t) (back != v) & (uint32_t) (fabsf(f) < INFINITY);
+    /* one step back where it was rounded away from zero */
+    const uint32_t u = __float_as_uint(f) - (off & (uint32_t) (fabs(back) > fabs(v)));
+    *p = kv_bf16(__uint_as_float(u | off));
+}
+
 /* ---------------------------------------------------------------- rope table */
 
 __global__ __launch_bounds__(256) void kv_rope_table_kernel(float * tab, int rows, int half, float theta) {

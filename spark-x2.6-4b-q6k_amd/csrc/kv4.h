@@ -7,7 +7,6 @@
 
 namespace sparkmv {
 
-constexpr int kKv4Block = 32;    /* elements that share a scale */
 constexpr int kKv4Low = 7;       /* scale bytes that an append writes: 2^-120 .. 2^125, or 255; */
 constexpr int kKv4High = 252;    /* any above this one is not a number */
 
@@ -42,7 +41,6 @@ __host__ __device__ inline int kv4_value_scale_at(int pos, int d, int hd) {
     return 66 * hd + ((pos >> 2 & 3) * (hd >> 5) + (d >> 5)) * 16 + (pos >> 5) * 8 + (pos >> 4 & 1) * 4 + (pos & 3);
 }
 
-typedef __bf16 kv4_b2 __attribute__((ext_vector_type(2)));
 typedef __bf16 kv4_b8 __attribute__((ext_vector_type(8)));
 
 /* byte B of four pairs of codes as bf16 with their scale, exactly (two significant
