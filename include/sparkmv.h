@@ -636,7 +636,7 @@ int sparkmv_kv_attend(const sparkmv_kv_cache * cache, const sparkmv_kv_batch * b
  * f0_i = theta^(-2 i / rope_dim) and
  *   NONE    f = f0
  *   LINEAR  f = f0 / factor
- *   NTK     theta factor^(d / (d - 2)) in place of theta (d = rope_dim, above 2)
+ *   NTK     theta factor^(d / (d - 2)) in place of theta (d = rope_dim; f0 where that is 2)
  *   YARN    c(r) = d ln(original / (2 pi r)) / (2 ln theta), lo = max(floor c(beta_fast), 0),
  *           hi = min(ceil c(beta_slow), d - 1), t = clamp((i - lo) / max(hi - lo, 0.001), 0, 1):
  *           f = f0 (1 - t) + f0 t / factor
@@ -697,7 +697,7 @@ int sparkmv_qk_rope(const sparkmv_qk_rows * rows, const sparkmv_head_turn * turn
  * Microscaling formats' E2M1 elements with E8M0 scales). The scale is the smallest
  * 2^e with |value| <= 7 * 2^e for all 32, -120 <= e <= 125; a value becomes the
  * nearest, of two as near the one with the even code (0 .. 7 in the order above), so
- * that it is off by at most 1 * 2^e. 32 elements one of which is not finite read as
+ * that it is off by at most 1 * 2^e (a value above 7 * 2^125 becomes 6 * 2^125). 32 elements one of which is not finite read as
  * NaN. Positions share nothing: no append changes another position, and what a
  * position holds depends on its own rows only.
  *
@@ -748,15 +748,16 @@ int sparkmv_kv4_read(const sparkmv_kv4_cache * cache, int nseq, const int * slot
                      void * v_out, int out_dtype, void * stream);
 
 /* Attention over the cache after the append, as sparkmv_kv_attend: causal within the
- * window, gated, zeros for a token none of whose positions has a page. Query elements
- * enter whole in a call of up to 48 columns (max_q tokens times query heads per kv head);
- * of more, an element is held to 2^-24 of the largest of its 32 neighbours (those
- * that share a scale of the keys), which is all of a bf16 one down to 2^-17 of that, or to
- * 2^-116 of the head's largest where that is more. A weight enters whole for f32 outputs; for bf16 ones it is held to 2^-17 of
- * itself. Scores, statistics and sums are f32, and scores have to lie
- * within its range. A position that reads as NaN, in any element of its key or value,
- * makes the tokens that see it NaN and no others. work: sparkmv_kv4_attend_work bytes
- * on the current device. */
+ * window, gated, zeros for a token none of whose positions has a page.
+ * Query elements enter whole (down to 2^-133) in a call of up to 48 columns (max_q tokens
+ * times query heads per kv head); of more, an element is held to 2^-24 of the largest of
+ * its 32 neighbours (those that share a scale of the keys), which is all of a bf16 one
+ * down to 2^-17 of that, or to 2^-116 of the head's largest where that is more. A weight
+ * enters whole for f32 outputs; for bf16 ones it is held to 2^-17 of itself. Scores,
+ * statistics and sums are f32: scores have to lie within its range, and so has 2^16
+ * times the sum of the values that a token sees. A position that reads as NaN, in any
+ * element of its key or value, makes the tokens that see it NaN and no others. work:
+ * sparkmv_kv4_attend_work bytes on the current device. */
 size_t sparkmv_kv4_attend_work(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch * batch, int heads);
 int sparkmv_kv4_attend(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch * batch, const sparkmv_kv_query * query,
                        void * stream);

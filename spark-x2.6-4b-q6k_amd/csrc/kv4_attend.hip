@@ -2,12 +2,13 @@
  *   out = sum_p softmax_p(scale * q . k_p) v_p (* sigmoid(gate))
  * over the positions p that a token sees.
  *
- * Codes become bf16 with their scale in one instruction a pair, exactly, and both
- * products run on the bf16 matrix instruction, 16 x 16 x 32, which keeps an f32 sum.
- * What meets the codes is an f32 query element or weight as a sum of bf16 numbers:
+ * Codes become bf16 with their scale in one instruction a pair, exactly, and products
+ * run on the bf16 matrix instruction, 16 x 16 x 32, which keeps an f32 sum; the scores
+ * of many columns on the one that takes 4-bit codes as they are (below). What meets the
+ * codes is an f32 query element or weight as a sum of bf16 numbers:
  *
- *   a query element as three, each the leading 8 bits of what the ones before left
- *   out, which is all of f32; bf16 queries need one;
+ *   few columns: a query element as three, each the leading 8 bits of what the ones
+ *   before left out, which is all of f32 down to bf16's 2^-133; bf16 queries need one;
  *
  *   a weight e^(s - m) as three for f32 outputs, again all of it, and as two for
  *   bf16 ones, 2^-17 of it at most being lost.
@@ -58,7 +59,7 @@ __device__ __forceinline__ uint32_t kv4_quad_part(const uint32_t * part, uint32_
 }
 
 constexpr int kKv4Cols = 16;      /* columns (token, query head) of a kv head that the flat kernels take at a time */
-/* pages that beginning a kv head of a sequence counts: with 4, 8, 12 and 16, 48 sequences of 12000 positions
+/* pages that beginning a kv head of a sequence counts: with 4, 8, 12 and 16, 48 sequences of up to 12000
  * take 70.0, 57.7, 54.3 and 54.3 us, 3 of 6000 with 8 tokens each 19.8, 20.2, 20.1 and 21.1 */
 constexpr int kKv4Item = 12;
 constexpr int kKv4Most = 1024;    /* workgroups of shares, at most */
@@ -90,9 +91,9 @@ constexpr int kv4_lds(int hd, int dq, int waves, int cmax) {
 /* ------------------------------------------------------------- few columns
  *
  * Sixteen columns of a kv head at a time: decode steps and short blocks. Bound by
- * reading the codes, 136 bytes a position of 256: with four heads of them, 131072
- * positions (143 MB) take 43.5 us and 48 sequences of 12000 (314 MB, partly cached from
- * call to call) 54.1 with the join's 5; one of 1004 takes 11.6, most of it latency.
+ * reading the codes, 272 bytes a kv head and position of 256: with four heads, 131072
+ * positions (143 MB) take 43.5 us and 48 sequences of up to 12000 (155313, 169 MB) 54.1,
+ * the joins' 5 and 6 included; one of 1004 takes 11.6, most of it latency.
  *
  * DQ 0, up to four columns: an instruction's sixteen columns are the four columns
  * times the parts of a query element or weight, so that f32's whole precision costs
@@ -624,11 +625,11 @@ __global__ __launch_bounds__(512) void kv4_flat_join_kernel(const Kv4Flat A) {
  * it is worked on: codes of keys as they lie, by direct loads; values as the bf16
  * operands that they become, converted once for all waves.
  *
- * 512 bf16 tokens of 16 heads of 256 at 16384 take 226 us with the join's 13: 139 GFLOP
- * as the formula counts them, 0.62 PFLOP/s, where a large bf16 product reaches 1.2. With
- * any one of the parts left out (scores, exponentials, conversion, the values' product)
- * a wave's time falls by a tenth at most: the vector and matrix pipes take turns, two
- * waves a SIMD being all that the registers hold.
+ * 512 bf16 tokens of 16 heads of 256 at 16384 take 220 us with the join's 13: 140 GFLOP
+ * as the formula counts them, 0.63 PFLOP/s, where a large bf16 product reaches 1.2. With
+ * four of the scores' five parts left out it would be 195, without the values' conversion
+ * 191, without their products 206, without exponentials no less: the vector and matrix
+ * pipes take turns, two waves a SIMD being all that the registers hold.
  *
  * The scores use the instruction that multiplies 4-bit codes as they are, 16 x 16 x 128
  * with a power of two for every 32 elements. A query element enters it as a sum of
@@ -637,15 +638,15 @@ __global__ __launch_bounds__(512) void kv4_flat_join_kernel(const Kv4Flat A) {
  * bf16's), at most 4 in magnitude and off by 1 / 8 at most: 2^-24 of the largest of the 32 is
  * what may be lost, and nothing of a bf16 element down to 2^-17 of it. Six parts for
  * head_dim 64, where an instruction takes two.
- * Two parts of 8 bits (E4M3) would do for bf16 (205 us for the call above), but for the
+ * Two parts of 8 bits (E4M3) would do for bf16 (205 us for the call above) but for the
  * sum: within 16 elements of a lane the instruction drops what lies below 2^-13 of the
  * largest product, which left outputs off by 1e-5. Products of a 6-bit part and a code
  * are multiples of 1 / 16 up to 24, so none of them is cut.
  *
  * Weights times values as in the flat kernels. */
 constexpr int kKv4Tile = 128;       /* columns of a workgroup */
-/* pages that beginning a tile's kv head counts: with 2, 6 and 12, 512 tokens at 16384
- * take 209, 205 and 217 us, at 1000 52.8, 51.6 and 53.2 */
+/* pages that beginning a tile's kv head counts: with 2, 4, 6 and 12, 512 tokens at 16384
+ * take 223, 222, 220 and 225 us, at 1000 54.9, 54.2, 54.5 and 55.5 */
 constexpr int kKv4TileItem = 6;
 constexpr int kKv4Tiles = 2048;     /* tiles that are split among equal shares, at most */
 constexpr int kKv4Ids = 256;        /* page numbers held at a time */
@@ -1309,9 +1310,9 @@ Kv4Plan kv4_plan(const sparkmv_kv4_cache * c, const sparkmv_kv_batch * b, int he
     const long in_window = ((long) window + kKvPage - 2) / kKvPage + 1, seen = window > 0 && in_window < pages ? in_window : pages;
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t o = off; off += (bytes + 255) & ~(size_t) 255; return o; };
-    /* few columns read a tile's pages again for each 16; blocks of 12 tokens with 4 heads
-     * each (48 columns) of 3 sequences of 6000 24.4 us, tiles of 128 28.7; of 16 tokens
-     * 32.6 and 32.5, of one sequence of 60000 60.3 and 55.5 */
+    /* few columns read a tile's pages again for each 16; blocks of 12 bf16 tokens with 4
+     * heads each (48 columns) of 3 sequences of up to 6000 23.8 us, tiles of 128 30.3, of one
+     * of 60000 49 and 55; of 16 tokens 29.8 and 33.8, 57.7 and 57.1 */
     p.flat = cols <= 3 * kKv4Cols;
     if (p.flat) {
         p.quad = cols <= 4;
@@ -1321,9 +1322,14 @@ Kv4Plan kv4_plan(const sparkmv_kv4_cache * c, const sparkmv_kv_batch * b, int he
          * us, 32 17.4 and 13.4; 9 pages of 24 sequences 10.7 and 19.6 */
         p.whole = cols <= kKv4Cols && seen <= 16;
         /* One workgroup a CU has fewer results to join than two, which keep more loads in
-         * flight. Two against one at head_dim 256: 500 pages 17.2 and 14.7 us, 2500 27.4
-         * and 22.0, 8192 45.9 and 44.3, 18000 40.1 and 42.3, 36000 58.3 and 63.3; at 128,
-         * with less to do for a page: 4000 13.1 and 12.4, 8000 15.4 and 16.6. */
+         * flight and even out lengths that differ. The host knows no lengths: `all` is what
+         * max_len allows, which sequences of unequal lengths do not reach. One against two
+         * with four kv heads, us. head_dim 256, one sequence of 8000 14.4 and 17.3, of 32000
+         * 21.0 and 25.3, of 128000 43.4 and 44.0; 16 of 16000 68 and 70, of 24000 93 and 100;
+         * of up to 16000 21.8 and 25.5, 48 of up to 12000 54.8 both, 32 of up to 32000 79
+         * and 77. 128: one of 64000 15.9 and 17.1, 16 of 8000 22.3 and 21.5, 64 of 16000 103
+         * and 111; 48 of up to 12000 27.9 and 25.3. 64: one of 64000 13.4 and 14.1, 16 of
+         * 8000 18.5 and 16.9, of 32000 45.6 and 35.9; 48 of up to 12000 23.4 and 20.7 */
         const long all = seen * p.seq_tiles * b->nseq * c->kv_heads;
         const long two = all >= (long) cu_count() * (hd == 256 ? 56 : 24) ? 2 : 1;
         const long most = two * cu_count() < kKv4Most ? two * cu_count() : kKv4Most;
@@ -1333,8 +1339,8 @@ Kv4Plan kv4_plan(const sparkmv_kv4_cache * c, const sparkmv_kv_batch * b, int he
         p.pml = take((size_t) p.groups * 2 * p.cmax * 2 * 4);
     } else {
         p.tiles = (long) b->ntok * G / kKv4Tile + b->nseq;
-        /* shares while their counts fit, one a CU: 512 tokens at 1000 53.2 us, with half as
-         * many 65.4 */
+        /* shares while their counts fit, one a CU: 512 tokens at 1000 54.4 us, with half as
+         * many 68.0 */
         if (p.tiles <= kKv4Tiles && p.tiles * ((long) c->max_pages + kKv4TileItem) <= 0x7fffffffl / c->kv_heads) {
             const long all = pages * p.tiles * c->kv_heads, most = cu_count();
             p.groups = (int) (all < 1 ? 1 : (all < most ? all : most));
@@ -1409,8 +1415,8 @@ int sparkmv_kv4_attend(const sparkmv_kv4_cache * cache, const sparkmv_kv_batch *
         t.pre = (int *) (mem + p.pre); t.po = (float *) (mem + p.po); t.pml = (float *) (mem + p.pml);
         const uint32_t lists = p.groups ? ((uint32_t) batch->nseq + (uint32_t) p.tiles + 1) * 4 : 0;
         const dim3 grid((unsigned) (p.groups ? p.groups : p.tiles * cache->kv_heads));
-        /* columns a wave of the join: one or two, with 12 tiles' kv heads 26.2 us for the call
-         * and 29.2, with 68 39.5 and 38.0 */
+        /* columns a wave of the join: one or two, with 12 tiles' kv heads 27.5 us for the call
+         * and 30.3, with 68 40.8 and 39.1 */
         const int each = p.tiles * cache->kv_heads * (kKv4Tile / 4) > 4 * cu_count() ? 2 : 1;
         const dim3 join((unsigned) p.tiles, (unsigned) cache->kv_heads, (unsigned) (kKv4Tile / 4 / each));
 #define KV4_TILE(H, DP)                                                                                              \

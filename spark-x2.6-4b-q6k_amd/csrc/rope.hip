@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTable A) {
  * token, queries' and then keys'. C and S (heads.h) are worked out once a workgroup, an
  * element a thread, and shared through LDS: loaded by every lane from the table and the
  * weights they are four times the bytes of the heads themselves, and what bounds (8192
- * tokens of 40 bf16 heads of 128 68.5 us). Now the rows in and out do: 36.9 us, 4.5 TB/s,
+ * tokens of 40 bf16 heads of 128 68.5 us). Now the rows in and out do: 37.3 us, 4.5 TB/s,
  * where a copy of them takes 33. */
 struct QkRope {
     sparkmv_qk_rows r;
